@@ -61,6 +61,11 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "gw_selftest_wait_timeout": (_i, [_i64, _vp]),
     "gw_dynamic_linear": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _i64, _i64, _d, _vp, _i, _vp, _i64,
                                _vp, _vp, _vp]),
+    "gw_rms_norm": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _d, _vp, _i64, _vp,
+                         _i64, _i64, _vp]),
+    "gw_rms_norm_q8": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _d, _vp, _i64, _vp,
+                            _i64, _i64, _vp, _vp]),
+    "gw_quantize_rows": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp]),
     "gw_gather_columns_dev": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _vp]),
     "gw_gather_rows_t_dev": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _vp]),
     "gw_gather_gemm_dev": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _i,
@@ -74,7 +79,7 @@ _api = None
 # binds; the same arguments as the ctypes functions, a fraction of the host time.
 FAST_ENTRIES = ("gw_gather_gemm", "gw_gather_gemm_dev", "gw_packed_gemm", "gw_gather_columns", "gw_dynamic_linear",
                 "gw_gather_rows_t", "gw_gather_columns_dev", "gw_gather_rows_t_dev", "gw_mask_compact",
-                "gw_gather_gemm_workspace_bytes")
+                "gw_rms_norm", "gw_rms_norm_q8", "gw_quantize_rows", "gw_gather_gemm_workspace_bytes")
 
 
 class _Api:
@@ -506,6 +511,42 @@ def dynamic_linear(x: torch.Tensor, weight: torch.Tensor, threshold: float, y: t
     if st != GW_OK and st != GW_ERR_UNSUPPORTED:
         _check(st, "gw_dynamic_linear")
     return st
+
+
+def _ld(t: torch.Tensor) -> int:
+    """Leading dimension of a row-major matrix (torch gives matrices of one row any stride)."""
+    return max(t.stride(0), t.shape[1])
+
+
+def rms_norm(x: torch.Tensor, residual: torch.Tensor | None, total: torch.Tensor | None,
+             weight: torch.Tensor | None, eps: float, idx: torch.Tensor | None, n: int, y: torch.Tensor,
+             scale: torch.Tensor | None = None) -> None:
+    """gw_rms_norm (scale None) or gw_rms_norm_q8 over row-major matrices; y is the whole
+    padded buffer, of which the first n columns are outputs and the rest is zeroed."""
+    _rowmajor(x, y)
+    rows, cols = x.shape
+    with _on_device(x.device):
+        head = (x.data_ptr(), dtype_code(x.dtype), rows, cols, _ld(x), _ptr(residual),
+                0 if residual is None else _ld(residual), _ptr(total), 0 if total is None else _ld(total),
+                _ptr(weight), float(eps), _ptr(idx), n, y.data_ptr(), _ld(y), y.shape[1])
+        if scale is None:
+            what, st = "gw_rms_norm", api().gw_rms_norm(*head, _stream(x.device))
+        else:
+            what, st = "gw_rms_norm_q8", api().gw_rms_norm_q8(*head, scale.data_ptr(), _stream(x.device))
+    if st:
+        _check(st, what)
+
+
+def quantize_rows(x: torch.Tensor, idx: torch.Tensor | None, n: int, q: torch.Tensor,
+                  scale: torch.Tensor) -> None:
+    """gw_quantize_rows over a row-major matrix; q is the whole padded buffer."""
+    _rowmajor(x, q)
+    rows, cols = x.shape
+    with _on_device(x.device):
+        st = api().gw_quantize_rows(x.data_ptr(), dtype_code(x.dtype), rows, cols, _ld(x), _ptr(idx), n,
+                                    q.data_ptr(), _ld(q), q.shape[1], scale.data_ptr(), _stream(x.device))
+    if st:
+        _check(st, "gw_quantize_rows")
 
 
 def validate_indices(idx: torch.Tensor, K: int) -> int:

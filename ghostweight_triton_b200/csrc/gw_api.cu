@@ -652,6 +652,80 @@ int gw_packed_gemm(const void* a, int dtype, int64_t M, int64_t K, int64_t lda,
   return e == cudaSuccess ? GW_OK : cuda_fail(e);
 }
 
+namespace {
+// The checks and the launch that the three row operators share.
+int run_rows(gw::RowParams& p, int dtype, bool q8, bool norm, cudaStream_t s) {
+  if (!valid_dtype(dtype)) return GW_ERR_DTYPE;
+  if (!matrix_ok(p.rows, p.cols, p.ldx) || p.n < 0 || p.pad < p.n ||
+      !matrix_ok(p.rows, p.pad, p.ldy))
+    return GW_ERR_SHAPE;
+  if (norm && p.rows > 0 && p.cols == 0) return GW_ERR_SHAPE;      // the mean of nothing
+  if (p.r && !matrix_ok(p.rows, p.cols, p.ldr)) return GW_ERR_SHAPE;
+  if (p.s && !matrix_ok(p.rows, p.cols, p.lds)) return GW_ERR_SHAPE;
+  if (!p.idx && p.n != p.cols && p.n != 0) return GW_ERR_NULL;
+  const gw::DeviceInfo* d = nullptr;
+  int st = current_device(&d);
+  if (st != GW_OK) return st;
+  if (p.rows == 0) return GW_OK;
+  if (p.cols > 0 && !p.x) return GW_ERR_NULL;
+  if (p.pad > 0 && !p.y) return GW_ERR_NULL;
+  if (q8 && !p.scale) return GW_ERR_NULL;
+  p.err = d->err_word;
+  cudaError_t e = gw::launch_rows(p, dtype, q8, norm, d->sm_count, s);
+  return e == cudaSuccess ? GW_OK : cuda_fail(e);
+}
+
+gw::RowParams row_params(const void* x, int64_t rows, int64_t cols, int64_t ldx,
+                         const void* residual, int64_t ldr, void* sum, int64_t lds,
+                         const void* weight, double eps, const int64_t* idx, int64_t n_idx, void* y,
+                         int64_t ldy, int64_t pad_to, float* scale) {
+  gw::RowParams p;
+  p.x = x;
+  p.ldx = ldx;
+  p.r = residual;
+  p.ldr = ldr;
+  p.s = sum;
+  p.lds = lds;
+  p.g = weight;
+  p.eps = static_cast<float>(eps);
+  p.idx = idx;
+  p.n = n_idx;
+  p.pad = pad_to;
+  p.y = y;
+  p.ldy = ldy;
+  p.scale = scale;
+  p.rows = rows;
+  p.cols = cols;
+  return p;
+}
+}  // namespace
+
+int gw_rms_norm(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx,
+                const void* residual, int64_t ldr, void* sum, int64_t lds, const void* weight,
+                double eps, const int64_t* idx, int64_t n_idx, void* y, int64_t ldy,
+                int64_t pad_to, void* stream) {
+  gw::RowParams p = row_params(x, rows, cols, ldx, residual, ldr, sum, lds, weight, eps, idx, n_idx,
+                               y, ldy, pad_to, nullptr);
+  return run_rows(p, dtype, false, true, static_cast<cudaStream_t>(stream));
+}
+
+int gw_rms_norm_q8(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx,
+                   const void* residual, int64_t ldr, void* sum, int64_t lds, const void* weight,
+                   double eps, const int64_t* idx, int64_t n_idx, void* q, int64_t ldq,
+                   int64_t pad_to, float* scale, void* stream) {
+  gw::RowParams p = row_params(x, rows, cols, ldx, residual, ldr, sum, lds, weight, eps, idx, n_idx,
+                               q, ldq, pad_to, scale);
+  return run_rows(p, dtype, true, true, static_cast<cudaStream_t>(stream));
+}
+
+int gw_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx,
+                     const int64_t* idx, int64_t n_idx, void* q, int64_t ldq, int64_t pad_to,
+                     float* scale, void* stream) {
+  gw::RowParams p = row_params(x, rows, cols, ldx, nullptr, 0, nullptr, 0, nullptr, 0.0, idx, n_idx,
+                               q, ldq, pad_to, scale);
+  return run_rows(p, dtype, true, false, static_cast<cudaStream_t>(stream));
+}
+
 int gw_gemm_plan(int64_t M, int64_t N, int64_t K, int* kernel, int* tile_n, int* split) {
   if (M < 0 || N < 0 || K < 0) return GW_ERR_SHAPE;
   if (!kernel) return GW_ERR_NULL;

@@ -62,6 +62,32 @@ cudaError_t launch_validate_indices(const int64_t* idx, int64_t n, int64_t K, in
 cudaError_t launch_index_runs(const int64_t* idx, int64_t n, int64_t K, int32_t* bad,
                               cudaStream_t stream);
 
+// gw_norm.cu: rows of x (+ r) normed and / or rounded to e4m3 over the alive
+// columns (see the file comment there for the formulas).
+struct RowParams {
+  const void* x = nullptr;          // [rows, cols], leading dimension ldx
+  int64_t ldx = 0;
+  const void* r = nullptr;          // residual [rows, cols] or null
+  int64_t ldr = 0;
+  void* s = nullptr;                // x + r out [rows, cols] (may be x or r itself) or null
+  int64_t lds = 0;
+  const void* g = nullptr;          // norm weight [cols] or null
+  float eps = 0.0f;
+  const int64_t* idx = nullptr;     // alive list (n entries) or null: all columns
+  int64_t n = 0;                    // outputs per row
+  int64_t pad = 0;                  // columns [n, pad) of y are written as zero
+  void* y = nullptr;                // [rows, pad] of x's type, or e4m3
+  int64_t ldy = 0;
+  float* scale = nullptr;           // e4m3: [rows]
+  int64_t rows = 0;
+  int64_t cols = 0;
+  unsigned int* err = nullptr;
+};
+// q8: y is e4m3 with scales. norm: the root-mean-square norm, else x as it is
+// (only with q8).
+cudaError_t launch_rows(const RowParams& p, int dtype, bool q8, bool norm, int sm_count,
+                        cudaStream_t stream);
+
 // gw_gemm_tc.cu: tcgen05 gather-GEMM / packed GEMM (fp16, bf16).
 // a_mode: 0 -> A is a dense [M, n_alive] matrix loaded by TMA (idx unused)
 //         1 -> producer warps gather x[:, idx] into shared memory

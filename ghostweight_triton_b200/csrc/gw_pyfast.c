@@ -148,6 +148,31 @@ static PyObject* fast_dynamic_linear(PyObject* self, PyObject* const* args, Py_s
                                            (int32_t*)a[13].p, (int32_t*)a[14].p, a[15].p));
 }
 
+static PyObject* fast_rms_norm(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  GW_PARSE("pilllplplpdplpllp")
+  return PyLong_FromLong(gw_rms_norm(a[0].p, a[1].i, a[2].l, a[3].l, a[4].l, a[5].p, a[6].l, a[7].p,
+                                     a[8].l, a[9].p, a[10].d, (const int64_t*)a[11].p, a[12].l,
+                                     a[13].p, a[14].l, a[15].l, a[16].p));
+}
+
+static PyObject* fast_rms_norm_q8(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  GW_PARSE("pilllplplpdplpllpp")
+  return PyLong_FromLong(gw_rms_norm_q8(a[0].p, a[1].i, a[2].l, a[3].l, a[4].l, a[5].p, a[6].l,
+                                        a[7].p, a[8].l, a[9].p, a[10].d, (const int64_t*)a[11].p,
+                                        a[12].l, a[13].p, a[14].l, a[15].l, (float*)a[16].p,
+                                        a[17].p));
+}
+
+static PyObject* fast_quantize_rows(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  GW_PARSE("pilllplpllpp")
+  return PyLong_FromLong(gw_quantize_rows(a[0].p, a[1].i, a[2].l, a[3].l, a[4].l,
+                                          (const int64_t*)a[5].p, a[6].l, a[7].p, a[8].l, a[9].l,
+                                          (float*)a[10].p, a[11].p));
+}
+
 static PyObject* fast_gather_gemm_workspace_bytes(PyObject* self, PyObject* const* args,
                                                   Py_ssize_t nargs) {
   (void)self;
@@ -178,6 +203,9 @@ static PyMethodDef gw_fast_methods[] = {
     GW_FAST(gather_rows_t_dev),
     GW_FAST(mask_compact),
     GW_FAST(dynamic_linear),
+    GW_FAST(rms_norm),
+    GW_FAST(rms_norm_q8),
+    GW_FAST(quantize_rows),
     GW_FAST(gather_gemm_workspace_bytes),
     GW_FAST(library_anchor),
     {NULL, NULL, 0, NULL},

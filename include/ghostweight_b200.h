@@ -337,6 +337,53 @@ GW_API int gw_packed_gemm(const void* a, int dtype, int64_t M, int64_t K, int64_
                           int epilogue, void* y, int64_t ldy, void* stream);
 
 /*
+ * Residual addition and root-mean-square norm of rows, written out over the
+ * alive columns of the layer that reads them:
+ *   s[m, k] = x[m, k] + residual[m, k]                       (all cols columns)
+ *   y[m, j] = s[m, idx[j]] * rsqrt(mean_k s[m, k]^2 + eps) * weight[idx[j]]
+ * for j < n_idx, and y[m, j] = 0 for n_idx <= j < pad_to (pad_to <= ldy; pass
+ * pad_to = n_idx for no padding). x [rows, cols] (ldx), residual [rows, cols]
+ * (ldr) or NULL (s = x), sum (lds): where s is written, or NULL; weight [cols]
+ * or NULL (ones); all of one dtype. idx NULL stands for all columns (n_idx =
+ * cols). The norm uses the fp32 sum before its rounding; y and sum are each
+ * rounded once. sum may be x or residual itself (same pointer and leading
+ * dimension); y overlaps none of the inputs. The list may have any order and
+ * repeats; an index outside [0, cols) gives a zero column and raises
+ * GW_DEVICE_ERR_BAD_INDEX. Entries of x outside the list count in the mean.
+ *
+ * No counterpart in the reference, whose layers take an activation that torch
+ * normed over the whole row and gather it again (kernels/gather.py:139-146).
+ */
+GW_API int gw_rms_norm(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx,
+                       const void* residual, int64_t ldr, void* sum, int64_t lds,
+                       const void* weight, double eps, const int64_t* idx, int64_t n_idx, void* y,
+                       int64_t ldy, int64_t pad_to, void* stream);
+
+/*
+ * gw_rms_norm with the output in 8 bits:
+ *   scale[m] = max(max_j |y[m, j]| / 448, 2^-126)              (float, [rows])
+ *   q[m, j]  = y[m, j] / scale[m] rounded to e4m3              (1 byte, ldq)
+ * y is the unrounded fp32 value; columns [n_idx, pad_to) of q are zero. A row
+ * with a NaN or an infinity among its outputs gets a scale that is one, so
+ * that its values read back as NaN.
+ */
+GW_API int gw_rms_norm_q8(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx,
+                          const void* residual, int64_t ldr, void* sum, int64_t lds,
+                          const void* weight, double eps, const int64_t* idx, int64_t n_idx,
+                          void* q, int64_t ldq, int64_t pad_to, float* scale, void* stream);
+
+/*
+ * Rows rounded to e4m3 with one scale each, as gw_rms_norm_q8 does it, of
+ * y[m, j] = x[m, idx[j]] (idx NULL: all columns). With x = nn.Linear.weight
+ * [N, K] it packs W[:, alive] for gw_packed_gemm_q8, with x an activation it
+ * makes that product's other operand. Entries of x outside the list are not
+ * looked at.
+ */
+GW_API int gw_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx,
+                            const int64_t* idx, int64_t n_idx, void* q, int64_t ldq,
+                            int64_t pad_to, float* scale, void* stream);
+
+/*
  * Counts indices outside [0, K) into *bad_count (int32, device, overwritten).
  * Debug helper for callers that want the reference's implicit "indices are
  * valid" contract checked (kernels/matmul.py:120 performs no check).
