@@ -61,6 +61,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "gw_selftest_wait_timeout": (_i, [_i64, _vp]),
     "gw_dynamic_linear": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _i64, _i64, _d, _vp, _i, _vp, _i64,
                                _vp, _vp, _vp]),
+    "gw_gather_gemm_residual": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i,
+                                     _vp, _i64, _vp, _i64, _i, _vp, _sz, _vp]),
+    "gw_gather_gemm_dev_residual": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _i,
+                                         _vp, _i64, _vp, _i64, _vp, _sz, _vp]),
+    "gw_dynamic_linear_residual": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _i64, _i64, _d, _vp, _i, _vp, _i64,
+                                        _vp, _i64, _vp, _vp, _vp]),
+    "gw_packed_gemm_residual": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i, _vp, _i64,
+                                     _vp, _i64, _vp]),
     "gw_rms_norm": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _d, _vp, _i64, _vp,
                          _i64, _i64, _vp]),
     "gw_rms_norm_q8": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _d, _vp, _i64, _vp,
@@ -79,7 +87,8 @@ _api = None
 # binds; the same arguments as the ctypes functions, a fraction of the host time.
 FAST_ENTRIES = ("gw_gather_gemm", "gw_gather_gemm_dev", "gw_packed_gemm", "gw_gather_columns", "gw_dynamic_linear",
                 "gw_gather_rows_t", "gw_gather_columns_dev", "gw_gather_rows_t_dev", "gw_mask_compact",
-                "gw_rms_norm", "gw_rms_norm_q8", "gw_quantize_rows", "gw_gather_gemm_workspace_bytes")
+                "gw_gather_gemm_residual", "gw_gather_gemm_dev_residual", "gw_dynamic_linear_residual",
+                "gw_packed_gemm_residual", "gw_rms_norm", "gw_rms_norm_q8", "gw_quantize_rows", "gw_gather_gemm_workspace_bytes")
 
 
 class _Api:
@@ -183,6 +192,11 @@ def _rowmajor(*ts: torch.Tensor) -> None:
     for t in ts:
         assert t.ndim == 2 and (t.stride(1) == 1 or t.shape[1] <= 1), (
             f"expected a row-major matrix, got shape {tuple(t.shape)} strides {t.stride()}")
+
+
+def _residual(t: torch.Tensor | None) -> tuple[int | None, int]:
+    """(pointer, leading dimension) of a residual matrix, or of none."""
+    return (None, 0) if t is None else (t.data_ptr(), max(t.stride(0), t.shape[1]))
 
 
 try:  # the raw cudaStream_t of torch's current stream, without building a Stream object
@@ -332,8 +346,9 @@ def gemm_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
 
 def gather_gemm(x: torch.Tensor, w_packed: torch.Tensor, idx: torch.Tensor, y: torch.Tensor,
                 bias: torch.Tensor | None = None, activation: str | None = None,
-                strategy: str = "auto", workspace: torch.Tensor | None = None) -> None:
-    """y = act(x[:, idx] @ w_packed[:, :len(idx)]^T + bias) on the current stream.
+                strategy: str = "auto", workspace: torch.Tensor | None = None,
+                residual: torch.Tensor | None = None) -> None:
+    """y = act(x[:, idx] @ w_packed[:, :len(idx)]^T + bias) + residual on the current stream.
 
     strategy "auto" uses the two-launch pregather path when `workspace` is large
     enough, else the single fused kernel; "fused" / "pregather" force one;
@@ -350,11 +365,11 @@ def gather_gemm(x: torch.Tensor, w_packed: torch.Tensor, idx: torch.Tensor, y: t
     if dev != cur:
         torch.cuda.set_device(dev)
     try:
-        st = api().gw_gather_gemm(
+        st = api().gw_gather_gemm_residual(
             x.data_ptr(), DTYPE_CODES[x.dtype], M, K, max(x.stride(0), K), w_packed.data_ptr(), N,
             max(w_packed.stride(0), n), idx.data_ptr(), n, _ptr(bias), epilogue_code(activation),
-            y.data_ptr(), max(y.stride(0), N), GEMM_STRATEGIES[strategy], ws_ptr, ws_bytes,
-            _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream)
+            *_residual(residual), y.data_ptr(), max(y.stride(0), N), GEMM_STRATEGIES[strategy], ws_ptr,
+            ws_bytes, _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream)
     finally:
         if dev != cur:
             torch.cuda.set_device(cur)
@@ -374,7 +389,8 @@ def prepare_gather_gemm(w_packed: torch.Tensor, idx: torch.Tensor, bias: torch.T
             idx.data_ptr(), n, _ptr(bias), epilogue_code(activation), GEMM_STRATEGIES[strategy])
 
 
-def gather_gemm_prepared(prep: tuple, x: torch.Tensor, y: torch.Tensor) -> None:
+def gather_gemm_prepared(prep: tuple, x: torch.Tensor, y: torch.Tensor,
+                         residual: torch.Tensor | None = None) -> None:
     """gather_gemm(x, ...) with the fixed arguments of :func:`prepare_gather_gemm`.
 
     x [M, K] must be contiguous and on the current device, y [M, N] contiguous.
@@ -392,9 +408,9 @@ def gather_gemm_prepared(prep: tuple, x: torch.Tensor, y: torch.Tensor) -> None:
             ws = gemm_workspace(x.device, ws_bytes)
             ws_ptr, ws_bytes = ws.data_ptr(), ws.numel()
     dev = x.get_device()
-    st = api().gw_gather_gemm(
-        x.data_ptr(), dtc, M, K, K, wptr, N, ldw, iptr, n, bptr, epi, y.data_ptr(), N, strat,
-        ws_ptr, ws_bytes, _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream)
+    st = api().gw_gather_gemm_residual(
+        x.data_ptr(), dtc, M, K, K, wptr, N, ldw, iptr, n, bptr, epi, *_residual(residual), y.data_ptr(), N,
+        strat, ws_ptr, ws_bytes, _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream)
     if st:
         _check(st, "gw_gather_gemm")
 
@@ -430,7 +446,8 @@ def gather_rows_t_dev(src: torch.Tensor, idx: torch.Tensor, n_dev: torch.Tensor,
 
 def gather_gemm_dev(x: torch.Tensor, w_packed: torch.Tensor, idx: torch.Tensor, n_dev: torch.Tensor,
                     y: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
-                    workspace: torch.Tensor | None = None) -> None:
+                    workspace: torch.Tensor | None = None,
+                    residual: torch.Tensor | None = None) -> None:
     """gather_gemm with K' = n_dev[0] read on the device (len(idx) is its upper bound)."""
     _rowmajor(x, w_packed, y)
     assert idx.dtype == torch.int64 and n_dev.dtype == torch.int32
@@ -442,10 +459,10 @@ def gather_gemm_dev(x: torch.Tensor, w_packed: torch.Tensor, idx: torch.Tensor, 
         workspace = gemm_workspace(x.device, nbytes) if nbytes else None
     ws_ptr, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
     with _on_device(x.device):
-        st = api().gw_gather_gemm_dev(
+        st = api().gw_gather_gemm_dev_residual(
             _ptr(x), dtype_code(x.dtype), M, K, max(x.stride(0), K), _ptr(w_packed), N,
             w_packed.stride(0), _ptr(idx), n, _ptr(n_dev), _ptr(bias), epilogue_code(activation),
-            _ptr(y), max(y.stride(0), N), ws_ptr, ws_bytes, _stream(x.device))
+            *_residual(residual), _ptr(y), max(y.stride(0), N), ws_ptr, ws_bytes, _stream(x.device))
     _check(st, "gw_gather_gemm_dev")
 
 
@@ -481,32 +498,35 @@ def gather_gemm_peers(x: torch.Tensor, w_packed: torch.Tensor, idx: torch.Tensor
 
 
 def packed_gemm(a: torch.Tensor, w_packed: torch.Tensor, y: torch.Tensor,
-                bias: torch.Tensor | None = None, activation: str | None = None) -> None:
-    """y = act(a @ w_packed[:, :K]^T + bias) with both operands loaded by TMA."""
+                bias: torch.Tensor | None = None, activation: str | None = None,
+                residual: torch.Tensor | None = None) -> None:
+    """y = act(a @ w_packed[:, :K]^T + bias) + residual with both operands loaded by TMA."""
     _rowmajor(a, w_packed, y)
     M, K = a.shape
     N = w_packed.shape[0]
     with _on_device(a.device):
-        st = api().gw_packed_gemm(
+        st = api().gw_packed_gemm_residual(
             _ptr(a), dtype_code(a.dtype), M, K, max(a.stride(0), K), _ptr(w_packed), N,
-            max(w_packed.stride(0), K), _ptr(bias), epilogue_code(activation), _ptr(y),
+            max(w_packed.stride(0), K), _ptr(bias), epilogue_code(activation), *_residual(residual), _ptr(y),
             max(y.stride(0), N), _stream(a.device))
     _check(st, "gw_packed_gemm")
 
 
 def dynamic_linear(x: torch.Tensor, weight: torch.Tensor, threshold: float, y: torch.Tensor,
                    bias: torch.Tensor | None = None, activation: str | None = None,
-                   count: torch.Tensor | None = None, mask: torch.Tensor | None = None) -> int:
+                   count: torch.Tensor | None = None, mask: torch.Tensor | None = None,
+                   residual: torch.Tensor | None = None) -> int:
     """Mask of x's columns and the sparse layer y = act(x[:, alive] @ weight[:, alive]^T + bias)
-    in one launch (gw_dynamic_linear). Returns the gw_status: GW_ERR_UNSUPPORTED for shapes
+    + residual in one launch (gw_dynamic_linear). Returns the gw_status: GW_ERR_UNSUPPORTED for shapes
     or layouts the single launch does not take (the caller then runs the separate kernels);
     raises on any other error."""
     M, K = x.shape
     N = weight.shape[0]
     with _on_device(x.device):
-        st = api().gw_dynamic_linear(
+        st = api().gw_dynamic_linear_residual(
             x.data_ptr(), DTYPE_CODES[x.dtype], M, K, x.stride(0), weight.data_ptr(), N,
-            weight.stride(0), float(threshold), _ptr(bias), epilogue_code(activation), y.data_ptr(),
+            weight.stride(0), float(threshold), _ptr(bias), epilogue_code(activation), *_residual(residual),
+            y.data_ptr(),
             y.stride(0), _ptr(count), _ptr(mask), _stream(x.device))
     if st != GW_OK and st != GW_ERR_UNSUPPORTED:
         _check(st, "gw_dynamic_linear")

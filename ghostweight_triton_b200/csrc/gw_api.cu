@@ -381,21 +381,23 @@ cudaError_t launch_dense_gemm(const void* a, int dtype, int64_t M, int64_t K, in
                               const void* w, int64_t N, int64_t ldw, const void* bias, int epilogue,
                               void* y, int64_t ldy, const gw::DeviceInfo* d, cudaStream_t s,
                               void* const* peers = nullptr, int n_peers = 0,
-                              const int64_t* a_cols = nullptr, int64_t a_width = 0) {
+                              const int64_t* a_cols = nullptr, int64_t a_width = 0,
+                              const gw::Residual& res = {}) {
   const GemmChoice c = choose_gemm(M, N, K, d);
   if (c.kernel == GW_KERNEL_PAIR)
     return gw::launch_gemm_tc2(a, dtype, M, K, lda, w, N, ldw, bias, epilogue, y, ldy,
-                               d->err_word, d->sm_count, s, peers, n_peers, a_cols, a_width);
+                               d->err_word, d->sm_count, s, peers, n_peers, a_cols, a_width, nullptr,
+                               nullptr, res);
   cudaError_t e;
   if (c.kernel == GW_KERNEL_DECODE)
     e = gw::launch_gemm_decode(c.dp, a, dtype, M, K, lda, w, N, ldw, bias, epilogue, y, ldy,
-                               d->err_word, s, a_cols, a_width);
+                               d->err_word, s, a_cols, a_width, res);
   else if (c.kernel == GW_KERNEL_SPLITK)
     e = gw::launch_gemm_splitk(c.sk, a, dtype, M, K, lda, w, N, ldw, bias, epilogue, y, ldy,
-                               d->err_word, s, a_cols, a_width);
+                               d->err_word, s, a_cols, a_width, res);
   else
     e = gw::launch_gemm_tc(0, a, dtype, M, a_cols ? a_width : K, lda, w, N, ldw, nullptr, K, bias,
-                           epilogue, y, ldy, d->err_word, d->sm_count, s, a_cols);
+                           epilogue, y, ldy, d->err_word, d->sm_count, s, a_cols, nullptr, res);
   if (e != cudaSuccess || n_peers == 0) return e;
   return gw::launch_copy_to_peers(y, M, N, ldy, peers, n_peers, d->sm_count, s);
 }
@@ -411,13 +413,22 @@ int gw_gather_gemm(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx,
                    const void* w_packed, int64_t N, int64_t ldw, const int64_t* idx,
                    int64_t n_alive, const void* bias, int epilogue, void* y, int64_t ldy,
                    int strategy, void* workspace, size_t workspace_bytes, void* stream) {
+  return gw_gather_gemm_residual(x, dtype, M, K, ldx, w_packed, N, ldw, idx, n_alive, bias, epilogue,
+                                 nullptr, 0, y, ldy, strategy, workspace, workspace_bytes, stream);
+}
+
+int gw_gather_gemm_residual(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx,
+                            const void* w_packed, int64_t N, int64_t ldw, const int64_t* idx,
+                            int64_t n_alive, const void* bias, int epilogue, const void* residual,
+                            int64_t ldr, void* y, int64_t ldy, int strategy, void* workspace,
+                            size_t workspace_bytes, void* stream) {
   if (!valid_dtype(dtype)) return GW_ERR_DTYPE;
   if (!valid_epi(epilogue)) return GW_ERR_UNSUPPORTED;
   if (strategy != GW_GEMM_AUTO && strategy != GW_GEMM_FUSED && strategy != GW_GEMM_PREGATHER &&
       strategy != GW_GEMM_OVERLAP && strategy != GW_GEMM_RUNS)
     return GW_ERR_UNSUPPORTED;
   if (!matrix_ok(M, K, ldx) || n_alive < 0 || !matrix_ok(N, n_alive, ldw) ||
-      !matrix_ok(M, N, ldy))
+      !matrix_ok(M, N, ldy) || (residual && !matrix_ok(M, N, ldr)))
     return GW_ERR_SHAPE;
   const gw::DeviceInfo* d = nullptr;
   int st = current_device(&d);
@@ -425,9 +436,10 @@ int gw_gather_gemm(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx,
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (M == 0 || N == 0) return GW_OK;
   if (!y) return GW_ERR_NULL;
+  const gw::Residual res{residual, ldr};
   cudaError_t e;
   if (n_alive == 0) {
-    e = gw::launch_fill_bias(y, dtype, M, N, ldy, bias, epilogue, s);
+    e = gw::launch_fill_bias(y, dtype, M, N, ldy, bias, epilogue, s, res);
     return e == cudaSuccess ? GW_OK : cuda_fail(e);
   }
   if (!x || !w_packed || !idx) return GW_ERR_NULL;
@@ -435,7 +447,7 @@ int gw_gather_gemm(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx,
     e = gw::launch_gemm_f32(static_cast<const float*>(x), M, K, ldx,
                             static_cast<const float*>(w_packed), N, ldw, idx, n_alive,
                             static_cast<const float*>(bias), epilogue, static_cast<float*>(y),
-                            ldy, d->err_word, s);
+                            ldy, d->err_word, s, nullptr, res);
     return e == cudaSuccess ? GW_OK : cuda_fail(e);
   }
   if (!aligned16(w_packed) || (ldw % 8) != 0) return GW_ERR_ALIGN;
@@ -444,7 +456,7 @@ int gw_gather_gemm(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx,
     if ((n_alive % 64) != 0) return GW_ERR_UNSUPPORTED;
     if (!aligned16(x) || (ldx % 8) != 0) return GW_ERR_ALIGN;
     e = launch_dense_gemm(x, dtype, M, n_alive, ldx, w_packed, N, ldw, bias, epilogue, y, ldy, d,
-                          s, nullptr, 0, idx, K);
+                          s, nullptr, 0, idx, K, res);
     return e == cudaSuccess ? GW_OK : cuda_fail(e);
   }
   if ((strategy == GW_GEMM_AUTO || strategy == GW_GEMM_FUSED) && M <= 4 && decode_gemm_enabled()) {
@@ -454,7 +466,7 @@ int gw_gather_gemm(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx,
     const gw::DecodePlan dp = gw::plan_decode(M, N, n_alive, d->sm_count);
     if (dp.split >= 2) {
       e = gw::launch_gemm_decode_gather(dp, x, dtype, M, K, ldx, idx, n_alive, w_packed, N, ldw,
-                                        bias, epilogue, y, ldy, d->err_word, s);
+                                        bias, epilogue, y, ldy, d->err_word, s, res);
       return e == cudaSuccess ? GW_OK : cuda_fail(e);
     }
   }
@@ -464,7 +476,7 @@ int gw_gather_gemm(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx,
   if (strat == GW_GEMM_AUTO) strat = ws_ok ? GW_GEMM_PREGATHER : GW_GEMM_FUSED;
   if (strat == GW_GEMM_FUSED) {
     e = gw::launch_gemm_tc(1, x, dtype, M, K, ldx, w_packed, N, ldw, idx, n_alive, bias,
-                           epilogue, y, ldy, d->err_word, d->sm_count, s);
+                           epilogue, y, ldy, d->err_word, d->sm_count, s, nullptr, nullptr, res);
     return e == cudaSuccess ? GW_OK : cuda_fail(e);
   }
   if (!workspace) return GW_ERR_NULL;
@@ -485,14 +497,15 @@ int gw_gather_gemm(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx,
     g.ldp = ldp;
     g.header = workspace;
     e = gw::launch_gemm_tc2(xg, dtype, M, n_alive, ldp, w_packed, N, ldw, bias, epilogue, y, ldy,
-                            d->err_word, d->sm_count, s, nullptr, 0, nullptr, 0, nullptr, &g);
+                            d->err_word, d->sm_count, s, nullptr, 0, nullptr, 0, nullptr, &g, res);
     return e == cudaSuccess ? GW_OK : cuda_fail(e);
   }
   // Pregather (also the overlap strategy's shapes that do not run on CTA pairs).
   e = gw::launch_gather_columns(x, dtype, M, ldx, K, idx, n_alive, xg, ldp, n_alive,
                                 d->err_word, d->sm_count, s, true);
   if (e != cudaSuccess) return cuda_fail(e);
-  e = launch_dense_gemm(xg, dtype, M, n_alive, ldp, w_packed, N, ldw, bias, epilogue, y, ldy, d, s);
+  e = launch_dense_gemm(xg, dtype, M, n_alive, ldp, w_packed, N, ldw, bias, epilogue, y, ldy, d, s,
+                        nullptr, 0, nullptr, 0, res);
   return e == cudaSuccess ? GW_OK : cuda_fail(e);
 }
 
@@ -501,10 +514,21 @@ int gw_gather_gemm_dev(const void* x, int dtype, int64_t M, int64_t K, int64_t l
                        int64_t n_alive_max, const int32_t* n_alive_dev, const void* bias,
                        int epilogue, void* y, int64_t ldy, void* workspace, size_t workspace_bytes,
                        void* stream) {
+  return gw_gather_gemm_dev_residual(x, dtype, M, K, ldx, w_packed, N, ldw, idx, n_alive_max,
+                                     n_alive_dev, bias, epilogue, nullptr, 0, y, ldy, workspace,
+                                     workspace_bytes, stream);
+}
+
+int gw_gather_gemm_dev_residual(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx,
+                                const void* w_packed, int64_t N, int64_t ldw, const int64_t* idx,
+                                int64_t n_alive_max, const int32_t* n_alive_dev, const void* bias,
+                                int epilogue, const void* residual, int64_t ldr, void* y,
+                                int64_t ldy, void* workspace, size_t workspace_bytes, void* stream) {
   if (!valid_dtype(dtype)) return GW_ERR_DTYPE;
   if (!valid_epi(epilogue)) return GW_ERR_UNSUPPORTED;
   if (!matrix_ok(M, K, ldx) || n_alive_max < 0 || n_alive_max > K ||
-      !matrix_ok(N, n_alive_max, ldw) || !matrix_ok(M, N, ldy))
+      !matrix_ok(N, n_alive_max, ldw) || !matrix_ok(M, N, ldy) ||
+      (residual && !matrix_ok(M, N, ldr)))
     return GW_ERR_SHAPE;
   const gw::DeviceInfo* d = nullptr;
   int st = current_device(&d);
@@ -512,9 +536,10 @@ int gw_gather_gemm_dev(const void* x, int dtype, int64_t M, int64_t K, int64_t l
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (M == 0 || N == 0) return GW_OK;
   if (!y) return GW_ERR_NULL;
+  const gw::Residual res{residual, ldr};
   cudaError_t e;
   if (n_alive_max == 0) {
-    e = gw::launch_fill_bias(y, dtype, M, N, ldy, bias, epilogue, s);
+    e = gw::launch_fill_bias(y, dtype, M, N, ldy, bias, epilogue, s, res);
     return e == cudaSuccess ? GW_OK : cuda_fail(e);
   }
   if (!x || !w_packed || !idx || !n_alive_dev) return GW_ERR_NULL;
@@ -522,7 +547,7 @@ int gw_gather_gemm_dev(const void* x, int dtype, int64_t M, int64_t K, int64_t l
     e = gw::launch_gemm_f32(static_cast<const float*>(x), M, K, ldx,
                             static_cast<const float*>(w_packed), N, ldw, idx, n_alive_max,
                             static_cast<const float*>(bias), epilogue, static_cast<float*>(y),
-                            ldy, d->err_word, s, n_alive_dev);
+                            ldy, d->err_word, s, n_alive_dev, res);
     return e == cudaSuccess ? GW_OK : cuda_fail(e);
   }
   const int64_t ldp = gemm_ld_pad(n_alive_max);
@@ -540,10 +565,10 @@ int gw_gather_gemm_dev(const void* x, int dtype, int64_t M, int64_t K, int64_t l
   // launch does not depend on it, read it (decode and split-K plans do).
   if (gw::use_pair_gemm(M, N, d->sm_count))
     e = gw::launch_gemm_tc2(xg, dtype, M, ldp, ldp, w_packed, N, ldw, bias, epilogue, y, ldy,
-                            d->err_word, d->sm_count, s, nullptr, 0, nullptr, 0, n_alive_dev);
+                            d->err_word, d->sm_count, s, nullptr, 0, nullptr, 0, n_alive_dev, nullptr, res);
   else
     e = gw::launch_gemm_tc(0, xg, dtype, M, ldp, ldp, w_packed, N, ldw, nullptr, ldp, bias,
-                           epilogue, y, ldy, d->err_word, d->sm_count, s, nullptr, n_alive_dev);
+                           epilogue, y, ldy, d->err_word, d->sm_count, s, nullptr, n_alive_dev, res);
   return e == cudaSuccess ? GW_OK : cuda_fail(e);
 }
 
@@ -604,9 +629,20 @@ int gw_dynamic_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ld
                       const void* w, int64_t N, int64_t ldw, double threshold, const void* bias,
                       int epilogue, void* y, int64_t ldy, int32_t* alive_count, int32_t* mask,
                       void* stream) {
+  return gw_dynamic_linear_residual(x, dtype, M, K, ldx, w, N, ldw, threshold, bias, epilogue, nullptr,
+                                    0, y, ldy, alive_count, mask, stream);
+}
+
+int gw_dynamic_linear_residual(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx,
+                               const void* w, int64_t N, int64_t ldw, double threshold,
+                               const void* bias, int epilogue, const void* residual, int64_t ldr,
+                               void* y, int64_t ldy, int32_t* alive_count, int32_t* mask,
+                               void* stream) {
   if (dtype != GW_DTYPE_F16 && dtype != GW_DTYPE_BF16) return GW_ERR_DTYPE;
   if (!valid_epi(epilogue)) return GW_ERR_UNSUPPORTED;
-  if (!matrix_ok(M, K, ldx) || !matrix_ok(N, K, ldw) || !matrix_ok(M, N, ldy)) return GW_ERR_SHAPE;
+  if (!matrix_ok(M, K, ldx) || !matrix_ok(N, K, ldw) || !matrix_ok(M, N, ldy) ||
+      (residual && !matrix_ok(M, N, ldr)))
+    return GW_ERR_SHAPE;
   if (!gw::dyn_linear_supported(M, K) || N > int64_t{65535} * 128) return GW_ERR_UNSUPPORTED;
   if (!aligned16(x) || !aligned16(w) || (ldx % 8) != 0 || (ldw % 8) != 0) return GW_ERR_UNSUPPORTED;
   const gw::DeviceInfo* d = nullptr;
@@ -623,16 +659,25 @@ int gw_dynamic_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ld
   // The reference passes the threshold as an fp32 kernel scalar (mask.py:100).
   cudaError_t e = gw::launch_dyn_linear(x, dtype, M, K, ldx, w, N, ldw, static_cast<float>(threshold),
                                         bias, epilogue, y, ldy, alive_count, mask, d->err_word,
-                                        static_cast<cudaStream_t>(stream));
+                                        static_cast<cudaStream_t>(stream), {residual, ldr});
   return e == cudaSuccess ? GW_OK : cuda_fail(e);
 }
 
 int gw_packed_gemm(const void* a, int dtype, int64_t M, int64_t K, int64_t lda,
                    const void* w_packed, int64_t N, int64_t ldw, const void* bias, int epilogue,
                    void* y, int64_t ldy, void* stream) {
+  return gw_packed_gemm_residual(a, dtype, M, K, lda, w_packed, N, ldw, bias, epilogue, nullptr, 0, y,
+                                 ldy, stream);
+}
+
+int gw_packed_gemm_residual(const void* a, int dtype, int64_t M, int64_t K, int64_t lda,
+                            const void* w_packed, int64_t N, int64_t ldw, const void* bias,
+                            int epilogue, const void* residual, int64_t ldr, void* y, int64_t ldy,
+                            void* stream) {
   if (dtype != GW_DTYPE_F16 && dtype != GW_DTYPE_BF16) return GW_ERR_DTYPE;
   if (!valid_epi(epilogue)) return GW_ERR_UNSUPPORTED;
-  if (!matrix_ok(M, K, lda) || !matrix_ok(N, K, ldw) || !matrix_ok(M, N, ldy))
+  if (!matrix_ok(M, K, lda) || !matrix_ok(N, K, ldw) || !matrix_ok(M, N, ldy) ||
+      (residual && !matrix_ok(M, N, ldr)))
     return GW_ERR_SHAPE;
   const gw::DeviceInfo* d = nullptr;
   int st = current_device(&d);
@@ -640,15 +685,17 @@ int gw_packed_gemm(const void* a, int dtype, int64_t M, int64_t K, int64_t lda,
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (M == 0 || N == 0) return GW_OK;
   if (!y) return GW_ERR_NULL;
+  const gw::Residual res{residual, ldr};
   cudaError_t e;
   if (K == 0) {
-    e = gw::launch_fill_bias(y, dtype, M, N, ldy, bias, epilogue, s);
+    e = gw::launch_fill_bias(y, dtype, M, N, ldy, bias, epilogue, s, res);
     return e == cudaSuccess ? GW_OK : cuda_fail(e);
   }
   if (!a || !w_packed) return GW_ERR_NULL;
   if (!aligned16(a) || !aligned16(w_packed) || (lda % 8) != 0 || (ldw % 8) != 0)
     return GW_ERR_ALIGN;
-  e = launch_dense_gemm(a, dtype, M, K, lda, w_packed, N, ldw, bias, epilogue, y, ldy, d, s);
+  e = launch_dense_gemm(a, dtype, M, K, lda, w_packed, N, ldw, bias, epilogue, y, ldy, d, s, nullptr, 0,
+                        nullptr, 0, res);
   return e == cudaSuccess ? GW_OK : cuda_fail(e);
 }
 

@@ -599,6 +599,53 @@ __device__ __forceinline__ void add_bias4(float (&f)[4], const uint16_t* bias, i
       if (n0 + j < N) f[j] += Elem<DT>::to_f(__ldg(bias + n0 + j));
   }
 }
+// Residual added in GEMM epilogues, after the activation and before the one
+// rounding: 32 (or 4) consecutive columns [n0, n0 + 32) of one row, as pairs
+// of 16-bit values, zeros at and past column N. Plain loads, not the
+// read-only path: the residual may be the output itself (each element is read
+// before the same thread or warp stores it).
+__device__ __forceinline__ void load_residual32(uint32_t (&v)[16], const uint16_t* row, int64_t n0,
+                                                int64_t N) {
+  const uint16_t* b = row + n0;
+  if (n0 + 32 <= N && (reinterpret_cast<uintptr_t>(b) & 15u) == 0) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint4 u = reinterpret_cast<const uint4*>(b)[q];
+      v[4 * q] = u.x; v[4 * q + 1] = u.y; v[4 * q + 2] = u.z; v[4 * q + 3] = u.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const uint32_t lo = n0 + 2 * j < N ? b[2 * j] : 0u;
+      const uint32_t hi = n0 + 2 * j + 1 < N ? b[2 * j + 1] : 0u;
+      v[j] = lo | (hi << 16);
+    }
+  }
+}
+template <int DT>
+__device__ __forceinline__ void add_residual32(float (&f)[32], const uint32_t (&v)[16]) {
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    f[2 * j] += Elem<DT>::to_f(static_cast<uint16_t>(v[j] & 0xFFFFu));
+    f[2 * j + 1] += Elem<DT>::to_f(static_cast<uint16_t>(v[j] >> 16));
+  }
+}
+__device__ __forceinline__ uint2 load_residual4(const uint16_t* row, int64_t n0, int64_t N) {
+  const uint16_t* b = row + n0;
+  if (n0 + 4 <= N && (reinterpret_cast<uintptr_t>(b) & 7u) == 0)
+    return *reinterpret_cast<const uint2*>(b);
+  uint32_t e[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) e[j] = n0 + j < N ? b[j] : 0u;
+  return make_uint2(e[0] | (e[1] << 16), e[2] | (e[3] << 16));
+}
+template <int DT>
+__device__ __forceinline__ void add_residual4(float (&f)[4], const uint2 v) {
+  f[0] += Elem<DT>::to_f(static_cast<uint16_t>(v.x & 0xFFFFu));
+  f[1] += Elem<DT>::to_f(static_cast<uint16_t>(v.x >> 16));
+  f[2] += Elem<DT>::to_f(static_cast<uint16_t>(v.y & 0xFFFFu));
+  f[3] += Elem<DT>::to_f(static_cast<uint16_t>(v.y >> 16));
+}
 // Activation chosen at compile time, so a kernel instantiation carries the
 // code of one activation only.
 template <int EPI>

@@ -190,15 +190,16 @@ gather_rows_t_kernel(const raw* __restrict__ src, int64_t rows_src, int64_t cols
 }
 
 template <int DT>
-__global__ void fill_bias_kernel(typename Elem<DT>::raw* __restrict__ y, int64_t M, int64_t N,
+__global__ void fill_bias_kernel(typename Elem<DT>::raw* y, int64_t M, int64_t N,
                                  int64_t ldy, const typename Elem<DT>::raw* __restrict__ bias,
-                                 int epi) {
+                                 int epi, const typename Elem<DT>::raw* res, int64_t ldr) {
   const int64_t total = M * N;
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; t < total;
        t += static_cast<int64_t>(gridDim.x) * blockDim.x) {
     const int64_t m = t / N, n = t - m * N;
     float v = bias ? Elem<DT>::to_f(bias[n]) : 0.0f;
     v = apply_epilogue(v, epi);
+    if (res) v += Elem<DT>::to_f(res[m * ldr + n]);
     y[m * ldy + n] = Elem<DT>::from_f(v);
   }
 }
@@ -363,21 +364,25 @@ cudaError_t launch_gather_rows_t(const void* src, int dtype, int64_t rows_src, i
 }
 
 cudaError_t launch_fill_bias(void* y, int dtype, int64_t M, int64_t N, int64_t ldy,
-                             const void* bias, int epilogue, cudaStream_t stream) {
+                             const void* bias, int epilogue, cudaStream_t stream,
+                             const Residual& res) {
   if (M == 0 || N == 0) return cudaSuccess;
   const unsigned grid = clamp_grid((M * N + 255) / 256, 148 * 32);
   switch (dtype) {
     case GW_DTYPE_F16:
       fill_bias_kernel<GW_DTYPE_F16><<<grid, 256, 0, stream>>>(
-          static_cast<uint16_t*>(y), M, N, ldy, static_cast<const uint16_t*>(bias), epilogue);
+          static_cast<uint16_t*>(y), M, N, ldy, static_cast<const uint16_t*>(bias), epilogue,
+          static_cast<const uint16_t*>(res.p), res.ld);
       break;
     case GW_DTYPE_BF16:
       fill_bias_kernel<GW_DTYPE_BF16><<<grid, 256, 0, stream>>>(
-          static_cast<uint16_t*>(y), M, N, ldy, static_cast<const uint16_t*>(bias), epilogue);
+          static_cast<uint16_t*>(y), M, N, ldy, static_cast<const uint16_t*>(bias), epilogue,
+          static_cast<const uint16_t*>(res.p), res.ld);
       break;
     default:
       fill_bias_kernel<GW_DTYPE_F32><<<grid, 256, 0, stream>>>(
-          static_cast<uint32_t*>(y), M, N, ldy, static_cast<const uint32_t*>(bias), epilogue);
+          static_cast<uint32_t*>(y), M, N, ldy, static_cast<const uint32_t*>(bias), epilogue,
+          static_cast<const uint32_t*>(res.p), res.ld);
       break;
   }
   return cudaGetLastError();

@@ -83,6 +83,8 @@ struct DcParams {
   uint16_t* y;
   int64_t ldy;
   int y_vec_ok;              // 8-byte stores of four outputs allowed
+  const uint16_t* res;       // residual (or null), leading dimension ldr
+  int64_t ldr;
   int num_kb;
   int split;                 // cluster size S
   int x_tx_bytes;            // bytes of one box of a (its rows: M rounded up to 8)
@@ -173,6 +175,8 @@ __device__ __forceinline__ void dc_finish(const DcParams& p, const float* recv, 
 #pragma unroll
       for (int j = 0; j < 4; ++j) f[j] = apply_epilogue16(f[j], p.epi);
     }
+    if (p.res)
+      add_residual4<DT>(f, load_residual4(p.res + static_cast<int64_t>(m) * p.ldr, n0, p.N));
     uint16_t* yp = p.y + static_cast<int64_t>(m) * p.ldy + n0;
     if (p.y_vec_ok && n0 + 4 <= p.N) {
       *reinterpret_cast<uint2*>(yp) = make_uint2(Elem<DT>::pack2(f[0], f[1]), Elem<DT>::pack2(f[2], f[3]));
@@ -415,6 +419,8 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap tmap_w,
                        mapa_shared(recv_bar, owner));
   }
 
+  // The residual may come from the previous kernel of the stream.
+  if (p.res) asm volatile("griddepcontrol.wait;" ::: "memory");
   // Every slot of this CTA's slice has landed: its own and the S - 1 peers'.
   const bool got = mbar_wait_cluster(recv_bar, 0u, nullptr, p.err);
   // Tell every sender that its copy into this CTA has landed.
@@ -606,7 +612,7 @@ cudaError_t launch_gemm_decode_gather(const DecodePlan& plan, const void* x, int
                                       int64_t K, int64_t ldx, const int64_t* idx, int64_t n_alive,
                                       const void* w, int64_t N, int64_t ldw, const void* bias,
                                       int epilogue, void* y, int64_t ldy, unsigned int* err,
-                                      cudaStream_t stream) {
+                                      cudaStream_t stream, const Residual& res) {
   if (plan.split < 2 || plan.split > 16 || plan.blocks <= 0 || plan.blocks > 65535 ||
       M <= 0 || M > plan.mp || n_alive <= 0)
     return cudaErrorInvalidValue;
@@ -617,6 +623,8 @@ cudaError_t launch_gemm_decode_gather(const DecodePlan& plan, const void* x, int
   p.x_cols = K;
   p.gidx = idx;
   p.n_alive = n_alive;
+  p.res = static_cast<const uint16_t*>(res.p);
+  p.ldr = res.ld;
   return launch_decode_params(plan, p, dtype, nullptr, 0, w, ldw, n_alive, stream);
 }
 
@@ -624,7 +632,7 @@ cudaError_t launch_gemm_decode(const DecodePlan& plan, const void* a, int dtype,
                                int64_t K, int64_t lda, const void* w, int64_t N, int64_t ldw,
                                const void* bias, int epilogue, void* y, int64_t ldy,
                                unsigned int* err, cudaStream_t stream, const int64_t* a_cols,
-                               int64_t a_width) {
+                               int64_t a_width, const Residual& res) {
   if (plan.split < 2 || plan.split > 16 || plan.blocks <= 0 || plan.blocks > 65535 ||
       M <= 0 || M > plan.mp)
     return cudaErrorInvalidValue;
@@ -633,6 +641,8 @@ cudaError_t launch_gemm_decode(const DecodePlan& plan, const void* a, int dtype,
   if (a_cols && (K % kDcK) != 0) return cudaErrorInvalidValue;
   p.a_cols = a_cols;
   p.a_width = a_width;
+  p.res = static_cast<const uint16_t*>(res.p);
+  p.ldr = res.ld;
   return launch_decode_params(plan, p, dtype, a, lda, w, ldw, K, stream);
 }
 

@@ -86,6 +86,8 @@ struct DyParams {
   float thr;
   const uint16_t* bias;
   int epi;
+  const uint16_t* res;       // residual (or null), leading dimension ldr
+  int64_t ldr;
   uint16_t* y;
   int64_t ldy;
   int y_vec_ok;
@@ -419,6 +421,7 @@ __global__ void __launch_bounds__(kDyThreads, 1) gemm_dyn_kernel(const DyParams 
           if (q < S) s += part_q[u][q];
         if (p.bias) s += Elem<DT>::to_f(__ldg(p.bias + n));
         s = apply_epilogue16(s, p.epi);
+        if (p.res) s += Elem<DT>::to_f(p.res[static_cast<int64_t>(m) * p.ldr + n]);
         p.y[static_cast<int64_t>(m) * p.ldy + n] = Elem<DT>::from_f(s);
       }
     }
@@ -475,7 +478,7 @@ bool dyn_linear_supported(int64_t M, int64_t K) {
 cudaError_t launch_dyn_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx,
                               const void* w, int64_t N, int64_t ldw, float thr, const void* bias,
                               int epilogue, void* y, int64_t ldy, int32_t* count, int32_t* mask,
-                              unsigned int* err, cudaStream_t stream) {
+                              unsigned int* err, cudaStream_t stream, const Residual& res) {
   if (!dyn_linear_supported(M, K) || N <= 0) return cudaErrorInvalidValue;
   const int64_t blocks = (N + kDyN - 1) / kDyN;
   if (blocks > 65535) return cudaErrorInvalidValue;
@@ -490,6 +493,8 @@ cudaError_t launch_dyn_linear(const void* x, int dtype, int64_t M, int64_t K, in
   p.thr = thr;
   p.bias = static_cast<const uint16_t*>(bias);
   p.epi = epilogue;
+  p.res = static_cast<const uint16_t*>(res.p);
+  p.ldr = res.ld;
   p.y = static_cast<uint16_t*>(y);
   p.ldy = ldy;
   p.split = static_cast<int>((K + kDyKS - 1) / kDyKS);

@@ -77,6 +77,8 @@ struct SkParams {
   uint16_t* y;
   int64_t ldy;
   int y_vec_ok;              // 8-byte stores of four outputs allowed
+  const uint16_t* res;       // residual (or null), leading dimension ldr
+  int64_t ldr;
   int num_kb;
   int m_tiles;
   int split;                 // cluster size S
@@ -120,10 +122,19 @@ __device__ __forceinline__ void reduce_slice(const SkParams& p, uint32_t red_loc
   const bool vec = p.y_vec_ok && n0 + 4 <= p.N;
   const int64_t y_step = static_cast<int64_t>(kStep) * p.ldy;
   uint16_t* yp = p.y + (static_cast<int64_t>(m_blk) * kSkBM + row0) * p.ldy + n0;
+  const uint16_t* rp = p.res ? p.res + (static_cast<int64_t>(m_blk) * kSkBM + row0) * p.ldr : nullptr;
+  const int64_t r_step = static_cast<int64_t>(kStep) * p.ldr;
   const uint32_t col_addr = red_local + static_cast<uint32_t>(col * 4);
   float sink = 0.f;
   for (int r = row0; r < rows_valid; r += kRows * kStep, yp += kRows * y_step) {
     float4 v[kRows][S];
+    uint2 rv[kRows];
+    if (rp) {
+#pragma unroll
+      for (int u = 0; u < kRows; ++u)
+        if (r + u * kStep < rows_valid) rv[u] = load_residual4(rp + u * r_step, n0, p.N);
+      rp += kRows * r_step;
+    }
 #pragma unroll
     for (int u = 0; u < kRows; ++u) {
       if (r + u * kStep < rows_valid) {
@@ -159,6 +170,7 @@ __device__ __forceinline__ void reduce_slice(const SkParams& p, uint32_t red_loc
         for (int j = 0; j < 4; ++j) f[j] += b[j];
       }
       activate4<EPI>(f);
+      if (p.res) add_residual4<DT>(f, rv[u]);
       uint16_t* yr = yp + u * y_step;
       if (vec) {
         const uint32_t lo = static_cast<uint32_t>(Elem<DT>::from_f(f[0])) |
@@ -353,6 +365,8 @@ gemm_splitk_kernel(const __grid_constant__ CUtensorMap tmap_b,
   cluster_sync();                      // every partial tile of the cluster is in shared memory
 
   // ------------------------------------------------------------ reduce-scatter over DSMEM
+  // The residual may come from the previous kernel of the stream.
+  if (p.res) asm volatile("griddepcontrol.wait;" ::: "memory");
   {
     const bool ok = *acc_ok != 0;
     if (p.split == 8) reduce_slice<8, BN, DT, EPI>(p, smem_u32(smem), rank, m_blk, n_blk, rows_valid, ok);
@@ -530,7 +544,7 @@ cudaError_t launch_gemm_splitk(const SplitKPlan& plan, const void* a, int dtype,
                                int64_t K, int64_t lda, const void* w, int64_t N, int64_t ldw,
                                const void* bias, int epilogue, void* y, int64_t ldy,
                                unsigned int* err, cudaStream_t stream, const int64_t* a_cols,
-                               int64_t a_width) {
+                               int64_t a_width, const Residual& res) {
   if (plan.split < 2 || plan.split > 8 || plan.tiles <= 0 || plan.tiles > 65535)
     return cudaErrorInvalidValue;
   SkParams p{};
@@ -547,6 +561,8 @@ cudaError_t launch_gemm_splitk(const SplitKPlan& plan, const void* a, int dtype,
   p.err = err;
   p.a_cols = a_cols;
   p.a_width = a_width;
+  p.res = static_cast<const uint16_t*>(res.p);
+  p.ldr = res.ld;
   if (p.num_kb < plan.split) return cudaErrorInvalidValue;
   if (a_cols && (K % kSkBK) != 0) return cudaErrorInvalidValue;
   // With fewer than 128 rows the x' box covers only the rows that exist; the

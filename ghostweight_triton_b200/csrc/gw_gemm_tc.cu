@@ -93,6 +93,8 @@ struct TcParams {
   int num_tiles;
   unsigned int* err;
   const int64_t* a_cols;        // kATma: k-block kb of A starts at x column a_cols[64 kb] (or null)
+  const uint16_t* res;          // residual (or null), leading dimension ldr
+  int64_t ldr;
   const int32_t* k_dev;         // kATma: K' on the device (num_kb an upper bound; see device_num_kb)
 };
 
@@ -300,6 +302,8 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmap_b,
     const int q = warp & 3;                       // TMEM lane quarter this warp may access
     const int part = (warp - (AMODE == kATma ? kWarpEpi0Dense : kWarpEpi0)) >> 2;
     const int row_in_tile = q * 32 + lane;
+    // The residual may come from the previous kernel of the stream.
+    if (p.res) asm volatile("griddepcontrol.wait;" ::: "memory");
     uint32_t lt = 0;
     for (int tile = blockIdx.x; tile < p.num_tiles; tile += gridDim.x, ++lt) {
       const int m_blk = tile % p.m_tiles;
@@ -326,6 +330,11 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmap_b,
         if (p.bias) add_bias32<DT>(f, p.bias, n_base, p.N);
         activate32<EPI>(f);
         if (row_ok) {
+          if (p.res) {
+            uint32_t rv[16];
+            load_residual32(rv, p.res + row * p.ldr, n_base, p.N);
+            add_residual32<DT>(f, rv);
+          }
           if (p.y_vec_ok && n_base + 32 <= p.N) {
             uint32_t packed[16];
 #pragma unroll
@@ -396,7 +405,8 @@ cudaError_t launch_gemm_tc(int a_mode, const void* x, int dtype, int64_t M, int6
                            int64_t ldx, const void* w, int64_t N, int64_t ldw,
                            const int64_t* idx, int64_t n_alive, const void* bias, int epilogue,
                            void* y, int64_t ldy, unsigned int* err, int sm_count,
-                           cudaStream_t stream, const int64_t* a_cols, const int32_t* k_dev) {
+                           cudaStream_t stream, const int64_t* a_cols, const int32_t* k_dev,
+                           const Residual& res) {
   // Tile width 256 (measured best on B200 where there are several waves:
   // wider tiles reuse A more per byte moved), 128 for narrow N. When 256-wide
   // tiles leave SMs idle in a single wave and 192-wide ones still fit in one
@@ -441,6 +451,8 @@ cudaError_t launch_gemm_tc(int a_mode, const void* x, int dtype, int64_t M, int6
   p.err = err;
   p.a_cols = a_mode == kATma ? a_cols : nullptr;
   p.k_dev = a_mode == kATma ? k_dev : nullptr;
+  p.res = static_cast<const uint16_t*>(res.p);
+  p.ldr = res.ld;
   if (p.a_cols && (n_alive % kBK) != 0) return cudaErrorInvalidValue;
 
   CUtensorMap tb, ta;

@@ -100,6 +100,8 @@ struct Tc2Params {
   int y_tma;                 // y stored through tmap_y (16-byte aligned rows)
   uint16_t* y;
   int64_t ldy;
+  const uint16_t* res;      // residual (or null), leading dimension ldr
+  int64_t ldr;
   int num_kb;               // 64-wide k atoms of K
   int num_ks;               // stages of kStageK2 per tile
   int m_tiles;
@@ -582,6 +584,8 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
       call = *reinterpret_cast<volatile unsigned long long*>(p.ghdr) + 1;
       gather_units<DT>(p, warp - 2, lane, claim_slot, call);
     }
+    // The residual may come from the previous kernel of the stream.
+    if (p.res) asm volatile("griddepcontrol.wait;" ::: "memory");
     uint32_t lt = 0;
     for (int job = pair; job < p.num_jobs; job += num_pairs, ++lt) {
       int m_blk, n_blk, sub;
@@ -620,6 +624,11 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
         }
         if (p.bias) add_bias32<DT>(f, p.bias, n_base, p.N);
         activate32<EPI>(f);
+        if (p.res && row_ok) {
+          uint32_t rv[16];
+          load_residual32(rv, p.res + row * p.ldr, n_base, p.N);
+          add_residual32<DT>(f, rv);
+        }
         uint32_t packed[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) packed[j] = Elem<DT>::pack2(f[2 * j], f[2 * j + 1]);
@@ -857,7 +866,7 @@ cudaError_t launch_gemm_tc2(const void* a, int dtype, int64_t M, int64_t K, int6
                             void* y, int64_t ldy, unsigned int* err, int sm_count,
                             cudaStream_t stream, void* const* peers, int n_peers,
                             const int64_t* a_cols, int64_t a_width, const int32_t* k_dev,
-                            const Tc2Gather* gather) {
+                            const Tc2Gather* gather, const Residual& res) {
   Tc2Params p{};
   p.M = M;
   p.N = N;
@@ -875,6 +884,8 @@ cudaError_t launch_gemm_tc2(const void* a, int dtype, int64_t M, int64_t K, int6
   p.a_cols = a_cols;
   p.a_width = a_width;
   p.k_dev = k_dev;
+  p.res = static_cast<const uint16_t*>(res.p);
+  p.ldr = res.ld;
   if (gather) {
     if (a_cols || k_dev || !gather->x || !gather->idx || !gather->xg || !gather->header ||
         (gather->ldp % 8) != 0 || gather->ldp < K)

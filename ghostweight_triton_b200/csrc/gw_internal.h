@@ -25,6 +25,13 @@ int current_device(const DeviceInfo** out, int* device = nullptr);
 // pending error and returns GW_ERR_CUDA.
 int cuda_fail(cudaError_t e);
 
+// The residual of a GEMM epilogue: y = act(...) + residual, [M, N] of y's type
+// (leading dimension ld); p null: none. It may be y itself (same ld).
+struct Residual {
+  const void* p = nullptr;
+  int64_t ld = 0;
+};
+
 // gw_mask.cu
 size_t mask_workspace_bytes(int64_t cols);
 cudaError_t launch_mask_compact(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld,
@@ -52,7 +59,8 @@ cudaError_t launch_gather_rows_t(const void* src, int dtype, int64_t rows_src, i
                                  int64_t ld_dst, int64_t pad_to, unsigned int* err,
                                  cudaStream_t stream, const int32_t* n_dev = nullptr);
 cudaError_t launch_fill_bias(void* y, int dtype, int64_t M, int64_t N, int64_t ldy,
-                             const void* bias, int epilogue, cudaStream_t stream);
+                             const void* bias, int epilogue, cudaStream_t stream,
+                             const Residual& res = {});
 // Copies y [rows, cols] (leading dimension ld, 16-bit, 16-byte aligned rows)
 // into each peer buffer at the same offsets.
 cudaError_t launch_copy_to_peers(const void* y, int64_t rows, int64_t cols, int64_t ld,
@@ -99,7 +107,7 @@ cudaError_t launch_gemm_tc(int a_mode, const void* x, int dtype, int64_t M, int6
                            const int64_t* idx, int64_t n_alive, const void* bias, int epilogue,
                            void* y, int64_t ldy, unsigned int* err, int sm_count,
                            cudaStream_t stream, const int64_t* a_cols = nullptr,
-                           const int32_t* k_dev = nullptr);
+                           const int32_t* k_dev = nullptr, const Residual& res = {});
 
 // gw_gemm_tc2.cu: CTA-pair (cta_group::2) tcgen05 GEMM, dense A [M, K] by TMA,
 // 256 x 256 tiles per pair. Chained to the previous kernel by programmatic
@@ -136,7 +144,8 @@ cudaError_t launch_gemm_tc2(const void* a, int dtype, int64_t M, int64_t K, int6
                             void* y, int64_t ldy, unsigned int* err, int sm_count,
                             cudaStream_t stream, void* const* peers = nullptr, int n_peers = 0,
                             const int64_t* a_cols = nullptr, int64_t a_width = 0,
-                            const int32_t* k_dev = nullptr, const Tc2Gather* gather = nullptr);
+                            const int32_t* k_dev = nullptr, const Tc2Gather* gather = nullptr,
+                            const Residual& res = {});
 // Whether the CTA-pair kernel serves a dense-A GEMM of this shape.
 bool use_pair_gemm(int64_t M, int64_t N, int sm_count);
 // Tile width (192 or 256) the pair kernel uses for an M x N output.
@@ -148,7 +157,7 @@ cudaError_t launch_gemm_f32(const float* x, int64_t M, int64_t K, int64_t ldx, c
                             int64_t N, int64_t ldw, const int64_t* idx, int64_t n_alive,
                             const float* bias, int epilogue, float* y, int64_t ldy,
                             unsigned int* err, cudaStream_t stream,
-                            const int32_t* n_dev = nullptr);
+                            const int32_t* n_dev = nullptr, const Residual& res = {});
 
 // gw_gemm_splitk.cu: split-K over a cluster of `split` CTAs reduced in DSMEM,
 // for dense-A GEMMs whose output has too few tiles to occupy the SMs.
@@ -163,7 +172,8 @@ cudaError_t launch_gemm_splitk(const SplitKPlan& plan, const void* a, int dtype,
                                int64_t K, int64_t lda, const void* w, int64_t N, int64_t ldw,
                                const void* bias, int epilogue, void* y, int64_t ldy,
                                unsigned int* err, cudaStream_t stream,
-                               const int64_t* a_cols = nullptr, int64_t a_width = 0);
+                               const int64_t* a_cols = nullptr, int64_t a_width = 0,
+                               const Residual& res = {});
 
 // gw_gemm_decode.cu: at most 32 rows of A; the MMA runs over 128-feature
 // blocks of W' (M = 128) and all rows of A padded to mp (N = 16 or 32),
@@ -178,14 +188,15 @@ cudaError_t launch_gemm_decode(const DecodePlan& plan, const void* a, int dtype,
                                int64_t K, int64_t lda, const void* w, int64_t N, int64_t ldw,
                                const void* bias, int epilogue, void* y, int64_t ldy,
                                unsigned int* err, cudaStream_t stream,
-                               const int64_t* a_cols = nullptr, int64_t a_width = 0);
+                               const int64_t* a_cols = nullptr, int64_t a_width = 0,
+                               const Residual& res = {});
 // Same, with A = x[:, idx] gathered inside the kernel (x [M, K], leading
 // dimension ldx; no alignment requirement on x): one launch, no x' in memory.
 cudaError_t launch_gemm_decode_gather(const DecodePlan& plan, const void* x, int dtype, int64_t M,
                                       int64_t K, int64_t ldx, const int64_t* idx, int64_t n_alive,
                                       const void* w, int64_t N, int64_t ldw, const void* bias,
                                       int epilogue, void* y, int64_t ldy, unsigned int* err,
-                                      cudaStream_t stream);
+                                      cudaStream_t stream, const Residual& res = {});
 
 // gw_gemm_dyn.cu: the per-forward activation mask, its compaction and the
 // gather-GEMM in one clustered launch, for at most 32 rows (fp16/bf16; x and
@@ -195,7 +206,7 @@ bool dyn_linear_supported(int64_t M, int64_t K);
 cudaError_t launch_dyn_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx,
                               const void* w, int64_t N, int64_t ldw, float thr, const void* bias,
                               int epilogue, void* y, int64_t ldy, int32_t* count, int32_t* mask,
-                              unsigned int* err, cudaStream_t stream);
+                              unsigned int* err, cudaStream_t stream, const Residual& res = {});
 
 // Driver entry point for cuTensorMapEncodeTiled (resolved once, no libcuda link).
 void* tensor_map_encoder();

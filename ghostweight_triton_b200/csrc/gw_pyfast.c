@@ -148,6 +148,41 @@ static PyObject* fast_dynamic_linear(PyObject* self, PyObject* const* args, Py_s
                                            (int32_t*)a[13].p, (int32_t*)a[14].p, a[15].p));
 }
 
+static PyObject* fast_gather_gemm_residual(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  GW_PARSE("pilllpllplpiplplipzp")
+  return PyLong_FromLong(gw_gather_gemm_residual(
+      a[0].p, a[1].i, a[2].l, a[3].l, a[4].l, a[5].p, a[6].l, a[7].l, (const int64_t*)a[8].p, a[9].l,
+      a[10].p, a[11].i, a[12].p, a[13].l, a[14].p, a[15].l, a[16].i, a[17].p, a[18].z, a[19].p));
+}
+
+static PyObject* fast_gather_gemm_dev_residual(PyObject* self, PyObject* const* args,
+                                               Py_ssize_t nargs) {
+  (void)self;
+  GW_PARSE("pilllpllplppiplplpzp")
+  return PyLong_FromLong(gw_gather_gemm_dev_residual(
+      a[0].p, a[1].i, a[2].l, a[3].l, a[4].l, a[5].p, a[6].l, a[7].l, (const int64_t*)a[8].p, a[9].l,
+      (const int32_t*)a[10].p, a[11].p, a[12].i, a[13].p, a[14].l, a[15].p, a[16].l, a[17].p, a[18].z,
+      a[19].p));
+}
+
+static PyObject* fast_packed_gemm_residual(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  GW_PARSE("pilllpllpiplplp")
+  return PyLong_FromLong(gw_packed_gemm_residual(a[0].p, a[1].i, a[2].l, a[3].l, a[4].l, a[5].p,
+                                                 a[6].l, a[7].l, a[8].p, a[9].i, a[10].p, a[11].l,
+                                                 a[12].p, a[13].l, a[14].p));
+}
+
+static PyObject* fast_dynamic_linear_residual(PyObject* self, PyObject* const* args,
+                                              Py_ssize_t nargs) {
+  (void)self;
+  GW_PARSE("pilllplldpiplplppp")
+  return PyLong_FromLong(gw_dynamic_linear_residual(
+      a[0].p, a[1].i, a[2].l, a[3].l, a[4].l, a[5].p, a[6].l, a[7].l, a[8].d, a[9].p, a[10].i,
+      a[11].p, a[12].l, a[13].p, a[14].l, (int32_t*)a[15].p, (int32_t*)a[16].p, a[17].p));
+}
+
 static PyObject* fast_rms_norm(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   (void)self;
   GW_PARSE("pilllplplpdplpllp")
@@ -203,6 +238,10 @@ static PyMethodDef gw_fast_methods[] = {
     GW_FAST(gather_rows_t_dev),
     GW_FAST(mask_compact),
     GW_FAST(dynamic_linear),
+    GW_FAST(gather_gemm_residual),
+    GW_FAST(gather_gemm_dev_residual),
+    GW_FAST(packed_gemm_residual),
+    GW_FAST(dynamic_linear_residual),
     GW_FAST(rms_norm),
     GW_FAST(rms_norm_q8),
     GW_FAST(quantize_rows),

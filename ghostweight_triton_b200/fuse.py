@@ -97,7 +97,9 @@ class GhostMLPChain(nn.Module):
         self._plan = (key, w_fc, b_fc, w_proj)
         return w_fc, b_fc, w_proj
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+        """The chain over x [..., in_features]; residual (the output's shape) is added in
+        proj's epilogue (behind the dropout, where a training-mode one is active)."""
         lead = x.shape[:-1]
         x2 = x.reshape(-1, self.fc.in_features)
         w_fc, b_fc, w_proj = self._operands(x2.dtype)
@@ -105,9 +107,17 @@ class GhostMLPChain(nn.Module):
         bias = self.proj.bias
         if bias is not None and bias.dtype != x2.dtype:
             bias = bias.to(x2.dtype)
-        y = packed_linear(h, w_proj, bias=bias)
-        if self.dropout is not None:
+        if residual is not None:
+            assert residual.shape == (*lead, self.proj.out_features), (
+                f"residual must have shape {(*lead, self.proj.out_features)}, got {tuple(residual.shape)}")
+        identity = self.dropout is None or (isinstance(self.dropout, nn.Dropout) and not self.dropout.training)
+        behind = residual is not None and not identity
+        fused = None if residual is None or behind else residual.reshape(-1, self.proj.out_features)
+        y = packed_linear(h, w_proj, bias=bias, residual=fused)
+        if self.dropout is not None and fused is None:
             y = self.dropout(y)
+        if behind:
+            y = y + residual.reshape(-1, self.proj.out_features)
         return y.reshape(*lead, self.proj.out_features)
 
 

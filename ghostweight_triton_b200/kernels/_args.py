@@ -1,0 +1,63 @@
+"""Argument checks shared by the operator wrappers (host side, no kernel)."""
+
+from __future__ import annotations
+
+import torch
+
+
+def refuse_grad(**tensors: torch.Tensor | None) -> None:
+    """Raise if a tensor would need a gradient that the operator cannot give."""
+    if torch.is_grad_enabled():
+        for name, t in tensors.items():
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{name} requires a gradient, and this operator has no backward pass: "
+                                   "call it under torch.no_grad() or on detached tensors")
+
+
+def rows(t: torch.Tensor, cols: int) -> torch.Tensor:
+    """t as a row-major [rows, cols] matrix (copied only when its strides are not such)."""
+    t = t.reshape(-1, cols)
+    if (t.stride(1) != 1 and cols > 1) or (t.shape[0] > 1 and t.stride(0) < cols):
+        t = t.contiguous()
+    return t
+
+
+def _span(m: torch.Tensor) -> tuple[int, int]:
+    return m.data_ptr(), m.data_ptr() + ((m.shape[0] - 1) * m.stride(0) + m.shape[1]) * m.element_size()
+
+
+def in_place_or_apart(what: str, out: torch.Tensor, *inputs: torch.Tensor | None) -> None:
+    """Assert that the matrix `out` takes the very place of an input matrix or none of its
+    memory (each element is read before it is written only if both have the same rows)."""
+    for t in inputs:
+        if t is None or not t.numel() or not out.numel():
+            continue
+        if (t.data_ptr() == out.data_ptr() and t.shape == out.shape
+                and (t.shape[0] <= 1 or t.stride(0) == out.stride(0))):
+            continue
+        (a0, a1), (b0, b1) = _span(t), _span(out)
+        assert a1 <= b0 or b1 <= a0, f"{what} overlaps an input without being the same rows"
+
+
+def out_matrix(what: str, out: torch.Tensor, like: torch.Tensor, *inputs: torch.Tensor | None) -> torch.Tensor:
+    """`out` as a matrix that results of `like`'s shape and type can be written to: rows that
+    do not overlap one another, and in_place_or_apart with the input matrices."""
+    assert out.shape == like.shape and out.dtype is like.dtype and out.device == like.device, (
+        f"{what} must have shape {tuple(like.shape)}, dtype {like.dtype} and be on {like.device}")
+    cols = like.shape[-1]
+    m = out.view(-1, cols) if out.is_contiguous() and cols else out
+    assert m.ndim == 2 and (m.stride(1) == 1 or cols <= 1) and (m.shape[0] <= 1 or m.stride(0) >= cols), (
+        f"{what} must be a row-major matrix (or contiguous)")
+    in_place_or_apart(what, m, *inputs)
+    return m
+
+
+def residual_matrix(residual: torch.Tensor, shape: tuple[int, int], like: torch.Tensor) -> torch.Tensor:
+    """The residual [M, N] of a product as a row-major matrix."""
+    assert residual.dtype is like.dtype and residual.device == like.device, (
+        f"residual must be {like.dtype} on {like.device}, got {residual.dtype} on {residual.device}")
+    assert tuple(residual.shape) == tuple(shape), f"residual must have shape {tuple(shape)}, got {tuple(residual.shape)}"
+    refuse_grad(residual=residual)
+    if (residual.stride(1) != 1 and shape[1] > 1) or (shape[0] > 1 and residual.stride(0) < shape[1]):
+        residual = residual.contiguous()
+    return residual

@@ -21,6 +21,7 @@ from __future__ import annotations
 import torch
 
 from ghostweight_triton_b200 import _native
+from ghostweight_triton_b200.kernels._args import in_place_or_apart, residual_matrix
 from ghostweight_triton_b200.kernels.gather import pack_weight
 
 
@@ -175,7 +176,7 @@ def clear_packed_cache() -> None:
     _packed_cache.clear()
 
 
-def _gemm(x, w_packed, idx, y, bias, activation, strategy):
+def _gemm(x, w_packed, idx, y, bias, activation, strategy, residual=None):
     ws = None
     if strategy == "runs" and (x.data_ptr() % 16 or x.stride(0) % 8):
         strategy = "auto"          # direct TMA of x needs 16-byte aligned rows
@@ -184,7 +185,7 @@ def _gemm(x, w_packed, idx, y, bias, activation, strategy):
         if nbytes:
             ws = _native.gemm_workspace(x.device, nbytes)
     _native.gather_gemm(x, w_packed, idx, y, bias=bias, activation=activation,
-                        strategy=strategy, workspace=ws)
+                        strategy=strategy, workspace=ws, residual=residual)
 
 
 def index_runs(alive_indices: torch.Tensor, K: int) -> int:
@@ -201,17 +202,36 @@ def ghost_linear(
     activation: str | None = None,
     out: torch.Tensor | None = None,
     strategy: str = "auto",
+    residual: torch.Tensor | None = None,
 ) -> torch.Tensor:
-    """y = act(x[:, alive] @ w_packed^T + bias) for x [M, K], w_packed [N, K_alive]."""
+    """y = act(x[:, alive] @ w_packed^T + bias) + residual for x [M, K], w_packed [N, K_alive].
+
+    residual [M, N] (x's dtype, rows may be strided) is added in the epilogue,
+    in fp32, before the one rounding; ``out`` may be the residual itself.
+    """
     assert x.ndim == 2 and x.is_cuda
     if not x.is_contiguous():
         x = x.contiguous()
     M = x.shape[0]
     N = w_packed.shape[0]
-    y = out if out is not None else torch.empty((M, N), dtype=x.dtype, device=x.device)
+    y, residual = _product_out(out, residual, M, N, x)
     if M and N:
-        _gemm(x, w_packed, alive_indices, y, bias, activation, strategy)
+        _gemm(x, w_packed, alive_indices, y, bias, activation, strategy, residual)
     return y
+
+
+def _product_out(out, residual, M, N, like):
+    """(output [M, N], residual as a row-major matrix or None) of a product. The output is
+    computed through the residual's rows, so it is these rows or lies apart from them."""
+    if residual is not None:
+        given = residual
+        residual = residual_matrix(residual, (M, N), like)
+        if out is not None:
+            in_place_or_apart("out", out, residual)
+            assert residual is given or out is not given, "a residual updated in place must have rows of adjacent elements"
+    if out is None:
+        out = torch.empty((M, N), dtype=like.dtype, device=like.device)
+    return out, residual
 
 
 def ghost_linear_dev(
@@ -222,6 +242,7 @@ def ghost_linear_dev(
     bias: torch.Tensor | None = None,
     activation: str | None = None,
     out: torch.Tensor | None = None,
+    residual: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """ghost_linear with K' = alive_count[0] read on the device (no host synchronisation).
 
@@ -232,10 +253,10 @@ def ghost_linear_dev(
     x = x.contiguous()
     M = x.shape[0]
     N = w_packed.shape[0]
-    y = out if out is not None else torch.empty((M, N), dtype=x.dtype, device=x.device)
+    y, residual = _product_out(out, residual, M, N, x)
     if M and N:
         _native.gather_gemm_dev(x, w_packed, alive_buffer, alive_count, y, bias=bias,
-                                activation=activation)
+                                activation=activation, residual=residual)
     return y
 
 
@@ -244,13 +265,22 @@ def packed_linear(
     w_packed: torch.Tensor,
     bias: torch.Tensor | None = None,
     activation: str | None = None,
+    residual: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
 ) -> torch.Tensor:
-    """y = act(a @ w_packed^T + bias) for an already compacted a [M, K_alive] (TMA operands)."""
+    """y = act(a @ w_packed^T + bias) + residual for an already compacted a [M, K_alive].
+
+    Both operands arrive by TMA: a's rows may be strided (as ``rms_norm``
+    returns them) if they stay 16-byte aligned, else they are copied. residual
+    [M, N] and ``out`` as for :func:`ghost_linear`.
+    """
     assert a.ndim == 2 and a.is_cuda
-    a = a.contiguous()
-    y = torch.empty((a.shape[0], w_packed.shape[0]), dtype=a.dtype, device=a.device)
+    if not a.is_contiguous() and (a.stride(1) != 1 or a.stride(0) % 8 or a.stride(0) < a.shape[1]
+                                  or a.data_ptr() % 16):
+        a = a.contiguous()
+    y, residual = _product_out(out, residual, a.shape[0], w_packed.shape[0], a)
     if y.numel():
-        _native.packed_gemm(a, w_packed, y, bias=bias, activation=activation)
+        _native.packed_gemm(a, w_packed, y, bias=bias, activation=activation, residual=residual)
     return y
 
 

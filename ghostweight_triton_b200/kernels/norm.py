@@ -16,30 +16,17 @@ gradients are refused, parameters are taken as constants.
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 from ghostweight_triton_b200 import _native
+from ghostweight_triton_b200.kernels._args import out_matrix, refuse_grad, rows
 from ghostweight_triton_b200.kernels.gather import PACK_ALIGN, _round_up
 
 # e4m3 rows keep a stride of a multiple of 128 bytes: one k-block of the
 # e4m3 product, so every TMA row starts 128-byte aligned. Padding is zero.
 PACK_ALIGN_Q8 = 128
-
-
-def _refuse_grad(**tensors: torch.Tensor | None) -> None:
-    if torch.is_grad_enabled():
-        for name, t in tensors.items():
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f"{name} requires a gradient, and this operator has no backward pass: "
-                                   "call it under torch.no_grad() or on detached tensors")
-
-
-def _rows(t: torch.Tensor, cols: int) -> torch.Tensor:
-    """t as a row-major [rows, cols] matrix (copied only when its strides are not such)."""
-    t = t.reshape(-1, cols)
-    if (t.stride(1) != 1 and cols > 1) or (t.shape[0] > 1 and t.stride(0) < cols):
-        t = t.contiguous()
-    return t
 
 
 def _alive(alive_indices: torch.Tensor | None, x: torch.Tensor) -> torch.Tensor | None:
@@ -53,35 +40,15 @@ def _alive(alive_indices: torch.Tensor | None, x: torch.Tensor) -> torch.Tensor 
     return alive_indices.contiguous()
 
 
-def _out_rows(residual_out: torch.Tensor, x: torch.Tensor, *inputs: torch.Tensor | None) -> torch.Tensor:
-    """residual_out as a matrix the sum can be written to: x's shape and type, rows that do
-    not overlap one another, and either the very place of an input or none of its memory."""
-    assert residual_out.shape == x.shape and residual_out.dtype is x.dtype and residual_out.device == x.device, (
-        "residual_out must have x's shape, dtype and device")
-    cols = x.shape[-1]
-    out = residual_out.view(-1, cols) if residual_out.is_contiguous() else residual_out
-    assert out.ndim == 2 and (out.stride(1) == 1 or cols <= 1) and (out.shape[0] <= 1 or out.stride(0) >= cols), (
-        "residual_out must be a row-major matrix (or contiguous)")
-    for t in inputs:
-        if t is None or not t.numel() or not out.numel():
-            continue
-        if t.data_ptr() == out.data_ptr() and (t.shape[0] <= 1 or t.stride(0) == out.stride(0)):
-            continue
-        span = lambda m: (m.data_ptr(), m.data_ptr() + ((m.shape[0] - 1) * m.stride(0) + cols) * m.element_size())
-        (a0, a1), (b0, b1) = span(t), span(out)
-        assert a1 <= b0 or b1 <= a0, "residual_out overlaps an input without being the same rows"
-    return out
-
-
 def _norm(x, weight, eps, residual, alive_indices, residual_out, q8):
     assert x.ndim >= 1 and x.is_cuda, "rms_norm runs on CUDA (sm_100) only"
     _native.dtype_code(x.dtype)
-    _refuse_grad(x=x, residual=residual)
+    refuse_grad(x=x, residual=residual)
     cols = x.shape[-1]
     assert cols > 0, "the norm of a row without columns is undefined"
     assert eps >= 0.0, f"eps must not be negative, got {eps}"
     lead = x.shape[:-1]
-    x_2d = _rows(x, cols)
+    x_2d = rows(x, cols)
     if weight is not None:
         assert weight.shape == (cols,), f"weight must have shape ({cols},), got {tuple(weight.shape)}"
         assert weight.device == x.device, "weight must be on x's device"
@@ -93,22 +60,22 @@ def _norm(x, weight, eps, residual, alive_indices, residual_out, q8):
     if residual is not None:
         assert residual.shape == x.shape and residual.dtype is x.dtype and residual.device == x.device, (
             "residual must have x's shape, dtype and device")
-        r_2d = _rows(residual, cols)
+        r_2d = rows(residual, cols)
         if residual_out is None:
             residual_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        total = _out_rows(residual_out, x, x_2d, r_2d)
+        total = out_matrix("residual_out", residual_out, x, x_2d, r_2d)
     else:
         assert residual_out is None, "residual_out needs a residual"
     idx = _alive(alive_indices, x)
     n = cols if idx is None else idx.numel()
-    rows = x_2d.shape[0]
+    M = x_2d.shape[0]
     if q8:
-        buf = torch.empty((rows, _round_up(n, PACK_ALIGN_Q8)), dtype=torch.float8_e4m3fn, device=x.device)
-        scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+        buf = torch.empty((M, _round_up(n, PACK_ALIGN_Q8)), dtype=torch.float8_e4m3fn, device=x.device)
+        scale = torch.empty(M, dtype=torch.float32, device=x.device)
     else:
-        buf = torch.empty((rows, n if idx is None else _round_up(n, PACK_ALIGN)), dtype=x.dtype, device=x.device)
+        buf = torch.empty((M, n if idx is None else _round_up(n, PACK_ALIGN)), dtype=x.dtype, device=x.device)
         scale = None
-    if rows:
+    if M:
         _native.rms_norm(x_2d, r_2d, total, weight, eps, idx, n, buf, scale)
     y = buf if buf.shape[1] == n else buf[:, :n]
     if x.ndim != 2:
@@ -184,18 +151,16 @@ def quantize_rows(
     """
     assert x.ndim >= 1 and x.is_cuda, "quantize_rows runs on CUDA (sm_100) only"
     _native.dtype_code(x.dtype)
-    _refuse_grad(x=x)
+    refuse_grad(x=x)
     cols = x.shape[-1]
     lead = x.shape[:-1]
     idx = _alive(alive_indices, x)
     n = cols if idx is None else idx.numel()
-    rows = 1
-    for d in lead:
-        rows *= d
-    buf = torch.empty((rows, _round_up(n, PACK_ALIGN_Q8)), dtype=torch.float8_e4m3fn, device=x.device)
-    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    if rows:
-        _native.quantize_rows(_rows(x, cols) if cols else x.reshape(rows, 0), idx, n, buf, scale)
+    M = math.prod(lead)
+    buf = torch.empty((M, _round_up(n, PACK_ALIGN_Q8)), dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty(M, dtype=torch.float32, device=x.device)
+    if M:
+        _native.quantize_rows(rows(x, cols) if cols else x.reshape(M, 0), idx, n, buf, scale)
     q = buf if buf.shape[1] == n else buf[:, :n]
     if x.ndim != 2:
         q, scale = q.view(*lead, n), scale.view(lead)

@@ -26,7 +26,7 @@ What changes underneath:
 Additions beyond the reference surface: ``freeze_weight_mask()`` freezes the
 mask from the per-input-column |W| reduction (the weight-side dead-column
 mask), ``from_conv1d`` wraps a transformers Conv1D, ``activation`` fuses a GELU
-into the epilogue, and the frozen index list survives state_dict round trips.
+into the epilogue and ``forward(x, residual)`` the residual's addition, and the frozen index list survives state_dict round trips.
 """
 
 from __future__ import annotations
@@ -36,6 +36,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from ghostweight_triton_b200 import _native
+from ghostweight_triton_b200.kernels._args import residual_matrix
 from ghostweight_triton_b200.kernels.gather import pack_weight, pack_weight_dev
 from ghostweight_triton_b200.kernels.mask import dead_neuron_mask_compact, alive_indices as _alive
 from ghostweight_triton_b200.kernels.matmul import ghost_linear, ghost_linear_dev, index_runs
@@ -241,8 +242,12 @@ class GhostLinear(nn.Module):
             r = self._runs = (alive, alive._version, index_runs(alive, self.in_features) == 0)
         return r[2]
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
-        """x : [..., in_features] -> [..., out_features] (arbitrary batch dims)."""
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+        """x : [..., in_features] -> [..., out_features] (arbitrary batch dims).
+
+        residual (optional, the output's shape, x's dtype) is added after the
+        activation, in the epilogue of the sparse product: y = act(x W^T + b) + residual.
+        """
         # Frozen mask, repeated call: everything the gather-GEMM needs was kept
         # by the last call (_fast), and is used again while the weight, bias
         # and alive list are the same tensors (same in-place versions and
@@ -267,18 +272,22 @@ class GhostLinear(nn.Module):
                 if not x_2d.is_contiguous():
                     x_2d = x_2d.contiguous()
                 out = x_2d.new_empty((x_2d.shape[0], out_f))
+                if residual is not None:
+                    residual = self._residual_2d(residual, x, x_2d)
                 if x_2d.shape[0]:
-                    _native.gather_gemm_prepared(prep, x_2d, out)
+                    _native.gather_gemm_prepared(prep, x_2d, out, residual)
                 d["_last_sparsity"] = sparsity
                 return out.reshape(*shape[:-1], out_f)
             d["_fast"] = None
         orig_shape = x.shape
         x_2d = x.reshape(-1, self.in_features)
         assert x_2d.is_cuda, "GhostLinear runs on CUDA (sm_100) only"
+        if residual is not None:
+            residual = self._residual_2d(residual, x, x_2d)
 
         frozen = self._mask_frozen and self._frozen_indices is not None
         if not frozen and self.sync_free:
-            return self._forward_sync_free(x_2d).reshape(*orig_shape[:-1], self.out_features)
+            return self._forward_sync_free(x_2d, residual).reshape(*orig_shape[:-1], self.out_features)
         if frozen:
             alive = self._frozen_indices
             k_alive = alive.shape[0]
@@ -297,6 +306,8 @@ class GhostLinear(nn.Module):
             out = F.linear(x_2d, self.weight.to(x_2d.dtype), bias)
             if self.activation is not None:
                 out = F.gelu(out, approximate="tanh" if self.activation == "gelu_tanh" else "none")
+            if residual is not None:
+                out = out + residual
         else:
             strategy = "auto"
             if frozen:
@@ -306,7 +317,7 @@ class GhostLinear(nn.Module):
             else:
                 w_packed = pack_weight(self.weight.detach(), alive, dtype=x_2d.dtype)
             out = ghost_linear(x_2d, w_packed, alive, bias=bias, activation=self.activation,
-                               strategy=strategy)
+                               strategy=strategy, residual=residual)
             if (frozen and not torch.cuda.is_current_stream_capturing()
                     and alive.dtype is torch.int64 and alive.is_contiguous()):
                 w, b = self.weight, self.bias
@@ -319,7 +330,12 @@ class GhostLinear(nn.Module):
                     float(sparsity))
         return out.reshape(*orig_shape[:-1], self.out_features)
 
-    def _forward_sync_free(self, x_2d: torch.Tensor) -> torch.Tensor:
+    def _residual_2d(self, residual: torch.Tensor, x: torch.Tensor, x_2d: torch.Tensor) -> torch.Tensor:
+        assert residual.shape[:-1] == x.shape[:-1] and residual.shape[-1] == self.out_features, (
+            f"residual must have shape {(*x.shape[:-1], self.out_features)}, got {tuple(residual.shape)}")
+        return residual_matrix(residual.reshape(-1, self.out_features), (x_2d.shape[0], self.out_features), x_2d)
+
+    def _forward_sync_free(self, x_2d: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
         """Dynamic-mask forward whose alive count never leaves the device."""
         bias = self.bias
         if bias is not None and bias.dtype != x_2d.dtype:
@@ -338,7 +354,7 @@ class GhostLinear(nn.Module):
                 y = torch.empty((x_2d.shape[0], self.out_features), dtype=x_2d.dtype, device=x_2d.device)
                 count = torch.empty(1, dtype=torch.int32, device=x_2d.device)
                 if _native.dynamic_linear(x_2d, w, self.threshold, y, bias=bias, activation=self.activation,
-                                          count=count) == _native.GW_OK:
+                                          count=count, residual=residual) == _native.GW_OK:
                     self._readback.record(count)
                     self._sparsity_pending = True
                     return y
@@ -347,9 +363,12 @@ class GhostLinear(nn.Module):
             out = F.linear(x_2d, self.weight.to(x_2d.dtype), bias)
             if self.activation is not None:
                 out = F.gelu(out, approximate="tanh" if self.activation == "gelu_tanh" else "none")
+            if residual is not None:
+                out = out + residual
         else:
             w_packed = pack_weight_dev(self.weight.detach(), buf, count, dtype=x_2d.dtype)
-            out = ghost_linear_dev(x_2d, w_packed, buf, count, bias=bias, activation=self.activation)
+            out = ghost_linear_dev(x_2d, w_packed, buf, count, bias=bias, activation=self.activation,
+                                   residual=residual)
         self._readback.record(count)
         self._sparsity_pending = True
         return out

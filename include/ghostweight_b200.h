@@ -337,6 +337,38 @@ GW_API int gw_packed_gemm(const void* a, int dtype, int64_t M, int64_t K, int64_
                           int epilogue, void* y, int64_t ldy, void* stream);
 
 /*
+ * The products above with a residual added in the epilogue, after the
+ * activation and before the one rounding:
+ *   y[m, n] = act( ... + bias[n] ) + residual[m, n]
+ * residual [M, N] (ldr) has y's type, needs no alignment, and may be y itself
+ * (same pointer and leading dimension) or lie apart from it; NULL gives the
+ * entry point without it. Everything else is as at gw_gather_gemm,
+ * gw_gather_gemm_dev, gw_dynamic_linear and gw_packed_gemm. The reference
+ * leaves the addition to torch, as it does the bias (module.py:116-117).
+ */
+GW_API int gw_gather_gemm_residual(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx,
+                                   const void* w_packed, int64_t N, int64_t ldw, const int64_t* idx,
+                                   int64_t n_alive, const void* bias, int epilogue,
+                                   const void* residual, int64_t ldr, void* y, int64_t ldy,
+                                   int strategy, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+GW_API int gw_gather_gemm_dev_residual(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx,
+                                       const void* w_packed, int64_t N, int64_t ldw,
+                                       const int64_t* idx, int64_t n_alive_max,
+                                       const int32_t* n_alive_dev, const void* bias, int epilogue,
+                                       const void* residual, int64_t ldr, void* y, int64_t ldy,
+                                       void* workspace, size_t workspace_bytes, void* stream);
+GW_API int gw_dynamic_linear_residual(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx,
+                                      const void* w, int64_t N, int64_t ldw, double threshold,
+                                      const void* bias, int epilogue, const void* residual,
+                                      int64_t ldr, void* y, int64_t ldy, int32_t* alive_count,
+                                      int32_t* mask, void* stream);
+GW_API int gw_packed_gemm_residual(const void* a, int dtype, int64_t M, int64_t K, int64_t lda,
+                                   const void* w_packed, int64_t N, int64_t ldw, const void* bias,
+                                   int epilogue, const void* residual, int64_t ldr, void* y,
+                                   int64_t ldy, void* stream);
+
+/*
  * Residual addition and root-mean-square norm of rows, written out over the
  * alive columns of the layer that reads them:
  *   s[m, k] = x[m, k] + residual[m, k]                       (all cols columns)

@@ -10,7 +10,8 @@ import pytest
 import torch
 
 from ghostweight_triton_b200 import _native
-from ghostweight_triton_b200.kernels.norm import _out_rows, pack_weight_q8, quantize_rows, rms_norm, rms_norm_q8
+from ghostweight_triton_b200.kernels._args import out_matrix
+from ghostweight_triton_b200.kernels.norm import pack_weight_q8, quantize_rows, rms_norm, rms_norm_q8
 
 SHAPE, DTYPE, NULL = _native.GW_ERR_SHAPE, _native.GW_ERR_DTYPE, _native.GW_ERR_NULL
 
@@ -44,6 +45,7 @@ def test_abi_refusals():
 
 
 def test_residual_out_checks_need_no_gpu():
+    _out_rows = lambda out, like, *ins: out_matrix("residual_out", out, like, *ins)
     x = torch.zeros(4, 6)
     r = torch.zeros(4, 6)
     assert _out_rows(x, x, x, r) is not None and _out_rows(torch.empty(4, 6), x, x, r) is not None
