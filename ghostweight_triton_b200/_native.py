@@ -69,6 +69,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                         _vp, _i64, _vp, _vp, _vp]),
     "gw_packed_gemm_residual": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i, _vp, _i64,
                                      _vp, _i64, _vp]),
+    "gw_packed_gemm_q8": (_i, [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i, _vp, _i64,
+                               _vp, _i, _i64, _vp]),
     "gw_rms_norm": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _d, _vp, _i64, _vp,
                          _i64, _i64, _vp]),
     "gw_rms_norm_q8": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _d, _vp, _i64, _vp,
@@ -88,7 +90,7 @@ _api = None
 FAST_ENTRIES = ("gw_gather_gemm", "gw_gather_gemm_dev", "gw_packed_gemm", "gw_gather_columns", "gw_dynamic_linear",
                 "gw_gather_rows_t", "gw_gather_columns_dev", "gw_gather_rows_t_dev", "gw_mask_compact",
                 "gw_gather_gemm_residual", "gw_gather_gemm_dev_residual", "gw_dynamic_linear_residual",
-                "gw_packed_gemm_residual", "gw_rms_norm", "gw_rms_norm_q8", "gw_quantize_rows", "gw_gather_gemm_workspace_bytes")
+                "gw_packed_gemm_residual", "gw_packed_gemm_q8", "gw_rms_norm", "gw_rms_norm_q8", "gw_quantize_rows", "gw_gather_gemm_workspace_bytes")
 
 
 class _Api:
@@ -510,6 +512,27 @@ def packed_gemm(a: torch.Tensor, w_packed: torch.Tensor, y: torch.Tensor,
             max(w_packed.stride(0), K), _ptr(bias), epilogue_code(activation), *_residual(residual), _ptr(y),
             max(y.stride(0), N), _stream(a.device))
     _check(st, "gw_packed_gemm")
+
+
+def packed_gemm_q8(a: torch.Tensor, a_scale: torch.Tensor, w_packed: torch.Tensor, w_scale: torch.Tensor,
+                   y: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
+                   residual: torch.Tensor | None = None) -> None:
+    """y = act(a_scale w_scale (a @ w_packed^T) + bias) + residual over e4m3 operands by TMA."""
+    _rowmajor(a, w_packed, y)
+    M, K = a.shape
+    N = w_packed.shape[0]
+    with _on_device(a.device):
+        st = api().gw_packed_gemm_q8(
+            a.data_ptr(), a_scale.data_ptr(), M, K, _ld16(a), w_packed.data_ptr(), w_scale.data_ptr(), N,
+            _ld16(w_packed), _ptr(bias), epilogue_code(activation), *_residual(residual), y.data_ptr(),
+            dtype_code(y.dtype), max(y.stride(0), N), _stream(a.device))
+    if st:
+        _check(st, "gw_packed_gemm_q8")
+
+
+def _ld16(t: torch.Tensor) -> int:
+    """Leading dimension of e4m3 rows; a matrix of one row has any, so a multiple of 16."""
+    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
 
 
 def dynamic_linear(x: torch.Tensor, weight: torch.Tensor, threshold: float, y: torch.Tensor,

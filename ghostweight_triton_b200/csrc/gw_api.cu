@@ -78,13 +78,13 @@ void* tensor_map_encoder() {
 }
 
 bool make_tmap_kmajor(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld,
-                      int box_cols, int box_rows) {
+                      int box_cols, int box_rows, int elem_bytes) {
   // A few recently encoded maps per host thread: the packed weight and the
   // reused workspace recur from call to call, and encoding is a driver call.
   struct Entry {
     const void* base;
     int64_t rows, cols, ld;
-    int box_cols, box_rows;
+    int box_cols, box_rows, elem_bytes;
     CUtensorMap map;
   };
   constexpr int kCache = 8;
@@ -93,7 +93,7 @@ bool make_tmap_kmajor(CUtensorMap* map, const void* base, int64_t rows, int64_t 
   for (int i = 0; i < filled; ++i) {
     const Entry& e = cache[i];
     if (e.base == base && e.rows == rows && e.cols == cols && e.ld == ld &&
-        e.box_cols == box_cols && e.box_rows == box_rows) {
+        e.box_cols == box_cols && e.box_rows == box_rows && e.elem_bytes == elem_bytes) {
       *map = e.map;
       return true;
     }
@@ -105,15 +105,15 @@ bool make_tmap_kmajor(CUtensorMap* map, const void* base, int64_t rows, int64_t 
   auto encode = reinterpret_cast<EncodeTiledFn>(tensor_map_encoder());
   if (!encode) return false;
   cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
-  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2u};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * static_cast<cuuint64_t>(elem_bytes)};
   cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
   cuuint32_t estr[2] = {1, 1};
-  if (encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(base), dims, strides,
+  if (encode(map, elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(base), dims, strides,
              box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return false;
   Entry& e = cache[next];
-  e = Entry{base, rows, cols, ld, box_cols, box_rows, *map};
+  e = Entry{base, rows, cols, ld, box_cols, box_rows, elem_bytes, *map};
   next = (next + 1) % kCache;
   if (filled < kCache) ++filled;
   return true;
@@ -382,22 +382,23 @@ cudaError_t launch_dense_gemm(const void* a, int dtype, int64_t M, int64_t K, in
                               void* y, int64_t ldy, const gw::DeviceInfo* d, cudaStream_t s,
                               void* const* peers = nullptr, int n_peers = 0,
                               const int64_t* a_cols = nullptr, int64_t a_width = 0,
-                              const gw::Residual& res = {}) {
-  const GemmChoice c = choose_gemm(M, N, K, d);
+                              const gw::Residual& res = {}, const gw::QScale& qs = {}) {
+  // The plans count 128-byte k-blocks: two e4m3 columns stand for one of 16 bits.
+  const GemmChoice c = choose_gemm(M, N, qs.a ? (K + 1) / 2 : K, d);
   if (c.kernel == GW_KERNEL_PAIR)
     return gw::launch_gemm_tc2(a, dtype, M, K, lda, w, N, ldw, bias, epilogue, y, ldy,
                                d->err_word, d->sm_count, s, peers, n_peers, a_cols, a_width, nullptr,
-                               nullptr, res);
+                               nullptr, res, qs);
   cudaError_t e;
   if (c.kernel == GW_KERNEL_DECODE)
     e = gw::launch_gemm_decode(c.dp, a, dtype, M, K, lda, w, N, ldw, bias, epilogue, y, ldy,
-                               d->err_word, s, a_cols, a_width, res);
+                               d->err_word, s, a_cols, a_width, res, qs);
   else if (c.kernel == GW_KERNEL_SPLITK)
     e = gw::launch_gemm_splitk(c.sk, a, dtype, M, K, lda, w, N, ldw, bias, epilogue, y, ldy,
-                               d->err_word, s, a_cols, a_width, res);
+                               d->err_word, s, a_cols, a_width, res, qs);
   else
     e = gw::launch_gemm_tc(0, a, dtype, M, a_cols ? a_width : K, lda, w, N, ldw, nullptr, K, bias,
-                           epilogue, y, ldy, d->err_word, d->sm_count, s, a_cols, nullptr, res);
+                           epilogue, y, ldy, d->err_word, d->sm_count, s, a_cols, nullptr, res, qs);
   if (e != cudaSuccess || n_peers == 0) return e;
   return gw::launch_copy_to_peers(y, M, N, ldy, peers, n_peers, d->sm_count, s);
 }
@@ -696,6 +697,35 @@ int gw_packed_gemm_residual(const void* a, int dtype, int64_t M, int64_t K, int6
     return GW_ERR_ALIGN;
   e = launch_dense_gemm(a, dtype, M, K, lda, w_packed, N, ldw, bias, epilogue, y, ldy, d, s, nullptr, 0,
                         nullptr, 0, res);
+  return e == cudaSuccess ? GW_OK : cuda_fail(e);
+}
+
+int gw_packed_gemm_q8(const void* a, const float* a_scale, int64_t M, int64_t K, int64_t lda,
+                      const void* w_packed, const float* w_scale, int64_t N, int64_t ldw,
+                      const void* bias, int epilogue, const void* residual, int64_t ldr, void* y,
+                      int dtype, int64_t ldy, void* stream) {
+  if (dtype != GW_DTYPE_F16 && dtype != GW_DTYPE_BF16) return GW_ERR_DTYPE;
+  if (!valid_epi(epilogue)) return GW_ERR_UNSUPPORTED;
+  if (!matrix_ok(M, K, lda) || !matrix_ok(N, K, ldw) || !matrix_ok(M, N, ldy) ||
+      (residual && !matrix_ok(M, N, ldr)) || K > 0x7FFFFFFFll - 128)
+    return GW_ERR_SHAPE;
+  const gw::DeviceInfo* d = nullptr;
+  int st = current_device(&d);
+  if (st != GW_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (M == 0 || N == 0) return GW_OK;
+  if (!y) return GW_ERR_NULL;
+  const gw::Residual res{residual, ldr};
+  cudaError_t e;
+  if (K == 0) {
+    e = gw::launch_fill_bias(y, dtype, M, N, ldy, bias, epilogue, s, res);
+    return e == cudaSuccess ? GW_OK : cuda_fail(e);
+  }
+  if (!a || !w_packed || !a_scale || !w_scale) return GW_ERR_NULL;
+  if (!aligned16(a) || !aligned16(w_packed) || (lda % 16) != 0 || (ldw % 16) != 0)
+    return GW_ERR_ALIGN;
+  e = launch_dense_gemm(a, dtype, M, K, lda, w_packed, N, ldw, bias, epilogue, y, ldy, d, s, nullptr,
+                        0, nullptr, 0, res, {a_scale, w_scale});
   return e == cudaSuccess ? GW_OK : cuda_fail(e);
 }
 

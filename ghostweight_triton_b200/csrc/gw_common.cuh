@@ -259,6 +259,26 @@ __device__ __forceinline__ void tc_mma_f16(uint32_t d_tmem, uint64_t a_desc, uin
       : "memory");
 }
 
+// The same for e4m3 operands (kind::f8f6f4, K = 32 per instruction). A row of
+// an operand atom is 128 bytes in both kinds and one instruction consumes 32 of
+// them, so descriptors, atoms and the 32-byte k steps are shared: an atom is
+// 64 columns of 16 bits or 128 columns of 8.
+__device__ __forceinline__ void tc_mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                          uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+template <bool Q8>
+__device__ __forceinline__ void tc_mma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                       uint32_t idesc, uint32_t accumulate) {
+  if constexpr (Q8) tc_mma_f8(d_tmem, a_desc, b_desc, idesc, accumulate);
+  else tc_mma_f16(d_tmem, a_desc, b_desc, idesc, accumulate);
+}
+
 // Arrive once on `bar` when every previously issued tcgen05 op of this thread completes.
 __device__ __forceinline__ void tc_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
@@ -319,6 +339,17 @@ __host__ __device__ constexpr uint32_t idesc_f16(uint32_t ab_format, uint32_t m,
        | ((n >> 3) << 17)          // N / 8
        | ((m >> 4) << 24);         // M / 16
 }
+// Kind f8f6f4, fp32 accumulate, A and B both e4m3 (format 0) and K-major.
+__host__ __device__ constexpr uint32_t idesc_e4m3(uint32_t m, uint32_t n) {
+  return (1u << 4) | (0u << 7) | (0u << 10) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+template <bool Q8, int DT>
+__host__ __device__ constexpr uint32_t idesc_for(uint32_t m, uint32_t n) {
+  return Q8 ? idesc_e4m3(m, n) : idesc_f16(DT == GW_DTYPE_BF16 ? 1u : 0u, m, n);
+}
+// Columns of one 128-byte operand atom.
+template <bool Q8>
+constexpr int atom_cols() { return Q8 ? 128 : 64; }
 
 // ----------------------------------------------------------------------------
 // Clusters of two CTAs (2-SM tcgen05 MMA). No TMA multicast anywhere: each CTA
@@ -448,6 +479,22 @@ __device__ __forceinline__ void tc_mma_f16_pair(uint32_t d_tmem, uint64_t a_desc
       "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
       :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+
+__device__ __forceinline__ void tc_mma_f8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                               uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+template <bool Q8>
+__device__ __forceinline__ void tc_mma_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                            uint32_t idesc, uint32_t accumulate) {
+  if constexpr (Q8) tc_mma_f8_pair(d_tmem, a_desc, b_desc, idesc, accumulate);
+  else tc_mma_f16_pair(d_tmem, a_desc, b_desc, idesc, accumulate);
 }
 
 // Arrive once on the barrier at this shared offset in every CTA of `mask` when
@@ -599,6 +646,28 @@ __device__ __forceinline__ void add_bias4(float (&f)[4], const uint16_t* bias, i
       if (n0 + j < N) f[j] += Elem<DT>::to_f(__ldg(bias + n0 + j));
   }
 }
+// Scales of e4m3 operands, applied to the fp32 accumulator in front of the bias:
+// f[j] * row * w[n0 + j]. First by the row's scale: the product of the two
+// scales alone could leave fp32's range.
+__device__ __forceinline__ void scale32(float (&f)[32], float row, const float* w, int64_t n0,
+                                        int64_t N) {
+  const float* s = w + n0;
+  if (n0 + 32 <= N && (reinterpret_cast<uintptr_t>(s) & 15u) == 0) {
+#pragma unroll
+    for (int v = 0; v < 8; ++v) {
+      const float4 q = __ldg(reinterpret_cast<const float4*>(s) + v);
+      f[4 * v] = f[4 * v] * row * q.x;
+      f[4 * v + 1] = f[4 * v + 1] * row * q.y;
+      f[4 * v + 2] = f[4 * v + 2] * row * q.z;
+      f[4 * v + 3] = f[4 * v + 3] * row * q.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (n0 + j < N) f[j] = f[j] * row * __ldg(s + j);
+  }
+}
+
 // Residual added in GEMM epilogues, after the activation and before the one
 // rounding: 32 (or 4) consecutive columns [n0, n0 + 32) of one row, as pairs
 // of 16-bit values, zeros at and past column N. Plain loads, not the

@@ -85,6 +85,8 @@ struct DcParams {
   int y_vec_ok;              // 8-byte stores of four outputs allowed
   const uint16_t* res;       // residual (or null), leading dimension ldr
   int64_t ldr;
+  const float* a_scale;      // Q8: scales of a's rows and of W's rows
+  const float* w_scale;
   int num_kb;
   int split;                 // cluster size S
   int x_tx_bytes;            // bytes of one box of a (its rows: M rounded up to 8)
@@ -148,7 +150,7 @@ __device__ __forceinline__ void dc_gather_tile(const DcParams& p, uint32_t xs, i
 // Once every slot of its receive buffer has landed it sums the S slots in rank
 // order and writes the slice out. One task = one row m x four features; rows
 // vary fastest across threads (conflict-free reads of the receive rows).
-template <int MP, int DT>
+template <int MP, int DT, bool Q8>
 __device__ __forceinline__ void dc_finish(const DcParams& p, const float* recv, int rank,
                                           int n_blk, int rows) {
   constexpr int kStride = DcCfg<MP>::kRecvStride;
@@ -166,6 +168,12 @@ __device__ __forceinline__ void dc_finish(const DcParams& p, const float* recv, 
     }
     const int64_t n0 = static_cast<int64_t>(n_blk) * kDcN + rank * F + 4 * g;
     if (n0 >= p.N) continue;
+    if constexpr (Q8) {
+      const float row = p.a_scale[m];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (n0 + j < p.N) f[j] = f[j] * row * __ldg(p.w_scale + n0 + j);
+    }
     if (p.bias) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -192,13 +200,13 @@ __device__ __forceinline__ void dc_finish(const DcParams& p, const float* recv, 
 // (local indices; `used` counts ring slots in order) into accumulator d, with
 // one commit per k-block to its stage's empty barrier, then one to tfull (or
 // raises the abort flag) and one to drain_bar.
-template <int MP, int DT, typename FullF, typename EmptyF>
+template <int MP, int DT, bool Q8, typename FullF, typename EmptyF>
 __device__ __forceinline__ void dc_issue(const DcParams& p, uint32_t sbase, uint32_t d, int nk,
                                          int first, int step, FullF full, EmptyF empty,
                                          uint32_t tfull, uint32_t drain_bar,
                                          volatile int* abort_flag) {
   using C = DcCfg<MP>;
-  constexpr uint32_t idesc = idesc_f16(DT == GW_DTYPE_BF16 ? 1u : 0u, kDcN, MP);
+  constexpr uint32_t idesc = idesc_for<Q8, DT>(kDcN, MP);
   bool ok = true;
   for (int used = first; used < nk; used += step) {
     const int s = used % C::kStages;
@@ -210,7 +218,7 @@ __device__ __forceinline__ void dc_issue(const DcParams& p, uint32_t sbase, uint
     const uint64_t a_desc = smem_desc_kmajor_sw128(w_s + kDcWBytes);
 #pragma unroll
     for (int k = 0; k < kDcK / 16; ++k)
-      tc_mma_f16(d, w_desc + 2u * k, a_desc + 2u * k, idesc, (used > first || k > 0) ? 1u : 0u);
+      tc_mma<Q8>(d, w_desc + 2u * k, a_desc + 2u * k, idesc, (used > first || k > 0) ? 1u : 0u);
     tc_commit(empty(s));
   }
   if (ok) tc_commit(tfull);
@@ -218,11 +226,13 @@ __device__ __forceinline__ void dc_issue(const DcParams& p, uint32_t sbase, uint
   tc_commit(drain_bar);
 }
 
-template <int MP, int DT>
+// Q8: a and W' in e4m3 with scales (never gathered here), else 16-bit of type DT.
+template <int MP, int DT, bool Q8>
 __global__ void __launch_bounds__(kDcThreads, 2)
 gemm_decode_kernel(const __grid_constant__ CUtensorMap tmap_w,
                    const __grid_constant__ CUtensorMap tmap_a, const DcParams p) {
   using C = DcCfg<MP>;
+  constexpr int kCols = atom_cols<Q8>();              // columns of one k-block
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_s = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + ((1024u - (raw_s & 1023u)) & 1023u);
@@ -302,9 +312,9 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap tmap_w,
       const int pre = nk < C::kStages ? nk : C::kStages;
       for (int i = 0; i < pre; ++i) {
         mbar_arrive_expect_tx(full(i), kDcWBytes + p.x_tx_bytes);
-        tma_load_2d(sbase + i * C::kStageBytes, &tmap_w, (kb0 + i) * kDcK, n_blk * kDcN, full(i));
+        tma_load_2d(sbase + i * C::kStageBytes, &tmap_w, (kb0 + i) * kCols, n_blk * kDcN, full(i));
       }
-      for (int kb = kb0 + pre; kb < kb1; ++kb) tma_prefetch_l2_2d(&tmap_w, kb * kDcK, n_blk * kDcN);
+      for (int kb = kb0 + pre; kb < kb1; ++kb) tma_prefetch_l2_2d(&tmap_w, kb * kCols, n_blk * kDcN);
       asm volatile("griddepcontrol.wait;" ::: "memory");
       int issued = 0;
       bool ok = true;
@@ -318,10 +328,10 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap tmap_w,
         if (issued >= pre) {
           if (!mbar_wait(empty(s), ph ^ 1u, abort_flag, p.err)) { ok = false; break; }
           mbar_arrive_expect_tx(full(s), kDcWBytes + p.x_tx_bytes);
-          tma_load_2d(w_s, &tmap_w, kb * kDcK, n_blk * kDcN, full(s));
+          tma_load_2d(w_s, &tmap_w, kb * kCols, n_blk * kDcN, full(s));
         }
         if (!p.gx) {
-          const int ax = p.a_cols ? run_start_check(cur, p.a_width, p.err) : kb * kDcK;
+          const int ax = p.a_cols ? run_start_check(cur, p.a_width, p.err) : kb * kCols;
           tma_load_2d(w_s + kDcWBytes, &tmap_a, ax, 0, full(s));
         }
       }
@@ -336,7 +346,7 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap tmap_w,
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (even k-blocks)
     if (lane == 0) {
-      dc_issue<MP, DT>(p, sbase, tmem_base, kb1 - kb0, 0, dual ? 2 : 1, full, empty, tfull,
+      dc_issue<MP, DT, Q8>(p, sbase, tmem_base, kb1 - kb0, 0, dual ? 2 : 1, full, empty, tfull,
                        drain_bar, abort_flag);
       // Every MMA (of both issuers) has finished writing TMEM before TMEM is freed.
       mbar_wait(drain_bar, 0u, nullptr, p.err, 100000000ull);
@@ -346,7 +356,7 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap tmap_w,
     if (dual && warp == 2) {
       // ---------------------------------------------------------- MMA issuer (odd k-blocks)
       if (lane == 0)
-        dc_issue<MP, DT>(p, sbase, tmem_base + MP, kb1 - kb0, 1, 2, full, empty, tfull, drain_bar,
+        dc_issue<MP, DT, Q8>(p, sbase, tmem_base + MP, kb1 - kb0, 1, 2, full, empty, tfull, drain_bar,
                          abort_flag);
       __syncwarp();
     }
@@ -419,21 +429,21 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap tmap_w,
                        mapa_shared(recv_bar, owner));
   }
 
-  // The residual may come from the previous kernel of the stream.
-  if (p.res) asm volatile("griddepcontrol.wait;" ::: "memory");
+  // The residual and the scales of a may come from the previous kernel of the stream.
+  if (Q8 || p.res) asm volatile("griddepcontrol.wait;" ::: "memory");
   // Every slot of this CTA's slice has landed: its own and the S - 1 peers'.
   const bool got = mbar_wait_cluster(recv_bar, 0u, nullptr, p.err);
   // Tell every sender that its copy into this CTA has landed.
   if (threadIdx.x < S) mbar_arrive_cluster(mapa_shared(sent_bar, threadIdx.x));
-  if (got) dc_finish<MP, DT>(p, recv, rank, n_blk, rows);
+  if (got) dc_finish<MP, DT, Q8>(p, recv, rank, n_blk, rows);
   // This CTA's ring is the source of its copies: it stays valid, and the CTA
   // alive, until every owner has received its slice.
   mbar_wait_cluster(sent_bar, 0u, nullptr, p.err);
 }
 
-template <int MP, int DT>
+template <int MP, int DT, bool Q8>
 cudaError_t set_decode_attrs() {
-  auto kern = gemm_decode_kernel<MP, DT>;
+  auto kern = gemm_decode_kernel<MP, DT, Q8>;
   cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kern), DcCfg<MP>::kSmemBytes);
   if (e != cudaSuccess) return e;
   // Clusters of 16 CTAs are a non-portable size; the occupancy query in
@@ -450,11 +460,11 @@ cudaError_t set_decode_attrs() {
   return cudaSuccess;
 }
 
-template <int MP, int DT>
+template <int MP, int DT, bool Q8>
 cudaError_t launch_dc(const CUtensorMap& tw, const CUtensorMap& ta, const DcParams& p,
                       int64_t blocks, cudaStream_t stream) {
-  auto kern = gemm_decode_kernel<MP, DT>;
-  cudaError_t e = set_decode_attrs<MP, DT>();
+  auto kern = gemm_decode_kernel<MP, DT, Q8>;
+  cudaError_t e = set_decode_attrs<MP, DT, Q8>();
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(p.split), static_cast<unsigned>(blocks));
@@ -481,8 +491,8 @@ struct DecodeTable {
 
 template <int MP>
 int query_decode_clusters(int s) {
-  auto kern = gemm_decode_kernel<MP, GW_DTYPE_F16>;
-  if (set_decode_attrs<MP, GW_DTYPE_F16>() != cudaSuccess) {
+  auto kern = gemm_decode_kernel<MP, GW_DTYPE_F16, false>;
+  if (set_decode_attrs<MP, GW_DTYPE_F16, false>() != cudaSuccess) {
     (void)cudaGetLastError();
     return 0;
   }
@@ -575,24 +585,30 @@ cudaError_t launch_decode_params(const DecodePlan& plan, DcParams& p, int dtype,
   const int a_rows = static_cast<int>((p.M + 7) / 8 * 8);
   p.x_tx_bytes = p.gx ? 0 : a_rows * kDcK * 2;
   CUtensorMap ta, tw;
-  if (!make_tmap_kmajor(&tw, w, p.N, K, ldw, kDcK, kDcN)) return cudaErrorInvalidValue;
+  const bool q8 = p.a_scale != nullptr;
+  const int kb_cols = q8 ? atom_cols<true>() : kDcK;
+  if (!make_tmap_kmajor(&tw, w, p.N, K, ldw, kb_cols, kDcN, q8 ? 1 : 2)) return cudaErrorInvalidValue;
   if (p.gx) {
     ta = tw;                          // unused: a is gathered in the kernel
-  } else if (!make_tmap_kmajor(&ta, a, p.M, p.a_cols ? p.a_width : K, lda, kDcK, a_rows)) {
+  } else if (!make_tmap_kmajor(&ta, a, p.M, p.a_cols ? p.a_width : K, lda, kb_cols, a_rows,
+                               q8 ? 1 : 2)) {
     return cudaErrorInvalidValue;
   }
   const bool bf = dtype == GW_DTYPE_BF16;
+#define GW_DC(MPV, Q)                                                              \
+  (bf ? launch_dc<MPV, GW_DTYPE_BF16, Q>(tw, ta, p, plan.blocks, stream)            \
+      : launch_dc<MPV, GW_DTYPE_F16, Q>(tw, ta, p, plan.blocks, stream))
   switch (plan.mp) {
-    case 16: return bf ? launch_dc<16, GW_DTYPE_BF16>(tw, ta, p, plan.blocks, stream)
-                       : launch_dc<16, GW_DTYPE_F16>(tw, ta, p, plan.blocks, stream);
-    case 32: return bf ? launch_dc<32, GW_DTYPE_BF16>(tw, ta, p, plan.blocks, stream)
-                       : launch_dc<32, GW_DTYPE_F16>(tw, ta, p, plan.blocks, stream);
+    case 16: return q8 ? GW_DC(16, true) : GW_DC(16, false);
+    case 32: return q8 ? GW_DC(32, true) : GW_DC(32, false);
     default: return cudaErrorInvalidValue;
   }
+#undef GW_DC
 }
 
 DcParams decode_params(const DecodePlan& plan, int64_t M, int64_t K, int64_t N, const void* bias,
-                       int epilogue, void* y, int64_t ldy, unsigned int* err) {
+                       int epilogue, void* y, int64_t ldy, unsigned int* err,
+                       const QScale& qs = {}) {
   DcParams p{};
   p.M = M;
   p.N = N;
@@ -601,7 +617,10 @@ DcParams decode_params(const DecodePlan& plan, int64_t M, int64_t K, int64_t N, 
   p.y = static_cast<uint16_t*>(y);
   p.ldy = ldy;
   p.y_vec_ok = ((reinterpret_cast<uintptr_t>(y) & 7u) == 0 && (ldy % 4) == 0) ? 1 : 0;
-  p.num_kb = static_cast<int>((K + kDcK - 1) / kDcK);
+  p.a_scale = qs.a;
+  p.w_scale = qs.w;
+  const int kb_cols = qs.a ? atom_cols<true>() : kDcK;
+  p.num_kb = static_cast<int>((K + kb_cols - 1) / kb_cols);
   p.split = plan.split;
   p.err = err;
   return p;
@@ -632,11 +651,12 @@ cudaError_t launch_gemm_decode(const DecodePlan& plan, const void* a, int dtype,
                                int64_t K, int64_t lda, const void* w, int64_t N, int64_t ldw,
                                const void* bias, int epilogue, void* y, int64_t ldy,
                                unsigned int* err, cudaStream_t stream, const int64_t* a_cols,
-                               int64_t a_width, const Residual& res) {
+                               int64_t a_width, const Residual& res, const QScale& qs) {
   if (plan.split < 2 || plan.split > 16 || plan.blocks <= 0 || plan.blocks > 65535 ||
       M <= 0 || M > plan.mp)
     return cudaErrorInvalidValue;
-  DcParams p = decode_params(plan, M, K, N, bias, epilogue, y, ldy, err);
+  if (qs.a && (!qs.w || a_cols)) return cudaErrorInvalidValue;
+  DcParams p = decode_params(plan, M, K, N, bias, epilogue, y, ldy, err, qs);
   if (p.num_kb < plan.split) return cudaErrorInvalidValue;
   if (a_cols && (K % kDcK) != 0) return cudaErrorInvalidValue;
   p.a_cols = a_cols;

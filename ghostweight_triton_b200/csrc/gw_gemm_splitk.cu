@@ -79,6 +79,8 @@ struct SkParams {
   int y_vec_ok;              // 8-byte stores of four outputs allowed
   const uint16_t* res;       // residual (or null), leading dimension ldr
   int64_t ldr;
+  const float* a_scale;      // Q8: scales of A's rows and of W's rows
+  const float* w_scale;
   int num_kb;
   int m_tiles;
   int split;                 // cluster size S
@@ -105,7 +107,7 @@ __device__ __forceinline__ float4 ld_dsmem_f4(uint32_t cluster_addr) {
 // order (the result does not depend on timing), applies the epilogue and
 // stores four outputs. (A mapping of one (row, group) task per iteration spent
 // about 200 cycles of dependent index arithmetic per task with six warps per SM.)
-template <int S, int BN, int DT, int EPI>
+template <int S, int BN, int DT, int EPI, bool Q8>
 __device__ __forceinline__ void reduce_slice(const SkParams& p, uint32_t red_local, int rank,
                                              int m_blk, int n_blk, int rows_valid, bool ok) {
   constexpr int kStride = SkCfg<BN>::kRedStride;
@@ -119,6 +121,12 @@ __device__ __forceinline__ void reduce_slice(const SkParams& p, uint32_t red_loc
   const int64_t n0 = static_cast<int64_t>(n_blk) * BN + col;
   float b[4] = {0.f, 0.f, 0.f, 0.f};
   if (p.bias) add_bias4<DT>(b, p.bias, n0, p.N);
+  float ws[4] = {1.f, 1.f, 1.f, 1.f};
+  if constexpr (Q8) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ws[j] = n0 + j < p.N ? __ldg(p.w_scale + n0 + j) : 0.0f;
+  }
+  const float* sp = Q8 ? p.a_scale + static_cast<int64_t>(m_blk) * kSkBM + row0 : nullptr;
   const bool vec = p.y_vec_ok && n0 + 4 <= p.N;
   const int64_t y_step = static_cast<int64_t>(kStep) * p.ldy;
   uint16_t* yp = p.y + (static_cast<int64_t>(m_blk) * kSkBM + row0) * p.ldy + n0;
@@ -128,6 +136,12 @@ __device__ __forceinline__ void reduce_slice(const SkParams& p, uint32_t red_loc
   float sink = 0.f;
   for (int r = row0; r < rows_valid; r += kRows * kStep, yp += kRows * y_step) {
     float4 v[kRows][S];
+    float rs[kRows];
+    if constexpr (Q8) {
+#pragma unroll
+      for (int u = 0; u < kRows; ++u) rs[u] = r + u * kStep < rows_valid ? sp[u * kStep] : 0.0f;
+      sp += kRows * kStep;
+    }
     uint2 rv[kRows];
     if (rp) {
 #pragma unroll
@@ -165,6 +179,10 @@ __device__ __forceinline__ void reduce_slice(const SkParams& p, uint32_t red_loc
         acc.x += v[u][s].x; acc.y += v[u][s].y; acc.z += v[u][s].z; acc.w += v[u][s].w;
       }
       float f[4] = {acc.x, acc.y, acc.z, acc.w};
+      if constexpr (Q8) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = f[j] * rs[u] * ws[j];
+      }
       if (p.bias) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) f[j] += b[j];
@@ -192,13 +210,13 @@ __device__ __forceinline__ void reduce_slice(const SkParams& p, uint32_t red_loc
 // (local indices) into accumulator d, one commit per k-block to its stage's
 // empty barrier, then one to tfull (or raises the abort flag) and one to
 // drain_bar.
-template <int BN, int DT, typename FullF, typename EmptyF>
+template <int BN, int DT, bool Q8, typename FullF, typename EmptyF>
 __device__ __forceinline__ void sk_issue(const SkParams& p, uint32_t sbase, uint32_t d, int nk,
                                          int first, int step, FullF full, EmptyF empty,
                                          uint32_t tfull, uint32_t drain_bar,
                                          volatile int* abort_flag) {
   using C = SkCfg<BN>;
-  constexpr uint32_t idesc = idesc_f16(DT == GW_DTYPE_BF16 ? 1u : 0u, kSkBM, BN);
+  constexpr uint32_t idesc = idesc_for<Q8, DT>(kSkBM, BN);
   bool ok = true;
   for (int used = first; used < nk; used += step) {
     const int s = used % C::kStages;
@@ -210,7 +228,7 @@ __device__ __forceinline__ void sk_issue(const SkParams& p, uint32_t sbase, uint
     const uint64_t b_desc = smem_desc_kmajor_sw128(a_s + C::kABytes);
 #pragma unroll
     for (int k = 0; k < kSkBK / 16; ++k)
-      tc_mma_f16(d, a_desc + 2u * k, b_desc + 2u * k, idesc, (used > first || k > 0) ? 1u : 0u);
+      tc_mma<Q8>(d, a_desc + 2u * k, b_desc + 2u * k, idesc, (used > first || k > 0) ? 1u : 0u);
     tc_commit(empty(s));
   }
   if (ok) tc_commit(tfull);
@@ -218,11 +236,13 @@ __device__ __forceinline__ void sk_issue(const SkParams& p, uint32_t sbase, uint
   tc_commit(drain_bar);
 }
 
-template <int BN, int DT, int EPI>
+// Q8: A and W' in e4m3 with scales, else 16-bit of type DT.
+template <int BN, int DT, int EPI, bool Q8>
 __global__ void __launch_bounds__(kSkThreads, 1)
 gemm_splitk_kernel(const __grid_constant__ CUtensorMap tmap_b,
                    const __grid_constant__ CUtensorMap tmap_a, const SkParams p) {
   using C = SkCfg<BN>;
+  constexpr int kCols = atom_cols<Q8>();              // columns of one k-block
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_s = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + ((1024u - (raw_s & 1023u)) & 1023u);
@@ -290,8 +310,8 @@ gemm_splitk_kernel(const __grid_constant__ CUtensorMap tmap_b,
         if (!mbar_wait(empty(s), ph ^ 1u, abort_flag, p.err)) { ok = false; break; }
         const uint32_t a_s = sbase + s * C::kStageBytes;
         mbar_arrive_expect_tx(full(s), C::kBBytes + p.a_tx_bytes);
-        tma_load_2d(a_s + C::kABytes, &tmap_b, kb * kSkBK, n_blk * BN, full(s));
-        const int ax = p.a_cols ? run_start_check(cur, p.a_width, p.err) : kb * kSkBK;
+        tma_load_2d(a_s + C::kABytes, &tmap_b, kb * kCols, n_blk * BN, full(s));
+        const int ax = p.a_cols ? run_start_check(cur, p.a_width, p.err) : kb * kCols;
         tma_load_2d(a_s, &tmap_a, ax, m_blk * kSkBM, full(s));
       }
       if (!ok) {
@@ -305,7 +325,7 @@ gemm_splitk_kernel(const __grid_constant__ CUtensorMap tmap_b,
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (even k-blocks)
     if (lane == 0) {
-      sk_issue<BN, DT>(p, sbase, tmem_base, kb1 - kb0, 0, dual ? 2 : 1, full, empty, tfull, drain_bar,
+      sk_issue<BN, DT, Q8>(p, sbase, tmem_base, kb1 - kb0, 0, dual ? 2 : 1, full, empty, tfull, drain_bar,
                        abort_flag);
       // Every MMA (of both issuers) has finished reading shared memory and
       // writing TMEM before the ring is reused as the reduction buffer and
@@ -317,7 +337,7 @@ gemm_splitk_kernel(const __grid_constant__ CUtensorMap tmap_b,
     if (dual && warp == 2) {
       // ---------------------------------------------------------- MMA issuer (odd k-blocks)
       if (lane == 0)
-        sk_issue<BN, DT>(p, sbase, tmem_base + BN, kb1 - kb0, 1, 2, full, empty, tfull, drain_bar,
+        sk_issue<BN, DT, Q8>(p, sbase, tmem_base + BN, kb1 - kb0, 1, 2, full, empty, tfull, drain_bar,
                          abort_flag);
       __syncwarp();
     }
@@ -365,13 +385,13 @@ gemm_splitk_kernel(const __grid_constant__ CUtensorMap tmap_b,
   cluster_sync();                      // every partial tile of the cluster is in shared memory
 
   // ------------------------------------------------------------ reduce-scatter over DSMEM
-  // The residual may come from the previous kernel of the stream.
-  if (p.res) asm volatile("griddepcontrol.wait;" ::: "memory");
+  // The residual and the scales of A may come from the previous kernel of the stream.
+  if (Q8 || p.res) asm volatile("griddepcontrol.wait;" ::: "memory");
   {
     const bool ok = *acc_ok != 0;
-    if (p.split == 8) reduce_slice<8, BN, DT, EPI>(p, smem_u32(smem), rank, m_blk, n_blk, rows_valid, ok);
-    else if (p.split == 4) reduce_slice<4, BN, DT, EPI>(p, smem_u32(smem), rank, m_blk, n_blk, rows_valid, ok);
-    else reduce_slice<2, BN, DT, EPI>(p, smem_u32(smem), rank, m_blk, n_blk, rows_valid, ok);
+    if (p.split == 8) reduce_slice<8, BN, DT, EPI, Q8>(p, smem_u32(smem), rank, m_blk, n_blk, rows_valid, ok);
+    else if (p.split == 4) reduce_slice<4, BN, DT, EPI, Q8>(p, smem_u32(smem), rank, m_blk, n_blk, rows_valid, ok);
+    else reduce_slice<2, BN, DT, EPI, Q8>(p, smem_u32(smem), rank, m_blk, n_blk, rows_valid, ok);
   }
 
   // Every DSMEM read of this thread has completed: its values were stored to y
@@ -385,16 +405,16 @@ gemm_splitk_kernel(const __grid_constant__ CUtensorMap tmap_b,
   }
 }
 
-template <int BN, int DT>
+template <int BN, int DT, bool Q8>
 cudaError_t launch_sk(const CUtensorMap& tb, const CUtensorMap& ta, const SkParams& p,
                       int64_t tiles, cudaStream_t stream) {
   using C = SkCfg<BN>;
   // One instantiation per activation: the reduction loop is unrolled over
   // 16 / S tasks, and runtime-selected activation code in it ran cold in the
   // instruction cache.
-  auto kern = p.epi == GW_EPI_GELU_ERF    ? gemm_splitk_kernel<BN, DT, GW_EPI_GELU_ERF>
-              : p.epi == GW_EPI_GELU_TANH ? gemm_splitk_kernel<BN, DT, GW_EPI_GELU_TANH>
-                                          : gemm_splitk_kernel<BN, DT, GW_EPI_NONE>;
+  auto kern = p.epi == GW_EPI_GELU_ERF    ? gemm_splitk_kernel<BN, DT, GW_EPI_GELU_ERF, Q8>
+              : p.epi == GW_EPI_GELU_TANH ? gemm_splitk_kernel<BN, DT, GW_EPI_GELU_TANH, Q8>
+                                          : gemm_splitk_kernel<BN, DT, GW_EPI_NONE, Q8>;
   cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kern), C::kSmemBytes);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
@@ -424,7 +444,7 @@ struct ClusterTable {
 
 template <int BN>
 int query_active_clusters(int s) {
-  auto kern = gemm_splitk_kernel<BN, GW_DTYPE_F16, GW_EPI_NONE>;
+  auto kern = gemm_splitk_kernel<BN, GW_DTYPE_F16, GW_EPI_NONE, false>;
   constexpr int smem = SkCfg<BN>::kSmemBytes;
   if (ensure_smem_attr(reinterpret_cast<const void*>(kern), smem) != cudaSuccess) return 0;
   cudaLaunchConfig_t cfg = {};
@@ -544,7 +564,7 @@ cudaError_t launch_gemm_splitk(const SplitKPlan& plan, const void* a, int dtype,
                                int64_t K, int64_t lda, const void* w, int64_t N, int64_t ldw,
                                const void* bias, int epilogue, void* y, int64_t ldy,
                                unsigned int* err, cudaStream_t stream, const int64_t* a_cols,
-                               int64_t a_width, const Residual& res) {
+                               int64_t a_width, const Residual& res, const QScale& qs) {
   if (plan.split < 2 || plan.split > 8 || plan.tiles <= 0 || plan.tiles > 65535)
     return cudaErrorInvalidValue;
   SkParams p{};
@@ -555,7 +575,12 @@ cudaError_t launch_gemm_splitk(const SplitKPlan& plan, const void* a, int dtype,
   p.y = static_cast<uint16_t*>(y);
   p.ldy = ldy;
   p.y_vec_ok = ((reinterpret_cast<uintptr_t>(y) & 7u) == 0 && (ldy % 4) == 0) ? 1 : 0;
-  p.num_kb = static_cast<int>((K + kSkBK - 1) / kSkBK);
+  const bool q8 = qs.a != nullptr;
+  if (q8 && (!qs.w || a_cols)) return cudaErrorInvalidValue;
+  const int kb_cols = q8 ? atom_cols<true>() : kSkBK;
+  p.a_scale = qs.a;
+  p.w_scale = qs.w;
+  p.num_kb = static_cast<int>((K + kb_cols - 1) / kb_cols);
   p.m_tiles = static_cast<int>((M + kSkBM - 1) / kSkBM);
   p.split = plan.split;
   p.err = err;
@@ -572,21 +597,21 @@ cudaError_t launch_gemm_splitk(const SplitKPlan& plan, const void* a, int dtype,
   p.a_tx_bytes = a_rows * kSkBK * 2;
 
   CUtensorMap ta, tb;
-  if (!make_tmap_kmajor(&ta, a, M, a_cols ? a_width : K, lda, kSkBK, a_rows))
+  if (!make_tmap_kmajor(&ta, a, M, a_cols ? a_width : K, lda, kb_cols, a_rows, q8 ? 1 : 2))
     return cudaErrorInvalidValue;
-  if (!make_tmap_kmajor(&tb, w, N, K, ldw, kSkBK, plan.bn)) return cudaErrorInvalidValue;
+  if (!make_tmap_kmajor(&tb, w, N, K, ldw, kb_cols, plan.bn, q8 ? 1 : 2)) return cudaErrorInvalidValue;
   const bool bf = dtype == GW_DTYPE_BF16;
+#define GW_SK(BNV, Q)                                                               \
+  (bf ? launch_sk<BNV, GW_DTYPE_BF16, Q>(tb, ta, p, plan.tiles, stream)              \
+      : launch_sk<BNV, GW_DTYPE_F16, Q>(tb, ta, p, plan.tiles, stream))
   switch (plan.bn) {
-    case 256: return bf ? launch_sk<256, GW_DTYPE_BF16>(tb, ta, p, plan.tiles, stream)
-                        : launch_sk<256, GW_DTYPE_F16>(tb, ta, p, plan.tiles, stream);
-    case 128: return bf ? launch_sk<128, GW_DTYPE_BF16>(tb, ta, p, plan.tiles, stream)
-                        : launch_sk<128, GW_DTYPE_F16>(tb, ta, p, plan.tiles, stream);
-    case 64: return bf ? launch_sk<64, GW_DTYPE_BF16>(tb, ta, p, plan.tiles, stream)
-                       : launch_sk<64, GW_DTYPE_F16>(tb, ta, p, plan.tiles, stream);
-    case 32: return bf ? launch_sk<32, GW_DTYPE_BF16>(tb, ta, p, plan.tiles, stream)
-                       : launch_sk<32, GW_DTYPE_F16>(tb, ta, p, plan.tiles, stream);
+    case 256: return q8 ? GW_SK(256, true) : GW_SK(256, false);
+    case 128: return q8 ? GW_SK(128, true) : GW_SK(128, false);
+    case 64: return q8 ? GW_SK(64, true) : GW_SK(64, false);
+    case 32: return q8 ? GW_SK(32, true) : GW_SK(32, false);
     default: return cudaErrorInvalidValue;
   }
+#undef GW_SK
 }
 
 }  // namespace gw

@@ -95,14 +95,19 @@ struct TcParams {
   const int64_t* a_cols;        // kATma: k-block kb of A starts at x column a_cols[64 kb] (or null)
   const uint16_t* res;          // residual (or null), leading dimension ldr
   int64_t ldr;
+  const float* a_scale;         // Q8: scales of A's rows and of W's rows
+  const float* w_scale;
   const int32_t* k_dev;         // kATma: K' on the device (num_kb an upper bound; see device_num_kb)
 };
 
-template <int BN, int DT, int AMODE, int EPI>
+// Q8: A and W in e4m3 with scales (kATma only), else 16-bit of type DT.
+template <int BN, int DT, int AMODE, int EPI, bool Q8>
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_tc_kernel(const __grid_constant__ CUtensorMap tmap_b,
                const __grid_constant__ CUtensorMap tmap_a, const TcParams p) {
   using C = TcCfg<BN>;
+  constexpr int kCols = atom_cols<Q8>();              // columns of one k-block
+  static_assert(!Q8 || AMODE == kATma, "e4m3 operands arrive by TMA");
   extern __shared__ uint8_t smem_raw[];
   // 1024-byte alignment (of the shared-window address) for the swizzled tiles.
   const uint32_t raw_s = smem_u32(smem_raw);
@@ -180,8 +185,8 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmap_b,
             tma_load_2d(b_s, &tmap_b, kb * kBK, n_blk * BN, full_b(s));
           } else {
             mbar_arrive_expect_tx(full_b(s), C::kBBytes + C::kABytes);
-            tma_load_2d(b_s, &tmap_b, kb * kBK, n_blk * BN, full_b(s));
-            const int ax = a_cols ? run_start_check(cur, p.K, p.err) : kb * kBK;
+            tma_load_2d(b_s, &tmap_b, kb * kCols, n_blk * BN, full_b(s));
+            const int ax = a_cols ? run_start_check(cur, p.K, p.err) : kb * kCols;
             tma_load_2d(a_s, &tmap_a, ax, m_blk * kBM, full_b(s));
           }
         }
@@ -196,7 +201,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmap_b,
   } else if (warp == kWarpMma) {
     // ------------------------------------------------------------ MMA issuer
     if (lane == 0) {
-      constexpr uint32_t idesc = idesc_f16(DT == GW_DTYPE_BF16 ? 1u : 0u, kBM, BN);
+      constexpr uint32_t idesc = idesc_for<Q8, DT>(kBM, BN);
       int num_kb = p.num_kb;
       if (AMODE == kATma && p.k_dev) {  // K' written by an earlier kernel: read it after the wait
         asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -221,8 +226,8 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmap_b,
           const uint64_t b_desc = smem_desc_kmajor_sw128(a_s + C::kABytes);
 #pragma unroll
           for (int k = 0; k < kBK / 16; ++k) {
-            // +32 bytes per 16-element k step inside the swizzle atom (>> 4 in the descriptor).
-            tc_mma_f16(d_tmem, a_desc + 2u * k, b_desc + 2u * k, idesc,
+            // +32 bytes per k step (one instruction) inside the swizzle atom (>> 4 in the descriptor).
+            tc_mma<Q8>(d_tmem, a_desc + 2u * k, b_desc + 2u * k, idesc,
                        (kb > 0 || k > 0) ? 1u : 0u);
           }
           tc_commit(empty(s));
@@ -297,13 +302,13 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmap_b,
     // 32-column tcgen05 load is issued before the current one is converted;
     // bias, activation, one packed rounding per pair, 16-byte stores.
     constexpr int kEpiWarps = epi_warps<AMODE>();
-    constexpr int kCols = BN / (kEpiWarps / 4);         // columns per warp
-    constexpr int kSteps = kCols / 32;
+    constexpr int kEpiCols = BN / (kEpiWarps / 4);      // columns per warp
+    constexpr int kSteps = kEpiCols / 32;
     const int q = warp & 3;                       // TMEM lane quarter this warp may access
     const int part = (warp - (AMODE == kATma ? kWarpEpi0Dense : kWarpEpi0)) >> 2;
     const int row_in_tile = q * 32 + lane;
-    // The residual may come from the previous kernel of the stream.
-    if (p.res) asm volatile("griddepcontrol.wait;" ::: "memory");
+    // The residual and the scales of A may come from the previous kernel of the stream.
+    if (Q8 || p.res) asm volatile("griddepcontrol.wait;" ::: "memory");
     uint32_t lt = 0;
     for (int tile = blockIdx.x; tile < p.num_tiles; tile += gridDim.x, ++lt) {
       const int m_blk = tile % p.m_tiles;
@@ -315,8 +320,9 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmap_b,
       const int64_t row = static_cast<int64_t>(m_blk) * kBM + row_in_tile;
       const bool row_ok = row < p.M;
       uint16_t* yrow = p.y + (row_ok ? row * p.ldy : 0);
-      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + b * BN + part * kCols;
-      const int64_t n_warp = static_cast<int64_t>(n_blk) * BN + part * kCols;
+      const float row_scale = Q8 && row_ok ? p.a_scale[row] : 0.0f;
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + b * BN + part * kEpiCols;
+      const int64_t n_warp = static_cast<int64_t>(n_blk) * BN + part * kEpiCols;
       uint32_t acc[32];
       tc_ld_32x32b_x32(t_row, acc);
 #pragma unroll 1
@@ -327,6 +333,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmap_b,
         for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(acc[j]);
         if (c + 1 < kSteps) tc_ld_32x32b_x32(t_row + (c + 1) * 32, acc);
         const int64_t n_base = n_warp + c * 32;
+        if constexpr (Q8) scale32(f, row_scale, p.w_scale, n_base, p.N);
         if (p.bias) add_bias32<DT>(f, p.bias, n_base, p.N);
         activate32<EPI>(f);
         if (row_ok) {
@@ -366,13 +373,13 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmap_b,
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-template <int BN, int DT, int AMODE>
+template <int BN, int DT, int AMODE, bool Q8>
 cudaError_t launch_tc(const CUtensorMap& tb, const CUtensorMap& ta, const TcParams& p,
                       int sm_count, cudaStream_t stream) {
   using C = TcCfg<BN>;
-  auto kern = p.epi == GW_EPI_GELU_ERF    ? gemm_tc_kernel<BN, DT, AMODE, GW_EPI_GELU_ERF>
-              : p.epi == GW_EPI_GELU_TANH ? gemm_tc_kernel<BN, DT, AMODE, GW_EPI_GELU_TANH>
-                                          : gemm_tc_kernel<BN, DT, AMODE, GW_EPI_NONE>;
+  auto kern = p.epi == GW_EPI_GELU_ERF    ? gemm_tc_kernel<BN, DT, AMODE, GW_EPI_GELU_ERF, Q8>
+              : p.epi == GW_EPI_GELU_TANH ? gemm_tc_kernel<BN, DT, AMODE, GW_EPI_GELU_TANH, Q8>
+                                          : gemm_tc_kernel<BN, DT, AMODE, GW_EPI_NONE, Q8>;
   // Opt in to the large dynamic shared-memory carve-out (idempotent, cheap).
   cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kern), C::kSmemBytes);
   if (e != cudaSuccess) return e;
@@ -406,7 +413,7 @@ cudaError_t launch_gemm_tc(int a_mode, const void* x, int dtype, int64_t M, int6
                            const int64_t* idx, int64_t n_alive, const void* bias, int epilogue,
                            void* y, int64_t ldy, unsigned int* err, int sm_count,
                            cudaStream_t stream, const int64_t* a_cols, const int32_t* k_dev,
-                           const Residual& res) {
+                           const Residual& res, const QScale& qs) {
   // Tile width 256 (measured best on B200 where there are several waves:
   // wider tiles reuse A more per byte moved), 128 for narrow N. When 256-wide
   // tiles leave SMs idle in a single wave and 192-wide ones still fit in one
@@ -428,7 +435,10 @@ cudaError_t launch_gemm_tc(int a_mode, const void* x, int dtype, int64_t M, int6
   const int64_t n_tiles = (N + BN - 1) / BN;
   const int64_t num_tiles = m_tiles * n_tiles;
   if (num_tiles > 0x7FFFFFFFll || m_tiles > 0x7FFFFFFFll) return cudaErrorInvalidValue;
-  const int64_t num_kb = (n_alive + kBK - 1) / kBK;
+  const bool q8 = qs.a != nullptr;
+  const int kb_cols = q8 ? atom_cols<true>() : kBK;
+  const int64_t num_kb = (n_alive + kb_cols - 1) / kb_cols;
+  if (q8 && (a_mode != kATma || a_cols || k_dev || !qs.w)) return cudaErrorInvalidValue;
   if (a_mode != kATma && a_mode != kASmemGather) return cudaErrorInvalidValue;
 
   TcParams p{};
@@ -453,22 +463,27 @@ cudaError_t launch_gemm_tc(int a_mode, const void* x, int dtype, int64_t M, int6
   p.k_dev = a_mode == kATma ? k_dev : nullptr;
   p.res = static_cast<const uint16_t*>(res.p);
   p.ldr = res.ld;
+  p.a_scale = qs.a;
+  p.w_scale = qs.w;
   if (p.a_cols && (n_alive % kBK) != 0) return cudaErrorInvalidValue;
 
   CUtensorMap tb, ta;
-  if (!make_tmap_kmajor(&tb, w, N, n_alive, ldw, kBK, BN)) return cudaErrorInvalidValue;
+  if (!make_tmap_kmajor(&tb, w, N, n_alive, ldw, kb_cols, BN, q8 ? 1 : 2)) return cudaErrorInvalidValue;
   if (a_mode == kASmemGather) {
     ta = tb;   // unused by the shared-memory gather variant
   } else if (a_mode == kATma) {
     // A is the compacted x' [M, n_alive], or x [M, K] itself with a_cols.
-    if (!make_tmap_kmajor(&ta, x, M, a_cols ? K : n_alive, ldx, kBK, kBM)) return cudaErrorInvalidValue;
+    if (!make_tmap_kmajor(&ta, x, M, a_cols ? K : n_alive, ldx, kb_cols, kBM, q8 ? 1 : 2))
+      return cudaErrorInvalidValue;
   }
 
 #define GW_TC_MODES(BNV, DTV)                                                                     \
   switch (a_mode) {                                                                              \
-    case kATma: return launch_tc<BNV, DTV, kATma>(tb, ta, p, static_cast<int>(sms), stream);      \
+    case kATma:                                                                                  \
+      return q8 ? launch_tc<BNV, DTV, kATma, true>(tb, ta, p, static_cast<int>(sms), stream)      \
+                : launch_tc<BNV, DTV, kATma, false>(tb, ta, p, static_cast<int>(sms), stream);    \
     default:                                                                                     \
-      return launch_tc<BNV, DTV, kASmemGather>(tb, ta, p, static_cast<int>(sms), stream);        \
+      return launch_tc<BNV, DTV, kASmemGather, false>(tb, ta, p, static_cast<int>(sms), stream); \
   }
   if (BN == 256) {
     if (dtype == GW_DTYPE_BF16) { GW_TC_MODES(256, GW_DTYPE_BF16) }

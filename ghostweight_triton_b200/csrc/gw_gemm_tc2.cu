@@ -102,7 +102,9 @@ struct Tc2Params {
   int64_t ldy;
   const uint16_t* res;      // residual (or null), leading dimension ldr
   int64_t ldr;
-  int num_kb;               // 64-wide k atoms of K
+  const float* a_scale;     // Q8: scales of A's rows and of W's rows
+  const float* w_scale;
+  int num_kb;               // k atoms of K (64 columns of 16 bits, 128 of 8)
   int num_ks;               // stages of kStageK2 per tile
   int m_tiles;
   int n_tiles;
@@ -359,7 +361,8 @@ __device__ __forceinline__ void gather_units(const Tc2Params& p, int e, int lane
   if (__any_sync(0xFFFFFFFFu, bad) && lane == 0) raise_error(p.err, GW_DERR_BAD_INDEX);
 }
 
-template <int BN, int DT, int EPI, bool GATHER>
+// Q8: A and W' in e4m3 with scales, else 16-bit of type DT.
+template <int BN, int DT, int EPI, bool GATHER, bool Q8>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads2, 1)
 gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
                 const __grid_constant__ CUtensorMap tmap_bh,
@@ -367,6 +370,8 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
                 const __grid_constant__ CUtensorMap tmap_y, const Tc2Params p) {
   using C = Tc2Cfg<BN>;
   constexpr int kHalfN = C::kHalfN;
+  constexpr int kCols = atom_cols<Q8>();              // columns of one k atom
+  static_assert(!(Q8 && GATHER), "the in-kernel gather moves 16-bit elements");
   constexpr int kStageBytes2 = C::kStageBytes;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_s = smem_u32(smem_raw);
@@ -499,7 +504,7 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
             if (!ok) break;
           } else {
             for (int a = 0; a < atoms; ++a) {
-              const int kx = (ks * kAtoms2 + a) * kBK2;
+              const int kx = (ks * kAtoms2 + a) * kCols;
               const int ax = p.a_cols ? run_start_check(a == 0 ? cur0 : cur1, p.a_width, p.err) : kx;
               tma_load_2d_pair(a_s + a * kAAtomBytes2, &tmap_a, ax, a_row, leader_full);
               tma_load_2d_pair(b_s + a * C::kBAtomBytes, tb, kx, b_row, leader_full);
@@ -516,8 +521,8 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (leader only)
     if (lane == 0 && rank == 0) {
-      constexpr uint32_t idesc_full = idesc_f16(DT == GW_DTYPE_BF16 ? 1u : 0u, kPairM, BN);
-      constexpr uint32_t idesc_half = idesc_f16(DT == GW_DTYPE_BF16 ? 1u : 0u, kPairM, 128);
+      constexpr uint32_t idesc_full = idesc_for<Q8, DT>(kPairM, BN);
+      constexpr uint32_t idesc_half = idesc_for<Q8, DT>(kPairM, 128);
       int num_kb = p.num_kb;
       if (p.k_dev) {                   // K' written by an earlier kernel: read it after the wait
         asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -545,15 +550,15 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
           const uint64_t b_desc = smem_desc_kmajor_sw128(a_s + kABytes2);
           const bool two = ks * kAtoms2 + 1 < num_kb;
           // Atom 1 of A and of B starts one atom further on (>> 4 in the
-          // descriptor); each 16-wide k step advances 32 bytes inside the atom.
+          // descriptor); each k step (one instruction) advances 32 bytes inside the atom.
 #pragma unroll
           for (int k = 0; k < kBK2 / 16; ++k)
-            tc_mma_f16_pair(d_tmem, a_desc + 2u * k, b_desc + 2u * k, idesc,
+            tc_mma_pair<Q8>(d_tmem, a_desc + 2u * k, b_desc + 2u * k, idesc,
                             (ks > 0 || k > 0) ? 1u : 0u);
           if (two) {
 #pragma unroll
             for (int k = 0; k < kBK2 / 16; ++k)
-              tc_mma_f16_pair(d_tmem, a_desc + (kAAtomBytes2 >> 4) + 2u * k,
+              tc_mma_pair<Q8>(d_tmem, a_desc + (kAAtomBytes2 >> 4) + 2u * k,
                               b_desc + (C::kBAtomBytes >> 4) + 2u * k, idesc, 1u);
           }
           tc_commit_pair_mc(empty(s), 0x3);
@@ -584,8 +589,8 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
       call = *reinterpret_cast<volatile unsigned long long*>(p.ghdr) + 1;
       gather_units<DT>(p, warp - 2, lane, claim_slot, call);
     }
-    // The residual may come from the previous kernel of the stream.
-    if (p.res) asm volatile("griddepcontrol.wait;" ::: "memory");
+    // The residual and the scales of A may come from the previous kernel of the stream.
+    if (Q8 || p.res) asm volatile("griddepcontrol.wait;" ::: "memory");
     uint32_t lt = 0;
     for (int job = pair; job < p.num_jobs; job += num_pairs, ++lt) {
       int m_blk, n_blk, sub;
@@ -598,6 +603,7 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
       const int64_t row = warp_row0 + lane;
       const bool row_ok = row < p.M;
       uint16_t* yrow = p.y + (row_ok ? row * p.ldy : 0);
+      const float row_scale = Q8 && row_ok ? p.a_scale[row] : 0.0f;
       // Whole tile: columns [0, 128) (half 0) or [128, BN) (half 1). Half
       // job: 64 columns each, [0, 64) and [64, 128) of its 128.
       const int col0 = sub < 0 ? half * C::kCols0 : half * 64;
@@ -622,6 +628,7 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
           if (lane == 0) bulk_wait_group_read<0>();
           __syncwarp();
         }
+        if constexpr (Q8) scale32(f, row_scale, p.w_scale, n_base, p.N);
         if (p.bias) add_bias32<DT>(f, p.bias, n_base, p.N);
         activate32<EPI>(f);
         if (p.res && row_ok) {
@@ -802,9 +809,12 @@ cudaError_t launch_tc2_bn(int dtype, Tc2Params& p, const void* a, int64_t M, int
   CUtensorMap ta, tb, tbh, ty;
   // With a_cols, A is x [M, a_width] (K = the alive count, a multiple of 64).
   if (p.a_cols && (K % kBK2) != 0) return cudaErrorInvalidValue;
-  if (!make_tmap_kmajor(&ta, a, M, p.a_cols ? p.a_width : K, lda, kBK2, kHalfM))
+  const bool q8 = p.a_scale != nullptr;
+  const int kb_cols = q8 ? atom_cols<true>() : kBK2;
+  const int eb = q8 ? 1 : 2;
+  if (!make_tmap_kmajor(&ta, a, M, p.a_cols ? p.a_width : K, lda, kb_cols, kHalfM, eb))
     return cudaErrorInvalidValue;
-  if (!make_tmap_kmajor(&tb, w, N, K, ldw, kBK2, C::kHalfN)) return cudaErrorInvalidValue;
+  if (!make_tmap_kmajor(&tb, w, N, K, ldw, kb_cols, C::kHalfN, eb)) return cudaErrorInvalidValue;
   tbh = tb;                  // read only by half jobs (set below)
   // TMA-store epilogue when y's rows are 16-byte aligned (else direct stores).
   p.y_tma = p.y_vec_ok && make_tmap_kmajor(&ty, y, M, N, ldy, kEpiCols, 32) ? 1 : 0;
@@ -820,7 +830,7 @@ cudaError_t launch_tc2_bn(int dtype, Tc2Params& p, const void* a, int64_t M, int
   p.num_jobs = p.num_tiles;
   const int64_t rem = num_tiles % pairs;
   if (BN == 256 && !p.ghdr && pair_tail_split_enabled() && rem > 0 && 2 * rem <= pairs) {
-    if (!make_tmap_kmajor(&tbh, w, N, K, ldw, kBK2, 64)) return cudaErrorInvalidValue;
+    if (!make_tmap_kmajor(&tbh, w, N, K, ldw, kb_cols, 64, eb)) return cudaErrorInvalidValue;
     p.num_full = static_cast<int>(num_tiles - rem);
     p.num_jobs = static_cast<int>(num_tiles + rem);
   }
@@ -835,16 +845,16 @@ cudaError_t launch_tc2_bn(int dtype, Tc2Params& p, const void* a, int64_t M, int
   }
 
   const bool bf = dtype == GW_DTYPE_BF16;
-#define GW_TC2_KERN(G)                                                          \
+#define GW_TC2_KERN(G, Q)                                                       \
   (p.epi == GW_EPI_GELU_ERF                                                     \
-       ? (bf ? gemm_tc2_kernel<BN, GW_DTYPE_BF16, GW_EPI_GELU_ERF, G>           \
-             : gemm_tc2_kernel<BN, GW_DTYPE_F16, GW_EPI_GELU_ERF, G>)           \
+       ? (bf ? gemm_tc2_kernel<BN, GW_DTYPE_BF16, GW_EPI_GELU_ERF, G, Q>        \
+             : gemm_tc2_kernel<BN, GW_DTYPE_F16, GW_EPI_GELU_ERF, G, Q>)        \
    : p.epi == GW_EPI_GELU_TANH                                                  \
-       ? (bf ? gemm_tc2_kernel<BN, GW_DTYPE_BF16, GW_EPI_GELU_TANH, G>          \
-             : gemm_tc2_kernel<BN, GW_DTYPE_F16, GW_EPI_GELU_TANH, G>)          \
-       : (bf ? gemm_tc2_kernel<BN, GW_DTYPE_BF16, GW_EPI_NONE, G>               \
-             : gemm_tc2_kernel<BN, GW_DTYPE_F16, GW_EPI_NONE, G>))
-  auto kern = p.ghdr ? GW_TC2_KERN(true) : GW_TC2_KERN(false);
+       ? (bf ? gemm_tc2_kernel<BN, GW_DTYPE_BF16, GW_EPI_GELU_TANH, G, Q>       \
+             : gemm_tc2_kernel<BN, GW_DTYPE_F16, GW_EPI_GELU_TANH, G, Q>)       \
+       : (bf ? gemm_tc2_kernel<BN, GW_DTYPE_BF16, GW_EPI_NONE, G, Q>            \
+             : gemm_tc2_kernel<BN, GW_DTYPE_F16, GW_EPI_NONE, G, Q>))
+  auto kern = q8 ? GW_TC2_KERN(false, true) : p.ghdr ? GW_TC2_KERN(true, false) : GW_TC2_KERN(false, false);
 #undef GW_TC2_KERN
   cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kern), C::kSmemBytes);
   if (e != cudaSuccess) return e;
@@ -866,7 +876,7 @@ cudaError_t launch_gemm_tc2(const void* a, int dtype, int64_t M, int64_t K, int6
                             void* y, int64_t ldy, unsigned int* err, int sm_count,
                             cudaStream_t stream, void* const* peers, int n_peers,
                             const int64_t* a_cols, int64_t a_width, const int32_t* k_dev,
-                            const Tc2Gather* gather, const Residual& res) {
+                            const Tc2Gather* gather, const Residual& res, const QScale& qs) {
   Tc2Params p{};
   p.M = M;
   p.N = N;
@@ -875,7 +885,11 @@ cudaError_t launch_gemm_tc2(const void* a, int dtype, int64_t M, int64_t K, int6
   p.y = static_cast<uint16_t*>(y);
   p.ldy = ldy;
   p.y_vec_ok = ((reinterpret_cast<uintptr_t>(y) & 15u) == 0 && (ldy % 8) == 0) ? 1 : 0;
-  p.num_kb = static_cast<int>((K + kBK2 - 1) / kBK2);
+  const int kb_cols = qs.a ? atom_cols<true>() : kBK2;
+  if (qs.a && (!qs.w || a_cols || k_dev || gather || n_peers)) return cudaErrorInvalidValue;
+  p.a_scale = qs.a;
+  p.w_scale = qs.w;
+  p.num_kb = static_cast<int>((K + kb_cols - 1) / kb_cols);
   p.num_ks = (p.num_kb + kAtoms2 - 1) / kAtoms2;
   p.err = err;
   if (n_peers < 0 || n_peers > kMaxPeers || (n_peers > 0 && !peers)) return cudaErrorInvalidValue;

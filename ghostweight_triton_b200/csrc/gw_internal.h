@@ -32,6 +32,14 @@ struct Residual {
   int64_t ld = 0;
 };
 
+// e4m3 operands of a GEMM: the scales of a's rows [M] and of W's rows [N] (both
+// null: 16-bit operands). K, lda and ldw then count 8-bit elements, and dtype is
+// the type of y, bias and residual.
+struct QScale {
+  const float* a = nullptr;
+  const float* w = nullptr;
+};
+
 // gw_mask.cu
 size_t mask_workspace_bytes(int64_t cols);
 cudaError_t launch_mask_compact(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld,
@@ -107,7 +115,8 @@ cudaError_t launch_gemm_tc(int a_mode, const void* x, int dtype, int64_t M, int6
                            const int64_t* idx, int64_t n_alive, const void* bias, int epilogue,
                            void* y, int64_t ldy, unsigned int* err, int sm_count,
                            cudaStream_t stream, const int64_t* a_cols = nullptr,
-                           const int32_t* k_dev = nullptr, const Residual& res = {});
+                           const int32_t* k_dev = nullptr, const Residual& res = {},
+                           const QScale& qs = {});
 
 // gw_gemm_tc2.cu: CTA-pair (cta_group::2) tcgen05 GEMM, dense A [M, K] by TMA,
 // 256 x 256 tiles per pair. Chained to the previous kernel by programmatic
@@ -145,7 +154,7 @@ cudaError_t launch_gemm_tc2(const void* a, int dtype, int64_t M, int64_t K, int6
                             cudaStream_t stream, void* const* peers = nullptr, int n_peers = 0,
                             const int64_t* a_cols = nullptr, int64_t a_width = 0,
                             const int32_t* k_dev = nullptr, const Tc2Gather* gather = nullptr,
-                            const Residual& res = {});
+                            const Residual& res = {}, const QScale& qs = {});
 // Whether the CTA-pair kernel serves a dense-A GEMM of this shape.
 bool use_pair_gemm(int64_t M, int64_t N, int sm_count);
 // Tile width (192 or 256) the pair kernel uses for an M x N output.
@@ -173,7 +182,7 @@ cudaError_t launch_gemm_splitk(const SplitKPlan& plan, const void* a, int dtype,
                                const void* bias, int epilogue, void* y, int64_t ldy,
                                unsigned int* err, cudaStream_t stream,
                                const int64_t* a_cols = nullptr, int64_t a_width = 0,
-                               const Residual& res = {});
+                               const Residual& res = {}, const QScale& qs = {});
 
 // gw_gemm_decode.cu: at most 32 rows of A; the MMA runs over 128-feature
 // blocks of W' (M = 128) and all rows of A padded to mp (N = 16 or 32),
@@ -189,7 +198,7 @@ cudaError_t launch_gemm_decode(const DecodePlan& plan, const void* a, int dtype,
                                const void* bias, int epilogue, void* y, int64_t ldy,
                                unsigned int* err, cudaStream_t stream,
                                const int64_t* a_cols = nullptr, int64_t a_width = 0,
-                               const Residual& res = {});
+                               const Residual& res = {}, const QScale& qs = {});
 // Same, with A = x[:, idx] gathered inside the kernel (x [M, K], leading
 // dimension ldx; no alignment requirement on x): one launch, no x' in memory.
 cudaError_t launch_gemm_decode_gather(const DecodePlan& plan, const void* x, int dtype, int64_t M,
@@ -210,9 +219,10 @@ cudaError_t launch_dyn_linear(const void* x, int dtype, int64_t M, int64_t K, in
 
 // Driver entry point for cuTensorMapEncodeTiled (resolved once, no libcuda link).
 void* tensor_map_encoder();
-// 2-D tile map over a [rows, cols] 16-bit row-major matrix with row stride ld
-// (elements): box = box_cols x box_rows, 128-byte swizzle, zero fill outside.
+// 2-D tile map over a [rows, cols] row-major matrix of elements of elem_bytes (2
+// or 1) with row stride ld (elements): box = box_cols x box_rows, 128-byte
+// swizzle, zero fill outside.
 bool make_tmap_kmajor(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld,
-                      int box_cols, int box_rows);
+                      int box_cols, int box_rows, int elem_bytes = 2);
 
 }  // namespace gw

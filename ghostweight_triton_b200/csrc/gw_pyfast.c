@@ -183,6 +183,14 @@ static PyObject* fast_dynamic_linear_residual(PyObject* self, PyObject* const* a
       a[11].p, a[12].l, a[13].p, a[14].l, (int32_t*)a[15].p, (int32_t*)a[16].p, a[17].p));
 }
 
+static PyObject* fast_packed_gemm_q8(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  GW_PARSE("pplllppllpiplpilp")
+  return PyLong_FromLong(gw_packed_gemm_q8(a[0].p, (const float*)a[1].p, a[2].l, a[3].l, a[4].l, a[5].p,
+                                           (const float*)a[6].p, a[7].l, a[8].l, a[9].p, a[10].i,
+                                           a[11].p, a[12].l, a[13].p, a[14].i, a[15].l, a[16].p));
+}
+
 static PyObject* fast_rms_norm(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   (void)self;
   GW_PARSE("pilllplplpdplpllp")
@@ -242,6 +250,7 @@ static PyMethodDef gw_fast_methods[] = {
     GW_FAST(gather_gemm_dev_residual),
     GW_FAST(packed_gemm_residual),
     GW_FAST(dynamic_linear_residual),
+    GW_FAST(packed_gemm_q8),
     GW_FAST(rms_norm),
     GW_FAST(rms_norm_q8),
     GW_FAST(quantize_rows),

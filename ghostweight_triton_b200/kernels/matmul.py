@@ -284,6 +284,64 @@ def packed_linear(
     return y
 
 
+def _q8_operand(what: str, q: torch.Tensor, scale: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """An e4m3 matrix whose rows TMA can load (16-byte aligned; copied into such rows if it
+    is not) and its scales [rows]."""
+    assert q.ndim == 2 and q.is_cuda and q.dtype is torch.float8_e4m3fn, (
+        f"{what} must be a float8_e4m3fn matrix on CUDA, got {q.dtype} {tuple(q.shape)}")
+    assert scale.dtype is torch.float32 and scale.shape == (q.shape[0],) and scale.device == q.device, (
+        f"{what}_scale must be float32 of shape ({q.shape[0]},) on {what}'s device")
+    if (q.shape[1] > 1 and q.stride(1) != 1) or q.data_ptr() % 16 or (
+            q.shape[0] > 1 and (q.stride(0) % 16 or q.stride(0) < q.shape[1])):
+        buf = torch.zeros((q.shape[0], (q.shape[1] + 15) // 16 * 16), dtype=q.dtype, device=q.device)
+        buf[:, : q.shape[1]] = q
+        q = buf[:, : q.shape[1]]
+    return q, scale.contiguous()
+
+
+def packed_linear_q8(
+    a: torch.Tensor,
+    a_scale: torch.Tensor,
+    w_packed: torch.Tensor,
+    w_scale: torch.Tensor,
+    bias: torch.Tensor | None = None,
+    activation: str | None = None,
+    residual: torch.Tensor | None = None,
+    dtype: torch.dtype | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """y = act(a_scale[:, None] * (a @ w_packed^T) * w_scale + bias) + residual in e4m3.
+
+    a [M, K_alive] with a_scale [M] (``rms_norm_q8``, ``quantize_rows``) and
+    w_packed [N, K_alive] with w_scale [N] (``pack_weight_q8``) are
+    float8_e4m3fn with float32 scales; the sum is accumulated and scaled in
+    fp32. ``dtype`` is y's type, float16 or bfloat16 (by default the residual's
+    or the output's, else float16 with a float16 bias, else bfloat16); residual
+    [M, N] has it too, bias is converted to it. ``out`` may be the residual itself.
+    """
+    a, a_scale = _q8_operand("a", a, a_scale)
+    w_packed, w_scale = _q8_operand("w_packed", w_packed, w_scale)
+    assert a.device == w_packed.device, "a and w_packed must be on one device"
+    assert a.shape[1] == w_packed.shape[1], f"K mismatch: a has {a.shape[1]} columns, w_packed {w_packed.shape[1]}"
+    M, N = a.shape[0], w_packed.shape[0]
+    if dtype is None:
+        dtype = next((t.dtype for t in (residual, out) if t is not None),
+                     bias.dtype if bias is not None and bias.dtype is torch.float16 else torch.bfloat16)
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"unsupported output dtype {dtype}; expected float16 or bfloat16")
+    y = torch.empty((M, N), dtype=dtype, device=a.device) if out is None else out
+    assert y.shape == (M, N) and y.dtype is dtype and y.device == a.device, (
+        f"out must be {dtype} of shape {(M, N)} on a's device")
+    if bias is not None:
+        assert bias.shape == (N,) and bias.device == a.device, f"bias must have shape ({N},) on a's device"
+        bias = bias.detach().to(dtype).contiguous()
+    y, residual = _product_out(y, residual, M, N, y)
+    if M and N:
+        _native.packed_gemm_q8(a, a_scale, w_packed, w_scale, y, bias=bias, activation=activation,
+                               residual=residual)
+    return y
+
+
 class _PipeState:
     """Per-device streams, events and x' buffers of ghost_linear_pipelined."""
 

@@ -369,6 +369,25 @@ GW_API int gw_packed_gemm_residual(const void* a, int dtype, int64_t M, int64_t 
                                    int64_t ldy, void* stream);
 
 /*
+ * Dense GEMM over e4m3 operands with a scale per row of each:
+ *   y[m, n] = act( a_scale[m] * w_scale[n] * sum_{j < K} a[m, j] * w_packed[n, j] + bias[n] )
+ *             + residual[m, n]
+ * a [M, K] (lda) and w_packed [N, K] (ldw) hold one byte per element, as
+ * gw_rms_norm_q8 and gw_quantize_rows write them (both 16-byte aligned, lda
+ * and ldw multiples of 16; what lies behind column K is not looked at),
+ * a_scale [M] and w_scale [N] are floats. bias, residual and y are fp16 or
+ * bf16 (dtype), bias and residual may be NULL, residual may be y itself. The
+ * sum is accumulated in fp32 and scaled in fp32; y is rounded once. K = 0
+ * gives act(bias) + residual. As with gw_gather_gemm, w_packed must not be
+ * the output of the GEMM call right before this one on the stream. No
+ * counterpart in the reference, which has no 8-bit types.
+ */
+GW_API int gw_packed_gemm_q8(const void* a, const float* a_scale, int64_t M, int64_t K, int64_t lda,
+                             const void* w_packed, const float* w_scale, int64_t N, int64_t ldw,
+                             const void* bias, int epilogue, const void* residual, int64_t ldr,
+                             void* y, int dtype, int64_t ldy, void* stream);
+
+/*
  * Residual addition and root-mean-square norm of rows, written out over the
  * alive columns of the layer that reads them:
  *   s[m, k] = x[m, k] + residual[m, k]                       (all cols columns)
