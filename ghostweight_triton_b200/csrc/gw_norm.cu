@@ -14,11 +14,10 @@
 // infinity an infinite one (its values then read back as NaN).
 //
 // e4m3 values are taken from u[m, j] = s[m, c_j] g[c_j], from which the norm's
-// factor cancels: y / scale = 448 u / max|u|, computed as (0.875 u) / (max|u| / 512).
-// With 16-bit inputs 0.875 u is mostly exact in fp32 (u has up to 21 bits), so a
-// quotient that lies exactly between two e4m3 values, which 16-bit data meets
-// often, comes out exact and rounds to even; dividing by a rounded scale would
-// send it either way.
+// factor cancels: y / scale = 448 u / max|u|. With 16-bit inputs u is mostly exact
+// in fp32, and quotients that lie exactly between two e4m3 values are common;
+// to_scale brings them out exact, so that they round to even, where dividing by a
+// rounded scale would send them either way.
 //
 // What bounds these kernels is HBM: a row is read and written once. rows_kernel
 // keeps a row in registers (E elements per thread, a warp or a CTA per row),
@@ -34,7 +33,7 @@ namespace gw {
 namespace {
 
 constexpr float kE4m3Max = 448.0f;                 // largest finite e4m3 value
-constexpr float kScaleMin = 1.17549435082e-38f;    // 2^-126: a row of zeros divides by it
+constexpr float kScaleMin = 0x1p-126f;             // a row of zeros divides by it
 
 // Two values rounded to e4m3 (nearest even, saturating, NaN kept): lo in bits 0-7.
 __device__ __forceinline__ uint32_t e4m3_pack2(float lo, float hi) {
@@ -46,22 +45,34 @@ __device__ __forceinline__ uint32_t e4m3_pack2(float lo, float hi) {
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
 // The scale of a row whose largest |u| is umax and whose norm factor is rstd,
-// and the divisor d for which y / scale = 0.875 u / d. NaN compares false and stays.
+// and the two factors that take u to y / scale (448 / umax, in two parts for a
+// tiny umax; rstd and 2^126 where the scale is at its floor: the product alone
+// may leave fp32's range).
 struct RowScale {
-  float scale, d;
+  float scale, m1, m2;
 };
 __device__ __forceinline__ RowScale row_scale(uint32_t umax_bits, float rstd) {
   const float umax = __uint_as_float(umax_bits);
   RowScale q;
-  q.scale = umax * rstd / kE4m3Max;
-  q.d = umax * (1.0f / 512.0f);
+  q.scale = umax * rstd / kE4m3Max;                // NaN compares false and stays
+  q.m2 = umax < 0x1p-64f ? 0x1p64f : 1.0f;
+  q.m1 = kE4m3Max / (umax * q.m2);
   if (q.scale < kScaleMin) {
     q.scale = kScaleMin;
-    q.d = 0.875f * kScaleMin / rstd;
+    q.m1 = rstd;
+    q.m2 = 0x1p126f;
   }
   return q;
 }
-__device__ __forceinline__ float to_scale(float u, float d) { return 0.875f * u / d; }
+// u m1 m2, rounded to 21 significant bits. m1 and the product are each off by at
+// most 2^-24, so a quotient that lies exactly between two e4m3 values (at most 5
+// bits) comes out as such and rounds to even. Splitting by 2^3 + 1 (Dekker)
+// gives the upper bits: three operations instead of a division's dozen.
+__device__ __forceinline__ float to_scale(float u, const RowScale& q) {
+  const float v = u * q.m1 * q.m2;
+  const float c = 9.0f * v;
+  return c - (c - v);
+}
 
 template <bool Q8, int DT> struct RowOut { using raw = typename Elem<DT>::raw; };
 template <int DT> struct RowOut<true, DT> { using raw = uint8_t; };
@@ -125,7 +136,7 @@ __global__ void __launch_bounds__(1024) rows_any_kernel(const RowParams p) {
       const float v = sum_at(c);
       return NORM && g ? v * Elem<DT>::to_f(g[c]) : v;
     };
-    RowScale q8 = {1.0f, 1.0f};
+    RowScale q8 = {1.0f, 1.0f, 1.0f};
     if constexpr (Q8) {
       uint32_t amax = 0;
       float unused = 0.0f;
@@ -136,7 +147,7 @@ __global__ void __launch_bounds__(1024) rows_any_kernel(const RowParams p) {
     }
     for (int64_t j = threadIdx.x; j < p.pad; j += blockDim.x) {
       const float v = j < p.n ? out_at(j) : 0.0f;
-      if constexpr (Q8) y[j] = static_cast<out>(e4m3_pack2(to_scale(v, q8.d), 0.0f));
+      if constexpr (Q8) y[j] = static_cast<out>(e4m3_pack2(to_scale(v, q8), 0.0f));
       else y[j] = Elem<DT>::from_f(v * rstd);
     }
     if (s) {
@@ -148,26 +159,37 @@ __global__ void __launch_bounds__(1024) rows_any_kernel(const RowParams p) {
 }
 
 // ---------------------------------------------------------------------------
-// Rows of up to 32768 columns, read and written once.
+// Rows read and written once.
 // ---------------------------------------------------------------------------
-// A group of G threads (a warp, or the whole CTA) holds a row: E elements per
-// thread, in 16-byte vectors (VEC: element k = (i G + t) V + j of vector i) or
-// one by one (k = i G + t). GATHER passes u = s g through shared memory and
-// picks the alive columns there; the list is kept there too, as 16-bit
-// positions, loaded once for all the rows of a CTA. For the e4m3 scale each
-// thread knows which of its columns the list names (one bit each), so the sum
-// of squares and the largest |u| take one reduction.
-constexpr int kRowsMaxCols = 32768;
+// A group of G threads (a warp for up to 1024 columns, else the CTA) works on a
+// row. One thread copies whole rows of x and r into a ring of stages in shared
+// memory (bulk copies counted on an mbarrier), up to kMaxStages rows ahead, so
+// that loads are in flight while a row is reduced and written. Loading a row
+// when its turn came left HBM idle during the reduction and the output: 34 us
+// instead of RINGUS for 4096 x 4096 fp16 with residual, half of the columns alive.
+//   kVec   rows of 16-byte vectors: thread t takes vectors i G + t of the stage;
+//   kAny   rows of any alignment: the 16-byte granules that hold the row are
+//          copied, thread t takes elements i G + t. Granules that reach past the
+//          matrix (its first and last row) are not copied; those rows are read
+//          from memory.
+//   kLong  rows of vectors too long for the registers: both passes read the stage.
+// In kVec and kAny each thread holds its E elements of u = s g in registers.
+// GATHER passes them through shared memory as fp32 and picks the alive columns
+// there; a thread's positions are the same in every row, so it keeps them in
+// registers too. For the e4m3 scale it knows which of its columns the list names
+// (one bit each), so the sum of squares and the largest |u| take one reduction.
+constexpr int kRowsHeldCols = 16384;               // 1024 threads x 16
+constexpr int kRowsMaxCols = 65535;                // 16-bit positions
+constexpr int kMaxStages = 4;
 constexpr uint32_t kNoColumn = 0xFFFFu;            // zero output (bad index or padding)
+enum RowMode { kVec = 0, kAny = 1, kLong = 2 };
 
-template <int DT>
-__device__ __forceinline__ uint4 ld_row_v4(const void* base, int64_t vec) {
-  // Read once: kept out of L1 (the residual may be written in place, so not the read-only path).
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(static_cast<const uint4*>(base) + vec) : "memory");
-  return v;
+// `bytes` (a multiple of 16, both addresses 16-byte aligned) of this GPU's memory
+// into shared memory, counted as transaction bytes on `bar`.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+      :: "r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
 // One 16-byte vector as floats.
@@ -204,14 +226,32 @@ __device__ __forceinline__ int row_pos(int k, int cols) {
     return k;
 }
 
-template <int DT, bool Q8, bool GATHER, bool VEC, int E, bool WARP, int MAXT>
-__global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, int y_vec) {
+// Shared memory of a CTA: [2][32] partial sums and maxima (512 bytes), mbarriers
+// (groups x kMaxStages), the abort flag, then the ring, the fp32 rows, kLong's
+// positions and (Q8) one bit per column.
+struct RowShared {
+  int stages = 0;            // rows in flight per group
+  int operand_bytes = 0;     // room for one operand of one row
+  int stage_bytes = 0;       // x and r of one row
+  int ring = 0;              // offsets
+  int srow = 0;
+  int spos = 0;
+  int bits = 0;
+  int bytes = 0;
+};
+constexpr int kRowHead = 512 + 4 * kMaxStages * 8 + 64;
+
+template <int DT, bool Q8, bool GATHER, int MODE, int E, bool WARP, int MAXT>
+__global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const RowShared sh, int y_vec) {
   using raw = typename Elem<DT>::raw;
   using out = typename RowOut<Q8, DT>::raw;
+  constexpr bool VEC = MODE != kAny;
   constexpr int V = VEC ? static_cast<int>(16 / sizeof(raw)) : 1;
   constexpr int I = E / V;                                        // vectors (or elements) per thread
   constexpr int kPack = Q8 ? 4 : sizeof(raw) == 2 ? 2 : 1;        // outputs per 4-byte store
-  extern __shared__ __align__(16) uint8_t smem[];
+  constexpr bool STAGED = GATHER && MODE != kLong;                // u passes through shared memory
+  constexpr int kGroupsOut = STAGED ? E / kPack : 1;              // output groups per thread
+  extern __shared__ __align__(128) uint8_t smem[];
   const int G = WARP ? 32 : static_cast<int>(blockDim.x);
   const int t = WARP ? (threadIdx.x & 31) : threadIdx.x;
   const int group = WARP ? (threadIdx.x >> 5) : 0;
@@ -221,36 +261,93 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, int y_vec
   const int pad = static_cast<int>(p.pad);
   float* red_v = reinterpret_cast<float*>(smem);                  // [2][32]
   uint32_t* red_m = reinterpret_cast<uint32_t*>(smem) + 64;       // [2][32]
-  float* srow = reinterpret_cast<float*>(smem + 512) + group * ((cols + 3) & ~3);
-  uint16_t* spos = reinterpret_cast<uint16_t*>(smem + 512 + groups * ((cols + 3) & ~3) * 4);
-  const int npos = (pad + 3) & ~3;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + 512 + 4 * kMaxStages * 8);
+  uint8_t* ring = smem + sh.ring + group * sh.stages * sh.stage_bytes;
+  float* srow = reinterpret_cast<float*>(smem + sh.srow) + group * ((cols + 3) & ~3);
+  uint16_t* spos = reinterpret_cast<uint16_t*>(smem + sh.spos);   // kLong
+  uint32_t* bits = reinterpret_cast<uint32_t*>(smem + sh.bits);   // Q8 and GATHER: one per column
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * groups + group;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * groups;
+  const uint32_t row_bytes = static_cast<uint32_t>(cols * sizeof(raw));
+  const uint32_t bar0 = smem_u32(smem + 512) + static_cast<uint32_t>(group * kMaxStages * 8);
+  const uint32_t ring_s = smem_u32(ring);
 
+  if (t == 0) {
+    for (int s = 0; s < sh.stages; ++s) mbar_init(bar0 + 8u * s, 1);
+    if (group == 0) *abort_flag = 0;
+    mbar_init_fence();
+  }
+  __syncthreads();
   // The inputs may come from the previous kernel of the stream.
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  // kAny: the granules that hold a row, and whether they lie within its matrix.
+  auto granules = [&](const void* base, int64_t ld, int64_t row, uintptr_t& lo, uint32_t& bytes) {
+    const uintptr_t first = reinterpret_cast<uintptr_t>(base);
+    const uintptr_t a = first + static_cast<uintptr_t>(row * ld) * sizeof(raw);
+    const uintptr_t last = first + static_cast<uintptr_t>((p.rows - 1) * ld) * sizeof(raw) + row_bytes;
+    lo = a & ~static_cast<uintptr_t>(15);
+    const uintptr_t hi = (a + row_bytes + 15) & ~static_cast<uintptr_t>(15);
+    bytes = static_cast<uint32_t>(hi - lo);
+    return lo >= first && hi <= last;
+  };
+  auto fetch = [&](int64_t row, int s) {           // one thread: x (and r) of the row into stage s
+    const uint32_t dst = ring_s + static_cast<uint32_t>(s * sh.stage_bytes);
+    const uint32_t bar = bar0 + 8u * s;
+    if constexpr (VEC) {
+      mbar_arrive_expect_tx(bar, p.r ? 2 * row_bytes : row_bytes);
+      bulk_load(dst, static_cast<const raw*>(p.x) + row * p.ldx, row_bytes, bar);
+      if (p.r) bulk_load(dst + sh.operand_bytes, static_cast<const raw*>(p.r) + row * p.ldr, row_bytes, bar);
+    } else {
+      uintptr_t xl, rl = 0;
+      uint32_t xb, rb = 0;
+      if (!granules(p.x, p.ldx, row, xl, xb)) xb = 0;
+      if (!p.r || !granules(p.r, p.ldr, row, rl, rb)) rb = 0;
+      mbar_arrive_expect_tx(bar, xb + rb);
+      if (xb) bulk_load(dst, reinterpret_cast<const void*>(xl), xb, bar);
+      if (rb) bulk_load(dst + sh.operand_bytes, reinterpret_cast<const void*>(rl), rb, bar);
+    }
+  };
+  if (t == 0)
+    for (int s = 0; s < sh.stages && row0 + s * step < p.rows; ++s) fetch(row0 + s * step, s);
+
   uint32_t named = 0xFFFFFFFFu;                                   // this thread's columns in the list
+  uint32_t pos[kGroupsOut * (kPack + 1) / 2];                     // its outputs' positions, two in each
   if constexpr (GATHER) {
-    bool bad = false;
-    uint32_t* bits = reinterpret_cast<uint32_t*>(spos + npos);    // Q8: one bit per column
     if constexpr (Q8) {
       for (int i = threadIdx.x; i < (cols + 31) / 32; i += blockDim.x) bits[i] = 0;
       __syncthreads();
     }
-    for (int j = threadIdx.x; j < npos; j += blockDim.x) {
-      uint32_t pos = kNoColumn;
-      if (j < n) {
-        const int64_t c = __ldg(p.idx + j);
-        if (c < 0 || c >= cols) {
-          bad = true;
+    bool bad = false;
+    auto position = [&](int j) -> uint32_t {
+      if (j >= n) return kNoColumn;
+      const int64_t c = __ldg(p.idx + j);
+      if (c < 0 || c >= cols) {
+        bad = true;
+        return kNoColumn;
+      }
+      if constexpr (Q8) atomicOr(&bits[c >> 5], 1u << (c & 31));
+      return MODE == kLong ? static_cast<uint32_t>(c) : row_pos<DT, VEC>(static_cast<int>(c), cols);
+    };
+    if constexpr (STAGED) {
+#pragma unroll
+      for (int i = 0; i < kGroupsOut; ++i) {
+        uint32_t q[kPack];
+#pragma unroll
+        for (int e = 0; e < kPack; ++e) q[e] = position((i * G + t) * kPack + e);
+        if constexpr (kPack == 1) {
+          if (i & 1) pos[i / 2] |= q[0] << 16;
+          else pos[i / 2] = q[0];
         } else {
-          pos = row_pos<DT, VEC>(static_cast<int>(c), cols);
-          if constexpr (Q8) atomicOr(&bits[c >> 5], 1u << (c & 31));
+#pragma unroll
+          for (int e = 0; e < kPack; e += 2) pos[(i * kPack + e) / 2] = q[e] | (q[e + 1] << 16);
         }
       }
-      spos[j] = static_cast<uint16_t>(pos);
+    } else {
+      for (int j = threadIdx.x; j < ((pad + 3) & ~3); j += blockDim.x) spos[j] = static_cast<uint16_t>(position(j));
     }
     if (bad && blockIdx.x == 0) raise_error(p.err, GW_DERR_BAD_INDEX);
-    __syncthreads();
-    if constexpr (Q8) {
+    if constexpr (Q8 || MODE == kLong) __syncthreads();
+    if constexpr (Q8 && STAGED) {
       named = 0;
 #pragma unroll
       for (int i = 0; i < I; ++i) {
@@ -260,98 +357,103 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, int y_vec
     }
   }
 
-  const int64_t step = static_cast<int64_t>(gridDim.x) * groups;
-  int buf = 0;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * groups + group; row < p.rows; row += step) {
-    const raw* x = static_cast<const raw*>(p.x) + row * p.ldx;
-    const raw* r = static_cast<const raw*>(p.r) + row * p.ldr;
-    raw* sum = static_cast<raw*>(p.s) + row * p.lds;
-    const raw* g = static_cast<const raw*>(p.g);
-    float u[E];
-    if constexpr (VEC) {
-      uint4 xv[I], rv[I];
+  int buf = 0, stage = 0;
+  uint32_t phase = 0;
+  const raw* g = static_cast<const raw*>(p.g);
+  for (int64_t row = row0; row < p.rows; row += step) {
+    raw* sum = p.s ? static_cast<raw*>(p.s) + row * p.lds : nullptr;
+    const uint8_t* xs = ring + stage * sh.stage_bytes;
+    const uint8_t* rs = xs + sh.operand_bytes;
+    // A wait that runs out raises the device error word and the abort flag; the
+    // rest of this CTA's rows are then worked off quickly, with undefined outputs.
+    mbar_wait(bar0 + 8u * stage, phase, abort_flag, p.err);
+    float u[MODE == kLong ? V : E];
+    float ss = 0.0f;
+    uint32_t umax = 0;
+    // Vector v of the row: the sum, rounded to `sum` when WRITE, times g.
+    auto vector = [&](int v, float* f, bool write) {
+      unpack16<DT>(reinterpret_cast<const uint4*>(xs)[v], f);
+      if (p.r) {
+        float q[V];
+        unpack16<DT>(reinterpret_cast<const uint4*>(rs)[v], q);
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[j] += q[j];
+      }
+      if (write) {
+        if (sum) reinterpret_cast<uint4*>(sum)[v] = pack16<DT>(f);
+#pragma unroll
+        for (int j = 0; j < V; ++j) ss = fmaf(f[j], f[j], ss);
+      }
+      if (g) {
+        float q[V];
+        unpack16<DT>(__ldg(reinterpret_cast<const uint4*>(g) + v), q);
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[j] *= q[j];
+      }
+    };
+    if constexpr (MODE == kVec) {
 #pragma unroll
       for (int i = 0; i < I; ++i) {
-        const int k = (i * G + t) * V;
-        xv[i] = k < cols ? ld_row_v4<DT>(x, i * G + t) : make_uint4(0, 0, 0, 0);
-      }
-      if (p.r) {
+        const int v = i * G + t;
+        float* f = u + i * V;
+        if (v * V < cols) {
+          vector(v, f, true);
+          if constexpr (STAGED) {
 #pragma unroll
-        for (int i = 0; i < I; ++i) {
-          const int k = (i * G + t) * V;
-          rv[i] = k < cols ? ld_row_v4<DT>(r, i * G + t) : make_uint4(0, 0, 0, 0);
+            for (int j = 0; j < V; j += 4)
+              *reinterpret_cast<float4*>(srow + row_pos<DT, VEC>(v * V + j, cols)) =
+                  make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; ++j) f[j] = 0.0f;
         }
       }
+      if constexpr (Q8) {
 #pragma unroll
-      for (int i = 0; i < I; ++i) unpack16<DT>(xv[i], u + i * V);
-      if (p.r) {
-#pragma unroll
-        for (int i = 0; i < I; ++i) {
-          float f[V];
-          unpack16<DT>(rv[i], f);
-#pragma unroll
-          for (int j = 0; j < V; ++j) u[i * V + j] += f[j];
-        }
+        for (int e = 0; e < E; ++e)
+          if (!GATHER || ((named >> e) & 1u)) umax = max(umax, abs_bits(u[e]));
       }
-      if (p.s) {
+    } else if constexpr (MODE == kLong) {
+      for (int v = t; v * V < cols; v += G) {
+        vector(v, u, true);
+        if constexpr (Q8) {
+          const uint32_t in = GATHER ? bits[v * V >> 5] >> (v * V & 31) : 0xFFFFFFFFu;
 #pragma unroll
-        for (int i = 0; i < I; ++i)
-          if ((i * G + t) * V < cols) reinterpret_cast<uint4*>(sum)[i * G + t] = pack16<DT>(u + i * V);
+          for (int j = 0; j < V; ++j)
+            if ((in >> j) & 1u) umax = max(umax, abs_bits(u[j]));
+        }
       }
     } else {
+      uintptr_t lo;
+      uint32_t bytes;
+      // Generic pointers: into the stage, or (first and last row) into memory.
+      const raw* x = static_cast<const raw*>(p.x) + row * p.ldx;
+      if (granules(p.x, p.ldx, row, lo, bytes)) x = reinterpret_cast<const raw*>(xs + (reinterpret_cast<uintptr_t>(x) & 15u));
+      const raw* r = nullptr;
+      if (p.r) {
+        r = static_cast<const raw*>(p.r) + row * p.ldr;
+        if (granules(p.r, p.ldr, row, lo, bytes)) r = reinterpret_cast<const raw*>(rs + (reinterpret_cast<uintptr_t>(r) & 15u));
+      }
 #pragma unroll
       for (int i = 0; i < I; ++i) {
         const int k = i * G + t;
-        u[i] = k < cols ? Elem<DT>::to_f(x[k]) : 0.0f;
-      }
-      if (p.r) {
-#pragma unroll
-        for (int i = 0; i < I; ++i)
-          if (i * G + t < cols) u[i] += Elem<DT>::to_f(r[i * G + t]);
-      }
-      if (p.s) {
-#pragma unroll
-        for (int i = 0; i < I; ++i)
-          if (i * G + t < cols) sum[i * G + t] = Elem<DT>::from_f(u[i]);
-      }
-    }
-    float ss = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) ss = fmaf(u[e], u[e], ss);
-    if (g) {
-#pragma unroll
-      for (int i = 0; i < I; ++i) {
-        const int k = (i * G + t) * V;
+        u[i] = 0.0f;
         if (k < cols) {
-          if constexpr (VEC) {
-            float f[V];
-            unpack16<DT>(__ldg(reinterpret_cast<const uint4*>(g) + i * G + t), f);
-#pragma unroll
-            for (int j = 0; j < V; ++j) u[i * V + j] *= f[j];
-          } else {
-            u[i] *= Elem<DT>::to_f(__ldg(g + k));
-          }
+          u[i] = Elem<DT>::to_f(x[k]);
+          if (r) u[i] += Elem<DT>::to_f(r[k]);
         }
       }
-    }
-    uint32_t umax = 0;
-    if constexpr (Q8) {
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (!GATHER || ((named >> e) & 1u)) umax = max(umax, abs_bits(u[e]));
-    }
-    if constexpr (GATHER) {
 #pragma unroll
       for (int i = 0; i < I; ++i) {
-        const int k = (i * G + t) * V;
+        const int k = i * G + t;
         if (k < cols) {
-          if constexpr (VEC) {
-#pragma unroll
-            for (int j = 0; j < V; j += 4)
-              *reinterpret_cast<float4*>(srow + row_pos<DT, VEC>(k + j, cols)) =
-                  make_float4(u[i * V + j], u[i * V + j + 1], u[i * V + j + 2], u[i * V + j + 3]);
-          } else {
-            srow[k] = u[i];
+          if (sum) sum[k] = Elem<DT>::from_f(u[i]);
+          ss = fmaf(u[i], u[i], ss);
+          if (g) u[i] *= Elem<DT>::to_f(__ldg(g + k));
+          if constexpr (STAGED) srow[k] = u[i];
+          if constexpr (Q8) {
+            if (!GATHER || ((named >> i) & 1u)) umax = max(umax, abs_bits(u[i]));
           }
         }
       }
@@ -369,6 +471,18 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, int y_vec
         red_m[buf * 32 + (t >> 5)] = umax;
       }
       __syncthreads();
+    }
+    auto refill = [&] {                              // every thread is done with the stage
+      const int64_t next = row + sh.stages * step;
+      if (t == 0 && next < p.rows && !*abort_flag) fetch(next, stage);
+      if (++stage == sh.stages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    };
+    if constexpr (MODE != kLong) refill();
+    if constexpr (!WARP) {
+      const int lane = t & 31;
       const bool in = lane < (G >> 5);
       ss = in ? red_v[buf * 32 + lane] : 0.0f;
 #pragma unroll
@@ -377,116 +491,189 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, int y_vec
       buf ^= 1;
     }
     const float rstd = p.norm ? rsqrtf(ss / static_cast<float>(cols) + p.eps) : 1.0f;
-    RowScale q8 = {1.0f, 1.0f};
+    RowScale q8 = {1.0f, 1.0f, 1.0f};
     if constexpr (Q8) {
       q8 = row_scale(umax, rstd);
       if (t == 0) p.scale[row] = q8.scale;
     }
     out* y = static_cast<out*>(p.y) + row * p.ldy;
-    auto value = [&](float v) { return Q8 ? to_scale(v, q8.d) : v * rstd; };
+    auto value = [&](float v) { return Q8 ? to_scale(v, q8) : v * rstd; };
     auto store1 = [&](int j, float v) {
       if constexpr (Q8) y[j] = static_cast<out>(e4m3_pack2(v, 0.0f));
       else y[j] = Elem<DT>::from_f(v);
     };
-    if constexpr (GATHER) {
+    auto store_pack = [&](int j, const float* v) {   // outputs j .. j + kPack - 1, up to pad
+      if (y_vec && j + kPack <= pad) {
+        uint32_t w;
+        if constexpr (Q8) w = e4m3_pack2(v[0], v[1]) | (e4m3_pack2(v[2], v[3]) << 16);
+        else if constexpr (kPack == 2) w = Elem<DT>::pack2(v[0], v[1]);
+        else w = __float_as_uint(v[0]);
+        *reinterpret_cast<uint32_t*>(y + j) = w;
+      } else {
+#pragma unroll
+        for (int q = 0; q < kPack; ++q)
+          if (j + q < pad) store1(j + q, v[q]);
+      }
+    };
+    auto store_vector = [&](int k, float* f) {       // outputs k .. k + V - 1 (aligned)
+#pragma unroll
+      for (int j = 0; j < V; ++j) f[j] = value(f[j]);
+      if constexpr (!VEC) {
+        store1(k, f[0]);
+      } else if constexpr (!Q8) {
+        *reinterpret_cast<uint4*>(y + k) = pack16<DT>(f);
+      } else {
+        const uint32_t lo = e4m3_pack2(f[0], f[1]) | (e4m3_pack2(f[2], f[3]) << 16);
+        if constexpr (V == 8) {
+          const uint32_t hi = e4m3_pack2(f[4], f[5]) | (e4m3_pack2(f[6], f[7]) << 16);
+          *reinterpret_cast<uint2*>(y + k) = make_uint2(lo, hi);
+        } else {
+          *reinterpret_cast<uint32_t*>(y + k) = lo;
+        }
+      }
+    };
+    if constexpr (STAGED) {
       // Neighbouring threads take neighbouring groups of outputs: 4-byte
       // stores, and shared-memory reads within a narrow window of the row.
-      for (int j = t * kPack; j < pad; j += G * kPack) {
-        float v[kPack];
-        uint16_t pos[kPack];
-        if constexpr (kPack == 4) *reinterpret_cast<uint2*>(pos) = *reinterpret_cast<const uint2*>(spos + j);
-        else if constexpr (kPack == 2) *reinterpret_cast<uint32_t*>(pos) = *reinterpret_cast<const uint32_t*>(spos + j);
-        else pos[0] = spos[j];
 #pragma unroll
-        for (int q = 0; q < kPack; ++q) v[q] = pos[q] == kNoColumn ? 0.0f : value(srow[pos[q]]);
-        if (y_vec && j + kPack <= pad) {
-          uint32_t w;
-          if constexpr (Q8) w = e4m3_pack2(v[0], v[1]) | (e4m3_pack2(v[2], v[3]) << 16);
-          else if constexpr (kPack == 2) w = Elem<DT>::pack2(v[0], v[1]);
-          else w = __float_as_uint(v[0]);
-          *reinterpret_cast<uint32_t*>(y + j) = w;
-        } else {
+      for (int i = 0; i < kGroupsOut; ++i) {
+        const int j = (i * G + t) * kPack;
+        if (j < pad) {
+          float v[kPack];
 #pragma unroll
-          for (int q = 0; q < kPack; ++q)
-            if (j + q < pad) store1(j + q, v[q]);
+          for (int e = 0; e < kPack; ++e) {
+            const int at = i * kPack + e;
+            const uint32_t c = (at & 1) ? pos[at / 2] >> 16 : pos[at / 2] & 0xFFFFu;
+            v[e] = c == kNoColumn ? 0.0f : value(srow[c]);
+          }
+          store_pack(j, v);
         }
       }
       // The next row overwrites srow.
       if constexpr (WARP) __syncwarp();
       else __syncthreads();
-    } else {
+    } else if constexpr (MODE == kLong && GATHER) {
+      const raw* x = reinterpret_cast<const raw*>(xs);
+      const raw* r = reinterpret_cast<const raw*>(rs);
+      for (int j = t * kPack; j < pad; j += G * kPack) {
+        float v[kPack];
 #pragma unroll
-      for (int i = 0; i < I; ++i) {
-        const int k = (i * G + t) * V;
-        if (k < cols) {
-#pragma unroll
-          for (int j = 0; j < V; ++j) u[i * V + j] = value(u[i * V + j]);
-          if constexpr (!VEC) {
-            store1(k, u[i]);
-          } else if constexpr (!Q8) {
-            *reinterpret_cast<uint4*>(y + k) = pack16<DT>(u + i * V);
-          } else {
-            const float* f = u + i * V;
-            const uint32_t lo = e4m3_pack2(f[0], f[1]) | (e4m3_pack2(f[2], f[3]) << 16);
-            if constexpr (V == 8) {
-              const uint32_t hi = e4m3_pack2(f[4], f[5]) | (e4m3_pack2(f[6], f[7]) << 16);
-              *reinterpret_cast<uint2*>(y + k) = make_uint2(lo, hi);
-            } else {
-              *reinterpret_cast<uint32_t*>(y + k) = lo;
-            }
+        for (int e = 0; e < kPack; ++e) {
+          const uint32_t c = spos[j + e];
+          v[e] = 0.0f;
+          if (c != kNoColumn) {
+            float f = Elem<DT>::to_f(x[c]);
+            if (p.r) f += Elem<DT>::to_f(r[c]);
+            if (g) f *= Elem<DT>::to_f(__ldg(g + c));
+            v[e] = value(f);
           }
         }
+        store_pack(j, v);
+      }
+      __syncthreads();
+      refill();
+    } else {
+      if constexpr (MODE == kLong) {
+        for (int v = t; v * V < cols; v += G) {
+          vector(v, u, false);
+          store_vector(v * V, u);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+          if ((i * G + t) * V < cols) store_vector((i * G + t) * V, u + i * V);
       }
       for (int j = n + t; j < pad; j += G) y[j] = 0;
+      if constexpr (MODE == kLong) {
+        __syncthreads();
+        refill();
+      }
     }
   }
+  // After a wait that ran out, copies may still be on their way into this CTA's
+  // shared memory: wait (bounded) for either phase of every stage once more.
+  if (t == 0 && *abort_flag)
+    for (int s = 0; s < sh.stages; ++s) {
+      mbar_wait(bar0 + 8u * s, 0u, nullptr, p.err, 100000000ull);
+      mbar_wait(bar0 + 8u * s, 1u, nullptr, p.err, 100000000ull);
+    }
 }
 
-template <int DT, bool Q8, bool GATHER, bool VEC, int E, bool WARP, int MAXT>
+template <int DT, bool Q8, bool GATHER, int MODE, int E, bool WARP, int MAXT>
 cudaError_t launch_rows_variant(const RowParams& p, int y_vec, int sm_count, cudaStream_t stream) {
-  auto kern = rows_kernel<DT, Q8, GATHER, VEC, E, WARP, MAXT>;
-  const int cols4 = static_cast<int>((p.cols + 3) & ~int64_t{3});
-  const int warps = WARP ? 4 : static_cast<int>((p.cols + 32 * E - 1) / (32 * E));
+  auto kern = rows_kernel<DT, Q8, GATHER, MODE, E, WARP, MAXT>;
+  constexpr int kSmemLimit = 232448;
+  const int cols = static_cast<int>(p.cols);
+  const int cols4 = (cols + 3) & ~3;
   const int groups = WARP ? 4 : 1;
-  const int npos = static_cast<int>((p.pad + 3) & ~int64_t{3});
-  int smem = 512;
-  if (GATHER) smem += groups * cols4 * 4 + npos * 2 + (Q8 ? (cols4 + 31) / 32 * 4 : 0);
-  if (smem > 232448) return cudaErrorInvalidValue;
+  const int warps = WARP ? groups : std::min(32, (cols + 32 * E - 1) / (32 * E));
+  const int threads = warps * 32;
+  // A thread's outputs are counted at compile time (kLong loops).
+  if (MODE != kLong && p.pad > static_cast<int64_t>(WARP ? 32 : threads) * E) return cudaErrorNotSupported;
+  const int npos = MODE == kLong && GATHER ? static_cast<int>((p.pad + 3) & ~int64_t{3}) : 0;
+  const bool staged = GATHER && MODE != kLong;
+  RowShared sh;
+  const int fixed = kRowHead + (staged ? groups * cols4 * 4 : 0) + npos * 2 +
+                    (GATHER && Q8 ? (cols4 + 31) / 32 * 4 : 0);
+  sh.operand_bytes = (cols * (DT == GW_DTYPE_F32 ? 4 : 2) + 15) / 16 * 16 + (MODE == kAny ? 16 : 0);
+  sh.stage_bytes = sh.operand_bytes * (p.r ? 2 : 1);
+  // As many CTAs as make 1024 threads per SM, each with up to four rows in
+  // flight; fewer CTAs where two rows each would not fit.
+  int per_sm = std::max(1, 1024 / threads);
+  for (;; per_sm = (per_sm + 1) / 2) {
+    sh.stages = ((kSmemLimit + 1024) / per_sm - 1024 - fixed) / (groups * sh.stage_bytes);
+    if (sh.stages >= 2 || per_sm == 1) break;
+  }
+  if (sh.stages < 1) return cudaErrorNotSupported;
+  sh.stages = std::min(sh.stages, kMaxStages);
+  sh.ring = kRowHead;
+  sh.srow = sh.ring + groups * sh.stages * sh.stage_bytes;
+  sh.spos = sh.srow + (staged ? groups * cols4 * 4 : 0);
+  sh.bits = sh.spos + npos * 2;
+  sh.bytes = fixed + groups * sh.stages * sh.stage_bytes;
   cudaError_t e = cudaSuccess;
-  if (smem > 48 * 1024) {
-    e = ensure_smem_attr(reinterpret_cast<const void*>(kern), 232448);
+  if (sh.bytes > 48 * 1024) {
+    e = ensure_smem_attr(reinterpret_cast<const void*>(kern), kSmemLimit);
     if (e != cudaSuccess) return e;
   }
-  // As many CTAs as the SMs can hold by threads and shared memory; each takes
-  // rows in steps of the grid, so the list is loaded once per CTA.
-  const int64_t per_sm = std::max(1, std::min(2048 / (warps * 32), 232448 / (smem + 1024)));
-  const int64_t grid = std::min<int64_t>((p.rows + groups - 1) / groups, per_sm * sm_count);
+  // Each CTA takes rows in steps of the grid, so the list is loaded once per CTA.
+  const int64_t grid = std::min<int64_t>((p.rows + groups - 1) / groups, static_cast<int64_t>(per_sm) * sm_count);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
-  cfg.blockDim = dim3(static_cast<unsigned>(warps * 32));
-  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = static_cast<size_t>(sh.bytes);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, p, y_vec);
+  return cudaLaunchKernelEx(&cfg, kern, p, sh, y_vec);
 }
 
-template <int DT, bool Q8, bool GATHER, bool VEC>
-cudaError_t launch_rows_fast(const RowParams& p, int y_vec, int sm_count, cudaStream_t stream) {
-  if (p.cols <= 256) return launch_rows_variant<DT, Q8, GATHER, VEC, 8, true, 128>(p, y_vec, sm_count, stream);
-  if (p.cols <= 1024) return launch_rows_variant<DT, Q8, GATHER, VEC, 32, true, 128>(p, y_vec, sm_count, stream);
-  if (p.cols <= 8192) return launch_rows_variant<DT, Q8, GATHER, VEC, 16, false, 512>(p, y_vec, sm_count, stream);
-  return launch_rows_variant<DT, Q8, GATHER, VEC, 32, false, 1024>(p, y_vec, sm_count, stream);
+template <int DT, bool Q8, bool GATHER>
+cudaError_t launch_rows_held(const RowParams& p, bool vec, int y_vec, int sm_count, cudaStream_t stream) {
+  if (vec) {
+    if (p.cols <= 256) return launch_rows_variant<DT, Q8, GATHER, kVec, 8, true, 128>(p, y_vec, sm_count, stream);
+    if (p.cols <= 1024) return launch_rows_variant<DT, Q8, GATHER, kVec, 32, true, 128>(p, y_vec, sm_count, stream);
+    cudaError_t e = cudaErrorNotSupported;
+    if (p.cols <= kRowsHeldCols)
+      e = launch_rows_variant<DT, Q8, GATHER, kVec, 16, false, 1024>(p, y_vec, sm_count, stream);
+    if (e != cudaErrorNotSupported) return e;
+    return launch_rows_variant<DT, Q8, GATHER, kLong, 16, false, 1024>(p, y_vec, sm_count, stream);
+  }
+  if (p.cols <= 256) return launch_rows_variant<DT, Q8, GATHER, kAny, 8, true, 128>(p, y_vec, sm_count, stream);
+  if (p.cols <= kRowsHeldCols)
+    return launch_rows_variant<DT, Q8, GATHER, kAny, 16, false, 1024>(p, y_vec, sm_count, stream);
+  return cudaErrorNotSupported;
 }
 
 // The rows_kernel for these operands, or cudaErrorNotSupported where only
-// rows_any_kernel takes them: longer rows, lists longer than the row.
+// rows_any_kernel takes them: rows too long for a stage (or too long and not
+// aligned), lists longer than the row.
 template <int DT, bool Q8>
-cudaError_t launch_rows_held(const RowParams& p, int sm_count, cudaStream_t stream) {
-  if (p.cols < 1 || p.cols > kRowsMaxCols || p.n > p.cols || p.pad > p.cols + 128) return cudaErrorNotSupported;
+cudaError_t launch_rows_once(const RowParams& p, int sm_count, cudaStream_t stream) {
+  if (p.cols < 1 || p.cols > kRowsMaxCols || p.n > p.cols) return cudaErrorNotSupported;
   constexpr int eb = DT == GW_DTYPE_F32 ? 4 : 2;
   constexpr int V = 16 / eb;
   const int ob = Q8 ? 1 : eb;                      // bytes of an output
@@ -498,16 +685,13 @@ cudaError_t launch_rows_held(const RowParams& p, int sm_count, cudaStream_t stre
              aligned(p.s, p.lds, 16, eb) && aligned(p.g, 0, 16, eb);
   if (!gather) vec = vec && aligned(p.y, p.ldy, V * ob, ob);
   const int y_vec = aligned(p.y, p.ldy, 4, ob) ? 1 : 0;
-  if (gather)
-    return vec ? launch_rows_fast<DT, Q8, true, true>(p, y_vec, sm_count, stream)
-               : launch_rows_fast<DT, Q8, true, false>(p, y_vec, sm_count, stream);
-  return vec ? launch_rows_fast<DT, Q8, false, true>(p, y_vec, sm_count, stream)
-             : launch_rows_fast<DT, Q8, false, false>(p, y_vec, sm_count, stream);
+  return gather ? launch_rows_held<DT, Q8, true>(p, vec, y_vec, sm_count, stream)
+                : launch_rows_held<DT, Q8, false>(p, vec, y_vec, sm_count, stream);
 }
 
 template <int DT, bool Q8, bool NORM>
 cudaError_t launch_rows_dt1(const RowParams& p, int sm_count, cudaStream_t stream) {
-  const cudaError_t e = launch_rows_held<DT, Q8>(p, sm_count, stream);
+  const cudaError_t e = launch_rows_once<DT, Q8>(p, sm_count, stream);
   if (e != cudaErrorNotSupported) return e;
   const int64_t width = std::max<int64_t>(p.cols, p.pad);
   const int threads = width <= 1024 ? 128 : width <= 8192 ? 256 : 1024;

@@ -16,6 +16,8 @@ rounded up. e4m3 halves a step of 2^-3 (2^-4 of the value), or 2^-10 below
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -83,14 +85,15 @@ def close(got, want, dtype, extra):
     assert bool((err <= bound).all()), f"off by {(err / bound).max().item():.3g} of the bound"
 
 
-def close_q8(q, scale, want, extra):
+def close_q8(q, scale, want, extra, tiny=0.0):
+    """`tiny`: what a product of fp32 subnormals may be off by, absolutely."""
     want_scale = (want.abs().amax(-1) / 448).clamp_min(2.0 ** -126) if want.shape[-1] else \
         torch.full(want.shape[:-1], 2.0 ** -126, dtype=torch.float64, device=want.device)
     assert q.dtype is torch.float8_e4m3fn and scale.dtype is torch.float32
     assert q.shape == want.shape and scale.shape == want.shape[:-1]
-    assert bool(((scale.double() - want_scale).abs() <= want_scale * (extra + 2.0 ** -23)).all())
+    assert bool(((scale.double() - want_scale).abs() <= want_scale * (extra + 2.0 ** -23) + tiny / 448).all())
     s = scale.double().unsqueeze(-1)
-    bound = torch.maximum(want.abs() / 16, s / 1024) + want.abs() * 2 * (extra + 2.0 ** -23)
+    bound = torch.maximum(want.abs() / 16, s / 1024) + want.abs() * 2 * (extra + 2.0 ** -23) + 2 * tiny
     err = (q.float().double() * s - want).abs()
     assert bool((err <= bound).all()), f"off by {(err / bound).max().item():.3g} of the bound"
 
@@ -291,6 +294,21 @@ def test_large_values_saturate_nothing():
         q, scale = quantize_rows(x)
         assert (q[:, 0].float() == -448).all()
         close_q8(q, scale, x.double(), 0.0)
+
+
+@pytest.mark.parametrize("K", [96, 2000])
+def test_tiny_rows_q8(K):
+    """Rows down to the subnormals: the factors between them and e4m3 stay within fp32.
+
+    The product of x with the weight rounds to a multiple of 2^-149 there, so it is off by up
+    to 2^-150, which the norm's factor (at most 1 / sqrt(eps)) enlarges."""
+    _, _, w = make(1, K, torch.float32, 14, residual=False)
+    x = torch.randn(12, K, device="cuda", generator=gen(15))
+    x *= torch.logspace(-44, -33, 12, device="cuda")[:, None]
+    q, scale = rms_norm_q8(x, w, EPS)
+    close_q8(q, scale, reference(x, None, w, None)[0], slack(K) + 2.0 ** -20, 2.0 ** -150 / math.sqrt(EPS))
+    q, scale = quantize_rows(x)
+    close_q8(q, scale, x.double(), 2.0 ** -20)
 
 
 def test_bad_indices():
