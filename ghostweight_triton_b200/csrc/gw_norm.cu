@@ -24,6 +24,7 @@
 // and passes it through shared memory only to pick alive columns from it;
 // rows_any_kernel takes what that one does not.
 #include <algorithm>
+#include <type_traits>
 
 #include "gw_common.cuh"
 #include "gw_internal.h"
@@ -175,13 +176,52 @@ __global__ void __launch_bounds__(1024) rows_any_kernel(const RowParams p) {
 //   kLong  rows of vectors too long for the registers: both passes read the stage.
 // In kVec and kAny each thread holds its E elements of u = s g in registers.
 // GATHER passes them through shared memory as fp32 and picks the alive columns
-// there; a thread's positions are the same in every row, so it keeps them in
-// registers too. For the e4m3 scale it knows which of its columns the list names
-// (one bit each), so the sum of squares and the largest |u| take one reduction.
+// there, through a table of 16-bit places that a CTA makes from the list once for
+// all its rows (kept in registers instead, the places and the weight behind them
+// took every thread's share of the list to set up: 24 us instead of N768US for
+// 8192 x 768 fp16, where a warp has three rows). For the e4m3 scale a thread
+// knows which of its columns the list names (one bit each), so the sum of squares
+// and the largest |u| take one reduction.
 constexpr int kRowsHeldCols = 16384;               // 1024 threads x 16
 constexpr int kRowsMaxCols = 65535;                // 16-bit positions
 constexpr int kMaxStages = 4;
 constexpr uint32_t kNoColumn = 0xFFFFu;            // zero output (bad index or padding)
+// The two 16-bit values of a word as floats.
+template <int DT>
+__device__ __forceinline__ float lo_f(uint32_t w) {
+  if constexpr (DT == GW_DTYPE_F16) return __low2float(*reinterpret_cast<const __half2*>(&w));
+  return __uint_as_float(w << 16);
+}
+template <int DT>
+__device__ __forceinline__ float hi_f(uint32_t w) {
+  if constexpr (DT == GW_DTYPE_F16) return __high2float(*reinterpret_cast<const __half2*>(&w));
+  return __uint_as_float(w & 0xFFFF0000u);
+}
+// Values of type DT kept in registers: two 16-bit ones in each.
+template <int DT, int N>
+struct Held {
+  static constexpr int kWords = DT == GW_DTYPE_F32 ? N : (N + 1) / 2;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0u;
+  }
+  // After clear(); i known at compile time, each once.
+  __device__ __forceinline__ void set(int i, typename Elem<DT>::raw v) {
+    if constexpr (DT == GW_DTYPE_F32) w[i] = v;
+    else w[i / 2] |= static_cast<uint32_t>(v) << (16 * (i & 1));
+  }
+  __device__ __forceinline__ void set16(int v, const uint4 q) {    // 16 bytes from value 16 / size * v on
+    w[4 * v] = q.x;
+    w[4 * v + 1] = q.y;
+    w[4 * v + 2] = q.z;
+    w[4 * v + 3] = q.w;
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (DT == GW_DTYPE_F32) return __uint_as_float(w[i]);
+    else return (i & 1) ? hi_f<DT>(w[i / 2]) : lo_f<DT>(w[i / 2]);
+  }
+};
 enum RowMode { kVec = 0, kAny = 1, kLong = 2 };
 
 // `bytes` (a multiple of 16, both addresses 16-byte aligned) of this GPU's memory
@@ -201,8 +241,8 @@ __device__ __forceinline__ void unpack16(const uint4 q, float* f) {
     if constexpr (DT == GW_DTYPE_F32) {
       f[i] = __uint_as_float(w[i]);
     } else {
-      f[2 * i] = Elem<DT>::to_f(static_cast<uint16_t>(w[i] & 0xFFFFu));
-      f[2 * i + 1] = Elem<DT>::to_f(static_cast<uint16_t>(w[i] >> 16));
+      f[2 * i] = lo_f<DT>(w[i]);
+      f[2 * i + 1] = hi_f<DT>(w[i]);
     }
   }
 }
@@ -227,8 +267,8 @@ __device__ __forceinline__ int row_pos(int k, int cols) {
 }
 
 // Shared memory of a CTA: [2][32] partial sums and maxima (512 bytes), mbarriers
-// (groups x kMaxStages), the abort flag, then the ring, the fp32 rows, kLong's
-// positions and (Q8) one bit per column.
+// (groups x kMaxStages), the abort flag, then the ring, the fp32 rows, the list's
+// places and (Q8) one bit per column.
 struct RowShared {
   int stages = 0;            // rows in flight per group
   int operand_bytes = 0;     // room for one operand of one row
@@ -250,7 +290,6 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
   constexpr int I = E / V;                                        // vectors (or elements) per thread
   constexpr int kPack = Q8 ? 4 : sizeof(raw) == 2 ? 2 : 1;        // outputs per 4-byte store
   constexpr bool STAGED = GATHER && MODE != kLong;                // u passes through shared memory
-  constexpr int kGroupsOut = STAGED ? E / kPack : 1;              // output groups per thread
   extern __shared__ __align__(128) uint8_t smem[];
   const int G = WARP ? 32 : static_cast<int>(blockDim.x);
   const int t = WARP ? (threadIdx.x & 31) : threadIdx.x;
@@ -264,7 +303,7 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + 512 + 4 * kMaxStages * 8);
   uint8_t* ring = smem + sh.ring + group * sh.stages * sh.stage_bytes;
   float* srow = reinterpret_cast<float*>(smem + sh.srow) + group * ((cols + 3) & ~3);
-  uint16_t* spos = reinterpret_cast<uint16_t*>(smem + sh.spos);   // kLong
+  uint16_t* spos = reinterpret_cast<uint16_t*>(smem + sh.spos);   // srow bytes, or kLong: columns
   uint32_t* bits = reinterpret_cast<uint32_t*>(smem + sh.bits);   // Q8 and GATHER: one per column
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * groups + group;
   const int64_t step = static_cast<int64_t>(gridDim.x) * groups;
@@ -311,42 +350,30 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
     for (int s = 0; s < sh.stages && row0 + s * step < p.rows; ++s) fetch(row0 + s * step, s);
 
   uint32_t named = 0xFFFFFFFFu;                                   // this thread's columns in the list
-  uint32_t pos[kGroupsOut * (kPack + 1) / 2];                     // its outputs' positions, two in each
+  bool checked = false;                                           // some output has no column
+  const raw* g = static_cast<const raw*>(p.g);
   if constexpr (GATHER) {
     if constexpr (Q8) {
       for (int i = threadIdx.x; i < (cols + 31) / 32; i += blockDim.x) bits[i] = 0;
       __syncthreads();
     }
     bool bad = false;
-    auto position = [&](int j) -> uint32_t {
-      if (j >= n) return kNoColumn;
-      const int64_t c = __ldg(p.idx + j);
-      if (c < 0 || c >= cols) {
-        bad = true;
-        return kNoColumn;
-      }
-      if constexpr (Q8) atomicOr(&bits[c >> 5], 1u << (c & 31));
-      return MODE == kLong ? static_cast<uint32_t>(c) : row_pos<DT, VEC>(static_cast<int>(c), cols);
-    };
-    if constexpr (STAGED) {
-#pragma unroll
-      for (int i = 0; i < kGroupsOut; ++i) {
-        uint32_t q[kPack];
-#pragma unroll
-        for (int e = 0; e < kPack; ++e) q[e] = position((i * G + t) * kPack + e);
-        if constexpr (kPack == 1) {
-          if (i & 1) pos[i / 2] |= q[0] << 16;
-          else pos[i / 2] = q[0];
+    for (int j = threadIdx.x; j < ((pad + 3) & ~3); j += blockDim.x) {
+      uint32_t place = kNoColumn;
+      if (j < n) {
+        const int64_t c64 = __ldg(p.idx + j);
+        const uint32_t c = static_cast<uint32_t>(c64);
+        if (static_cast<uint64_t>(c64) >= static_cast<uint64_t>(cols)) {
+          bad = true;
         } else {
-#pragma unroll
-          for (int e = 0; e < kPack; e += 2) pos[(i * kPack + e) / 2] = q[e] | (q[e + 1] << 16);
+          if constexpr (Q8) atomicOr(&bits[c >> 5], 1u << (c & 31));
+          place = MODE == kLong ? c : 4u * row_pos<DT, VEC>(static_cast<int>(c), cols);
         }
       }
-    } else {
-      for (int j = threadIdx.x; j < ((pad + 3) & ~3); j += blockDim.x) spos[j] = static_cast<uint16_t>(position(j));
+      spos[j] = static_cast<uint16_t>(place);
     }
     if (bad && blockIdx.x == 0) raise_error(p.err, GW_DERR_BAD_INDEX);
-    if constexpr (Q8 || MODE == kLong) __syncthreads();
+    checked = __syncthreads_or(bad ? 1 : 0) != 0;
     if constexpr (Q8 && STAGED) {
       named = 0;
 #pragma unroll
@@ -356,10 +383,21 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
       }
     }
   }
+  Held<DT, MODE == kLong ? 1 : E> gain;                           // this thread's share of the weight
+  gain.clear();
+  if (MODE != kLong && g) {
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      const int k = (i * G + t) * V;
+      if (k < cols) {
+        if constexpr (VEC) gain.set16(i, __ldg(reinterpret_cast<const uint4*>(g) + i * G + t));
+        else gain.set(i, __ldg(g + k));
+      }
+    }
+  }
 
   int buf = 0, stage = 0;
   uint32_t phase = 0;
-  const raw* g = static_cast<const raw*>(p.g);
   for (int64_t row = row0; row < p.rows; row += step) {
     raw* sum = p.s ? static_cast<raw*>(p.s) + row * p.lds : nullptr;
     const uint8_t* xs = ring + stage * sh.stage_bytes;
@@ -371,7 +409,7 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
     float ss = 0.0f;
     uint32_t umax = 0;
     // Vector v of the row: the sum, rounded to `sum` when WRITE, times g.
-    auto vector = [&](int v, float* f, bool write) {
+    auto vector = [&](int v, int i, float* f, bool write) {
       unpack16<DT>(reinterpret_cast<const uint4*>(xs)[v], f);
       if (p.r) {
         float q[V];
@@ -385,10 +423,15 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
         for (int j = 0; j < V; ++j) ss = fmaf(f[j], f[j], ss);
       }
       if (g) {
-        float q[V];
-        unpack16<DT>(__ldg(reinterpret_cast<const uint4*>(g) + v), q);
+        if constexpr (MODE == kLong) {
+          float q[V];
+          unpack16<DT>(__ldg(reinterpret_cast<const uint4*>(g) + v), q);
 #pragma unroll
-        for (int j = 0; j < V; ++j) f[j] *= q[j];
+          for (int j = 0; j < V; ++j) f[j] *= q[j];
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; ++j) f[j] *= gain.get(i * V + j);
+        }
       }
     };
     if constexpr (MODE == kVec) {
@@ -397,7 +440,7 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
         const int v = i * G + t;
         float* f = u + i * V;
         if (v * V < cols) {
-          vector(v, f, true);
+          vector(v, i, f, true);
           if constexpr (STAGED) {
 #pragma unroll
             for (int j = 0; j < V; j += 4)
@@ -416,7 +459,7 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
       }
     } else if constexpr (MODE == kLong) {
       for (int v = t; v * V < cols; v += G) {
-        vector(v, u, true);
+        vector(v, 0, u, true);
         if constexpr (Q8) {
           const uint32_t in = GATHER ? bits[v * V >> 5] >> (v * V & 31) : 0xFFFFFFFFu;
 #pragma unroll
@@ -425,23 +468,31 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
         }
       }
     } else {
+      const raw* x = static_cast<const raw*>(p.x) + row * p.ldx;
+      const raw* r = p.r ? static_cast<const raw*>(p.r) + row * p.ldr : nullptr;
       uintptr_t lo;
       uint32_t bytes;
-      // Generic pointers: into the stage, or (first and last row) into memory.
-      const raw* x = static_cast<const raw*>(p.x) + row * p.ldx;
-      if (granules(p.x, p.ldx, row, lo, bytes)) x = reinterpret_cast<const raw*>(xs + (reinterpret_cast<uintptr_t>(x) & 15u));
-      const raw* r = nullptr;
-      if (p.r) {
-        r = static_cast<const raw*>(p.r) + row * p.ldr;
-        if (granules(p.r, p.ldr, row, lo, bytes)) r = reinterpret_cast<const raw*>(rs + (reinterpret_cast<uintptr_t>(r) & 15u));
-      }
+      const bool in_x = granules(p.x, p.ldx, row, lo, bytes);
+      const bool in_r = !r || granules(p.r, p.ldr, row, lo, bytes);
+      if (in_x && in_r) {
+        const raw* xr = reinterpret_cast<const raw*>(xs + (reinterpret_cast<uintptr_t>(x) & 15u));
+        const raw* rr = reinterpret_cast<const raw*>(rs + (reinterpret_cast<uintptr_t>(r) & 15u));
 #pragma unroll
-      for (int i = 0; i < I; ++i) {
-        const int k = i * G + t;
-        u[i] = 0.0f;
-        if (k < cols) {
-          u[i] = Elem<DT>::to_f(x[k]);
-          if (r) u[i] += Elem<DT>::to_f(r[k]);
+        for (int i = 0; i < I; ++i) u[i] = i * G + t < cols ? Elem<DT>::to_f(xr[i * G + t]) : 0.0f;
+        if (r) {
+#pragma unroll
+          for (int i = 0; i < I; ++i)
+            if (i * G + t < cols) u[i] += Elem<DT>::to_f(rr[i * G + t]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+          const int k = i * G + t;
+          u[i] = 0.0f;
+          if (k < cols) {
+            u[i] = Elem<DT>::to_f(x[k]);
+            if (r) u[i] += Elem<DT>::to_f(r[k]);
+          }
         }
       }
 #pragma unroll
@@ -450,7 +501,7 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
         if (k < cols) {
           if (sum) sum[k] = Elem<DT>::from_f(u[i]);
           ss = fmaf(u[i], u[i], ss);
-          if (g) u[i] *= Elem<DT>::to_f(__ldg(g + k));
+          if (g) u[i] *= gain.get(i);
           if constexpr (STAGED) srow[k] = u[i];
           if constexpr (Q8) {
             if (!GATHER || ((named >> i) & 1u)) umax = max(umax, abs_bits(u[i]));
@@ -535,19 +586,37 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
     if constexpr (STAGED) {
       // Neighbouring threads take neighbouring groups of outputs: 4-byte
       // stores, and shared-memory reads within a narrow window of the row.
-#pragma unroll
-      for (int i = 0; i < kGroupsOut; ++i) {
-        const int j = (i * G + t) * kPack;
-        if (j < pad) {
-          float v[kPack];
-#pragma unroll
-          for (int e = 0; e < kPack; ++e) {
-            const int at = i * kPack + e;
-            const uint32_t c = (at & 1) ? pos[at / 2] >> 16 : pos[at / 2] & 0xFFFFu;
-            v[e] = c == kNoColumn ? 0.0f : value(srow[c]);
-          }
-          store_pack(j, v);
+      const uint8_t* sr = reinterpret_cast<const uint8_t*>(srow);
+      auto read = [&](int j, uint32_t* c) {          // the places of outputs j .. j + kPack - 1
+        if constexpr (kPack == 4) {
+          const uint2 q = *reinterpret_cast<const uint2*>(spos + j);
+          c[0] = q.x & 0xFFFFu; c[1] = q.x >> 16; c[2] = q.y & 0xFFFFu; c[3] = q.y >> 16;
+        } else if constexpr (kPack == 2) {
+          const uint32_t q = *reinterpret_cast<const uint32_t*>(spos + j);
+          c[0] = q & 0xFFFFu; c[1] = q >> 16;
+        } else {
+          c[0] = spos[j];
         }
+      };
+      const int whole = checked ? 0 : n / kPack * kPack;   // outputs that all have a column
+      int j = t * kPack;
+#pragma unroll 4
+      for (; j < whole; j += G * kPack) {
+        uint32_t c[kPack];
+        float v[kPack];
+        read(j, c);
+#pragma unroll
+        for (int e = 0; e < kPack; ++e) v[e] = value(*reinterpret_cast<const float*>(sr + c[e]));
+        store_pack(j, v);
+      }
+      for (; j < pad; j += G * kPack) {
+        uint32_t c[kPack];
+        float v[kPack];
+        read(j, c);
+#pragma unroll
+        for (int e = 0; e < kPack; ++e)
+          v[e] = c[e] == kNoColumn ? 0.0f : value(*reinterpret_cast<const float*>(sr + c[e]));
+        store_pack(j, v);
       }
       // The next row overwrites srow.
       if constexpr (WARP) __syncwarp();
@@ -575,7 +644,7 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
     } else {
       if constexpr (MODE == kLong) {
         for (int v = t; v * V < cols; v += G) {
-          vector(v, u, false);
+          vector(v, 0, u, false);
           store_vector(v * V, u);
         }
       } else {
@@ -608,9 +677,7 @@ cudaError_t launch_rows_variant(const RowParams& p, int y_vec, int sm_count, cud
   const int groups = WARP ? 4 : 1;
   const int warps = WARP ? groups : std::min(32, (cols + 32 * E - 1) / (32 * E));
   const int threads = warps * 32;
-  // A thread's outputs are counted at compile time (kLong loops).
-  if (MODE != kLong && p.pad > static_cast<int64_t>(WARP ? 32 : threads) * E) return cudaErrorNotSupported;
-  const int npos = MODE == kLong && GATHER ? static_cast<int>((p.pad + 3) & ~int64_t{3}) : 0;
+  const int npos = GATHER ? static_cast<int>((p.pad + 3) & ~int64_t{3}) : 0;
   const bool staged = GATHER && MODE != kLong;
   RowShared sh;
   const int fixed = kRowHead + (staged ? groups * cols4 * 4 : 0) + npos * 2 +
@@ -663,6 +730,7 @@ cudaError_t launch_rows_held(const RowParams& p, bool vec, int y_vec, int sm_cou
     return launch_rows_variant<DT, Q8, GATHER, kLong, 16, false, 1024>(p, y_vec, sm_count, stream);
   }
   if (p.cols <= 256) return launch_rows_variant<DT, Q8, GATHER, kAny, 8, true, 128>(p, y_vec, sm_count, stream);
+  if (p.cols <= 4096) return launch_rows_variant<DT, Q8, GATHER, kAny, 16, false, 256>(p, y_vec, sm_count, stream);
   if (p.cols <= kRowsHeldCols)
     return launch_rows_variant<DT, Q8, GATHER, kAny, 16, false, 1024>(p, y_vec, sm_count, stream);
   return cudaErrorNotSupported;
@@ -673,7 +741,7 @@ cudaError_t launch_rows_held(const RowParams& p, bool vec, int y_vec, int sm_cou
 // aligned), lists longer than the row.
 template <int DT, bool Q8>
 cudaError_t launch_rows_once(const RowParams& p, int sm_count, cudaStream_t stream) {
-  if (p.cols < 1 || p.cols > kRowsMaxCols || p.n > p.cols) return cudaErrorNotSupported;
+  if (p.cols < 1 || p.cols > kRowsMaxCols || p.n > p.cols || p.pad > p.cols + 128) return cudaErrorNotSupported;
   constexpr int eb = DT == GW_DTYPE_F32 ? 4 : 2;
   constexpr int V = 16 / eb;
   const int ob = Q8 ? 1 : eb;                      // bytes of an output
