@@ -518,14 +518,22 @@ def packed_gemm_q8(a: torch.Tensor, a_scale: torch.Tensor, w_packed: torch.Tenso
                    y: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
                    residual: torch.Tensor | None = None) -> None:
     """y = act(a_scale w_scale (a @ w_packed^T) + bias) + residual over e4m3 operands by TMA."""
-    _rowmajor(a, w_packed, y)
+    _rowmajor(y)
     M, K = a.shape
     N = w_packed.shape[0]
-    with _on_device(a.device):
+    dev = a.get_device()
+    cur = torch.cuda.current_device()
+    if dev != cur:
+        torch.cuda.set_device(dev)
+    try:
         st = api().gw_packed_gemm_q8(
             a.data_ptr(), a_scale.data_ptr(), M, K, _ld16(a), w_packed.data_ptr(), w_scale.data_ptr(), N,
             _ld16(w_packed), _ptr(bias), epilogue_code(activation), *_residual(residual), y.data_ptr(),
-            dtype_code(y.dtype), max(y.stride(0), N), _stream(a.device))
+            dtype_code(y.dtype), max(y.stride(0), N),
+            _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream)
+    finally:
+        if dev != cur:
+            torch.cuda.set_device(cur)
     if st:
         _check(st, "gw_packed_gemm_q8")
 
@@ -566,16 +574,24 @@ def rms_norm(x: torch.Tensor, residual: torch.Tensor | None, total: torch.Tensor
              scale: torch.Tensor | None = None) -> None:
     """gw_rms_norm (scale None) or gw_rms_norm_q8 over row-major matrices; y is the whole
     padded buffer, of which the first n columns are outputs and the rest is zeroed."""
-    _rowmajor(x, y)
     rows, cols = x.shape
-    with _on_device(x.device):
-        head = (x.data_ptr(), dtype_code(x.dtype), rows, cols, _ld(x), _ptr(residual),
-                0 if residual is None else _ld(residual), _ptr(total), 0 if total is None else _ld(total),
-                _ptr(weight), float(eps), _ptr(idx), n, y.data_ptr(), _ld(y), y.shape[1])
+    pad = y.shape[1]
+    dev = x.get_device()
+    cur = torch.cuda.current_device()
+    if dev != cur:
+        torch.cuda.set_device(dev)
+    try:
+        stream = _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
+        head = (x.data_ptr(), dtype_code(x.dtype), rows, cols, _ld(x), *_residual(residual), *_residual(total),
+                None if weight is None else weight.data_ptr(), eps, None if idx is None else idx.data_ptr(), n,
+                y.data_ptr(), pad, pad)
         if scale is None:
-            what, st = "gw_rms_norm", api().gw_rms_norm(*head, _stream(x.device))
+            what, st = "gw_rms_norm", api().gw_rms_norm(*head, stream)
         else:
-            what, st = "gw_rms_norm_q8", api().gw_rms_norm_q8(*head, scale.data_ptr(), _stream(x.device))
+            what, st = "gw_rms_norm_q8", api().gw_rms_norm_q8(*head, scale.data_ptr(), stream)
+    finally:
+        if dev != cur:
+            torch.cuda.set_device(cur)
     if st:
         _check(st, what)
 
@@ -583,11 +599,20 @@ def rms_norm(x: torch.Tensor, residual: torch.Tensor | None, total: torch.Tensor
 def quantize_rows(x: torch.Tensor, idx: torch.Tensor | None, n: int, q: torch.Tensor,
                   scale: torch.Tensor) -> None:
     """gw_quantize_rows over a row-major matrix; q is the whole padded buffer."""
-    _rowmajor(x, q)
     rows, cols = x.shape
-    with _on_device(x.device):
-        st = api().gw_quantize_rows(x.data_ptr(), dtype_code(x.dtype), rows, cols, _ld(x), _ptr(idx), n,
-                                    q.data_ptr(), _ld(q), q.shape[1], scale.data_ptr(), _stream(x.device))
+    pad = q.shape[1]
+    dev = x.get_device()
+    cur = torch.cuda.current_device()
+    if dev != cur:
+        torch.cuda.set_device(dev)
+    try:
+        st = api().gw_quantize_rows(
+            x.data_ptr(), dtype_code(x.dtype), rows, cols, _ld(x), None if idx is None else idx.data_ptr(), n,
+            q.data_ptr(), pad, pad, scale.data_ptr(),
+            _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream)
+    finally:
+        if dev != cur:
+            torch.cuda.set_device(cur)
     if st:
         _check(st, "gw_quantize_rows")
 

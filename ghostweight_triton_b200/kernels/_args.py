@@ -54,10 +54,13 @@ def out_matrix(what: str, out: torch.Tensor, like: torch.Tensor, *inputs: torch.
 
 def residual_matrix(residual: torch.Tensor, shape: tuple[int, int], like: torch.Tensor) -> torch.Tensor:
     """The residual [M, N] of a product as a row-major matrix."""
-    assert residual.dtype is like.dtype and residual.device == like.device, (
+    assert residual.dtype is like.dtype and residual.is_cuda and residual.get_device() == like.get_device(), (
         f"residual must be {like.dtype} on {like.device}, got {residual.dtype} on {residual.device}")
-    assert tuple(residual.shape) == tuple(shape), f"residual must have shape {tuple(shape)}, got {tuple(residual.shape)}"
-    refuse_grad(residual=residual)
+    assert residual.shape == shape, f"residual must have shape {tuple(shape)}, got {tuple(residual.shape)}"
+    if torch.is_grad_enabled():
+        refuse_grad(residual=residual)
+    if residual.is_contiguous():
+        return residual
     if (residual.stride(1) != 1 and shape[1] > 1) or (shape[0] > 1 and residual.stride(0) < shape[1]):
         residual = residual.contiguous()
     return residual

@@ -287,16 +287,18 @@ def packed_linear(
 def _q8_operand(what: str, q: torch.Tensor, scale: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """An e4m3 matrix whose rows TMA can load (16-byte aligned; copied into such rows if it
     is not) and its scales [rows]."""
-    assert q.ndim == 2 and q.is_cuda and q.dtype is torch.float8_e4m3fn, (
+    assert q.is_cuda and q.dtype is torch.float8_e4m3fn and q.dim() == 2, (
         f"{what} must be a float8_e4m3fn matrix on CUDA, got {q.dtype} {tuple(q.shape)}")
-    assert scale.dtype is torch.float32 and scale.shape == (q.shape[0],) and scale.device == q.device, (
-        f"{what}_scale must be float32 of shape ({q.shape[0]},) on {what}'s device")
-    if (q.shape[1] > 1 and q.stride(1) != 1) or q.data_ptr() % 16 or (
-            q.shape[0] > 1 and (q.stride(0) % 16 or q.stride(0) < q.shape[1])):
-        buf = torch.zeros((q.shape[0], (q.shape[1] + 15) // 16 * 16), dtype=q.dtype, device=q.device)
-        buf[:, : q.shape[1]] = q
-        q = buf[:, : q.shape[1]]
-    return q, scale.contiguous()
+    rows, cols = q.shape
+    assert (scale.dtype is torch.float32 and scale.dim() == 1 and scale.numel() == rows and scale.is_cuda
+            and scale.get_device() == q.get_device()), (
+        f"{what}_scale must be float32 of shape ({rows},) on {what}'s device")
+    s0, s1 = q.stride()
+    if (cols > 1 and s1 != 1) or q.data_ptr() % 16 or (rows > 1 and (s0 % 16 or s0 < cols)):
+        buf = torch.zeros((rows, (cols + 15) // 16 * 16), dtype=q.dtype, device=q.device)
+        buf[:, :cols] = q
+        q = buf[:, :cols]
+    return q, scale if scale.is_contiguous() else scale.contiguous()
 
 
 def packed_linear_q8(
@@ -321,21 +323,28 @@ def packed_linear_q8(
     """
     a, a_scale = _q8_operand("a", a, a_scale)
     w_packed, w_scale = _q8_operand("w_packed", w_packed, w_scale)
-    assert a.device == w_packed.device, "a and w_packed must be on one device"
-    assert a.shape[1] == w_packed.shape[1], f"K mismatch: a has {a.shape[1]} columns, w_packed {w_packed.shape[1]}"
-    M, N = a.shape[0], w_packed.shape[0]
+    dev = a.get_device()
+    assert dev == w_packed.get_device(), "a and w_packed must be on one device"
+    (M, K), (N, K_w) = a.shape, w_packed.shape
+    assert K == K_w, f"K mismatch: a has {K} columns, w_packed {K_w}"
     if dtype is None:
         dtype = next((t.dtype for t in (residual, out) if t is not None),
                      bias.dtype if bias is not None and bias.dtype is torch.float16 else torch.bfloat16)
     if dtype not in (torch.float16, torch.bfloat16):
         raise TypeError(f"unsupported output dtype {dtype}; expected float16 or bfloat16")
-    y = torch.empty((M, N), dtype=dtype, device=a.device) if out is None else out
-    assert y.shape == (M, N) and y.dtype is dtype and y.device == a.device, (
-        f"out must be {dtype} of shape {(M, N)} on a's device")
     if bias is not None:
-        assert bias.shape == (N,) and bias.device == a.device, f"bias must have shape ({N},) on a's device"
-        bias = bias.detach().to(dtype).contiguous()
-    y, residual = _product_out(y, residual, M, N, y)
+        assert bias.dim() == 1 and bias.numel() == N and bias.is_cuda and bias.get_device() == dev, (
+            f"bias must have shape ({N},) on a's device")
+        if bias.dtype is not dtype or not bias.is_contiguous():
+            bias = bias.detach().to(dtype).contiguous()
+    if out is None:
+        y = torch.empty((M, N), dtype=dtype, device=a.device)
+        if residual is not None:
+            residual = residual_matrix(residual, (M, N), y)
+    else:
+        assert out.shape == (M, N) and out.dtype is dtype and out.is_cuda and out.get_device() == dev, (
+            f"out must be {dtype} of shape {(M, N)} on a's device")
+        y, residual = _product_out(out, residual, M, N, out)
     if M and N:
         _native.packed_gemm_q8(a, a_scale, w_packed, w_scale, y, bias=bias, activation=activation,
                                residual=residual)

@@ -29,60 +29,74 @@ from ghostweight_triton_b200.kernels.gather import PACK_ALIGN, _round_up
 PACK_ALIGN_Q8 = 128
 
 
-def _alive(alive_indices: torch.Tensor | None, x: torch.Tensor) -> torch.Tensor | None:
-    if alive_indices is None:
-        return None
-    assert alive_indices.ndim == 1, f"alive_indices must be one list, got shape {tuple(alive_indices.shape)}"
-    if alive_indices.dtype is not torch.int64 or alive_indices.device != x.device:
+def _alive(alive_indices: torch.Tensor, dev: int) -> torch.Tensor:
+    """The list as contiguous int64 on CUDA device `dev`."""
+    assert alive_indices.dim() == 1, f"alive_indices must be one list, got shape {tuple(alive_indices.shape)}"
+    if alive_indices.dtype is not torch.int64 or not alive_indices.is_cuda or alive_indices.get_device() != dev:
         assert not alive_indices.is_floating_point() and alive_indices.dtype is not torch.bool, \
             f"alive_indices must be integers, got {alive_indices.dtype}"
-        alive_indices = alive_indices.to(device=x.device, dtype=torch.int64)
-    return alive_indices.contiguous()
+        alive_indices = alive_indices.to(device=torch.device("cuda", dev), dtype=torch.int64)
+    return alive_indices if alive_indices.is_contiguous() else alive_indices.contiguous()
 
 
 def _norm(x, weight, eps, residual, alive_indices, residual_out, q8):
-    assert x.ndim >= 1 and x.is_cuda, "rms_norm runs on CUDA (sm_100) only"
-    _native.dtype_code(x.dtype)
-    refuse_grad(x=x, residual=residual)
-    cols = x.shape[-1]
+    # Small calls are bound by this function, not by the kernel (4 us for one
+    # row of 4096): attribute reads and integer compares, no tensor operation
+    # that the operands do not need.
+    assert x.is_cuda and x.dim() >= 1, "rms_norm runs on CUDA (sm_100) only"
+    dtype = x.dtype
+    _native.dtype_code(dtype)
+    if torch.is_grad_enabled():
+        refuse_grad(x=x, residual=residual)
+    dev = x.get_device()
+    flat = x.dim() == 2
+    shape = x.shape
+    cols = shape[-1]
     assert cols > 0, "the norm of a row without columns is undefined"
     assert eps >= 0.0, f"eps must not be negative, got {eps}"
-    lead = x.shape[:-1]
-    x_2d = rows(x, cols)
+    x_2d = x if flat and x.is_contiguous() else rows(x, cols)
+    M = x_2d.shape[0]
     if weight is not None:
-        assert weight.shape == (cols,), f"weight must have shape ({cols},), got {tuple(weight.shape)}"
-        assert weight.device == x.device, "weight must be on x's device"
-        weight = weight.detach()
-        if weight.dtype is not x.dtype:
-            weight = weight.to(x.dtype)
-        weight = weight.contiguous()
+        assert weight.dim() == 1 and weight.numel() == cols, (
+            f"weight must have shape ({cols},), got {tuple(weight.shape)}")
+        assert weight.is_cuda and weight.get_device() == dev, "weight must be on x's device"
+        if weight.dtype is not dtype:
+            weight = weight.detach().to(dtype)
+        if not weight.is_contiguous():
+            weight = weight.contiguous()
     total = r_2d = None
     if residual is not None:
-        assert residual.shape == x.shape and residual.dtype is x.dtype and residual.device == x.device, (
-            "residual must have x's shape, dtype and device")
-        r_2d = rows(residual, cols)
+        assert (residual.shape == shape and residual.dtype is dtype and residual.is_cuda
+                and residual.get_device() == dev), "residual must have x's shape, dtype and device"
+        r_2d = residual if flat and residual.is_contiguous() else rows(residual, cols)
         if residual_out is None:
-            residual_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        total = out_matrix("residual_out", residual_out, x, x_2d, r_2d)
+            residual_out = x.new_empty(shape)
+            total = residual_out if flat else residual_out.view(-1, cols)
+        else:
+            total = out_matrix("residual_out", residual_out, x, x_2d, r_2d)
     else:
         assert residual_out is None, "residual_out needs a residual"
-    idx = _alive(alive_indices, x)
-    n = cols if idx is None else idx.numel()
-    M = x_2d.shape[0]
+    idx, n, ld = None, cols, cols
+    if alive_indices is not None:
+        idx = _alive(alive_indices, dev)
+        n = idx.numel()
+        ld = _round_up(n, PACK_ALIGN)
+    scale = None
     if q8:
-        buf = torch.empty((M, _round_up(n, PACK_ALIGN_Q8)), dtype=torch.float8_e4m3fn, device=x.device)
+        ld = _round_up(n, PACK_ALIGN_Q8)
+        buf = torch.empty((M, ld), dtype=torch.float8_e4m3fn, device=x.device)
         scale = torch.empty(M, dtype=torch.float32, device=x.device)
     else:
-        buf = torch.empty((M, n if idx is None else _round_up(n, PACK_ALIGN)), dtype=x.dtype, device=x.device)
-        scale = None
+        buf = x.new_empty((M, ld))
     if M:
         _native.rms_norm(x_2d, r_2d, total, weight, eps, idx, n, buf, scale)
-    y = buf if buf.shape[1] == n else buf[:, :n]
-    if x.ndim != 2:
-        y = y.view(*lead, n)
-        scale = scale.view(lead) if q8 else None
-    out = (y, scale) if q8 else (y,)
-    return out if residual is None else (*out, residual_out)
+    y = buf if ld == n else buf.narrow(1, 0, n)
+    if not flat:
+        y = y.view(*shape[:-1], n)
+        scale = scale.view(shape[:-1]) if q8 else None
+    if residual is None:
+        return (y, scale) if q8 else (y,)
+    return (y, scale, residual_out) if q8 else (y, residual_out)
 
 
 def rms_norm(
@@ -149,21 +163,28 @@ def quantize_rows(
     q * scale ~ x[..., alive], as :func:`rms_norm_q8` rounds its output.
     Columns outside the list are not looked at.
     """
-    assert x.ndim >= 1 and x.is_cuda, "quantize_rows runs on CUDA (sm_100) only"
+    assert x.is_cuda and x.dim() >= 1, "quantize_rows runs on CUDA (sm_100) only"
     _native.dtype_code(x.dtype)
-    refuse_grad(x=x)
-    cols = x.shape[-1]
-    lead = x.shape[:-1]
-    idx = _alive(alive_indices, x)
-    n = cols if idx is None else idx.numel()
-    M = math.prod(lead)
-    buf = torch.empty((M, _round_up(n, PACK_ALIGN_Q8)), dtype=torch.float8_e4m3fn, device=x.device)
+    if torch.is_grad_enabled():
+        refuse_grad(x=x)
+    shape = x.shape
+    flat = x.dim() == 2
+    cols = shape[-1]
+    idx, n = None, cols
+    if alive_indices is not None:
+        idx = _alive(alive_indices, x.get_device())
+        n = idx.numel()
+    M = shape[0] if flat else math.prod(shape[:-1])
+    ld = _round_up(n, PACK_ALIGN_Q8)
+    buf = torch.empty((M, ld), dtype=torch.float8_e4m3fn, device=x.device)
     scale = torch.empty(M, dtype=torch.float32, device=x.device)
     if M:
-        _native.quantize_rows(rows(x, cols) if cols else x.reshape(M, 0), idx, n, buf, scale)
-    q = buf if buf.shape[1] == n else buf[:, :n]
-    if x.ndim != 2:
-        q, scale = q.view(*lead, n), scale.view(lead)
+        if not (flat and x.is_contiguous()):
+            x = rows(x, cols) if cols else x.reshape(M, 0)
+        _native.quantize_rows(x, idx, n, buf, scale)
+    q = buf if ld == n else buf.narrow(1, 0, n)
+    if not flat:
+        q, scale = q.view(*shape[:-1], n), scale.view(shape[:-1])
     return q, scale
 
 
