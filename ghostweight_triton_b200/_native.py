@@ -569,31 +569,33 @@ def _ld(t: torch.Tensor) -> int:
     return max(t.stride(0), t.shape[1])
 
 
-def rms_norm(x: torch.Tensor, residual: torch.Tensor | None, total: torch.Tensor | None,
-             weight: torch.Tensor | None, eps: float, idx: torch.Tensor | None, n: int, y: torch.Tensor,
+def rms_norm(x: torch.Tensor, rows: int, cols: int, ldx: int, residual: torch.Tensor | None, ldr: int,
+             total: torch.Tensor | None, lds: int, weight: torch.Tensor | None, eps: float,
+             idx: torch.Tensor | None, n: int, y: torch.Tensor, pad: int,
              scale: torch.Tensor | None = None) -> None:
     """gw_rms_norm (scale None) or gw_rms_norm_q8 over row-major matrices; y is the whole
-    padded buffer, of which the first n columns are outputs and the rest is zeroed."""
-    rows, cols = x.shape
-    pad = y.shape[1]
+    [rows, pad] buffer, of which the first n columns are outputs and the rest is zeroed."""
     dev = x.get_device()
     cur = torch.cuda.current_device()
     if dev != cur:
         torch.cuda.set_device(dev)
     try:
         stream = _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
-        head = (x.data_ptr(), dtype_code(x.dtype), rows, cols, _ld(x), *_residual(residual), *_residual(total),
-                None if weight is None else weight.data_ptr(), eps, None if idx is None else idx.data_ptr(), n,
-                y.data_ptr(), pad, pad)
+        r_ptr = None if residual is None else residual.data_ptr()
+        s_ptr = None if total is None else total.data_ptr()
+        g_ptr = None if weight is None else weight.data_ptr()
+        i_ptr = None if idx is None else idx.data_ptr()
         if scale is None:
-            what, st = "gw_rms_norm", api().gw_rms_norm(*head, stream)
+            st = api().gw_rms_norm(x.data_ptr(), DTYPE_CODES[x.dtype], rows, cols, ldx, r_ptr, ldr, s_ptr, lds,
+                                   g_ptr, eps, i_ptr, n, y.data_ptr(), pad, pad, stream)
         else:
-            what, st = "gw_rms_norm_q8", api().gw_rms_norm_q8(*head, scale.data_ptr(), stream)
+            st = api().gw_rms_norm_q8(x.data_ptr(), DTYPE_CODES[x.dtype], rows, cols, ldx, r_ptr, ldr, s_ptr, lds,
+                                      g_ptr, eps, i_ptr, n, y.data_ptr(), pad, pad, scale.data_ptr(), stream)
     finally:
         if dev != cur:
             torch.cuda.set_device(cur)
     if st:
-        _check(st, what)
+        _check(st, "gw_rms_norm" if scale is None else "gw_rms_norm_q8")
 
 
 def quantize_rows(x: torch.Tensor, idx: torch.Tensor | None, n: int, q: torch.Tensor,

@@ -55,7 +55,7 @@ struct RowScale {
 __device__ __forceinline__ RowScale row_scale(uint32_t umax_bits, float rstd) {
   const float umax = __uint_as_float(umax_bits);
   RowScale q;
-  q.scale = umax * rstd / kE4m3Max;                // NaN compares false and stays
+  q.scale = umax * rstd * (1.0f / kE4m3Max);       // NaN compares false and stays
   q.m2 = umax < 0x1p-64f ? 0x1p64f : 1.0f;
   q.m1 = kE4m3Max / (umax * q.m2);
   if (q.scale < kScaleMin) {
@@ -73,6 +73,47 @@ __device__ __forceinline__ float to_scale(float u, const RowScale& q) {
   const float v = u * q.m1 * q.m2;
   const float c = 9.0f * v;
   return c - (c - v);
+}
+
+// Two fp32 operations in one instruction, each rounded on its own.
+__device__ __forceinline__ uint64_t pair_bits(float2 v) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+  return r;
+}
+__device__ __forceinline__ float2 bits_pair(uint64_t r) {
+  float2 v;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
+  return v;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)));
+  return bits_pair(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)));
+  return bits_pair(r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)), "l"(pair_bits(c)));
+  return bits_pair(r);
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+// to_scale for two values.
+__device__ __forceinline__ float2 to_scale2(float2 u, const RowScale& q) {
+  float2 v = mul2(u, both(q.m1));
+  if (q.m2 != 1.0f) v = mul2(v, both(q.m2));
+  const float2 c = mul2(v, both(9.0f));
+  return fma2(fma2(v, both(-1.0f), c), both(-1.0f), c);
+}
+// max(a, |b|), NaN if either is (its bits then lie above infinity's).
+__device__ __forceinline__ float max_abs(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+  return r;
 }
 
 template <bool Q8, int DT> struct RowOut { using raw = typename Elem<DT>::raw; };
@@ -217,9 +258,9 @@ struct Held {
     w[4 * v + 2] = q.z;
     w[4 * v + 3] = q.w;
   }
-  __device__ __forceinline__ float get(int i) const {
-    if constexpr (DT == GW_DTYPE_F32) return __uint_as_float(w[i]);
-    else return (i & 1) ? hi_f<DT>(w[i / 2]) : lo_f<DT>(w[i / 2]);
+  __device__ __forceinline__ float2 get2(int i) const {             // values i (even) and i + 1
+    if constexpr (DT == GW_DTYPE_F32) return make_float2(__uint_as_float(w[i]), __uint_as_float(w[i + 1]));
+    else return make_float2(lo_f<DT>(w[i / 2]), hi_f<DT>(w[i / 2]));
   }
 };
 enum RowMode { kVec = 0, kAny = 1, kLong = 2 };
@@ -396,6 +437,7 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
     }
   }
 
+  const float inv_cols = 1.0f / static_cast<float>(cols);
   int buf = 0, stage = 0;
   uint32_t phase = 0;
   for (int64_t row = row0; row < p.rows; row += step) {
@@ -405,33 +447,30 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
     // A wait that runs out raises the device error word and the abort flag; the
     // rest of this CTA's rows are then worked off quickly, with undefined outputs.
     mbar_wait(bar0 + 8u * stage, phase, abort_flag, p.err);
-    float u[MODE == kLong ? V : E];
-    float ss = 0.0f;
-    uint32_t umax = 0;
-    // Vector v of the row: the sum, rounded to `sum` when WRITE, times g.
-    auto vector = [&](int v, int i, float* f, bool write) {
+    __align__(16) float u[MODE == kLong ? V : E];
+    float2 ss2 = make_float2(0.0f, 0.0f);
+    float uabs = 0.0f;
+    // Vector v of the row (the thread's i-th): the sum, rounded to `sum` and
+    // squared into ss2 when `first`, times the weight.
+    auto vector = [&](int v, int i, float* f, bool first) {
       unpack16<DT>(reinterpret_cast<const uint4*>(xs)[v], f);
+      float2* f2 = reinterpret_cast<float2*>(f);
+      float q[V];
       if (p.r) {
-        float q[V];
         unpack16<DT>(reinterpret_cast<const uint4*>(rs)[v], q);
 #pragma unroll
-        for (int j = 0; j < V; ++j) f[j] += q[j];
+        for (int j = 0; j < V / 2; ++j) f2[j] = add2(f2[j], make_float2(q[2 * j], q[2 * j + 1]));
       }
-      if (write) {
+      if (first) {
         if (sum) reinterpret_cast<uint4*>(sum)[v] = pack16<DT>(f);
 #pragma unroll
-        for (int j = 0; j < V; ++j) ss = fmaf(f[j], f[j], ss);
+        for (int j = 0; j < V / 2; ++j) ss2 = fma2(f2[j], f2[j], ss2);
       }
       if (g) {
-        if constexpr (MODE == kLong) {
-          float q[V];
-          unpack16<DT>(__ldg(reinterpret_cast<const uint4*>(g) + v), q);
+        if constexpr (MODE == kLong) unpack16<DT>(__ldg(reinterpret_cast<const uint4*>(g) + v), q);
 #pragma unroll
-          for (int j = 0; j < V; ++j) f[j] *= q[j];
-        } else {
-#pragma unroll
-          for (int j = 0; j < V; ++j) f[j] *= gain.get(i * V + j);
-        }
+        for (int j = 0; j < V / 2; ++j)
+          f2[j] = mul2(f2[j], MODE == kLong ? make_float2(q[2 * j], q[2 * j + 1]) : gain.get2(i * V + 2 * j));
       }
     };
     if constexpr (MODE == kVec) {
@@ -455,7 +494,7 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
       if constexpr (Q8) {
 #pragma unroll
         for (int e = 0; e < E; ++e)
-          if (!GATHER || ((named >> e) & 1u)) umax = max(umax, abs_bits(u[e]));
+          if (!GATHER || ((named >> e) & 1u)) uabs = max_abs(uabs, u[e]);
       }
     } else if constexpr (MODE == kLong) {
       for (int v = t; v * V < cols; v += G) {
@@ -464,7 +503,7 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
           const uint32_t in = GATHER ? bits[v * V >> 5] >> (v * V & 31) : 0xFFFFFFFFu;
 #pragma unroll
           for (int j = 0; j < V; ++j)
-            if ((in >> j) & 1u) umax = max(umax, abs_bits(u[j]));
+            if ((in >> j) & 1u) uabs = max_abs(uabs, u[j]);
         }
       }
     } else {
@@ -495,20 +534,29 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
           }
         }
       }
+      if (sum) {
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+          if (i * G + t < cols) sum[i * G + t] = Elem<DT>::from_f(u[i]);
+      }
+      float2* u2 = reinterpret_cast<float2*>(u);
+#pragma unroll
+      for (int i = 0; i < E / 2; ++i) {
+        ss2 = fma2(u2[i], u2[i], ss2);
+        if (g) u2[i] = mul2(u2[i], gain.get2(2 * i));
+      }
 #pragma unroll
       for (int i = 0; i < I; ++i) {
-        const int k = i * G + t;
-        if (k < cols) {
-          if (sum) sum[k] = Elem<DT>::from_f(u[i]);
-          ss = fmaf(u[i], u[i], ss);
-          if (g) u[i] *= gain.get(i);
-          if constexpr (STAGED) srow[k] = u[i];
-          if constexpr (Q8) {
-            if (!GATHER || ((named >> i) & 1u)) umax = max(umax, abs_bits(u[i]));
-          }
+        if constexpr (STAGED) {
+          if (i * G + t < cols) srow[i * G + t] = u[i];
+        }
+        if constexpr (Q8) {
+          if (!GATHER || ((named >> i) & 1u)) uabs = max_abs(uabs, u[i]);
         }
       }
     }
+    float ss = ss2.x + ss2.y;
+    uint32_t umax = __float_as_uint(uabs);
     // Sum of squares and largest |u| of the row; publishes srow too.
 #pragma unroll
     for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
@@ -541,7 +589,7 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
       if constexpr (Q8) umax = __reduce_max_sync(0xFFFFFFFFu, in ? red_m[buf * 32 + lane] : 0u);
       buf ^= 1;
     }
-    const float rstd = p.norm ? rsqrtf(ss / static_cast<float>(cols) + p.eps) : 1.0f;
+    const float rstd = p.norm ? rsqrtf(ss * inv_cols + p.eps) : 1.0f;
     RowScale q8 = {1.0f, 1.0f, 1.0f};
     if constexpr (Q8) {
       q8 = row_scale(umax, rstd);
@@ -549,6 +597,7 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
     }
     out* y = static_cast<out*>(p.y) + row * p.ldy;
     auto value = [&](float v) { return Q8 ? to_scale(v, q8) : v * rstd; };
+    auto value2 = [&](float2 v) { return Q8 ? to_scale2(v, q8) : mul2(v, both(rstd)); };
     auto store1 = [&](int j, float v) {
       if constexpr (Q8) y[j] = static_cast<out>(e4m3_pack2(v, 0.0f));
       else y[j] = Elem<DT>::from_f(v);
@@ -567,10 +616,13 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
       }
     };
     auto store_vector = [&](int k, float* f) {       // outputs k .. k + V - 1 (aligned)
+      if constexpr (VEC) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) f[j] = value(f[j]);
+        for (int j = 0; j < V; j += 2)
+          *reinterpret_cast<float2*>(f + j) = value2(*reinterpret_cast<const float2*>(f + j));
+      }
       if constexpr (!VEC) {
-        store1(k, f[0]);
+        store1(k, value(f[0]));
       } else if constexpr (!Q8) {
         *reinterpret_cast<uint4*>(y + k) = pack16<DT>(f);
       } else {
@@ -603,15 +655,22 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
 #pragma unroll 4
       for (; j < whole; j += G * kPack) {
         uint32_t c[kPack];
-        float v[kPack];
+        __align__(16) float v[kPack];
         read(j, c);
 #pragma unroll
-        for (int e = 0; e < kPack; ++e) v[e] = value(*reinterpret_cast<const float*>(sr + c[e]));
+        for (int e = 0; e < kPack; ++e) v[e] = *reinterpret_cast<const float*>(sr + c[e]);
+        if constexpr (kPack == 1) {
+          v[0] = value(v[0]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < kPack; e += 2)
+            *reinterpret_cast<float2*>(v + e) = value2(*reinterpret_cast<const float2*>(v + e));
+        }
         store_pack(j, v);
       }
       for (; j < pad; j += G * kPack) {
         uint32_t c[kPack];
-        float v[kPack];
+        __align__(16) float v[kPack];
         read(j, c);
 #pragma unroll
         for (int e = 0; e < kPack; ++e)

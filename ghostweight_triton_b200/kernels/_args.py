@@ -22,6 +22,11 @@ def rows(t: torch.Tensor, cols: int) -> torch.Tensor:
     return t
 
 
+def leading(m: torch.Tensor) -> int:
+    """Leading dimension of a row-major matrix (torch gives matrices of one row any stride)."""
+    return max(m.stride(0), m.shape[1])
+
+
 def _span(m: torch.Tensor) -> tuple[int, int]:
     return m.data_ptr(), m.data_ptr() + ((m.shape[0] - 1) * m.stride(0) + m.shape[1]) * m.element_size()
 

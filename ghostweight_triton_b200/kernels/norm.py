@@ -21,7 +21,7 @@ import math
 import torch
 
 from ghostweight_triton_b200 import _native
-from ghostweight_triton_b200.kernels._args import out_matrix, refuse_grad, rows
+from ghostweight_triton_b200.kernels._args import leading, out_matrix, refuse_grad, rows
 from ghostweight_triton_b200.kernels.gather import PACK_ALIGN, _round_up
 
 # e4m3 rows keep a stride of a multiple of 128 bytes: one k-block of the
@@ -45,8 +45,9 @@ def _norm(x, weight, eps, residual, alive_indices, residual_out, q8):
     # that the operands do not need.
     assert x.is_cuda and x.dim() >= 1, "rms_norm runs on CUDA (sm_100) only"
     dtype = x.dtype
-    _native.dtype_code(dtype)
-    if torch.is_grad_enabled():
+    if dtype not in _native.DTYPE_CODES:
+        _native.dtype_code(dtype)                # raises
+    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
         refuse_grad(x=x, residual=residual)
     dev = x.get_device()
     flat = x.dim() == 2
@@ -54,8 +55,11 @@ def _norm(x, weight, eps, residual, alive_indices, residual_out, q8):
     cols = shape[-1]
     assert cols > 0, "the norm of a row without columns is undefined"
     assert eps >= 0.0, f"eps must not be negative, got {eps}"
-    x_2d = x if flat and x.is_contiguous() else rows(x, cols)
-    M = x_2d.shape[0]
+    if flat and x.is_contiguous():
+        x_2d, M, ldx = x, shape[0], cols
+    else:
+        x_2d = rows(x, cols)
+        M, ldx = x_2d.shape[0], leading(x_2d)
     if weight is not None:
         assert weight.dim() == 1 and weight.numel() == cols, (
             f"weight must have shape ({cols},), got {tuple(weight.shape)}")
@@ -65,31 +69,37 @@ def _norm(x, weight, eps, residual, alive_indices, residual_out, q8):
         if not weight.is_contiguous():
             weight = weight.contiguous()
     total = r_2d = None
+    ldr = lds = 0
     if residual is not None:
         assert (residual.shape == shape and residual.dtype is dtype and residual.is_cuda
                 and residual.get_device() == dev), "residual must have x's shape, dtype and device"
-        r_2d = residual if flat and residual.is_contiguous() else rows(residual, cols)
+        if flat and residual.is_contiguous():
+            r_2d, ldr = residual, cols
+        else:
+            r_2d = rows(residual, cols)
+            ldr = leading(r_2d)
         if residual_out is None:
-            residual_out = x.new_empty(shape)
-            total = residual_out if flat else residual_out.view(-1, cols)
+            total = residual_out = x.new_empty(shape)
+            lds = cols
         else:
             total = out_matrix("residual_out", residual_out, x, x_2d, r_2d)
+            lds = leading(total)
     else:
         assert residual_out is None, "residual_out needs a residual"
     idx, n, ld = None, cols, cols
     if alive_indices is not None:
         idx = _alive(alive_indices, dev)
         n = idx.numel()
-        ld = _round_up(n, PACK_ALIGN)
+        ld = (n + PACK_ALIGN - 1) // PACK_ALIGN * PACK_ALIGN
     scale = None
     if q8:
-        ld = _round_up(n, PACK_ALIGN_Q8)
+        ld = (n + PACK_ALIGN_Q8 - 1) // PACK_ALIGN_Q8 * PACK_ALIGN_Q8
         buf = torch.empty((M, ld), dtype=torch.float8_e4m3fn, device=x.device)
         scale = torch.empty(M, dtype=torch.float32, device=x.device)
     else:
         buf = x.new_empty((M, ld))
     if M:
-        _native.rms_norm(x_2d, r_2d, total, weight, eps, idx, n, buf, scale)
+        _native.rms_norm(x_2d, M, cols, ldx, r_2d, ldr, total, lds, weight, eps, idx, n, buf, ld, scale)
     y = buf if ld == n else buf.narrow(1, 0, n)
     if not flat:
         y = y.view(*shape[:-1], n)
