@@ -399,19 +399,29 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
       __syncthreads();
     }
     bool bad = false;
-    for (int j = threadIdx.x; j < ((pad + 3) & ~3); j += blockDim.x) {
-      uint32_t place = kNoColumn;
-      if (j < n) {
-        const int64_t c64 = __ldg(p.idx + j);
-        const uint32_t c = static_cast<uint32_t>(c64);
-        if (static_cast<uint64_t>(c64) >= static_cast<uint64_t>(cols)) {
-          bad = true;
-        } else {
+    // Eight entries per thread at a time, all loaded before the first is used.
+    const int entries = (pad + 3) & ~3;
+    for (int j0 = threadIdx.x; j0 < entries; j0 += 8 * blockDim.x) {
+      int64_t c64[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int j = j0 + i * static_cast<int>(blockDim.x);
+        c64[i] = j < n ? __ldg(p.idx + j) : -1;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int j = j0 + i * static_cast<int>(blockDim.x);
+        if (j >= entries) break;
+        const uint32_t c = static_cast<uint32_t>(c64[i]);
+        uint32_t place = kNoColumn;
+        if (static_cast<uint64_t>(c64[i]) < static_cast<uint64_t>(cols)) {
           if constexpr (Q8) atomicOr(&bits[c >> 5], 1u << (c & 31));
           place = MODE == kLong ? c : 4u * row_pos<DT, VEC>(static_cast<int>(c), cols);
+        } else if (j < n) {
+          bad = true;
         }
+        spos[j] = static_cast<uint16_t>(place);
       }
-      spos[j] = static_cast<uint16_t>(place);
     }
     if (bad && blockIdx.x == 0) raise_error(p.err, GW_DERR_BAD_INDEX);
     checked = __syncthreads_or(bad ? 1 : 0) != 0;
@@ -734,7 +744,8 @@ cudaError_t launch_rows_variant(const RowParams& p, int y_vec, int sm_count, cud
   const int cols = static_cast<int>(p.cols);
   const int cols4 = (cols + 3) & ~3;
   const int groups = WARP ? 4 : 1;
-  const int warps = WARP ? groups : std::min(32, (cols + 32 * E - 1) / (32 * E));
+  const int warps = WARP ? groups : MODE == kLong ? (cols <= kRowsHeldCols ? 16 : 32)
+                                                  : std::min(32, (cols + 32 * E - 1) / (32 * E));
   const int threads = warps * 32;
   const int npos = GATHER ? static_cast<int>((p.pad + 3) & ~int64_t{3}) : 0;
   const bool staged = GATHER && MODE != kLong;
@@ -745,10 +756,10 @@ cudaError_t launch_rows_variant(const RowParams& p, int y_vec, int sm_count, cud
   sh.stage_bytes = sh.operand_bytes * (p.r ? 2 : 1);
   // As many CTAs as make 1024 threads per SM, each with up to four rows in
   // flight; fewer CTAs where two rows each would not fit.
-  int per_sm = std::max(1, 1024 / threads);
+  int per_sm = std::max(1, (MODE == kLong ? 2048 : 1024) / threads);
   for (;; per_sm = (per_sm + 1) / 2) {
     sh.stages = ((kSmemLimit + 1024) / per_sm - 1024 - fixed) / (groups * sh.stage_bytes);
-    if (sh.stages >= 2 || per_sm == 1) break;
+    if (sh.stages >= (MODE == kLong && per_sm == 2 ? 1 : 2) || per_sm == 1) break;
   }
   if (sh.stages < 1) return cudaErrorNotSupported;
   sh.stages = std::min(sh.stages, kMaxStages);
@@ -783,7 +794,7 @@ cudaError_t launch_rows_held(const RowParams& p, bool vec, int y_vec, int sm_cou
     if (p.cols <= 256) return launch_rows_variant<DT, Q8, GATHER, kVec, 8, true, 128>(p, y_vec, sm_count, stream);
     if (p.cols <= 1024) return launch_rows_variant<DT, Q8, GATHER, kVec, 32, true, 128>(p, y_vec, sm_count, stream);
     cudaError_t e = cudaErrorNotSupported;
-    if (p.cols <= kRowsHeldCols)
+    if (p.cols <= kRowsHeldCols && (GATHER || p.cols <= 4096))
       e = launch_rows_variant<DT, Q8, GATHER, kVec, 16, false, 1024>(p, y_vec, sm_count, stream);
     if (e != cudaErrorNotSupported) return e;
     return launch_rows_variant<DT, Q8, GATHER, kLong, 16, false, 1024>(p, y_vec, sm_count, stream);
