@@ -309,7 +309,7 @@ __device__ __forceinline__ int row_pos(int k, int cols) {
 
 // Shared memory of a CTA: [2][32] partial sums and maxima (512 bytes), mbarriers
 // (groups x kMaxStages), the abort flag, then the ring, the fp32 rows, the list's
-// places and (Q8) one bit per column.
+// places and (Q8) one byte per column.
 struct RowShared {
   int stages = 0;            // rows in flight per group
   int operand_bytes = 0;     // room for one operand of one row
@@ -317,7 +317,7 @@ struct RowShared {
   int ring = 0;              // offsets
   int srow = 0;
   int spos = 0;
-  int bits = 0;
+  int flags = 0;
   int bytes = 0;
 };
 constexpr int kRowHead = 512 + 4 * kMaxStages * 8 + 64;
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
   uint8_t* ring = smem + sh.ring + group * sh.stages * sh.stage_bytes;
   float* srow = reinterpret_cast<float*>(smem + sh.srow) + group * ((cols + 3) & ~3);
   uint16_t* spos = reinterpret_cast<uint16_t*>(smem + sh.spos);   // srow bytes, or kLong: columns
-  uint32_t* bits = reinterpret_cast<uint32_t*>(smem + sh.bits);   // Q8 and GATHER: one per column
+  uint8_t* flags = smem + sh.flags;                               // Q8 and GATHER: 1 per listed column
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * groups + group;
   const int64_t step = static_cast<int64_t>(gridDim.x) * groups;
   const uint32_t row_bytes = static_cast<uint32_t>(cols * sizeof(raw));
@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
   const raw* g = static_cast<const raw*>(p.g);
   if constexpr (GATHER) {
     if constexpr (Q8) {
-      for (int i = threadIdx.x; i < (cols + 31) / 32; i += blockDim.x) bits[i] = 0;
+      for (int i = threadIdx.x; i < (cols + 3) / 4; i += blockDim.x) reinterpret_cast<uint32_t*>(flags)[i] = 0;
       __syncthreads();
     }
     bool bad = false;
@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
         const uint32_t c = static_cast<uint32_t>(c64[i]);
         uint32_t place = kNoColumn;
         if (static_cast<uint64_t>(c64[i]) < static_cast<uint64_t>(cols)) {
-          if constexpr (Q8) atomicOr(&bits[c >> 5], 1u << (c & 31));
+          if constexpr (Q8) flags[c] = 1;
           place = MODE == kLong ? c : 4u * row_pos<DT, VEC>(static_cast<int>(c), cols);
         } else if (j < n) {
           bad = true;
@@ -430,7 +430,10 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
 #pragma unroll
       for (int i = 0; i < I; ++i) {
         const int k = (i * G + t) * V;
-        if (k < cols) named |= ((bits[k >> 5] >> (k & 31)) & ((1u << V) - 1u)) << (i * V);
+        if (k < cols) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) named |= static_cast<uint32_t>(flags[k + j]) << (i * V + j);
+        }
       }
     }
   }
@@ -473,8 +476,10 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
       }
       if (first) {
         if (sum) reinterpret_cast<uint4*>(sum)[v] = pack16<DT>(f);
+        if (p.norm) {
 #pragma unroll
-        for (int j = 0; j < V / 2; ++j) ss2 = fma2(f2[j], f2[j], ss2);
+          for (int j = 0; j < V / 2; ++j) ss2 = fma2(f2[j], f2[j], ss2);
+        }
       }
       if (g) {
         if constexpr (MODE == kLong) unpack16<DT>(__ldg(reinterpret_cast<const uint4*>(g) + v), q);
@@ -510,10 +515,9 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
       for (int v = t; v * V < cols; v += G) {
         vector(v, 0, u, true);
         if constexpr (Q8) {
-          const uint32_t in = GATHER ? bits[v * V >> 5] >> (v * V & 31) : 0xFFFFFFFFu;
 #pragma unroll
           for (int j = 0; j < V; ++j)
-            if ((in >> j) & 1u) uabs = max_abs(uabs, u[j]);
+            if (!GATHER || flags[v * V + j]) uabs = max_abs(uabs, u[j]);
         }
       }
     } else {
@@ -751,7 +755,7 @@ cudaError_t launch_rows_variant(const RowParams& p, int y_vec, int sm_count, cud
   const bool staged = GATHER && MODE != kLong;
   RowShared sh;
   const int fixed = kRowHead + (staged ? groups * cols4 * 4 : 0) + npos * 2 +
-                    (GATHER && Q8 ? (cols4 + 31) / 32 * 4 : 0);
+                    (GATHER && Q8 ? cols4 : 0);
   sh.operand_bytes = (cols * (DT == GW_DTYPE_F32 ? 4 : 2) + 15) / 16 * 16 + (MODE == kAny ? 16 : 0);
   sh.stage_bytes = sh.operand_bytes * (p.r ? 2 : 1);
   // As many CTAs as make 1024 threads per SM, each with up to four rows in
@@ -766,7 +770,7 @@ cudaError_t launch_rows_variant(const RowParams& p, int y_vec, int sm_count, cud
   sh.ring = kRowHead;
   sh.srow = sh.ring + groups * sh.stages * sh.stage_bytes;
   sh.spos = sh.srow + (staged ? groups * cols4 * 4 : 0);
-  sh.bits = sh.spos + npos * 2;
+  sh.flags = sh.spos + npos * 2;
   sh.bytes = fixed + groups * sh.stages * sh.stage_bytes;
   cudaError_t e = cudaSuccess;
   if (sh.bytes > 48 * 1024) {
