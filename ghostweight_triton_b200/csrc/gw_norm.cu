@@ -47,8 +47,9 @@ __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v
 
 // The scale of a row whose largest |u| is umax and whose norm factor is rstd,
 // and the two factors that take u to y / scale (448 / umax, in two parts for a
-// tiny umax; rstd and 2^126 where the scale is at its floor: the product alone
-// may leave fp32's range).
+// tiny or a huge umax; rstd and 2^126 where the scale is at its floor: the
+// product alone may leave fp32's range). The reciprocal is the hardware's
+// approximation after one Newton step.
 struct RowScale {
   float scale, m1, m2;
 };
@@ -56,8 +57,11 @@ __device__ __forceinline__ RowScale row_scale(uint32_t umax_bits, float rstd) {
   const float umax = __uint_as_float(umax_bits);
   RowScale q;
   q.scale = umax * rstd * (1.0f / kE4m3Max);       // NaN compares false and stays
-  q.m2 = umax < 0x1p-64f ? 0x1p64f : 1.0f;
-  q.m1 = kE4m3Max / (umax * q.m2);
+  q.m2 = umax < 0x1p-64f ? 0x1p64f : umax > 0x1p64f ? 0x1p-64f : 1.0f;
+  const float v = umax * q.m2;
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  q.m1 = kE4m3Max * fmaf(r, fmaf(-v, r, 1.0f), r);
   if (q.scale < kScaleMin) {
     q.scale = kScaleMin;
     q.m1 = rstd;
@@ -65,8 +69,8 @@ __device__ __forceinline__ RowScale row_scale(uint32_t umax_bits, float rstd) {
   }
   return q;
 }
-// u m1 m2, rounded to 21 significant bits. m1 and the product are each off by at
-// most 2^-24, so a quotient that lies exactly between two e4m3 values (at most 5
+// u m1 m2, rounded to 21 significant bits. m1 is off by at most 2^-23 (its Newton
+// step and the factor 448 round once each), the product by 2^-24 more, so a quotient that lies exactly between two e4m3 values (at most 5
 // bits) comes out as such and rounds to even. Splitting by 2^3 + 1 (Dekker)
 // gives the upper bits: three operations instead of a division's dozen.
 __device__ __forceinline__ float to_scale(float u, const RowScale& q) {
@@ -453,8 +457,12 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
   const float inv_cols = 1.0f / static_cast<float>(cols);
   int buf = 0, stage = 0;
   uint32_t phase = 0;
-  for (int64_t row = row0; row < p.rows; row += step) {
-    raw* sum = p.s ? static_cast<raw*>(p.s) + row * p.lds : nullptr;
+  // The row's place in each output, moved along with the row.
+  raw* sum = p.s ? static_cast<raw*>(p.s) + row0 * p.lds : nullptr;
+  out* y = static_cast<out*>(p.y) + row0 * p.ldy;
+  const int64_t sum_step = p.s ? step * p.lds : 0;
+  const int64_t y_step = step * p.ldy;
+  for (int64_t row = row0; row < p.rows; row += step, sum += sum_step, y += y_step) {
     const uint8_t* xs = ring + stage * sh.stage_bytes;
     const uint8_t* rs = xs + sh.operand_bytes;
     // A wait that runs out raises the device error word and the abort flag; the
@@ -609,7 +617,6 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
       q8 = row_scale(umax, rstd);
       if (t == 0) p.scale[row] = q8.scale;
     }
-    out* y = static_cast<out*>(p.y) + row * p.ldy;
     auto value = [&](float v) { return Q8 ? to_scale(v, q8) : v * rstd; };
     auto value2 = [&](float2 v) { return Q8 ? to_scale2(v, q8) : mul2(v, both(rstd)); };
     auto store1 = [&](int j, float v) {
@@ -664,23 +671,30 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
           c[0] = spos[j];
         }
       };
-      const int whole = checked ? 0 : n / kPack * kPack;   // outputs that all have a column
       int j = t * kPack;
+      if (y_vec && !checked) {
+        // Every output of these groups has a column: no checks.
+        const int whole = n / kPack * kPack;
+        uint32_t* yw = reinterpret_cast<uint32_t*>(y + j);
 #pragma unroll 4
-      for (; j < whole; j += G * kPack) {
-        uint32_t c[kPack];
-        __align__(16) float v[kPack];
-        read(j, c);
+        for (; j < whole; j += G * kPack, yw += G) {
+          uint32_t c[kPack];
+          __align__(16) float v[kPack];
+          read(j, c);
 #pragma unroll
-        for (int e = 0; e < kPack; ++e) v[e] = *reinterpret_cast<const float*>(sr + c[e]);
-        if constexpr (kPack == 1) {
-          v[0] = value(v[0]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < kPack; e += 2)
-            *reinterpret_cast<float2*>(v + e) = value2(*reinterpret_cast<const float2*>(v + e));
+          for (int e = 0; e < kPack; ++e) v[e] = *reinterpret_cast<const float*>(sr + c[e]);
+          if constexpr (kPack == 1) {
+            *yw = __float_as_uint(value(v[0]));
+          } else {
+            const float2 a = value2(make_float2(v[0], v[1]));
+            if constexpr (!Q8) {
+              *yw = Elem<DT>::pack2(a.x, a.y);
+            } else {
+              const float2 b = value2(make_float2(v[2], v[3]));
+              *yw = e4m3_pack2(a.x, a.y) | (e4m3_pack2(b.x, b.y) << 16);
+            }
+          }
         }
-        store_pack(j, v);
       }
       for (; j < pad; j += G * kPack) {
         uint32_t c[kPack];
