@@ -198,13 +198,22 @@ def _rowmajor(*ts: torch.Tensor) -> None:
 
 def _residual(t: torch.Tensor | None) -> tuple[int | None, int]:
     """(pointer, leading dimension) of a residual matrix, or of none."""
-    return (None, 0) if t is None else (t.data_ptr(), max(t.stride(0), t.shape[1]))
+    if t is None:
+        return None, 0
+    ld, cols = t.stride(0), t.shape[1]
+    return t.data_ptr(), ld if ld > cols else cols
 
 
 try:  # the raw cudaStream_t of torch's current stream, without building a Stream object
     _raw_stream = torch._C._cuda_getCurrentRawStream
 except AttributeError:  # pragma: no cover - older torch
     _raw_stream = None
+
+
+try:  # torch.cuda.is_current_stream_capturing without its wrapper
+    _capturing = torch._C._cuda_isCurrentStreamCapturing
+except AttributeError:  # pragma: no cover - older torch
+    _capturing = torch.cuda.is_current_stream_capturing
 
 
 def _stream(device: torch.device) -> int:
@@ -332,7 +341,7 @@ _gemm_ws: dict[tuple[int, int], torch.Tensor] = {}
 
 
 def gemm_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
     dev = device.index if device.index is not None else torch.cuda.current_device()
     key = (dev, _stream(device))
@@ -356,10 +365,12 @@ def gather_gemm(x: torch.Tensor, w_packed: torch.Tensor, idx: torch.Tensor, y: t
     enough, else the single fused kernel; "fused" / "pregather" force one;
     "runs" loads x directly (idx must be 64-column runs: see index_runs).
     """
-    _rowmajor(x, w_packed, y)
-    assert idx.dtype == torch.int64 and idx.is_contiguous()
+    assert idx.dtype is torch.int64 and idx.is_contiguous()
     M, K = x.shape
-    N = w_packed.shape[0]
+    N, wk = w_packed.shape
+    (sx, ux), (sw, uw), (sy, uy) = x.stride(), w_packed.stride(), y.stride()
+    if (ux != 1 and K > 1) or (uw != 1 and wk > 1) or (uy != 1 and y.shape[1] > 1):
+        _rowmajor(x, w_packed, y)                # raises
     n = idx.numel()
     ws_ptr, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
     dev = x.get_device()
@@ -367,11 +378,13 @@ def gather_gemm(x: torch.Tensor, w_packed: torch.Tensor, idx: torch.Tensor, y: t
     if dev != cur:
         torch.cuda.set_device(dev)
     try:
+        r_ptr, ldr = _residual(residual) if residual is not None else (None, 0)
         st = api().gw_gather_gemm_residual(
-            x.data_ptr(), DTYPE_CODES[x.dtype], M, K, max(x.stride(0), K), w_packed.data_ptr(), N,
-            max(w_packed.stride(0), n), idx.data_ptr(), n, _ptr(bias), epilogue_code(activation),
-            *_residual(residual), y.data_ptr(), max(y.stride(0), N), GEMM_STRATEGIES[strategy], ws_ptr,
-            ws_bytes, _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream)
+            x.data_ptr(), DTYPE_CODES[x.dtype], M, K, sx if sx > K else K, w_packed.data_ptr(), N,
+            sw if sw > n else n, idx.data_ptr(), n, None if bias is None else bias.data_ptr(),
+            EPILOGUES[activation] if activation in EPILOGUES else epilogue_code(activation),
+            r_ptr, ldr, y.data_ptr(), sy if sy > N else N, GEMM_STRATEGIES[strategy], ws_ptr, ws_bytes,
+            _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream)
     finally:
         if dev != cur:
             torch.cuda.set_device(cur)
@@ -514,33 +527,28 @@ def packed_gemm(a: torch.Tensor, w_packed: torch.Tensor, y: torch.Tensor,
     _check(st, "gw_packed_gemm")
 
 
-def packed_gemm_q8(a: torch.Tensor, a_scale: torch.Tensor, w_packed: torch.Tensor, w_scale: torch.Tensor,
-                   y: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
+def packed_gemm_q8(a: torch.Tensor, a_scale: torch.Tensor, M: int, K: int, lda: int, w_packed: torch.Tensor,
+                   w_scale: torch.Tensor, N: int, ldw: int, y: torch.Tensor, ldy: int,
+                   bias: torch.Tensor | None = None, activation: str | None = None,
                    residual: torch.Tensor | None = None) -> None:
     """y = act(a_scale w_scale (a @ w_packed^T) + bias) + residual over e4m3 operands by TMA."""
-    _rowmajor(y)
-    M, K = a.shape
-    N = w_packed.shape[0]
     dev = a.get_device()
     cur = torch.cuda.current_device()
     if dev != cur:
         torch.cuda.set_device(dev)
     try:
+        r_ptr, ldr = _residual(residual) if residual is not None else (None, 0)
         st = api().gw_packed_gemm_q8(
-            a.data_ptr(), a_scale.data_ptr(), M, K, _ld16(a), w_packed.data_ptr(), w_scale.data_ptr(), N,
-            _ld16(w_packed), _ptr(bias), epilogue_code(activation), *_residual(residual), y.data_ptr(),
-            dtype_code(y.dtype), max(y.stride(0), N),
+            a.data_ptr(), a_scale.data_ptr(), M, K, lda, w_packed.data_ptr(), w_scale.data_ptr(), N, ldw,
+            None if bias is None else bias.data_ptr(),
+            EPILOGUES[activation] if activation in EPILOGUES else epilogue_code(activation),
+            r_ptr, ldr, y.data_ptr(), DTYPE_CODES[y.dtype], ldy,
             _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream)
     finally:
         if dev != cur:
             torch.cuda.set_device(cur)
     if st:
         _check(st, "gw_packed_gemm_q8")
-
-
-def _ld16(t: torch.Tensor) -> int:
-    """Leading dimension of e4m3 rows; a matrix of one row has any, so a multiple of 16."""
-    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
 
 
 def dynamic_linear(x: torch.Tensor, weight: torch.Tensor, threshold: float, y: torch.Tensor,

@@ -214,7 +214,12 @@ def ghost_linear(
         x = x.contiguous()
     M = x.shape[0]
     N = w_packed.shape[0]
-    y, residual = _product_out(out, residual, M, N, x)
+    if out is None:
+        y = x.new_empty((M, N))
+        if residual is not None:
+            residual = residual_matrix(residual, (M, N), x)
+    else:
+        y, residual = _product_out(out, residual, M, N, x)
     if M and N:
         _gemm(x, w_packed, alive_indices, y, bias, activation, strategy, residual)
     return y
@@ -284,21 +289,27 @@ def packed_linear(
     return y
 
 
-def _q8_operand(what: str, q: torch.Tensor, scale: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """An e4m3 matrix whose rows TMA can load (16-byte aligned; copied into such rows if it
-    is not) and its scales [rows]."""
-    assert q.is_cuda and q.dtype is torch.float8_e4m3fn and q.dim() == 2, (
-        f"{what} must be a float8_e4m3fn matrix on CUDA, got {q.dtype} {tuple(q.shape)}")
+def _q8_operand(what: str, q: torch.Tensor, scale: torch.Tensor, dev: int) -> tuple:
+    """(matrix, rows, columns, leading dimension, scales) of an e4m3 operand, in rows that TMA
+    can load (16-byte aligned; copied into such rows if they are not)."""
+    assert q.dtype is torch.float8_e4m3fn and q.dim() == 2 and q.is_cuda and q.get_device() == dev, (
+        f"{what} must be a float8_e4m3fn matrix on one CUDA device with the others, got {q.dtype} "
+        f"{tuple(q.shape)} on {q.device}")
     rows, cols = q.shape
     assert (scale.dtype is torch.float32 and scale.dim() == 1 and scale.numel() == rows and scale.is_cuda
-            and scale.get_device() == q.get_device()), (
+            and scale.get_device() == dev), (
         f"{what}_scale must be float32 of shape ({rows},) on {what}'s device")
-    s0, s1 = q.stride()
-    if (cols > 1 and s1 != 1) or q.data_ptr() % 16 or (rows > 1 and (s0 % 16 or s0 < cols)):
-        buf = torch.zeros((rows, (cols + 15) // 16 * 16), dtype=q.dtype, device=q.device)
+    if not scale.is_contiguous():
+        scale = scale.contiguous()
+    ld, unit = q.stride()
+    if (unit != 1 and cols > 1) or q.data_ptr() % 16 or (rows > 1 and (ld % 16 or ld < cols)):
+        ld = (cols + 15) // 16 * 16
+        buf = torch.zeros((rows, ld), dtype=q.dtype, device=q.device)
         buf[:, :cols] = q
-        q = buf[:, :cols]
-    return q, scale if scale.is_contiguous() else scale.contiguous()
+        q = buf
+    elif rows <= 1:
+        ld = (cols + 15) // 16 * 16
+    return q, rows, cols, ld, scale
 
 
 def packed_linear_q8(
@@ -321,16 +332,14 @@ def packed_linear_q8(
     or the output's, else float16 with a float16 bias, else bfloat16); residual
     [M, N] has it too, bias is converted to it. ``out`` may be the residual itself.
     """
-    a, a_scale = _q8_operand("a", a, a_scale)
-    w_packed, w_scale = _q8_operand("w_packed", w_packed, w_scale)
-    dev = a.get_device()
-    assert dev == w_packed.get_device(), "a and w_packed must be on one device"
-    (M, K), (N, K_w) = a.shape, w_packed.shape
+    dev = a.get_device() if a.is_cuda else -1
+    a, M, K, lda, a_scale = _q8_operand("a", a, a_scale, dev)
+    w_packed, N, K_w, ldw, w_scale = _q8_operand("w_packed", w_packed, w_scale, dev)
     assert K == K_w, f"K mismatch: a has {K} columns, w_packed {K_w}"
     if dtype is None:
         dtype = next((t.dtype for t in (residual, out) if t is not None),
                      bias.dtype if bias is not None and bias.dtype is torch.float16 else torch.bfloat16)
-    if dtype not in (torch.float16, torch.bfloat16):
+    if dtype is not torch.float16 and dtype is not torch.bfloat16:
         raise TypeError(f"unsupported output dtype {dtype}; expected float16 or bfloat16")
     if bias is not None:
         assert bias.dim() == 1 and bias.numel() == N and bias.is_cuda and bias.get_device() == dev, (
@@ -338,16 +347,17 @@ def packed_linear_q8(
         if bias.dtype is not dtype or not bias.is_contiguous():
             bias = bias.detach().to(dtype).contiguous()
     if out is None:
-        y = torch.empty((M, N), dtype=dtype, device=a.device)
+        y, ldy = a.new_empty((M, N), dtype=dtype), N
         if residual is not None:
             residual = residual_matrix(residual, (M, N), y)
     else:
         assert out.shape == (M, N) and out.dtype is dtype and out.is_cuda and out.get_device() == dev, (
             f"out must be {dtype} of shape {(M, N)} on a's device")
+        assert (out.stride(1) == 1 or N <= 1) and (out.stride(0) >= N or M <= 1), "out must be a row-major matrix"
         y, residual = _product_out(out, residual, M, N, out)
+        ldy = max(y.stride(0), N)
     if M and N:
-        _native.packed_gemm_q8(a, a_scale, w_packed, w_scale, y, bias=bias, activation=activation,
-                               residual=residual)
+        _native.packed_gemm_q8(a, a_scale, M, K, lda, w_packed, w_scale, N, ldw, y, ldy, bias, activation, residual)
     return y
 
 
