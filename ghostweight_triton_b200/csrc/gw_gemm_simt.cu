@@ -3,12 +3,19 @@
 // The reference runs fp32 inputs through tl.dot with allow_tf32=False
 // (ghostweight_triton/kernels/matmul.py:127-130) so results hold a 1e-4
 // tolerance; tcgen05 has no exact-fp32 kind, so fp32 uses FFMA:
-//   y[m, n] = act( sum_j x[m, idx[j]] * w[n, j] + bias[n] )
-// Tiles of 128 x 128 outputs, k-steps of 8, 256 threads each owning an 8 x 8
-// register micro-tile; the A tile is gathered through the index list while it
-// is staged into shared memory (k-major), the packed weight tile is read with
-// consecutive threads on consecutive k. Double-buffered shared memory, one
-// __syncthreads per k-step.
+//   y[m, n] = act( sum_j x[m, idx[j]] * w[n, j] + bias[n] ) + residual[m, n]
+// Every output is one chain of fused multiply-adds over j in ascending order,
+// whatever the tile, so its bits do not depend on the tile chosen.
+//
+// What bounds it is the FP32 pipe for tall outputs (74 TFLOP/s at 148 x 128
+// lanes and 1.96 GHz) and the latency of the k loop for small ones. Tiles of
+// BM x BN outputs, BK columns per stage; both operands arrive by cp.async, the
+// alive columns of x as single elements through the list (loaded a stage
+// ahead), W' as 16-byte vectors, S - 1 stages ahead of the arithmetic. Shared
+// rows hold BK + 4 floats: a thread reads four columns of a row as one vector,
+// and eight neighbouring rows cover all 32 banks.
+// Tiles of 64 x 64 outputs where they make four CTAs per SM, 32 x 64 below (their
+// finer grain evens out the SMs' shares), 16 x 32 for at most 16 rows.
 #include "gw_common.cuh"
 #include "gw_internal.h"
 
@@ -16,116 +23,233 @@ namespace gw {
 
 namespace {
 
-constexpr int kSBM = 128;
-constexpr int kSBN = 128;
-constexpr int kSBK = 8;
-constexpr int kSThreads = 256;
+__device__ __forceinline__ void cp_async4(uint32_t dst, const float* src, bool valid) {
+  const uint32_t bytes = valid ? 4u : 0u;          // 0: the destination becomes zero
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" :: "r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const float* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory");
+}
 
-__global__ void __launch_bounds__(kSThreads)
-gemm_f32_kernel(const float* __restrict__ x, int64_t M, int64_t K, int64_t ldx,
-                const float* __restrict__ w, int64_t N, int64_t ldw,
-                const int64_t* __restrict__ idx, int64_t n_alive,
-                const float* __restrict__ bias, int epi, float* y, int64_t ldy,
-                unsigned int* err, const int32_t* __restrict__ n_dev, const float* res,
-                int64_t ldr) {
-  // n_dev: the alive count on the device (n_alive is then an upper bound).
-  if (n_dev) n_alive = min(n_alive, static_cast<int64_t>(max(*n_dev, 0)));
-  // +4 floats per k-row: conflict-free loader stores, rows stay 16-byte aligned.
-  __shared__ __align__(16) float As[2][kSBK][kSBM + 4];
-  __shared__ __align__(16) float Bs[2][kSBK][kSBN + 4];
+struct SimtParams {
+  const float* x;
+  int64_t M;
+  int64_t K;
+  int64_t ldx;
+  const float* w;
+  int64_t N;
+  int64_t ldw;
+  const int64_t* idx;
+  int64_t n_alive;
+  const float* bias;
+  int epi;
+  float* y;
+  int64_t ldy;
+  unsigned int* err;
+  const int32_t* n_dev;      // the alive count on the device (n_alive is then an upper bound)
+  const float* res;          // residual (or null), leading dimension ldr
+  int64_t ldr;
+  int w_vec;                 // W' rows may be read as 16-byte vectors
+};
 
+template <int BM, int BN, int BK, int TM, int TN, int S>
+struct SimtCfg {
+  static constexpr int kThreads = (BM / TM) * (BN / TN);
+  static constexpr int kRow = BK + 4;                              // floats per shared row
+  static constexpr int kStageFloats = (BM + BN) * kRow;
+  static constexpr int kSmemBytes = S * kStageFloats * 4;
+  static constexpr int kARows = kThreads / BK;                     // rows of x per pass of the threads
+  static constexpr int kAPer = BM / kARows;                        // elements of x per thread and stage
+  static constexpr int kBVecs = BN * (BK / 4);                     // vectors of W' per stage
+  static constexpr int kBPer = (kBVecs + kThreads - 1) / kThreads;
+  static_assert(kThreads % BK == 0 && BM % kARows == 0, "whole passes over the tile of x");
+};
+
+template <int BM, int BN, int BK, int TM, int TN, int S>
+__global__ void __launch_bounds__((BM / TM) * (BN / TN))
+gemm_f32_kernel(const SimtParams p) {
+  using C = SimtCfg<BM, BN, BK, TM, TN, S>;
+  extern __shared__ __align__(16) float smem_f[];
+  const uint32_t smem_s = smem_u32(smem_f);
+  int64_t n_alive = p.n_alive;
+  if (p.n_dev) n_alive = min(n_alive, static_cast<int64_t>(max(*p.n_dev, 0)));
   const int tid = threadIdx.x;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * kSBM;
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * kSBN;
-
-  // Loader mapping: 128 rows x 8 k per tile = 1024 elements, 4 per thread.
-  // Thread t loads k = t % 8 for rows t / 8 + 32 * i (i = 0..3).
-  const int lk = tid & 7;
-  const int lr = tid >> 3;   // 0..31
-
-  // Compute mapping: 16 x 16 threads, each 8 x 8 outputs (rows ty*4 + {0..3, 64..67}).
-  const int tx = tid & 15;
-  const int ty = tid >> 4;
-
-  float acc[8][8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[i][j] = 0.0f;
-
-  const int64_t nk = (n_alive + kSBK - 1) / kSBK;
+  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * BM;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * BN;
+  // A warp is 4 x 8 threads: a vector load of W' touches eight rows (all 32
+  // banks), one of x four, each shared by the threads beside or below.
+  const int lane = tid & 31;
+  constexpr int kWarpsN = BN / (8 * TN);
+  const int row_t = (tid >> 5) / kWarpsN * (4 * TM) + (lane >> 3);   // rows row_t + 4 i
+  const int col_t = (tid >> 5) % kWarpsN * (8 * TN) + (lane & 7);    // columns col_t + 8 j
+  const int lk = tid % BK;                           // this thread's column of x tiles
+  const int lr = tid / BK;
+  const int nk = static_cast<int>((n_alive + BK - 1) / BK);
   bool bad = false;
 
-  auto load_tile = [&](int64_t kt, float (&a_reg)[4], float (&b_reg)[4]) {
-    const int64_t kk = kt * kSBK + lk;
-    int64_t col = -1;
-    if (kk < n_alive) {
-      col = __ldg(idx + kk);
-      if (col < 0 || col >= K) { bad = true; col = -1; }
-    }
+  auto column = [&](int kt) {                        // the alive column this thread loads in step kt
+    const int64_t j = static_cast<int64_t>(kt) * BK + lk;
+    if (j >= n_alive) return int64_t{-1};
+    const int64_t c = __ldg(p.idx + j);
+    if (c >= 0 && c < p.K) return c;
+    bad = true;
+    return int64_t{-1};
+  };
+  // This thread's rows of x and vectors of W', and where they go in a stage.
+  const float* x_row[C::kAPer];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t m = m0 + lr + 32 * i;
-      a_reg[i] = (m < M && col >= 0) ? __ldg(x + m * ldx + col) : 0.0f;
-      const int64_t n = n0 + lr + 32 * i;
-      b_reg[i] = (n < N && kk < n_alive) ? __ldg(w + n * ldw + kk) : 0.0f;
+  for (int i = 0; i < C::kAPer; ++i) {
+    const int64_t m = m0 + lr + i * C::kARows;
+    x_row[i] = m < p.M ? p.x + m * p.ldx : nullptr;
+  }
+  const uint32_t a_dst = static_cast<uint32_t>((lr * C::kRow + lk) * 4);
+  const float* w_vec[C::kBPer];
+#pragma unroll
+  for (int i = 0; i < C::kBPer; ++i) {
+    const int v = tid + i * C::kThreads;
+    const int64_t n = n0 + v / (BK / 4);
+    w_vec[i] = v < C::kBVecs && n < p.N ? p.w + n * p.ldw + (v % (BK / 4)) * 4 : nullptr;
+  }
+  const uint32_t b_dst = static_cast<uint32_t>((BM * C::kRow + tid / (BK / 4) * C::kRow + (tid % (BK / 4)) * 4) * 4);
+  static_assert(C::kThreads % (BK / 4) == 0, "a thread's vectors of W' share one column");
+  const int n_cols = static_cast<int>(n_alive);
+  auto load = [&](int kt, int stage, int64_t col) {  // both tiles of k step kt
+    const uint32_t st = smem_s + static_cast<uint32_t>(stage * C::kStageFloats * 4);
+#pragma unroll
+    for (int i = 0; i < C::kAPer; ++i) {
+      const bool ok = col >= 0 && x_row[i] != nullptr;
+      cp_async4(st + a_dst + i * C::kARows * C::kRow * 4, ok ? x_row[i] + col : p.x, ok);
+    }
+    if (p.w_vec) {
+      const int left = n_cols - (kt * BK + (tid % (BK / 4)) * 4);
+      const uint32_t want = left >= 4 ? 16u : left > 0 ? static_cast<uint32_t>(left) * 4u : 0u;
+#pragma unroll
+      for (int i = 0; i < C::kBPer; ++i) {
+        if (C::kBVecs % C::kThreads == 0 || tid + i * C::kThreads < C::kBVecs) {
+          const uint32_t bytes = w_vec[i] ? want : 0u;
+          cp_async16(st + b_dst + i * (C::kThreads / (BK / 4)) * C::kRow * 4, bytes ? w_vec[i] + kt * BK : p.w, bytes);
+        }
+      }
+    } else {
+      for (int e = tid; e < BN * BK; e += C::kThreads) {
+        const int r = e / BK;
+        const int64_t k = static_cast<int64_t>(kt) * BK + e % BK;
+        const bool ok = n0 + r < p.N && k < n_alive;
+        cp_async4(st + static_cast<uint32_t>((BM * C::kRow + r * C::kRow + e % BK) * 4),
+                  ok ? p.w + (n0 + r) * p.ldw + k : p.w, ok);
+      }
     }
   };
-  auto store_tile = [&](int buf, const float (&a_reg)[4], const float (&b_reg)[4]) {
+
+  float acc[TM][TN];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      As[buf][lk][lr + 32 * i] = a_reg[i];
-      Bs[buf][lk][lr + 32 * i] = b_reg[i];
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = 0.0f;
+
+  // One commit per stage, empty at the end, so that the count of groups in
+  // flight says which stage has landed. The list is read four stages ahead of
+  // the loads that need it: an entry on its way from L2 held up every stage of
+  // a small tile otherwise.
+  constexpr int kAhead = 4;
+  int64_t cols[S - 1 + kAhead];
+#pragma unroll
+  for (int s = 0; s < S - 1 + kAhead; ++s) cols[s] = s < nk ? column(s) : -1;
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) {
+    if (s < nk) load(s, s, cols[s]);
+    cp_async_commit();
+  }
+  int64_t next[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) next[i] = cols[S - 1 + i];
+  int stage = 0, free_stage = S - 1;                 // of step kt, and of step kt + S - 1
+  for (int kt = 0; kt < nk; ++kt) {
+    cp_async_wait<S - 2>();
+    __syncthreads();                                 // stage kt landed; stage kt - 1 is free
+    if (kt + S - 1 < nk) load(kt + S - 1, free_stage, next[0]);
+    free_stage = stage;
+    cp_async_commit();
+#pragma unroll
+    for (int i = 0; i + 1 < kAhead; ++i) next[i] = next[i + 1];
+    next[kAhead - 1] = kt + S - 1 + kAhead < nk ? column(kt + S - 1 + kAhead) : -1;
+    const float* a_t = smem_f + stage * C::kStageFloats;
+    if (++stage == S) stage = 0;
+    const float* b_t = a_t + BM * C::kRow;
+#pragma unroll
+    for (int k = 0; k < BK; k += 4) {
+      float4 b[TN];
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+        b[j] = *reinterpret_cast<const float4*>(b_t + (col_t + 8 * j) * C::kRow + k);
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const float4 a = *reinterpret_cast<const float4*>(a_t + (row_t + 4 * i) * C::kRow + k);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          float v = fmaf(a.x, b[j].x, acc[i][j]);
+          v = fmaf(a.y, b[j].y, v);
+          v = fmaf(a.z, b[j].z, v);
+          acc[i][j] = fmaf(a.w, b[j].w, v);
+        }
+      }
+    }
+  }
+  cp_async_wait<0>();
+  if (bad) raise_error(p.err, GW_DERR_BAD_INDEX);
+
+  auto store = [&](const float (*r)[TN]) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const int64_t m = m0 + row_t + 4 * i;
+      if (m >= p.M) continue;
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int64_t n = n0 + col_t + 8 * j;
+        if (n >= p.N) continue;
+        float v = acc[i][j];
+        if (p.bias) v += __ldg(p.bias + n);
+        v = apply_epilogue(v, p.epi);
+        if (r) v += r[i][j];
+        p.y[m * p.ldy + n] = v;
+      }
     }
   };
-
-  float a_reg[4], b_reg[4];
-  if (nk > 0) {
-    load_tile(0, a_reg, b_reg);
-    store_tile(0, a_reg, b_reg);
-  }
-  __syncthreads();
-
-  for (int64_t kt = 0; kt < nk; ++kt) {
-    const int buf = static_cast<int>(kt & 1);
-    const bool more = (kt + 1 < nk);
-    if (more) load_tile(kt + 1, a_reg, b_reg);
+  if (p.res) {
+    // All of the residual before the first store: y may be the residual, so a
+    // load behind a store would wait for it.
+    float r[TM][TN];
 #pragma unroll
-    for (int k = 0; k < kSBK; ++k) {
-      float a[8], b[8];
-      const float4 a0 = *reinterpret_cast<const float4*>(&As[buf][k][ty * 4]);
-      const float4 a1 = *reinterpret_cast<const float4*>(&As[buf][k][ty * 4 + 64]);
-      const float4 b0 = *reinterpret_cast<const float4*>(&Bs[buf][k][tx * 4]);
-      const float4 b1 = *reinterpret_cast<const float4*>(&Bs[buf][k][tx * 4 + 64]);
-      a[0] = a0.x; a[1] = a0.y; a[2] = a0.z; a[3] = a0.w;
-      a[4] = a1.x; a[5] = a1.y; a[6] = a1.z; a[7] = a1.w;
-      b[0] = b0.x; b[1] = b0.y; b[2] = b0.z; b[3] = b0.w;
-      b[4] = b1.x; b[5] = b1.y; b[6] = b1.z; b[7] = b1.w;
+    for (int i = 0; i < TM; ++i) {
+      const int64_t m = m0 + row_t + 4 * i;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
+      for (int j = 0; j < TN; ++j) {
+        const int64_t n = n0 + col_t + 8 * j;
+        r[i][j] = m < p.M && n < p.N ? p.res[m * p.ldr + n] : 0.0f;
+      }
     }
-    if (more) store_tile(buf ^ 1, a_reg, b_reg);
-    __syncthreads();
+    store(r);
+  } else {
+    store(nullptr);
   }
-  if (bad) raise_error(err, GW_DERR_BAD_INDEX);
+}
 
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t m = m0 + ty * 4 + (i & 3) + (i >= 4 ? 64 : 0);
-    if (m >= M) continue;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int64_t n = n0 + tx * 4 + (j & 3) + (j >= 4 ? 64 : 0);
-      if (n >= N) continue;
-      float v = acc[i][j];
-      if (bias) v += __ldg(bias + n);
-      v = apply_epilogue(v, epi);
-      if (res) v += res[m * ldr + n];
-      y[m * ldy + n] = v;
-    }
-  }
+template <int BM, int BN, int BK, int TM, int TN, int S>
+cudaError_t launch_simt(const SimtParams& p, cudaStream_t stream) {
+  using C = SimtCfg<BM, BN, BK, TM, TN, S>;
+  const int64_t gx = (p.N + BN - 1) / BN;
+  const int64_t gy = (p.M + BM - 1) / BM;
+  if (gx > 0x7FFFFFFFll || gy > 65535) return cudaErrorInvalidValue;
+  auto kern = gemm_f32_kernel<BM, BN, BK, TM, TN, S>;
+  cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kern), C::kSmemBytes);
+  if (e != cudaSuccess) return e;
+  kern<<<dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy)), C::kThreads, C::kSmemBytes, stream>>>(p);
+  return cudaGetLastError();
 }
 
 }  // namespace
@@ -136,14 +260,35 @@ cudaError_t launch_gemm_f32(const float* x, int64_t M, int64_t K, int64_t ldx, c
                             unsigned int* err, cudaStream_t stream, const int32_t* n_dev,
                             const Residual& res) {
   if (M == 0 || N == 0) return cudaSuccess;
-  const int64_t gx = (N + kSBN - 1) / kSBN;
-  const int64_t gy = (M + kSBM - 1) / kSBM;
-  if (gx > 0x7FFFFFFFll || gy > 65535) return cudaErrorInvalidValue;
-  dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(gy));
-  gemm_f32_kernel<<<grid, kSThreads, 0, stream>>>(x, M, K, ldx, w, N, ldw, idx, n_alive, bias,
-                                                  epilogue, y, ldy, err, n_dev,
-                                                  static_cast<const float*>(res.p), res.ld);
-  return cudaGetLastError();
+  SimtParams p{};
+  p.x = x;
+  p.M = M;
+  p.K = K;
+  p.ldx = ldx;
+  p.w = w;
+  p.N = N;
+  p.ldw = ldw;
+  p.idx = idx;
+  p.n_alive = n_alive;
+  p.bias = bias;
+  p.epi = epilogue;
+  p.y = y;
+  p.ldy = ldy;
+  p.err = err;
+  p.n_dev = n_dev;
+  p.res = static_cast<const float*>(res.p);
+  p.ldr = res.ld;
+  p.w_vec = ((reinterpret_cast<uintptr_t>(w) & 15u) == 0 && (N <= 1 || ldw % 4 == 0)) ? 1 : 0;
+  // Measured (us) for M x N x K' = 1024 x 768 x 384, 100 x 4096 x 2048, 1024 x
+  // 4096 x 2048 and 4096 x 4096 x 2048: 64 x 64 tiles 32, 116, 532 and 1792; 32
+  // x 64 tiles 27, 99, 605 and 2234; 128 x 128 tiles (one or two CTAs per SM hold
+  // their registers) 92, 408, 565 and 2000. 16 x 4096 x 2048: 16 x 32 tiles with
+  // 64 columns a stage 42, with 32 columns 62; 32 x 32 tiles 71.
+  auto ctas = [&](int64_t bm, int64_t bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
+  constexpr int64_t kSms = 148;
+  if (M <= 16) return launch_simt<16, 32, 64, 2, 2, 4>(p, stream);
+  if (ctas(64, 64) < 4 * kSms) return launch_simt<32, 64, 32, 4, 4, 3>(p, stream);
+  return launch_simt<64, 64, 32, 8, 4, 3>(p, stream);
 }
 
 }  // namespace gw
