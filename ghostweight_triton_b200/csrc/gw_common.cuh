@@ -646,6 +646,33 @@ __device__ __forceinline__ void add_bias4(float (&f)[4], const uint16_t* bias, i
       if (n0 + j < N) f[j] += Elem<DT>::to_f(__ldg(bias + n0 + j));
   }
 }
+// Two fp32 operations in one instruction, each rounded on its own.
+__device__ __forceinline__ uint64_t pair_bits(float2 v) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+  return r;
+}
+__device__ __forceinline__ float2 bits_pair(uint64_t r) {
+  float2 v;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
+  return v;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)));
+  return bits_pair(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)));
+  return bits_pair(r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)), "l"(pair_bits(c)));
+  return bits_pair(r);
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 // Scales of e4m3 operands, applied to the fp32 accumulator in front of the bias:
 // f[j] * row * w[n0 + j]. First by the row's scale: the product of the two
 // scales alone could leave fp32's range.
@@ -656,15 +683,65 @@ __device__ __forceinline__ void scale32(float (&f)[32], float row, const float* 
 #pragma unroll
     for (int v = 0; v < 8; ++v) {
       const float4 q = __ldg(reinterpret_cast<const float4*>(s) + v);
-      f[4 * v] = f[4 * v] * row * q.x;
-      f[4 * v + 1] = f[4 * v + 1] * row * q.y;
-      f[4 * v + 2] = f[4 * v + 2] * row * q.z;
-      f[4 * v + 3] = f[4 * v + 3] * row * q.w;
+      const float2 a = mul2(mul2(make_float2(f[4 * v], f[4 * v + 1]), both(row)), make_float2(q.x, q.y));
+      const float2 b = mul2(mul2(make_float2(f[4 * v + 2], f[4 * v + 3]), both(row)), make_float2(q.z, q.w));
+      f[4 * v] = a.x; f[4 * v + 1] = a.y; f[4 * v + 2] = b.x; f[4 * v + 3] = b.y;
     }
   } else {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
       if (n0 + j < N) f[j] = f[j] * row * __ldg(s + j);
+  }
+}
+// Bias and activation behind scale32, two values at a time. The tanh form of the
+// GELU as v / (1 + 2^(v (k1 + k2 v^2))), with k1 = -2 sqrt(2 / pi) log2(e) and
+// k2 = 0.044715 k1: five operations and two approximations (ex2, rcp) a value,
+// each a few ulp of fp32, far below the 16-bit rounding behind it. With a tensor
+// core twice as fast as for 16-bit operands the epilogue has half the time.
+template <int DT, int EPI>
+__device__ __forceinline__ void bias_activate32(float (&f)[32], const uint16_t* bias, int64_t n0, int64_t N) {
+  if (bias) {
+    const uint16_t* b = bias + n0;
+    if (n0 + 32 <= N && (reinterpret_cast<uintptr_t>(b) & 15u) == 0) {
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const uint4 q = __ldg(reinterpret_cast<const uint4*>(b) + v);
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int j = 8 * v + 2 * k;
+          const float2 a = add2(make_float2(f[j], f[j + 1]),
+                                make_float2(Elem<DT>::to_f(static_cast<uint16_t>(w[k] & 0xFFFFu)),
+                                            Elem<DT>::to_f(static_cast<uint16_t>(w[k] >> 16))));
+          f[j] = a.x; f[j + 1] = a.y;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (n0 + j < N) f[j] += Elem<DT>::to_f(__ldg(b + j));
+    }
+  }
+  if constexpr (EPI == GW_EPI_GELU_TANH) {
+    constexpr float k1 = -2.0f * 0.79788456080286535588f * 1.44269504088896340736f;
+    constexpr float k2 = 0.044715f * k1;
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+      const float2 v = make_float2(f[j], f[j + 1]);
+      const float2 x = mul2(v, fma2(mul2(v, v), both(k2), both(k1)));
+      float2 e;
+      asm("ex2.approx.f32 %0, %1;" : "=f"(e.x) : "f"(x.x));
+      asm("ex2.approx.f32 %0, %1;" : "=f"(e.y) : "f"(x.y));
+      e = add2(e, both(1.0f));
+      float2 r;
+      asm("rcp.approx.f32 %0, %1;" : "=f"(r.x) : "f"(e.x));
+      asm("rcp.approx.f32 %0, %1;" : "=f"(r.y) : "f"(e.y));
+      r = mul2(v, r);
+      f[j] = r.x; f[j + 1] = r.y;
+    }
+  } else if constexpr (EPI == GW_EPI_GELU_ERF) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) f[j] = apply_epilogue16(f[j], EPI);
   }
 }
 

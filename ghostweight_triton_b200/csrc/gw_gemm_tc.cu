@@ -333,9 +333,13 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmap_b,
         for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(acc[j]);
         if (c + 1 < kSteps) tc_ld_32x32b_x32(t_row + (c + 1) * 32, acc);
         const int64_t n_base = n_warp + c * 32;
-        if constexpr (Q8) scale32(f, row_scale, p.w_scale, n_base, p.N);
-        if (p.bias) add_bias32<DT>(f, p.bias, n_base, p.N);
-        activate32<EPI>(f);
+        if constexpr (Q8) {
+          scale32(f, row_scale, p.w_scale, n_base, p.N);
+          bias_activate32<DT, EPI>(f, p.bias, n_base, p.N);
+        } else {
+          if (p.bias) add_bias32<DT>(f, p.bias, n_base, p.N);
+          activate32<EPI>(f);
+        }
         if (row_ok) {
           if (p.res) {
             uint32_t rv[16];

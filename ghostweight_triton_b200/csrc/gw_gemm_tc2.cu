@@ -102,6 +102,7 @@ struct Tc2Params {
   int64_t ldy;
   const uint16_t* res;      // residual (or null), leading dimension ldr
   int64_t ldr;
+  int res_tile;             // residual rows are 16-byte aligned and y is stored by TMA
   const float* a_scale;     // Q8: scales of A's rows and of W's rows
   const float* w_scale;
   int num_kb;               // k atoms of K (64 columns of 16 bits, 128 of 8)
@@ -361,8 +362,10 @@ __device__ __forceinline__ void gather_units(const Tc2Params& p, int e, int lane
   if (__any_sync(0xFFFFFFFFu, bad) && lane == 0) raise_error(p.err, GW_DERR_BAD_INDEX);
 }
 
-// Q8: A and W' in e4m3 with scales, else 16-bit of type DT.
-template <int BN, int DT, int EPI, bool GATHER, bool Q8>
+// Q8: A and W' in e4m3 with scales, else 16-bit of type DT. RES: with a residual
+// (an instantiation of its own: its loads cost the plain epilogue 10% where the
+// epilogue bounds the kernel).
+template <int BN, int DT, int EPI, bool GATHER, bool Q8, bool RES>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads2, 1)
 gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
                 const __grid_constant__ CUtensorMap tmap_bh,
@@ -590,15 +593,13 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
       gather_units<DT>(p, warp - 2, lane, claim_slot, call);
     }
     // The residual and the scales of A may come from the previous kernel of the stream.
-    if (Q8 || p.res) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (Q8 || RES) asm volatile("griddepcontrol.wait;" ::: "memory");
     uint32_t lt = 0;
     for (int job = pair; job < p.num_jobs; job += num_pairs, ++lt) {
       int m_blk, n_blk, sub;
       job_coords(job, p, m_blk, n_blk, sub);
       const uint32_t b = lt & 1u;
       const uint32_t aph = (lt >> 1) & 1u;
-      if (!mbar_wait_cluster(tfull(b), aph, abort_flag, p.err)) break;
-      tc_fence_after();
       const int64_t warp_row0 = static_cast<int64_t>(m_blk) * kPairM + rank * kHalfM + q * 32;
       const int64_t row = warp_row0 + lane;
       const bool row_ok = row < p.M;
@@ -610,6 +611,44 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + b * BN + col0;
       const int64_t n_warp = static_cast<int64_t>(n_blk) * BN + (sub < 0 ? 0 : sub * 128) + col0;
       const int steps = sub < 0 ? (half ? C::kCols1 : C::kCols0) / 32 : 2;   // 32-column loads (even)
+      // The residual of a 64-column chunk is loaded one chunk ahead (the first one
+      // while the MMAs run), eight lanes per row and four rows per load, and goes
+      // through the staging tile to the lanes that own the rows. A lane loading
+      // its own row touches 32 lines per instruction, which the L1 looks up one by
+      // one: 47.9 us instead of RES512 for 8192 x 4096 x 512.
+      uint4 rt[8];
+      const uint16_t* rsrc = nullptr;
+      int r_rows = 0;                                 // of this lane's eight rows, those in y
+      if (RES && p.res_tile) {
+        const int64_t r0 = warp_row0 + (lane >> 3);
+        rsrc = p.res + r0 * p.ldr + (lane & 7) * 8;
+        const int64_t left = p.M - r0;
+        r_rows = left <= 0 ? 0 : left >= 32 ? 8 : static_cast<int>((left + 3) / 4);
+      }
+      auto residual_chunk = [&](int64_t n_chunk) {
+        const int64_t cols = p.N - n_chunk - (lane & 7) * 8;          // of this lane's eight
+#pragma unroll
+        for (int i = 0; i < 8; ++i) rt[i] = make_uint4(0, 0, 0, 0);
+        if (cols >= 8) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i < r_rows) rt[i] = *reinterpret_cast<const uint4*>(rsrc + 4 * i * p.ldr + n_chunk);
+        } else if (cols > 0) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint16_t* e = rsrc + 4 * i * p.ldr + n_chunk;
+            uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int j = 0; j < 7; ++j)
+              if (i < r_rows && j < cols) w[j / 2] |= static_cast<uint32_t>(e[j]) << (16 * (j & 1));
+            rt[i] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      };
+      if (RES && p.res_tile) residual_chunk(n_warp);
+      const uint16_t* rrow = RES && !p.res_tile && row_ok ? p.res + row * p.ldr : nullptr;
+      if (!mbar_wait_cluster(tfull(b), aph, abort_flag, p.err)) break;
+      tc_fence_after();
       uint32_t acc[32];
       tc_ld_32x32b_x32(t_row, acc);
 #pragma unroll 1
@@ -627,13 +666,36 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
           // The staging tile's previous TMA store must have read it.
           if (lane == 0) bulk_wait_group_read<0>();
           __syncwarp();
+          if (RES && p.res_tile) {
+            // Row r of the staging tile, unit v at v ^ (r & 7), as the output goes there.
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int r = 4 * i + (lane >> 3);
+              *reinterpret_cast<uint4*>(sb + r * (kEpiCols * 2) + (((lane & 7) ^ (r & 7)) << 4)) = rt[i];
+            }
+            __syncwarp();
+            if (st + 2 < steps) residual_chunk(n_chunk + kEpiCols);
+          }
         }
-        if constexpr (Q8) scale32(f, row_scale, p.w_scale, n_base, p.N);
-        if (p.bias) add_bias32<DT>(f, p.bias, n_base, p.N);
-        activate32<EPI>(f);
-        if (p.res && row_ok) {
+        if constexpr (Q8) {
+          scale32(f, row_scale, p.w_scale, n_base, p.N);
+          bias_activate32<DT, EPI>(f, p.bias, n_base, p.N);
+        } else {
+          if (p.bias) add_bias32<DT>(f, p.bias, n_base, p.N);
+          activate32<EPI>(f);
+        }
+        if (RES && p.res_tile) {
           uint32_t rv[16];
-          load_residual32(rv, p.res + row * p.ldr, n_base, p.N);
+          const uint4* srow = reinterpret_cast<const uint4*>(sb + lane * (kEpiCols * 2));
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const uint4 u = srow[(h * 4 + v) ^ (lane & 7)];
+            rv[4 * v] = u.x; rv[4 * v + 1] = u.y; rv[4 * v + 2] = u.z; rv[4 * v + 3] = u.w;
+          }
+          add_residual32<DT>(f, rv);
+        } else if (RES && rrow) {
+          uint32_t rv[16];
+          load_residual32(rv, rrow, n_base, p.N);
           add_residual32<DT>(f, rv);
         }
         uint32_t packed[16];
@@ -819,6 +881,7 @@ cudaError_t launch_tc2_bn(int dtype, Tc2Params& p, const void* a, int64_t M, int
   // TMA-store epilogue when y's rows are 16-byte aligned (else direct stores).
   p.y_tma = p.y_vec_ok && make_tmap_kmajor(&ty, y, M, N, ldy, kEpiCols, 32) ? 1 : 0;
   if (!p.y_tma) ty = ta;     // not read by the kernel
+  p.res_tile = p.res && p.y_tma && (reinterpret_cast<uintptr_t>(p.res) & 15u) == 0 && (p.ldr % 8) == 0 ? 1 : 0;
   if (p.n_peers > 0 && !p.y_tma) return cudaErrorInvalidValue;   // peer stores ride the TMA path
 
   const int64_t pairs = std::max<int64_t>(1, (sm_count > 0 ? sm_count : 148) / 2);
@@ -845,16 +908,20 @@ cudaError_t launch_tc2_bn(int dtype, Tc2Params& p, const void* a, int64_t M, int
   }
 
   const bool bf = dtype == GW_DTYPE_BF16;
-#define GW_TC2_KERN(G, Q)                                                       \
+#define GW_TC2_KERN(G, Q, R)                                                    \
   (p.epi == GW_EPI_GELU_ERF                                                     \
-       ? (bf ? gemm_tc2_kernel<BN, GW_DTYPE_BF16, GW_EPI_GELU_ERF, G, Q>        \
-             : gemm_tc2_kernel<BN, GW_DTYPE_F16, GW_EPI_GELU_ERF, G, Q>)        \
+       ? (bf ? gemm_tc2_kernel<BN, GW_DTYPE_BF16, GW_EPI_GELU_ERF, G, Q, R>     \
+             : gemm_tc2_kernel<BN, GW_DTYPE_F16, GW_EPI_GELU_ERF, G, Q, R>)     \
    : p.epi == GW_EPI_GELU_TANH                                                  \
-       ? (bf ? gemm_tc2_kernel<BN, GW_DTYPE_BF16, GW_EPI_GELU_TANH, G, Q>       \
-             : gemm_tc2_kernel<BN, GW_DTYPE_F16, GW_EPI_GELU_TANH, G, Q>)       \
-       : (bf ? gemm_tc2_kernel<BN, GW_DTYPE_BF16, GW_EPI_NONE, G, Q>            \
-             : gemm_tc2_kernel<BN, GW_DTYPE_F16, GW_EPI_NONE, G, Q>))
-  auto kern = q8 ? GW_TC2_KERN(false, true) : p.ghdr ? GW_TC2_KERN(true, false) : GW_TC2_KERN(false, false);
+       ? (bf ? gemm_tc2_kernel<BN, GW_DTYPE_BF16, GW_EPI_GELU_TANH, G, Q, R>    \
+             : gemm_tc2_kernel<BN, GW_DTYPE_F16, GW_EPI_GELU_TANH, G, Q, R>)    \
+       : (bf ? gemm_tc2_kernel<BN, GW_DTYPE_BF16, GW_EPI_NONE, G, Q, R>         \
+             : gemm_tc2_kernel<BN, GW_DTYPE_F16, GW_EPI_NONE, G, Q, R>))
+  const bool gather = p.ghdr != nullptr;
+  auto kern = p.res ? (q8 ? GW_TC2_KERN(false, true, true)
+                       : gather ? GW_TC2_KERN(true, false, true) : GW_TC2_KERN(false, false, true))
+                    : (q8 ? GW_TC2_KERN(false, true, false)
+                       : gather ? GW_TC2_KERN(true, false, false) : GW_TC2_KERN(false, false, false));
 #undef GW_TC2_KERN
   cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kern), C::kSmemBytes);
   if (e != cudaSuccess) return e;

@@ -79,33 +79,6 @@ __device__ __forceinline__ float to_scale(float u, const RowScale& q) {
   return c - (c - v);
 }
 
-// Two fp32 operations in one instruction, each rounded on its own.
-__device__ __forceinline__ uint64_t pair_bits(float2 v) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
-  return r;
-}
-__device__ __forceinline__ float2 bits_pair(uint64_t r) {
-  float2 v;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
-  return v;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)));
-  return bits_pair(r);
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)));
-  return bits_pair(r);
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)), "l"(pair_bits(c)));
-  return bits_pair(r);
-}
-__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 // to_scale for two values.
 __device__ __forceinline__ float2 to_scale2(float2 u, const RowScale& q) {
   float2 v = mul2(u, both(q.m1));
