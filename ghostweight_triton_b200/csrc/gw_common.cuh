@@ -602,50 +602,6 @@ __device__ __forceinline__ float apply_epilogue16(float v, int epi) {
   return apply_epilogue(v, epi);
 }
 
-// Epilogue arithmetic for 32 consecutive output columns [n0, n0 + 32) of one
-// row (the 32 values a lane holds after one 32-column TMEM load).
-// Bias: four 16-byte loads when the 32 values lie inside [0, N) and are
-// 16-byte aligned (every lane of the warp reads the same addresses), else one
-// load per element.
-template <int DT>
-__device__ __forceinline__ void add_bias32(float (&f)[32], const uint16_t* bias, int64_t n0,
-                                           int64_t N) {
-  const uint16_t* b = bias + n0;
-  if (n0 + 32 <= N && (reinterpret_cast<uintptr_t>(b) & 15u) == 0) {
-#pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      const uint4 q = __ldg(reinterpret_cast<const uint4*>(b) + v);
-      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        f[8 * v + 2 * k] += Elem<DT>::to_f(static_cast<uint16_t>(w[k] & 0xFFFFu));
-        f[8 * v + 2 * k + 1] += Elem<DT>::to_f(static_cast<uint16_t>(w[k] >> 16));
-      }
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (n0 + j < N) f[j] += Elem<DT>::to_f(__ldg(bias + n0 + j));
-  }
-}
-// The same for four consecutive columns [n0, n0 + 4): one 8-byte load when
-// they lie inside [0, N) and are 8-byte aligned.
-template <int DT>
-__device__ __forceinline__ void add_bias4(float (&f)[4], const uint16_t* bias, int64_t n0,
-                                          int64_t N) {
-  const uint16_t* b = bias + n0;
-  if (n0 + 4 <= N && (reinterpret_cast<uintptr_t>(b) & 7u) == 0) {
-    const uint2 q = __ldg(reinterpret_cast<const uint2*>(b));
-    f[0] += Elem<DT>::to_f(static_cast<uint16_t>(q.x & 0xFFFFu));
-    f[1] += Elem<DT>::to_f(static_cast<uint16_t>(q.x >> 16));
-    f[2] += Elem<DT>::to_f(static_cast<uint16_t>(q.y & 0xFFFFu));
-    f[3] += Elem<DT>::to_f(static_cast<uint16_t>(q.y >> 16));
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (n0 + j < N) f[j] += Elem<DT>::to_f(__ldg(bias + n0 + j));
-  }
-}
 // Two fp32 operations in one instruction, each rounded on its own.
 __device__ __forceinline__ uint64_t pair_bits(float2 v) {
   uint64_t r;
@@ -673,6 +629,54 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return bits_pair(r);
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+// Epilogue arithmetic for 32 consecutive output columns [n0, n0 + 32) of one
+// row (the 32 values a lane holds after one 32-column TMEM load).
+// Bias: four 16-byte loads when the 32 values lie inside [0, N) and are
+// 16-byte aligned (every lane of the warp reads the same addresses), else one
+// load per element.
+template <int DT>
+__device__ __forceinline__ void add_bias32(float (&f)[32], const uint16_t* bias, int64_t n0,
+                                           int64_t N) {
+  const uint16_t* b = bias + n0;
+  if (n0 + 32 <= N && (reinterpret_cast<uintptr_t>(b) & 15u) == 0) {
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const uint4 q = __ldg(reinterpret_cast<const uint4*>(b) + v);
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int j = 8 * v + 2 * k;
+        const float2 a = add2(make_float2(f[j], f[j + 1]),
+                              make_float2(Elem<DT>::to_f(static_cast<uint16_t>(w[k] & 0xFFFFu)),
+                                          Elem<DT>::to_f(static_cast<uint16_t>(w[k] >> 16))));
+        f[j] = a.x;
+        f[j + 1] = a.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (n0 + j < N) f[j] += Elem<DT>::to_f(__ldg(bias + n0 + j));
+  }
+}
+// The same for four consecutive columns [n0, n0 + 4): one 8-byte load when
+// they lie inside [0, N) and are 8-byte aligned.
+template <int DT>
+__device__ __forceinline__ void add_bias4(float (&f)[4], const uint16_t* bias, int64_t n0,
+                                          int64_t N) {
+  const uint16_t* b = bias + n0;
+  if (n0 + 4 <= N && (reinterpret_cast<uintptr_t>(b) & 7u) == 0) {
+    const uint2 q = __ldg(reinterpret_cast<const uint2*>(b));
+    f[0] += Elem<DT>::to_f(static_cast<uint16_t>(q.x & 0xFFFFu));
+    f[1] += Elem<DT>::to_f(static_cast<uint16_t>(q.x >> 16));
+    f[2] += Elem<DT>::to_f(static_cast<uint16_t>(q.y & 0xFFFFu));
+    f[3] += Elem<DT>::to_f(static_cast<uint16_t>(q.y >> 16));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (n0 + j < N) f[j] += Elem<DT>::to_f(__ldg(bias + n0 + j));
+  }
+}
 // Scales of e4m3 operands, applied to the fp32 accumulator in front of the bias:
 // f[j] * row * w[n0 + j]. First by the row's scale: the product of the two
 // scales alone could leave fp32's range.
@@ -700,28 +704,7 @@ __device__ __forceinline__ void scale32(float (&f)[32], float row, const float* 
 // core twice as fast as for 16-bit operands the epilogue has half the time.
 template <int DT, int EPI>
 __device__ __forceinline__ void bias_activate32(float (&f)[32], const uint16_t* bias, int64_t n0, int64_t N) {
-  if (bias) {
-    const uint16_t* b = bias + n0;
-    if (n0 + 32 <= N && (reinterpret_cast<uintptr_t>(b) & 15u) == 0) {
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const uint4 q = __ldg(reinterpret_cast<const uint4*>(b) + v);
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int j = 8 * v + 2 * k;
-          const float2 a = add2(make_float2(f[j], f[j + 1]),
-                                make_float2(Elem<DT>::to_f(static_cast<uint16_t>(w[k] & 0xFFFFu)),
-                                            Elem<DT>::to_f(static_cast<uint16_t>(w[k] >> 16))));
-          f[j] = a.x; f[j + 1] = a.y;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (n0 + j < N) f[j] += Elem<DT>::to_f(__ldg(b + j));
-    }
-  }
+  if (bias) add_bias32<DT>(f, bias, n0, N);
   if constexpr (EPI == GW_EPI_GELU_TANH) {
     constexpr float k1 = -2.0f * 0.79788456080286535588f * 1.44269504088896340736f;
     constexpr float k2 = 0.044715f * k1;
@@ -772,8 +755,11 @@ template <int DT>
 __device__ __forceinline__ void add_residual32(float (&f)[32], const uint32_t (&v)[16]) {
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
-    f[2 * j] += Elem<DT>::to_f(static_cast<uint16_t>(v[j] & 0xFFFFu));
-    f[2 * j + 1] += Elem<DT>::to_f(static_cast<uint16_t>(v[j] >> 16));
+    const float2 a = add2(make_float2(f[2 * j], f[2 * j + 1]),
+                          make_float2(Elem<DT>::to_f(static_cast<uint16_t>(v[j] & 0xFFFFu)),
+                                      Elem<DT>::to_f(static_cast<uint16_t>(v[j] >> 16))));
+    f[2 * j] = a.x;
+    f[2 * j + 1] = a.y;
   }
 }
 __device__ __forceinline__ uint2 load_residual4(const uint16_t* row, int64_t n0, int64_t N) {
