@@ -506,6 +506,12 @@ __device__ __forceinline__ void tc_commit_pair_mc(uint32_t bar, uint16_t mask) {
       :: "r"(bar), "h"(mask) : "memory");
 }
 
+// Host: what the rows of a matrix of 16-bit values are aligned to (16, 4 or 2 bytes).
+inline int row_alignment(const void* p, int64_t ld) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(ld * 2);
+  return (a & 15u) == 0 ? 16 : (a & 3u) == 0 ? 4 : 2;
+}
+
 // Host: raise `kern`'s dynamic shared-memory limit to `bytes` once per device
 // (the attribute sticks to the function; re-setting it on every launch costs a
 // driver call).
@@ -729,28 +735,126 @@ __device__ __forceinline__ void bias_activate32(float (&f)[32], const uint16_t* 
 }
 
 // Residual added in GEMM epilogues, after the activation and before the one
-// rounding: 32 (or 4) consecutive columns [n0, n0 + 32) of one row, as pairs
-// of 16-bit values, zeros at and past column N. Plain loads, not the
-// read-only path: the residual may be the output itself (each element is read
-// before the same thread or warp stores it).
-__device__ __forceinline__ void load_residual32(uint32_t (&v)[16], const uint16_t* row, int64_t n0,
-                                                int64_t N) {
-  const uint16_t* b = row + n0;
-  if (n0 + 32 <= N && (reinterpret_cast<uintptr_t>(b) & 15u) == 0) {
+// rounding. Plain loads, not the read-only path: the residual may be the output
+// itself (each element is read before the same thread or warp stores it).
+//
+// Tile of a warp's epilogue: 32 rows of COLS 16-bit values in shared memory,
+// 16-byte units swizzled by the row so that a lane's accesses to its own row
+// (32 lanes, 32 rows) and to the units of whole rows are both without bank
+// conflicts. Residuals come in through it and outputs whose rows are not aligned
+// for TMA or vector stores go out through it: in both directions lanes side by
+// side access adjacent memory. A lane that reads or writes its own row touches 32
+// lines per instruction, which the L1 looks up one by one.
+template <int COLS>
+struct WarpTile {
+  static constexpr int kRowBytes = COLS * 2;
+  static constexpr int kBytes = 32 * kRowBytes;
+  static constexpr int kUnits = kRowBytes / 16;            // 16-byte units of a row
+  static constexpr int kWords = COLS / 2;                  // 4-byte words of a row
+  static constexpr int kRegs = 32 * kWords / 32;           // words per lane of a whole tile
+  static_assert(COLS == 64 || COLS == 32, "tile width");
+  uint8_t* base;
+  int lane;
+  __device__ __forceinline__ uint4* unit(int r, int v) const {
+    const int sw = COLS == 64 ? (r & 7) : ((r >> 1) & 3);
+    return reinterpret_cast<uint4*>(base + r * kRowBytes + ((v ^ sw) << 4));
+  }
+  __device__ __forceinline__ uint32_t* word(int r, int w) const {
+    return reinterpret_cast<uint32_t*>(unit(r, w >> 2)) + (w & 3);
+  }
+  // Rows [row0, row0 + 32) and columns [n0, n0 + COLS) of src [M, N] into this
+  // lane's registers (zeros outside): 16-byte units where its rows are 16-byte
+  // aligned (`align` 16; n0 is a multiple of 8), words of two values where they
+  // are 4-byte aligned, else single values. No branch inside the loops, so that
+  // all loads of a tile are in flight at once.
+  __device__ __forceinline__ void load(uint32_t (&v)[kRegs], const uint16_t* src, int64_t ld, int align,
+                                       int64_t row0, int64_t M, int64_t n0, int64_t N) const {
+    if (align == 16) {
+      constexpr int kRows = 32 / kUnits;                   // rows per pass
+      const int64_t cols = N - n0 - (lane % kUnits) * 8;
+      const uint16_t* p = src + (row0 + lane / kUnits) * ld + n0 + (lane % kUnits) * 8;
+      const int64_t left = M - row0 - lane / kUnits;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const uint4 u = reinterpret_cast<const uint4*>(b)[q];
-      v[4 * q] = u.x; v[4 * q + 1] = u.y; v[4 * q + 2] = u.z; v[4 * q + 3] = u.w;
-    }
-  } else {
+      for (int i = 0; i < 32 / kRows; ++i) {
+        uint4 q = make_uint4(0, 0, 0, 0);
+        if (i * kRows < left && cols > 0) {
+          const uint16_t* e = p + i * kRows * ld;
+          if (cols >= 8) {
+            q = *reinterpret_cast<const uint4*>(e);
+          } else {
+            uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const uint32_t lo = n0 + 2 * j < N ? b[2 * j] : 0u;
-      const uint32_t hi = n0 + 2 * j + 1 < N ? b[2 * j + 1] : 0u;
-      v[j] = lo | (hi << 16);
+            for (int j = 0; j < 7; ++j)
+              if (j < cols) w[j / 2] |= static_cast<uint32_t>(e[j]) << (16 * (j & 1));
+            q = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
+      }
+    } else {
+      constexpr int kRows = 32 / kWords;
+      const int64_t cols = N - n0 - (lane % kWords) * 2;
+      const uint16_t* p = src + (row0 + lane / kWords) * ld + n0 + (lane % kWords) * 2;
+      const int64_t left = M - row0 - lane / kWords;
+      if (align == 4 && cols != 1) {
+#pragma unroll
+        for (int i = 0; i < kRegs; ++i)
+          v[i] = i * kRows < left && cols > 1 ? *reinterpret_cast<const uint32_t*>(p + i * kRows * ld) : 0u;
+      } else {
+#pragma unroll
+        for (int i = 0; i < kRegs; ++i) {
+          const uint32_t lo = i * kRows < left && cols > 0 ? p[i * kRows * ld] : 0u;
+          const uint32_t hi = i * kRows < left && cols > 1 ? p[i * kRows * ld + 1] : 0u;
+          v[i] = lo | (hi << 16);
+        }
+      }
     }
   }
-}
+  __device__ __forceinline__ void put(const uint32_t (&v)[kRegs], int align) const {   // what load() took
+    if (align == 16) {
+      constexpr int kRows = 32 / kUnits;
+#pragma unroll
+      for (int i = 0; i < 32 / kRows; ++i)
+        *unit(i * kRows + lane / kUnits, lane % kUnits) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    } else {
+      constexpr int kRows = 32 / kWords;
+#pragma unroll
+      for (int i = 0; i < kRegs; ++i) *word(i * kRows + lane / kWords, lane % kWords) = v[i];
+    }
+  }
+  // This lane's own row, 32 values from column 32 h on.
+  __device__ __forceinline__ void own_row(uint32_t (&v)[16], int h) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 q = *unit(lane, h * 4 + i);
+      v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
+    }
+  }
+  __device__ __forceinline__ void set_own_row(const uint32_t (&v)[16], int h) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *unit(lane, h * 4 + i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  }
+  // The tile to rows of any alignment of dst [M, N].
+  __device__ __forceinline__ void store(uint16_t* dst, int64_t ld, int64_t row0, int64_t M, int64_t n0, int64_t N) const {
+    constexpr int kRows = 32 / kWords;
+    const int64_t cols = N - n0 - (lane % kWords) * 2;
+    uint16_t* p = dst + (row0 + lane / kWords) * ld + n0 + (lane % kWords) * 2;
+    const int64_t left = M - row0 - lane / kWords;
+    if (cols <= 0) return;
+#pragma unroll 8
+    for (int i = 0; i < kRegs; ++i) {
+      if (i * kRows >= left) break;
+      uint16_t* e = p + i * kRows * ld;
+      const uint32_t v = *word(i * kRows + lane / kWords, lane % kWords);
+      if (cols >= 2 && (reinterpret_cast<uintptr_t>(e) & 3u) == 0) {
+        *reinterpret_cast<uint32_t*>(e) = v;
+      } else {
+        e[0] = static_cast<uint16_t>(v);
+        if (cols >= 2) e[1] = static_cast<uint16_t>(v >> 16);
+      }
+    }
+  }
+};
 template <int DT>
 __device__ __forceinline__ void add_residual32(float (&f)[32], const uint32_t (&v)[16]) {
 #pragma unroll

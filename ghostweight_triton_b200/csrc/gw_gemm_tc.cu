@@ -71,7 +71,9 @@ struct TcCfg {
   static constexpr int kStages = kStagesFit > kMaxStages ? kMaxStages : kStagesFit;
   static constexpr int kTmemCols = pow2_at_least(2 * BN);   // two accumulator buffers
   static constexpr int kBarBytes = 256;
-  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kBarBytes;
+  static constexpr int kEpiBytes = 8 * WarpTile<32>::kBytes;     // an epilogue tile per warp
+  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kEpiBytes + kBarBytes;
+  static_assert(kSmemBytes <= 232448, "shared memory budget per CTA");
 };
 
 struct TcParams {
@@ -95,13 +97,17 @@ struct TcParams {
   const int64_t* a_cols;        // kATma: k-block kb of A starts at x column a_cols[64 kb] (or null)
   const uint16_t* res;          // residual (or null), leading dimension ldr
   int64_t ldr;
+  int res_align;                // alignment of its rows (row_alignment)
   const float* a_scale;         // Q8: scales of A's rows and of W's rows
   const float* w_scale;
   const int32_t* k_dev;         // kATma: K' on the device (num_kb an upper bound; see device_num_kb)
 };
 
-// Q8: A and W in e4m3 with scales (kATma only), else 16-bit of type DT.
-template <int BN, int DT, int AMODE, int EPI, bool Q8>
+// Q8: A and W in e4m3 with scales (kATma only), else 16-bit of type DT. STAGED:
+// with a residual or with rows of y that are not 16-byte aligned, which pass
+// through a tile in shared memory (an instantiation of its own: 1024 x 4096 x
+// 1024 without either takes 9.0 us, 10.5 with the tile's code beside it).
+template <int BN, int DT, int AMODE, int EPI, bool Q8, bool STAGED>
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_tc_kernel(const __grid_constant__ CUtensorMap tmap_b,
                const __grid_constant__ CUtensorMap tmap_a, const TcParams p) {
@@ -114,7 +120,8 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmap_b,
   uint8_t* smem = smem_raw + ((1024u - (raw_s & 1023u)) & 1023u);
   const uint32_t sbase = smem_u32(smem);
 
-  uint8_t* bar_region = smem + C::kStages * C::kStageBytes;
+  uint8_t* epi_stage = smem + C::kStages * C::kStageBytes;
+  uint8_t* bar_region = epi_stage + C::kEpiBytes;
   const uint32_t bar0 = smem_u32(bar_region);
   // barriers: full_a[S] full_b[S] empty[S] tfull[2] tempty[2] drain
   auto full_a = [&](int s) { return bar0 + 8u * s; };
@@ -307,22 +314,28 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmap_b,
     const int q = warp & 3;                       // TMEM lane quarter this warp may access
     const int part = (warp - (AMODE == kATma ? kWarpEpi0Dense : kWarpEpi0)) >> 2;
     const int row_in_tile = q * 32 + lane;
+    const WarpTile<32> wt{epi_stage + (warp - (AMODE == kATma ? kWarpEpi0Dense : kWarpEpi0)) * WarpTile<32>::kBytes, lane};
     // The residual and the scales of A may come from the previous kernel of the stream.
-    if (Q8 || p.res) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (Q8 || (STAGED && p.res)) asm volatile("griddepcontrol.wait;" ::: "memory");
     uint32_t lt = 0;
     for (int tile = blockIdx.x; tile < p.num_tiles; tile += gridDim.x, ++lt) {
       const int m_blk = tile % p.m_tiles;
       const int n_blk = tile / p.m_tiles;
       const uint32_t b = lt & 1u;
       const uint32_t aph = (lt >> 1) & 1u;
-      if (!mbar_wait(tfull(b), aph, abort_flag, p.err)) break;
-      tc_fence_after();
-      const int64_t row = static_cast<int64_t>(m_blk) * kBM + row_in_tile;
+      const int64_t warp_row0 = static_cast<int64_t>(m_blk) * kBM + q * 32;
+      const int64_t row = warp_row0 + lane;
       const bool row_ok = row < p.M;
       uint16_t* yrow = p.y + (row_ok ? row * p.ldy : 0);
       const float row_scale = Q8 && row_ok ? p.a_scale[row] : 0.0f;
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + b * BN + part * kEpiCols;
       const int64_t n_warp = static_cast<int64_t>(n_blk) * BN + part * kEpiCols;
+      // The residual of a step is loaded one step ahead, the first one while the
+      // MMAs run, and goes through the warp's tile to the lanes that own the rows.
+      uint32_t rt[16];
+      if (STAGED && p.res) wt.load(rt, p.res, p.ldr, p.res_align, warp_row0, p.M, n_warp, p.N);
+      if (!mbar_wait(tfull(b), aph, abort_flag, p.err)) break;
+      tc_fence_after();
       uint32_t acc[32];
       tc_ld_32x32b_x32(t_row, acc);
 #pragma unroll 1
@@ -340,26 +353,40 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmap_b,
           if (p.bias) add_bias32<DT>(f, p.bias, n_base, p.N);
           activate32<EPI>(f);
         }
-        if (row_ok) {
-          if (p.res) {
-            uint32_t rv[16];
-            load_residual32(rv, p.res + row * p.ldr, n_base, p.N);
-            add_residual32<DT>(f, rv);
-          }
-          if (p.y_vec_ok && n_base + 32 <= p.N) {
-            uint32_t packed[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) packed[j] = Elem<DT>::pack2(f[2 * j], f[2 * j + 1]);
-            uint4* dst = reinterpret_cast<uint4*>(yrow + n_base);
-#pragma unroll
-            for (int v = 0; v < 4; ++v)
-              dst[v] = make_uint4(packed[4 * v], packed[4 * v + 1], packed[4 * v + 2], packed[4 * v + 3]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (n_base + j < p.N) yrow[n_base + j] = Elem<DT>::from_f(f[j]);
-          }
+        if (STAGED && p.res) {
+          wt.put(rt, p.res_align);
+          __syncwarp();
+          if (c + 1 < kSteps) wt.load(rt, p.res, p.ldr, p.res_align, warp_row0, p.M, n_base + 32, p.N);
+          uint32_t rv[16];
+          wt.own_row(rv, 0);
+          add_residual32<DT>(f, rv);
         }
+        if (!STAGED || p.y_vec_ok) {
+          if (row_ok) {
+            if (n_base + 32 <= p.N) {
+              uint32_t packed[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) packed[j] = Elem<DT>::pack2(f[2 * j], f[2 * j + 1]);
+              uint4* dst = reinterpret_cast<uint4*>(yrow + n_base);
+#pragma unroll
+              for (int v = 0; v < 4; ++v)
+                dst[v] = make_uint4(packed[4 * v], packed[4 * v + 1], packed[4 * v + 2], packed[4 * v + 3]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (n_base + j < p.N) yrow[n_base + j] = Elem<DT>::from_f(f[j]);
+            }
+          }
+        } else {
+          // Rows of any alignment leave through the warp's tile.
+          uint32_t packed[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) packed[j] = Elem<DT>::pack2(f[2 * j], f[2 * j + 1]);
+          wt.set_own_row(packed, 0);
+          __syncwarp();
+          wt.store(p.y, p.ldy, warp_row0, p.M, n_base, p.N);
+        }
+        if constexpr (STAGED) __syncwarp();          // the tile is free for the next step
       }
       tc_fence_before();
       __syncwarp();
@@ -377,13 +404,13 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmap_b,
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-template <int BN, int DT, int AMODE, bool Q8>
+template <int BN, int DT, int AMODE, bool Q8, bool STAGED>
 cudaError_t launch_tc(const CUtensorMap& tb, const CUtensorMap& ta, const TcParams& p,
                       int sm_count, cudaStream_t stream) {
   using C = TcCfg<BN>;
-  auto kern = p.epi == GW_EPI_GELU_ERF    ? gemm_tc_kernel<BN, DT, AMODE, GW_EPI_GELU_ERF, Q8>
-              : p.epi == GW_EPI_GELU_TANH ? gemm_tc_kernel<BN, DT, AMODE, GW_EPI_GELU_TANH, Q8>
-                                          : gemm_tc_kernel<BN, DT, AMODE, GW_EPI_NONE, Q8>;
+  auto kern = p.epi == GW_EPI_GELU_ERF    ? gemm_tc_kernel<BN, DT, AMODE, GW_EPI_GELU_ERF, Q8, STAGED>
+              : p.epi == GW_EPI_GELU_TANH ? gemm_tc_kernel<BN, DT, AMODE, GW_EPI_GELU_TANH, Q8, STAGED>
+                                          : gemm_tc_kernel<BN, DT, AMODE, GW_EPI_NONE, Q8, STAGED>;
   // Opt in to the large dynamic shared-memory carve-out (idempotent, cheap).
   cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kern), C::kSmemBytes);
   if (e != cudaSuccess) return e;
@@ -467,6 +494,7 @@ cudaError_t launch_gemm_tc(int a_mode, const void* x, int dtype, int64_t M, int6
   p.k_dev = a_mode == kATma ? k_dev : nullptr;
   p.res = static_cast<const uint16_t*>(res.p);
   p.ldr = res.ld;
+  p.res_align = row_alignment(p.res, p.ldr);
   p.a_scale = qs.a;
   p.w_scale = qs.w;
   if (p.a_cols && (n_alive % kBK) != 0) return cudaErrorInvalidValue;
@@ -481,13 +509,16 @@ cudaError_t launch_gemm_tc(int a_mode, const void* x, int dtype, int64_t M, int6
       return cudaErrorInvalidValue;
   }
 
+  const bool staged = res.p != nullptr || !p.y_vec_ok;
+#define GW_TC_LAUNCH(BNV, DTV, MODE, Q)                                                            \
+  (staged ? launch_tc<BNV, DTV, MODE, Q, true>(tb, ta, p, static_cast<int>(sms), stream)           \
+          : launch_tc<BNV, DTV, MODE, Q, false>(tb, ta, p, static_cast<int>(sms), stream))
 #define GW_TC_MODES(BNV, DTV)                                                                     \
   switch (a_mode) {                                                                              \
     case kATma:                                                                                  \
-      return q8 ? launch_tc<BNV, DTV, kATma, true>(tb, ta, p, static_cast<int>(sms), stream)      \
-                : launch_tc<BNV, DTV, kATma, false>(tb, ta, p, static_cast<int>(sms), stream);    \
+      return q8 ? GW_TC_LAUNCH(BNV, DTV, kATma, true) : GW_TC_LAUNCH(BNV, DTV, kATma, false);    \
     default:                                                                                     \
-      return launch_tc<BNV, DTV, kASmemGather, false>(tb, ta, p, static_cast<int>(sms), stream); \
+      return GW_TC_LAUNCH(BNV, DTV, kASmemGather, false);                                        \
   }
   if (BN == 256) {
     if (dtype == GW_DTYPE_BF16) { GW_TC_MODES(256, GW_DTYPE_BF16) }
@@ -500,6 +531,7 @@ cudaError_t launch_gemm_tc(int a_mode, const void* x, int dtype, int64_t M, int6
     GW_TC_MODES(128, GW_DTYPE_F16)
   }
 #undef GW_TC_MODES
+#undef GW_TC_LAUNCH
 }
 
 }  // namespace gw

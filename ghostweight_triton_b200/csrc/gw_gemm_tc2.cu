@@ -12,7 +12,8 @@
 //   * MMA completion is multicast to both CTAs (tcgen05.commit ... multicast)
 //     to free their stages and publish finished accumulators;
 //   * each CTA's four epilogue warps drain its own TMEM (bias, GELU, one
-//     rounding) into swizzled staging tiles that the TMA unit stores to y,
+//     rounding) into swizzled staging tiles that the TMA unit stores to y (the
+//     warps themselves where y's rows are not 16-byte aligned),
 //     and arrive on the leader's accumulator-empty barrier (remote arrive for
 //     the second CTA) as soon as their TMEM reads are done;
 //   * launch_dependents right after the prologue lets the next kernel of the
@@ -102,7 +103,7 @@ struct Tc2Params {
   int64_t ldy;
   const uint16_t* res;      // residual (or null), leading dimension ldr
   int64_t ldr;
-  int res_tile;             // residual rows are 16-byte aligned and y is stored by TMA
+  int res_align;            // alignment of its rows (row_alignment)
   const float* a_scale;     // Q8: scales of A's rows and of W's rows
   const float* w_scale;
   int num_kb;               // k atoms of K (64 columns of 16 bits, 128 of 8)
@@ -586,6 +587,8 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
     const uint32_t leader_tempty0 = mapa_shared(tempty(0), 0);
     const uint32_t leader_tempty1 = mapa_shared(tempty(1), 0);
     uint8_t* sb = epi_stage + (warp - 2) * kEpiTileBytes;
+    const WarpTile<kEpiCols> tile{sb, lane};
+    static_assert(WarpTile<kEpiCols>::kBytes == kEpiTileBytes, "staging tile");
     if constexpr (GATHER) {
       // x, the alive list and the workspace may come from the previous kernel.
       asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -603,7 +606,6 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
       const int64_t warp_row0 = static_cast<int64_t>(m_blk) * kPairM + rank * kHalfM + q * 32;
       const int64_t row = warp_row0 + lane;
       const bool row_ok = row < p.M;
-      uint16_t* yrow = p.y + (row_ok ? row * p.ldy : 0);
       const float row_scale = Q8 && row_ok ? p.a_scale[row] : 0.0f;
       // Whole tile: columns [0, 128) (half 0) or [128, BN) (half 1). Half
       // job: 64 columns each, [0, 64) and [64, 128) of its 128.
@@ -611,42 +613,11 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + b * BN + col0;
       const int64_t n_warp = static_cast<int64_t>(n_blk) * BN + (sub < 0 ? 0 : sub * 128) + col0;
       const int steps = sub < 0 ? (half ? C::kCols1 : C::kCols0) / 32 : 2;   // 32-column loads (even)
-      // The residual of a 64-column chunk is loaded one chunk ahead (the first one
-      // while the MMAs run), eight lanes per row and four rows per load, and goes
-      // through the staging tile to the lanes that own the rows. A lane loading
-      // its own row touches 32 lines per instruction, which the L1 looks up one by
-      // one: 47.9 us instead of RES512 for 8192 x 4096 x 512.
-      uint4 rt[8];
-      const uint16_t* rsrc = nullptr;
-      int r_rows = 0;                                 // of this lane's eight rows, those in y
-      if (RES && p.res_tile) {
-        const int64_t r0 = warp_row0 + (lane >> 3);
-        rsrc = p.res + r0 * p.ldr + (lane & 7) * 8;
-        const int64_t left = p.M - r0;
-        r_rows = left <= 0 ? 0 : left >= 32 ? 8 : static_cast<int>((left + 3) / 4);
-      }
-      auto residual_chunk = [&](int64_t n_chunk) {
-        const int64_t cols = p.N - n_chunk - (lane & 7) * 8;          // of this lane's eight
-#pragma unroll
-        for (int i = 0; i < 8; ++i) rt[i] = make_uint4(0, 0, 0, 0);
-        if (cols >= 8) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (i < r_rows) rt[i] = *reinterpret_cast<const uint4*>(rsrc + 4 * i * p.ldr + n_chunk);
-        } else if (cols > 0) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint16_t* e = rsrc + 4 * i * p.ldr + n_chunk;
-            uint32_t w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-            for (int j = 0; j < 7; ++j)
-              if (i < r_rows && j < cols) w[j / 2] |= static_cast<uint32_t>(e[j]) << (16 * (j & 1));
-            rt[i] = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        }
-      };
-      if (RES && p.res_tile) residual_chunk(n_warp);
-      const uint16_t* rrow = RES && !p.res_tile && row_ok ? p.res + row * p.ldr : nullptr;
+      // The residual of a 64-column chunk is loaded one chunk ahead, the first one
+      // while the MMAs run, and goes through the staging tile to the lanes that own
+      // the rows (8192 x 4096 x 512: 39.5 us; 47.9 with lanes loading their own rows).
+      uint32_t rt[RES ? WarpTile<kEpiCols>::kRegs : 1];
+      if constexpr (RES) tile.load(rt, p.res, p.ldr, p.res_align, warp_row0, p.M, n_warp, p.N);
       if (!mbar_wait_cluster(tfull(b), aph, abort_flag, p.err)) break;
       tc_fence_after();
       uint32_t acc[32];
@@ -662,19 +633,14 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
         const int h = st & 1;                           // its 32-column half
         const int64_t n_chunk = n_warp + c * kEpiCols;
         const int64_t n_base = n_chunk + h * 32;
-        if (p.y_tma && h == 0) {
+        if (h == 0) {
           // The staging tile's previous TMA store must have read it.
-          if (lane == 0) bulk_wait_group_read<0>();
+          if (p.y_tma && lane == 0) bulk_wait_group_read<0>();
           __syncwarp();
-          if (RES && p.res_tile) {
-            // Row r of the staging tile, unit v at v ^ (r & 7), as the output goes there.
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int r = 4 * i + (lane >> 3);
-              *reinterpret_cast<uint4*>(sb + r * (kEpiCols * 2) + (((lane & 7) ^ (r & 7)) << 4)) = rt[i];
-            }
+          if constexpr (RES) {
+            tile.put(rt, p.res_align);
             __syncwarp();
-            if (st + 2 < steps) residual_chunk(n_chunk + kEpiCols);
+            if (st + 2 < steps) tile.load(rt, p.res, p.ldr, p.res_align, warp_row0, p.M, n_chunk + kEpiCols, p.N);
           }
         }
         if constexpr (Q8) {
@@ -684,31 +650,16 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
           if (p.bias) add_bias32<DT>(f, p.bias, n_base, p.N);
           activate32<EPI>(f);
         }
-        if (RES && p.res_tile) {
+        if constexpr (RES) {
           uint32_t rv[16];
-          const uint4* srow = reinterpret_cast<const uint4*>(sb + lane * (kEpiCols * 2));
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            const uint4 u = srow[(h * 4 + v) ^ (lane & 7)];
-            rv[4 * v] = u.x; rv[4 * v + 1] = u.y; rv[4 * v + 2] = u.z; rv[4 * v + 3] = u.w;
-          }
-          add_residual32<DT>(f, rv);
-        } else if (RES && rrow) {
-          uint32_t rv[16];
-          load_residual32(rv, rrow, n_base, p.N);
+          tile.own_row(rv, h);
           add_residual32<DT>(f, rv);
         }
         uint32_t packed[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) packed[j] = Elem<DT>::pack2(f[2 * j], f[2 * j + 1]);
+        tile.set_own_row(packed, h);      // the 128-byte swizzle that the TMA store reads
         if (p.y_tma) {
-          // Row `lane` of the staging tile, 128-byte swizzle: 16-byte unit
-          // v of the row lives at unit (v ^ (row & 7)).
-          uint4* srow = reinterpret_cast<uint4*>(sb + lane * (kEpiCols * 2));
-#pragma unroll
-          for (int v = 0; v < 4; ++v)
-            srow[(h * 4 + v) ^ (lane & 7)] =
-                make_uint4(packed[4 * v], packed[4 * v + 1], packed[4 * v + 2], packed[4 * v + 3]);
           if (h == 1) {
             fence_proxy_async_smem();    // staging writes -> visible to the TMA unit
             __syncwarp();
@@ -742,17 +693,10 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
               }
             }
           }
-        } else if (row_ok) {
-          if (p.y_vec_ok && n_base + 32 <= p.N) {
-            uint4* dst = reinterpret_cast<uint4*>(yrow + n_base);
-#pragma unroll
-            for (int v = 0; v < 4; ++v)
-              dst[v] = make_uint4(packed[4 * v], packed[4 * v + 1], packed[4 * v + 2], packed[4 * v + 3]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (n_base + j < p.N) yrow[n_base + j] = Elem<DT>::from_f(f[j]);
-          }
+        } else if (h == 1) {
+          __syncwarp();
+          tile.store(p.y, p.ldy, warp_row0, p.M, n_chunk, p.N);
+          __syncwarp();
         }
       }
       // All TMEM reads of this accumulator are complete: hand it back. After
@@ -881,7 +825,7 @@ cudaError_t launch_tc2_bn(int dtype, Tc2Params& p, const void* a, int64_t M, int
   // TMA-store epilogue when y's rows are 16-byte aligned (else direct stores).
   p.y_tma = p.y_vec_ok && make_tmap_kmajor(&ty, y, M, N, ldy, kEpiCols, 32) ? 1 : 0;
   if (!p.y_tma) ty = ta;     // not read by the kernel
-  p.res_tile = p.res && p.y_tma && (reinterpret_cast<uintptr_t>(p.res) & 15u) == 0 && (p.ldr % 8) == 0 ? 1 : 0;
+  p.res_align = row_alignment(p.res, p.ldr);
   if (p.n_peers > 0 && !p.y_tma) return cudaErrorInvalidValue;   // peer stores ride the TMA path
 
   const int64_t pairs = std::max<int64_t>(1, (sm_count > 0 ? sm_count : 148) / 2);
