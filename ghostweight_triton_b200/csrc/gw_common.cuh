@@ -792,21 +792,32 @@ struct WarpTile {
         v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
       }
     } else {
+      // Lanes outside read a place inside (the last row or column), and drop it.
       constexpr int kRows = 32 / kWords;
-      const int64_t cols = N - n0 - (lane % kWords) * 2;
-      const uint16_t* p = src + (row0 + lane / kWords) * ld + n0 + (lane % kWords) * 2;
       const int64_t left = M - row0 - lane / kWords;
-      if (align == 4 && cols != 1) {
+      const int64_t col = n0 + (lane % kWords) * 2;
+      const int last = left <= 0 ? 0 : left < 32 ? static_cast<int>(left) - 1 : 31;
+      const uint16_t* p = src + (left > 0 ? (row0 + lane / kWords) * ld : 0);
+      if (align == 4 && (N & 1) == 0) {
+        const uint16_t* e = p + (col < N ? col : 0);
 #pragma unroll
-        for (int i = 0; i < kRegs; ++i)
-          v[i] = i * kRows < left && cols > 1 ? *reinterpret_cast<const uint32_t*>(p + i * kRows * ld) : 0u;
+        for (int i = 0; i < kRegs; ++i) v[i] = *reinterpret_cast<const uint32_t*>(e + min(i * kRows, last) * ld);
+        if (col >= N) {
+#pragma unroll
+          for (int i = 0; i < kRegs; ++i) v[i] = 0u;
+        }
       } else {
+        const uint16_t* e0 = p + (col < N ? col : 0);
+        const uint16_t* e1 = p + (col + 1 < N ? col + 1 : 0);
+        const uint32_t m0 = col < N ? 0xFFFFu : 0u, m1 = col + 1 < N ? 0xFFFF0000u : 0u;
+        uint16_t lo[kRegs], hi[kRegs];
 #pragma unroll
         for (int i = 0; i < kRegs; ++i) {
-          const uint32_t lo = i * kRows < left && cols > 0 ? p[i * kRows * ld] : 0u;
-          const uint32_t hi = i * kRows < left && cols > 1 ? p[i * kRows * ld + 1] : 0u;
-          v[i] = lo | (hi << 16);
+          lo[i] = e0[min(i * kRows, last) * ld];
+          hi[i] = e1[min(i * kRows, last) * ld];
         }
+#pragma unroll
+        for (int i = 0; i < kRegs; ++i) v[i] = (lo[i] & m0) | ((static_cast<uint32_t>(hi[i]) << 16) & m1);
       }
     }
   }

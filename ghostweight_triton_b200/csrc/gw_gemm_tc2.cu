@@ -615,7 +615,10 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
       const int steps = sub < 0 ? (half ? C::kCols1 : C::kCols0) / 32 : 2;   // 32-column loads (even)
       // The residual of a 64-column chunk is loaded one chunk ahead, the first one
       // while the MMAs run, and goes through the staging tile to the lanes that own
-      // the rows (8192 x 4096 x 512: 39.5 us; 47.9 with lanes loading their own rows).
+      // the rows. 8192 x 4096 x 512 bf16: 39.5 us (31.2 without a residual); 47.9
+      // with lanes loading their own rows, 51 when a chunk is requested only behind
+      // the last bias load of the one before (loads return in order, but the
+      // residual's latency is the longer one).
       uint32_t rt[RES ? WarpTile<kEpiCols>::kRegs : 1];
       if constexpr (RES) tile.load(rt, p.res, p.ldr, p.res_align, warp_row0, p.M, n_warp, p.N);
       if (!mbar_wait_cluster(tfull(b), aph, abort_flag, p.err)) break;
