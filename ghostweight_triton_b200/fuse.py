@@ -13,6 +13,11 @@ columns of the second weight are zero. The fused chain therefore
   already is the second layer's compacted input x'; and
 * feeds that straight into the second GEMM (both operands by TMA, no gather).
 
+``GhostPreNormMLP`` puts the residual stream and the root-mean-square norm in
+front of the same chain, so that a whole pre-norm MLP block is three launches
+(five in e4m3): the residual's addition, the norm and the first layer's gather
+are one kernel, and the second addition is the last GEMM's epilogue.
+
 One gather launch and the dead part of the first GEMM disappear; the result
 equals the unfused chain's (the skipped terms are products with zero weights),
 up to the one rounding of the intermediate that the fused GELU saves. This is
@@ -26,7 +31,9 @@ import torch
 import torch.nn as nn
 
 from ghostweight_triton_b200.kernels.gather import pack_weight
-from ghostweight_triton_b200.kernels.matmul import ghost_linear, packed_linear
+from ghostweight_triton_b200.kernels._args import refuse_grad
+from ghostweight_triton_b200.kernels.matmul import ghost_linear, packed_linear, packed_linear_q8
+from ghostweight_triton_b200.kernels.norm import quantize_rows, rms_norm, rms_norm_q8
 from ghostweight_triton_b200.module import GhostLinear
 
 # Activation modules (by class name) that the GEMM epilogue reproduces.
@@ -119,6 +126,81 @@ class GhostMLPChain(nn.Module):
         if behind:
             y = y + residual.reshape(-1, self.proj.out_features)
         return y.reshape(*lead, self.proj.out_features)
+
+
+class GhostPreNormMLP(GhostMLPChain):
+    """s = x + residual;  y = s + proj(activation(fc(rms_norm(s)))).
+
+    ``norm`` is a root-mean-square norm over fc's input features (torch.nn.RMSNorm,
+    or a module with ``weight`` and ``eps`` or ``variance_epsilon``), ``fc`` and
+    ``proj`` are GhostLinears with frozen masks, joined by the GELU ``activation``
+    ("gelu" or "gelu_tanh"); all stay registered, so parameters and state-dict
+    keys are theirs. fp16 and bf16 inputs. ``precision="e4m3"`` runs both
+    products on e4m3 operands (weights rounded once with a scale per feature,
+    activations with one per token), with fp32 sums and the residual stream in
+    the input's type.
+    """
+
+    def __init__(self, norm: nn.Module, fc: GhostLinear, proj: GhostLinear, activation: str,
+                 dropout: nn.Module | None = None, precision: str = "input"):
+        super().__init__(fc, proj, activation, dropout)
+        if precision not in ("input", "e4m3"):
+            raise ValueError(f"precision must be 'input' or 'e4m3', got {precision!r}")
+        assert proj.out_features == fc.in_features, "the block adds its output to its input"
+        assert not isinstance(norm, nn.LayerNorm) and getattr(norm, "bias", None) is None, (
+            "norm must be a root-mean-square norm (no mean, no bias)")
+        weight = getattr(norm, "weight", None)
+        assert weight is None or weight.shape == (fc.in_features,), (
+            f"norm must be over fc's {fc.in_features} input features")
+        self.norm = norm
+        self.precision = precision
+        self._plan_q8: tuple | None = None
+
+    def refresh_packed(self) -> None:
+        super().refresh_packed()
+        self._plan_q8 = None
+
+    def _eps(self, dtype: torch.dtype) -> float:
+        eps = getattr(self.norm, "eps", getattr(self.norm, "variance_epsilon", None))
+        return torch.finfo(dtype).eps if eps is None else float(eps)       # None: torch.nn.RMSNorm's default
+
+    def _operands_q8(self, dtype: torch.dtype):
+        w_fc, b_fc, w_proj = self._operands(dtype)
+        if self._plan_q8 is None or self._plan_q8[0] is not w_fc:
+            self._plan_q8 = (w_fc, quantize_rows(w_fc), quantize_rows(w_proj))
+        return self._plan_q8[1], b_fc, self._plan_q8[2]
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+        """x [..., features], and optionally a residual of its shape added in front of the norm."""
+        assert x.dtype in (torch.float16, torch.bfloat16), f"GhostPreNormMLP runs fp16 and bf16, got {x.dtype}"
+        if not (_frozen(self.fc) and _frozen(self.proj)):
+            raise RuntimeError("GhostPreNormMLP needs frozen masks on fc and proj (freeze_mask or freeze_weight_mask)")
+        refuse_grad(x=x, residual=residual)
+        features = self.fc.in_features
+        x2 = x.reshape(-1, features)
+        r2 = None if residual is None else residual.reshape(-1, features)
+        norm = dict(weight=getattr(self.norm, "weight", None), eps=self._eps(x.dtype), residual=r2,
+                    alive_indices=self.fc._frozen_indices)
+        bias = self.proj.bias
+        if bias is not None and bias.dtype != x.dtype:
+            bias = bias.to(x.dtype)
+        identity = self.dropout is None or (isinstance(self.dropout, nn.Dropout) and not self.dropout.training)
+        if self.precision == "e4m3":
+            (w_fc, s_fc), b_fc, (w_proj, s_proj) = self._operands_q8(x.dtype)
+            q, scale, *rest = rms_norm_q8(x2, **norm)
+            s = rest[0] if rest else x2
+            h = packed_linear_q8(q, scale, w_fc, s_fc, bias=b_fc, activation=self.activation, dtype=x.dtype)
+            q, scale = quantize_rows(h)
+            y = packed_linear_q8(q, scale, w_proj, s_proj, bias=bias, residual=s if identity else None, dtype=x.dtype)
+        else:
+            w_fc, b_fc, w_proj = self._operands(x.dtype)
+            out = rms_norm(x2, **norm)
+            n, s = out if r2 is not None else (out, x2)
+            h = packed_linear(n, w_fc, bias=b_fc, activation=self.activation)
+            y = packed_linear(h, w_proj, bias=bias, residual=s if identity else None)
+        if not identity:
+            y = s + self.dropout(y)
+        return y.reshape(x.shape)
 
 
 def _frozen(m: nn.Module) -> bool:
