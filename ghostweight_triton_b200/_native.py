@@ -373,21 +373,12 @@ def gather_gemm(x: torch.Tensor, w_packed: torch.Tensor, idx: torch.Tensor, y: t
         _rowmajor(x, w_packed, y)                # raises
     n = idx.numel()
     ws_ptr, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
-    dev = x.get_device()
-    cur = torch.cuda.current_device()
-    if dev != cur:
-        torch.cuda.set_device(dev)
-    try:
-        r_ptr, ldr = _residual(residual) if residual is not None else (None, 0)
-        st = api().gw_gather_gemm_residual(
-            x.data_ptr(), DTYPE_CODES[x.dtype], M, K, sx if sx > K else K, w_packed.data_ptr(), N,
-            sw if sw > n else n, idx.data_ptr(), n, None if bias is None else bias.data_ptr(),
-            EPILOGUES[activation] if activation in EPILOGUES else epilogue_code(activation),
-            r_ptr, ldr, y.data_ptr(), sy if sy > N else N, GEMM_STRATEGIES[strategy], ws_ptr, ws_bytes,
-            _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream)
-    finally:
-        if dev != cur:
-            torch.cuda.set_device(cur)
+    r_ptr, ldr = _residual(residual) if residual is not None else (None, 0)
+    st = _call((_api or api()).gw_gather_gemm_residual,
+               (x.data_ptr(), DTYPE_CODES[x.dtype], M, K, sx if sx > K else K, w_packed.data_ptr(), N,
+                sw if sw > n else n, idx.data_ptr(), n, None if bias is None else bias.data_ptr(),
+                epilogue_code(activation), r_ptr, ldr, y.data_ptr(), sy if sy > N else N, GEMM_STRATEGIES[strategy],
+                ws_ptr, ws_bytes), x.get_device())
     if st:
         _check(st, "gw_gather_gemm")
 
@@ -532,21 +523,11 @@ def packed_gemm_q8(a: torch.Tensor, a_scale: torch.Tensor, M: int, K: int, lda: 
                    bias: torch.Tensor | None = None, activation: str | None = None,
                    residual: torch.Tensor | None = None) -> None:
     """y = act(a_scale w_scale (a @ w_packed^T) + bias) + residual over e4m3 operands by TMA."""
-    dev = a.get_device()
-    cur = torch.cuda.current_device()
-    if dev != cur:
-        torch.cuda.set_device(dev)
-    try:
-        r_ptr, ldr = _residual(residual) if residual is not None else (None, 0)
-        st = api().gw_packed_gemm_q8(
-            a.data_ptr(), a_scale.data_ptr(), M, K, lda, w_packed.data_ptr(), w_scale.data_ptr(), N, ldw,
-            None if bias is None else bias.data_ptr(),
-            EPILOGUES[activation] if activation in EPILOGUES else epilogue_code(activation),
-            r_ptr, ldr, y.data_ptr(), DTYPE_CODES[y.dtype], ldy,
-            _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream)
-    finally:
-        if dev != cur:
-            torch.cuda.set_device(cur)
+    r_ptr, ldr = _residual(residual) if residual is not None else (None, 0)
+    st = _call((_api or api()).gw_packed_gemm_q8,
+               (a.data_ptr(), a_scale.data_ptr(), M, K, lda, w_packed.data_ptr(), w_scale.data_ptr(), N, ldw,
+                None if bias is None else bias.data_ptr(), epilogue_code(activation), r_ptr, ldr, y.data_ptr(),
+                DTYPE_CODES[y.dtype], ldy), a.get_device())
     if st:
         _check(st, "gw_packed_gemm_q8")
 
@@ -577,6 +558,24 @@ def _ld(t: torch.Tensor) -> int:
     return max(t.stride(0), t.shape[1])
 
 
+try:  # the current device without torch.cuda's wrapper (the caller's tensor has initialised CUDA)
+    _current_device = torch._C._cuda_getDevice
+except AttributeError:  # pragma: no cover - older torch
+    _current_device = torch.cuda.current_device
+
+
+def _call(fn, args: tuple, dev: int) -> int:
+    """fn(*args, torch's current stream of device `dev`), with that device current."""
+    cur = _current_device()
+    if dev == cur:
+        return fn(*args, _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream)
+    torch.cuda.set_device(dev)
+    try:
+        return fn(*args, _stream(torch.device("cuda", dev)))
+    finally:
+        torch.cuda.set_device(cur)
+
+
 def rms_norm(x: torch.Tensor, rows: int, cols: int, ldx: int, residual: torch.Tensor | None, ldr: int,
              total: torch.Tensor | None, lds: int, weight: torch.Tensor | None, eps: float,
              idx: torch.Tensor | None, n: int, y: torch.Tensor, pad: int,
@@ -584,24 +583,14 @@ def rms_norm(x: torch.Tensor, rows: int, cols: int, ldx: int, residual: torch.Te
     """gw_rms_norm (scale None) or gw_rms_norm_q8 over row-major matrices; y is the whole
     [rows, pad] buffer, of which the first n columns are outputs and the rest is zeroed."""
     dev = x.get_device()
-    cur = torch.cuda.current_device()
-    if dev != cur:
-        torch.cuda.set_device(dev)
-    try:
-        stream = _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
-        r_ptr = None if residual is None else residual.data_ptr()
-        s_ptr = None if total is None else total.data_ptr()
-        g_ptr = None if weight is None else weight.data_ptr()
-        i_ptr = None if idx is None else idx.data_ptr()
-        if scale is None:
-            st = api().gw_rms_norm(x.data_ptr(), DTYPE_CODES[x.dtype], rows, cols, ldx, r_ptr, ldr, s_ptr, lds,
-                                   g_ptr, eps, i_ptr, n, y.data_ptr(), pad, pad, stream)
-        else:
-            st = api().gw_rms_norm_q8(x.data_ptr(), DTYPE_CODES[x.dtype], rows, cols, ldx, r_ptr, ldr, s_ptr, lds,
-                                      g_ptr, eps, i_ptr, n, y.data_ptr(), pad, pad, scale.data_ptr(), stream)
-    finally:
-        if dev != cur:
-            torch.cuda.set_device(cur)
+    args = (x.data_ptr(), DTYPE_CODES[x.dtype], rows, cols, ldx, None if residual is None else residual.data_ptr(),
+            ldr, None if total is None else total.data_ptr(), lds, None if weight is None else weight.data_ptr(), eps,
+            None if idx is None else idx.data_ptr(), n, y.data_ptr(), pad, pad)
+    lib = _api or api()
+    if scale is None:
+        st = _call(lib.gw_rms_norm, args, dev)
+    else:
+        st = _call(lib.gw_rms_norm_q8, (*args, scale.data_ptr()), dev)
     if st:
         _check(st, "gw_rms_norm" if scale is None else "gw_rms_norm_q8")
 
@@ -611,18 +600,9 @@ def quantize_rows(x: torch.Tensor, idx: torch.Tensor | None, n: int, q: torch.Te
     """gw_quantize_rows over a row-major matrix; q is the whole padded buffer."""
     rows, cols = x.shape
     pad = q.shape[1]
-    dev = x.get_device()
-    cur = torch.cuda.current_device()
-    if dev != cur:
-        torch.cuda.set_device(dev)
-    try:
-        st = api().gw_quantize_rows(
-            x.data_ptr(), dtype_code(x.dtype), rows, cols, _ld(x), None if idx is None else idx.data_ptr(), n,
-            q.data_ptr(), pad, pad, scale.data_ptr(),
-            _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream)
-    finally:
-        if dev != cur:
-            torch.cuda.set_device(cur)
+    st = _call((_api or api()).gw_quantize_rows,
+               (x.data_ptr(), DTYPE_CODES[x.dtype], rows, cols, _ld(x), None if idx is None else idx.data_ptr(), n,
+                q.data_ptr(), pad, pad, scale.data_ptr()), x.get_device())
     if st:
         _check(st, "gw_quantize_rows")
 

@@ -81,12 +81,13 @@ gemm_f32_kernel(const SimtParams p) {
   const int tid = threadIdx.x;
   const int64_t m0 = static_cast<int64_t>(blockIdx.y) * BM;
   const int64_t n0 = static_cast<int64_t>(blockIdx.x) * BN;
-  // A warp is 4 x 8 threads: a vector load of W' touches eight rows (all 32
-  // banks), one of x four, each shared by the threads beside or below.
+  // A warp is 4 x 8 threads, eight neighbouring lanes 2 x 4 of them: a vector load
+  // takes four rows of W' (two of x) for each eight lanes. 3 to 5% faster than
+  // eight lanes along a row.
   const int lane = tid & 31;
   constexpr int kWarpsN = BN / (8 * TN);
-  const int row_t = (tid >> 5) / kWarpsN * (4 * TM) + (lane >> 3);   // rows row_t + 4 i
-  const int col_t = (tid >> 5) % kWarpsN * (8 * TN) + (lane & 7);    // columns col_t + 8 j
+  const int row_t = (tid >> 5) / kWarpsN * (4 * TM) + (((lane >> 4) << 1) | (lane & 1));   // rows row_t + 4 i
+  const int col_t = (tid >> 5) % kWarpsN * (8 * TN) + ((lane >> 1) & 7);                  // columns col_t + 8 j
   const int lk = tid % BK;                           // this thread's column of x tiles
   const int lr = tid / BK;
   const int nk = static_cast<int>((n_alive + BK - 1) / BK);
@@ -279,15 +280,15 @@ cudaError_t launch_gemm_f32(const float* x, int64_t M, int64_t K, int64_t ldx, c
   p.res = static_cast<const float*>(res.p);
   p.ldr = res.ld;
   p.w_vec = ((reinterpret_cast<uintptr_t>(w) & 15u) == 0 && (N <= 1 || ldw % 4 == 0)) ? 1 : 0;
-  // Measured (us) for M x N x K' = 1024 x 768 x 384, 100 x 4096 x 2048, 1024 x
-  // 4096 x 2048 and 4096 x 4096 x 2048: 64 x 64 tiles 32, 116, 532 and 1792; 32
-  // x 64 tiles 27, 99, 605 and 2234; 128 x 128 tiles (one or two CTAs per SM hold
-  // their registers) 92, 408, 565 and 2000. 16 x 4096 x 2048: 16 x 32 tiles with
-  // 64 columns a stage 42, with 32 columns 62; 32 x 32 tiles 71.
+  // Measured (us) for M x N x K' = 1024 x 768 x 384, 100 x 4096 x 2048 and 4096 x
+  // 4096 x 2048: 64 x 64 tiles 32, 116 and 1745; 32 x 64 tiles 26, 81 and 1904
+  // (with 32 columns a stage 27, 98 and 2234); 128 x 128 tiles 92, 408 and 2000
+  // (one CTA per SM holds their registers). 16 x 4096 x 2048: 16 x 32 tiles with 64
+  // columns a stage 42, with 32 columns 62; 32 x 32 tiles 71.
   auto ctas = [&](int64_t bm, int64_t bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
   constexpr int64_t kSms = 148;
   if (M <= 16) return launch_simt<16, 32, 64, 2, 2, 4>(p, stream);
-  if (ctas(64, 64) < 4 * kSms) return launch_simt<32, 64, 32, 4, 4, 3>(p, stream);
+  if (ctas(64, 64) < 4 * kSms) return launch_simt<32, 64, 64, 4, 4, 2>(p, stream);
   return launch_simt<64, 64, 32, 8, 4, 3>(p, stream);
 }
 

@@ -177,15 +177,33 @@ def clear_packed_cache() -> None:
 
 
 def _gemm(x, w_packed, idx, y, bias, activation, strategy, residual=None):
-    ws = None
+    """gw_gather_gemm_residual for a contiguous x; w_packed and y are row-major."""
     if strategy == "runs" and (x.data_ptr() % 16 or x.stride(0) % 8):
         strategy = "auto"          # direct TMA of x needs 16-byte aligned rows
-    if strategy != "fused" and strategy != "runs" and x.dtype is not torch.float32:
-        nbytes = _native.gather_gemm_workspace_bytes(x.shape[0], idx.numel(), x.dtype)
+    dtype = x.dtype
+    M, K = x.shape
+    N, wk = w_packed.shape
+    ldw, uw = w_packed.stride()
+    ldy, uy = y.stride()
+    assert idx.dtype is torch.int64 and idx.is_contiguous()
+    if (uw != 1 and wk > 1) or (uy != 1 and N > 1) or dtype not in _native.DTYPE_CODES:
+        _native.dtype_code(dtype)                # raises
+        _native._rowmajor(w_packed, y)
+    n = idx.numel()
+    ws_ptr, ws_bytes = None, 0
+    if strategy != "fused" and strategy != "runs" and dtype is not torch.float32:
+        nbytes = _native.gather_gemm_workspace_bytes(M, n, dtype)
         if nbytes:
             ws = _native.gemm_workspace(x.device, nbytes)
-    _native.gather_gemm(x, w_packed, idx, y, bias=bias, activation=activation,
-                        strategy=strategy, workspace=ws, residual=residual)
+            ws_ptr, ws_bytes = ws.data_ptr(), ws.numel()
+    r_ptr, ldr = (None, 0) if residual is None else (residual.data_ptr(), max(residual.stride(0), N))
+    st = _native._call((_native._api or _native.api()).gw_gather_gemm_residual,
+                       (x.data_ptr(), _native.DTYPE_CODES[dtype], M, K, K, w_packed.data_ptr(), N, ldw if ldw > n else n,
+                        idx.data_ptr(), n, None if bias is None else bias.data_ptr(), _native.epilogue_code(activation),
+                        r_ptr, ldr, y.data_ptr(), ldy if ldy > N else N, _native.GEMM_STRATEGIES[strategy], ws_ptr,
+                        ws_bytes), x.get_device())
+    if st:
+        _native._check(st, "gw_gather_gemm")
 
 
 def index_runs(alive_indices: torch.Tensor, K: int) -> int:
