@@ -89,7 +89,6 @@ struct RowParams {
   int64_t lds = 0;
   const void* g = nullptr;          // norm weight [cols] or null
   float eps = 0.0f;
-  int norm = 0;                     // set by launch_rows
   const int64_t* idx = nullptr;     // alive list (n entries) or null: all columns
   int64_t n = 0;                    // outputs per row
   int64_t pad = 0;                  // columns [n, pad) of y are written as zero
@@ -102,7 +101,7 @@ struct RowParams {
 };
 // q8: y is e4m3 with scales. norm: the root-mean-square norm, else x as it is
 // (only with q8).
-cudaError_t launch_rows(RowParams p, int dtype, bool q8, bool norm, int sm_count,
+cudaError_t launch_rows(const RowParams& p, int dtype, bool q8, bool norm, int sm_count,
                         cudaStream_t stream);
 
 // gw_gemm_tc.cu: tcgen05 gather-GEMM / packed GEMM (fp16, bf16).

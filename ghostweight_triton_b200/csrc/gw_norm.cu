@@ -299,7 +299,8 @@ struct RowShared {
 };
 constexpr int kRowHead = 512 + 4 * kMaxStages * 8 + 64;
 
-template <int DT, bool Q8, bool GATHER, int MODE, int E, bool WARP, int MAXT>
+// NORM: residual, norm and weight; else (Q8) the rows as they are.
+template <int DT, bool Q8, bool NORM, bool GATHER, int MODE, int E, bool WARP, int MAXT>
 __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const RowShared sh, int y_vec) {
   using raw = typename Elem<DT>::raw;
   using out = typename RowOut<Q8, DT>::raw;
@@ -308,6 +309,10 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
   constexpr int I = E / V;                                        // vectors (or elements) per thread
   constexpr int kPack = Q8 ? 4 : sizeof(raw) == 2 ? 2 : 1;        // outputs per 4-byte store
   constexpr bool STAGED = GATHER && MODE != kLong;                // u passes through shared memory
+  static_assert(NORM || Q8, "plain rows are only rounded");
+  // Plain rows of 16-bit vectors: the largest magnitude of two values at a time,
+  // on their bits (see the file comment), without turning them into floats.
+  constexpr bool kBits16 = !NORM && !GATHER && VEC && sizeof(raw) == 2;
   extern __shared__ __align__(128) uint8_t smem[];
   const int G = WARP ? 32 : static_cast<int>(blockDim.x);
   const int t = WARP ? (threadIdx.x & 31) : threadIdx.x;
@@ -351,14 +356,14 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
     const uint32_t dst = ring_s + static_cast<uint32_t>(s * sh.stage_bytes);
     const uint32_t bar = bar0 + 8u * s;
     if constexpr (VEC) {
-      mbar_arrive_expect_tx(bar, p.r ? 2 * row_bytes : row_bytes);
+      mbar_arrive_expect_tx(bar, NORM && p.r ? 2 * row_bytes : row_bytes);
       bulk_load(dst, static_cast<const raw*>(p.x) + row * p.ldx, row_bytes, bar);
-      if (p.r) bulk_load(dst + sh.operand_bytes, static_cast<const raw*>(p.r) + row * p.ldr, row_bytes, bar);
+      if (NORM && p.r) bulk_load(dst + sh.operand_bytes, static_cast<const raw*>(p.r) + row * p.ldr, row_bytes, bar);
     } else {
       uintptr_t xl, rl = 0;
       uint32_t xb, rb = 0;
       if (!granules(p.x, p.ldx, row, xl, xb)) xb = 0;
-      if (!p.r || !granules(p.r, p.ldr, row, rl, rb)) rb = 0;
+      if (!NORM || !p.r || !granules(p.r, p.ldr, row, rl, rb)) rb = 0;
       mbar_arrive_expect_tx(bar, xb + rb);
       if (xb) bulk_load(dst, reinterpret_cast<const void*>(xl), xb, bar);
       if (rb) bulk_load(dst + sh.operand_bytes, reinterpret_cast<const void*>(rl), rb, bar);
@@ -369,7 +374,7 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
 
   uint32_t named = 0xFFFFFFFFu;                                   // this thread's columns in the list
   bool checked = false;                                           // some output has no column
-  const raw* g = static_cast<const raw*>(p.g);
+  const raw* g = NORM ? static_cast<const raw*>(p.g) : nullptr;
   if constexpr (GATHER) {
     if constexpr (Q8) {
       for (int i = threadIdx.x; i < (cols + 3) / 4; i += blockDim.x) reinterpret_cast<uint32_t*>(flags)[i] = 0;
@@ -414,13 +419,13 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
       }
     }
   }
-  Held<DT, MODE == kLong ? 1 : E> gain;                           // this thread's share of the weight
+  Held<DT, MODE == kLong || !NORM ? 1 : E> gain;                  // this thread's share of the weight
   gain.clear();
-  if (MODE != kLong && g) {
+  if constexpr (NORM && MODE != kLong) {
 #pragma unroll
     for (int i = 0; i < I; ++i) {
       const int k = (i * G + t) * V;
-      if (k < cols) {
+      if (g && k < cols) {
         if constexpr (VEC) gain.set16(i, __ldg(reinterpret_cast<const uint4*>(g) + i * G + t));
         else gain.set(i, __ldg(g + k));
       }
@@ -431,9 +436,9 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
   int buf = 0, stage = 0;
   uint32_t phase = 0;
   // The row's place in each output, moved along with the row.
-  raw* sum = p.s ? static_cast<raw*>(p.s) + row0 * p.lds : nullptr;
+  raw* sum = NORM && p.s ? static_cast<raw*>(p.s) + row0 * p.lds : nullptr;
   out* y = static_cast<out*>(p.y) + row0 * p.ldy;
-  const int64_t sum_step = p.s ? step * p.lds : 0;
+  const int64_t sum_step = NORM && p.s ? step * p.lds : 0;
   const int64_t y_step = step * p.ldy;
   for (int64_t row = row0; row < p.rows; row += step, sum += sum_step, y += y_step) {
     const uint8_t* xs = ring + stage * sh.stage_bytes;
@@ -448,26 +453,35 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
     // squared into ss2 when `first`, times the weight.
     auto vector = [&](int v, int i, float* f, bool first) {
       unpack16<DT>(reinterpret_cast<const uint4*>(xs)[v], f);
-      float2* f2 = reinterpret_cast<float2*>(f);
-      float q[V];
-      if (p.r) {
-        unpack16<DT>(reinterpret_cast<const uint4*>(rs)[v], q);
+      if constexpr (NORM) {
+        float2* f2 = reinterpret_cast<float2*>(f);
+        float q[V];
+        if (p.r) {
+          unpack16<DT>(reinterpret_cast<const uint4*>(rs)[v], q);
 #pragma unroll
-        for (int j = 0; j < V / 2; ++j) f2[j] = add2(f2[j], make_float2(q[2 * j], q[2 * j + 1]));
-      }
-      if (first) {
-        if (sum) reinterpret_cast<uint4*>(sum)[v] = pack16<DT>(f);
-        if (p.norm) {
+          for (int j = 0; j < V / 2; ++j) f2[j] = add2(f2[j], make_float2(q[2 * j], q[2 * j + 1]));
+        }
+        if (first) {
+          if (sum) reinterpret_cast<uint4*>(sum)[v] = pack16<DT>(f);
 #pragma unroll
           for (int j = 0; j < V / 2; ++j) ss2 = fma2(f2[j], f2[j], ss2);
         }
-      }
-      if (g) {
-        if constexpr (MODE == kLong) unpack16<DT>(__ldg(reinterpret_cast<const uint4*>(g) + v), q);
+        if (g) {
+          if constexpr (MODE == kLong) unpack16<DT>(__ldg(reinterpret_cast<const uint4*>(g) + v), q);
 #pragma unroll
-        for (int j = 0; j < V / 2; ++j)
-          f2[j] = mul2(f2[j], MODE == kLong ? make_float2(q[2 * j], q[2 * j + 1]) : gain.get2(i * V + 2 * j));
+          for (int j = 0; j < V / 2; ++j) {
+            if constexpr (MODE == kLong) f2[j] = mul2(f2[j], make_float2(q[2 * j], q[2 * j + 1]));
+            else f2[j] = mul2(f2[j], gain.get2(i * V + 2 * j));
+          }
+        }
       }
+    };
+    // kBits16: the largest bits of |x| so far, two 16-bit values.
+    uint32_t largest = 0;
+    auto vector_bits = [&](int v) {
+      const uint4 q = reinterpret_cast<const uint4*>(xs)[v];
+      largest = __vmaxu2(largest, __vmaxu2(__vmaxu2(q.x & 0x7FFF7FFFu, q.y & 0x7FFF7FFFu),
+                                           __vmaxu2(q.z & 0x7FFF7FFFu, q.w & 0x7FFF7FFFu)));
     };
     if constexpr (MODE == kVec) {
 #pragma unroll
@@ -476,6 +490,7 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
         float* f = u + i * V;
         if (v * V < cols) {
           vector(v, i, f, true);
+          if constexpr (kBits16) vector_bits(v);
           if constexpr (STAGED) {
 #pragma unroll
             for (int j = 0; j < V; j += 4)
@@ -487,13 +502,18 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
           for (int j = 0; j < V; ++j) f[j] = 0.0f;
         }
       }
-      if constexpr (Q8) {
+      if constexpr (Q8 && !kBits16) {
 #pragma unroll
         for (int e = 0; e < E; ++e)
           if (!GATHER || ((named >> e) & 1u)) uabs = max_abs(uabs, u[e]);
       }
     } else if constexpr (MODE == kLong) {
+#pragma unroll 4
       for (int v = t; v * V < cols; v += G) {
+        if constexpr (kBits16) {
+          vector_bits(v);
+          continue;
+        }
         vector(v, 0, u, true);
         if constexpr (Q8) {
 #pragma unroll
@@ -503,7 +523,7 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
       }
     } else {
       const raw* x = static_cast<const raw*>(p.x) + row * p.ldx;
-      const raw* r = p.r ? static_cast<const raw*>(p.r) + row * p.ldr : nullptr;
+      const raw* r = NORM && p.r ? static_cast<const raw*>(p.r) + row * p.ldr : nullptr;
       uintptr_t lo;
       uint32_t bytes;
       const bool in_x = granules(p.x, p.ldx, row, lo, bytes);
@@ -537,8 +557,10 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
       float2* u2 = reinterpret_cast<float2*>(u);
 #pragma unroll
       for (int i = 0; i < E / 2; ++i) {
-        ss2 = fma2(u2[i], u2[i], ss2);
-        if (g) u2[i] = mul2(u2[i], gain.get2(2 * i));
+        if constexpr (NORM) {
+          ss2 = fma2(u2[i], u2[i], ss2);
+          if (g) u2[i] = mul2(u2[i], gain.get2(2 * i));
+        }
       }
 #pragma unroll
       for (int i = 0; i < I; ++i) {
@@ -552,9 +574,13 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
     }
     float ss = ss2.x + ss2.y;
     uint32_t umax = __float_as_uint(uabs);
+    if constexpr (kBits16)
+      umax = __float_as_uint(Elem<DT>::to_f(static_cast<raw>(max(largest & 0xFFFFu, largest >> 16))));
     // Sum of squares and largest |u| of the row; publishes srow too.
+    if constexpr (NORM) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+      for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+    }
     if constexpr (Q8) umax = __reduce_max_sync(0xFFFFFFFFu, umax);
     if constexpr (WARP) {
       __syncwarp();
@@ -578,13 +604,15 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
     if constexpr (!WARP) {
       const int lane = t & 31;
       const bool in = lane < (G >> 5);
-      ss = in ? red_v[buf * 32 + lane] : 0.0f;
+      if constexpr (NORM) {
+        ss = in ? red_v[buf * 32 + lane] : 0.0f;
 #pragma unroll
-      for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+        for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+      }
       if constexpr (Q8) umax = __reduce_max_sync(0xFFFFFFFFu, in ? red_m[buf * 32 + lane] : 0u);
       buf ^= 1;
     }
-    const float rstd = p.norm ? rsqrtf(ss * inv_cols + p.eps) : 1.0f;
+    const float rstd = NORM ? rsqrtf(ss * inv_cols + p.eps) : 1.0f;
     RowScale q8 = {1.0f, 1.0f, 1.0f};
     if constexpr (Q8) {
       q8 = row_scale(umax, rstd);
@@ -692,7 +720,7 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
           v[e] = 0.0f;
           if (c != kNoColumn) {
             float f = Elem<DT>::to_f(x[c]);
-            if (p.r) f += Elem<DT>::to_f(r[c]);
+            if (NORM && p.r) f += Elem<DT>::to_f(r[c]);
             if (g) f *= Elem<DT>::to_f(__ldg(g + c));
             v[e] = value(f);
           }
@@ -703,9 +731,11 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
       refill();
     } else {
       if constexpr (MODE == kLong) {
+#pragma unroll 2
         for (int v = t; v * V < cols; v += G) {
-          vector(v, 0, u, false);
-          store_vector(v * V, u);
+          __align__(16) float f[V];
+          vector(v, 0, f, false);
+          store_vector(v * V, f);
         }
       } else {
 #pragma unroll
@@ -728,9 +758,9 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
     }
 }
 
-template <int DT, bool Q8, bool GATHER, int MODE, int E, bool WARP, int MAXT>
+template <int DT, bool Q8, bool NORM, bool GATHER, int MODE, int E, bool WARP, int MAXT>
 cudaError_t launch_rows_variant(const RowParams& p, int y_vec, int sm_count, cudaStream_t stream) {
-  auto kern = rows_kernel<DT, Q8, GATHER, MODE, E, WARP, MAXT>;
+  auto kern = rows_kernel<DT, Q8, NORM, GATHER, MODE, E, WARP, MAXT>;
   constexpr int kSmemLimit = 232448;
   const int cols = static_cast<int>(p.cols);
   const int cols4 = (cols + 3) & ~3;
@@ -779,28 +809,28 @@ cudaError_t launch_rows_variant(const RowParams& p, int y_vec, int sm_count, cud
   return cudaLaunchKernelEx(&cfg, kern, p, sh, y_vec);
 }
 
-template <int DT, bool Q8, bool GATHER>
+template <int DT, bool Q8, bool NORM, bool GATHER>
 cudaError_t launch_rows_held(const RowParams& p, bool vec, int y_vec, int sm_count, cudaStream_t stream) {
   if (vec) {
-    if (p.cols <= 256) return launch_rows_variant<DT, Q8, GATHER, kVec, 8, true, 128>(p, y_vec, sm_count, stream);
-    if (p.cols <= 1024) return launch_rows_variant<DT, Q8, GATHER, kVec, 32, true, 128>(p, y_vec, sm_count, stream);
+    if (p.cols <= 256) return launch_rows_variant<DT, Q8, NORM, GATHER, kVec, 8, true, 128>(p, y_vec, sm_count, stream);
+    if (p.cols <= 1024) return launch_rows_variant<DT, Q8, NORM, GATHER, kVec, 32, true, 128>(p, y_vec, sm_count, stream);
     cudaError_t e = cudaErrorNotSupported;
     if (p.cols <= kRowsHeldCols && (GATHER || p.cols <= 4096))
-      e = launch_rows_variant<DT, Q8, GATHER, kVec, 16, false, 1024>(p, y_vec, sm_count, stream);
+      e = launch_rows_variant<DT, Q8, NORM, GATHER, kVec, 16, false, 1024>(p, y_vec, sm_count, stream);
     if (e != cudaErrorNotSupported) return e;
-    return launch_rows_variant<DT, Q8, GATHER, kLong, 16, false, 1024>(p, y_vec, sm_count, stream);
+    return launch_rows_variant<DT, Q8, NORM, GATHER, kLong, 16, false, 1024>(p, y_vec, sm_count, stream);
   }
-  if (p.cols <= 256) return launch_rows_variant<DT, Q8, GATHER, kAny, 8, true, 128>(p, y_vec, sm_count, stream);
-  if (p.cols <= 4096) return launch_rows_variant<DT, Q8, GATHER, kAny, 16, false, 256>(p, y_vec, sm_count, stream);
+  if (p.cols <= 256) return launch_rows_variant<DT, Q8, NORM, GATHER, kAny, 8, true, 128>(p, y_vec, sm_count, stream);
+  if (p.cols <= 4096) return launch_rows_variant<DT, Q8, NORM, GATHER, kAny, 16, false, 256>(p, y_vec, sm_count, stream);
   if (p.cols <= kRowsHeldCols)
-    return launch_rows_variant<DT, Q8, GATHER, kAny, 16, false, 1024>(p, y_vec, sm_count, stream);
+    return launch_rows_variant<DT, Q8, NORM, GATHER, kAny, 16, false, 1024>(p, y_vec, sm_count, stream);
   return cudaErrorNotSupported;
 }
 
 // The rows_kernel for these operands, or cudaErrorNotSupported where only
 // rows_any_kernel takes them: rows too long for a stage (or too long and not
 // aligned), lists longer than the row.
-template <int DT, bool Q8>
+template <int DT, bool Q8, bool NORM>
 cudaError_t launch_rows_once(const RowParams& p, int sm_count, cudaStream_t stream) {
   if (p.cols < 1 || p.cols > kRowsMaxCols || p.n > p.cols || p.pad > p.cols + 128) return cudaErrorNotSupported;
   constexpr int eb = DT == GW_DTYPE_F32 ? 4 : 2;
@@ -814,13 +844,13 @@ cudaError_t launch_rows_once(const RowParams& p, int sm_count, cudaStream_t stre
              aligned(p.s, p.lds, 16, eb) && aligned(p.g, 0, 16, eb);
   if (!gather) vec = vec && aligned(p.y, p.ldy, V * ob, ob);
   const int y_vec = aligned(p.y, p.ldy, 4, ob) ? 1 : 0;
-  return gather ? launch_rows_held<DT, Q8, true>(p, vec, y_vec, sm_count, stream)
-                : launch_rows_held<DT, Q8, false>(p, vec, y_vec, sm_count, stream);
+  return gather ? launch_rows_held<DT, Q8, NORM, true>(p, vec, y_vec, sm_count, stream)
+                : launch_rows_held<DT, Q8, NORM, false>(p, vec, y_vec, sm_count, stream);
 }
 
 template <int DT, bool Q8, bool NORM>
 cudaError_t launch_rows_dt1(const RowParams& p, int sm_count, cudaStream_t stream) {
-  const cudaError_t e = launch_rows_once<DT, Q8>(p, sm_count, stream);
+  const cudaError_t e = launch_rows_once<DT, Q8, NORM>(p, sm_count, stream);
   if (e != cudaErrorNotSupported) return e;
   const int64_t width = std::max<int64_t>(p.cols, p.pad);
   const int threads = width <= 1024 ? 128 : width <= 8192 ? 256 : 1024;
@@ -840,10 +870,9 @@ cudaError_t launch_rows_dt(const RowParams& p, int dtype, int sm_count, cudaStre
 
 }  // namespace
 
-cudaError_t launch_rows(RowParams p, int dtype, bool q8, bool norm, int sm_count,
+cudaError_t launch_rows(const RowParams& p, int dtype, bool q8, bool norm, int sm_count,
                         cudaStream_t stream) {
   if (p.rows == 0) return cudaSuccess;
-  p.norm = norm ? 1 : 0;
   if (q8) return norm ? launch_rows_dt<true, true>(p, dtype, sm_count, stream)
                       : launch_rows_dt<true, false>(p, dtype, sm_count, stream);
   return launch_rows_dt<false, true>(p, dtype, sm_count, stream);
