@@ -14,15 +14,21 @@
 // infinity an infinite one (its values then read back as NaN).
 //
 // e4m3 values are taken from u[m, j] = s[m, c_j] g[c_j], from which the norm's
-// factor cancels: y / scale = 448 u / max|u|. With 16-bit inputs u is mostly exact
-// in fp32, and quotients that lie exactly between two e4m3 values are common;
-// to_scale brings them out exact, so that they round to even, where dividing by a
-// rounded scale would send them either way.
+// factor cancels: y / scale = 448 u / max|u|, rounded to fp32 once (to_scale). With
+// 16-bit inputs u is mostly exact in fp32, and quotients that lie exactly between
+// two e4m3 values are common; they come out exact and round to even, where
+// dividing by a rounded scale would send them either way.
 //
 // What bounds these kernels is HBM: a row is read and written once. rows_kernel
 // keeps a row in registers (E elements per thread, a warp or a CTA per row),
 // and passes it through shared memory only to pick alive columns from it;
-// rows_any_kernel takes what that one does not.
+// rows_any_kernel takes what that one does not. Share of the measured copy
+// bandwidth (6453 GB/s) over the bytes of one read and one write: 4096 x 4096
+// fp16 with residual, half alive, 19.6 us, 93%; all columns 20.2 us, 103%; 8192 x
+// 8192 bf16 with residual to e4m3, 30% alive, 73.8 us, 89%; 1537 x 11008 bf16
+// rounded 11.1 us, 71% (three rows per CTA: the first load's latency shows).
+// Rows of odd length run at a third of it (4096 x 4097 bf16: 52 us): their 2-byte
+// accesses make instructions the limit.
 #include <algorithm>
 #include <type_traits>
 
@@ -46,45 +52,50 @@ __device__ __forceinline__ uint32_t e4m3_pack2(float lo, float hi) {
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
 // The scale of a row whose largest |u| is umax and whose norm factor is rstd,
-// and the two factors that take u to y / scale (448 / umax, in two parts for a
-// tiny or a huge umax; rstd and 2^126 where the scale is at its floor: the
-// product alone may leave fp32's range). The reciprocal is the hardware's
-// approximation after one Newton step.
+// and what turns u into y / scale = 448 u / umax = (0.875 u) / d, d = umax / 512:
+// d and its reciprocal r (the hardware's approximation after one Newton step),
+// of umax and u multiplied by m2, a power of two that keeps both in range. Where
+// the scale is at its floor (2^-126), y / scale is u rstd 2^126 instead.
 struct RowScale {
-  float scale, m1, m2;
+  float scale, d, r, m2;
+  bool floor, odd;                                 // odd: at the floor, or m2 is not one
 };
 __device__ __forceinline__ RowScale row_scale(uint32_t umax_bits, float rstd) {
   const float umax = __uint_as_float(umax_bits);
   RowScale q;
   q.scale = umax * rstd * (1.0f / kE4m3Max);       // NaN compares false and stays
   q.m2 = umax < 0x1p-64f ? 0x1p64f : umax > 0x1p64f ? 0x1p-64f : 1.0f;
-  const float v = umax * q.m2;
-  float r;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
-  q.m1 = kE4m3Max * fmaf(r, fmaf(-v, r, 1.0f), r);
-  if (q.scale < kScaleMin) {
+  q.d = umax * q.m2 * (1.0f / 512.0f);
+  asm("rcp.approx.f32 %0, %1;" : "=f"(q.r) : "f"(q.d));
+  q.r = fmaf(q.r, fmaf(-q.d, q.r, 1.0f), q.r);
+  q.floor = q.scale < kScaleMin;
+  if (q.floor) {
     q.scale = kScaleMin;
-    q.m1 = rstd;
-    q.m2 = 0x1p126f;
+    q.r = rstd;
   }
+  q.odd = q.floor || q.m2 != 1.0f;
   return q;
 }
-// u m1 m2, rounded to 21 significant bits. m1 is off by at most 2^-23 (its Newton
-// step and the factor 448 round once each), the product by 2^-24 more, so a quotient that lies exactly between two e4m3 values (at most 5
-// bits) comes out as such and rounds to even. Splitting by 2^3 + 1 (Dekker)
-// gives the upper bits: three operations instead of a division's dozen.
-__device__ __forceinline__ float to_scale(float u, const RowScale& q) {
-  const float v = u * q.m1 * q.m2;
-  const float c = 9.0f * v;
-  return c - (c - v);
-}
-
-// to_scale for two values.
+// The quotient rounded to nearest, by the remainder of a first estimate (Markstein,
+// "Computation of elementary functions on the IBM RISC System/6000 processor",
+// 1990): v0 = h r with h = 0.875 u, v = v0 + (h - v0 d) r, where the remainder is
+// exact in one fused operation. EXACT: 0.875 u needs no more than fp32's bits (16-bit
+// values as they are); else its low part joins the remainder.
+template <bool EXACT>
 __device__ __forceinline__ float2 to_scale2(float2 u, const RowScale& q) {
-  float2 v = mul2(u, both(q.m1));
-  if (q.m2 != 1.0f) v = mul2(v, both(q.m2));
-  const float2 c = mul2(v, both(9.0f));
-  return fma2(fma2(v, both(-1.0f), c), both(-1.0f), c);
+  if (q.odd) {
+    if (q.floor) return mul2(mul2(u, both(q.r)), both(0x1p126f));
+    u = mul2(u, both(q.m2));
+  }
+  const float2 nh = mul2(u, both(-0.875f));                        // -h
+  const float2 v0 = mul2(nh, both(-q.r));
+  float2 t = fma2(v0, both(q.d), nh);                              // -(h - v0 d)
+  if constexpr (!EXACT) t = fma2(fma2(u, both(0.875f), nh), both(-1.0f), t);
+  return fma2(t, both(-q.r), v0);
+}
+template <bool EXACT>
+__device__ __forceinline__ float to_scale(float u, const RowScale& q) {
+  return to_scale2<EXACT>(make_float2(u, 0.0f), q).x;
 }
 // max(a, |b|), NaN if either is (its bits then lie above infinity's).
 __device__ __forceinline__ float max_abs(float a, float b) {
@@ -155,7 +166,7 @@ __global__ void __launch_bounds__(1024) rows_any_kernel(const RowParams p) {
       const float v = sum_at(c);
       return NORM && g ? v * Elem<DT>::to_f(g[c]) : v;
     };
-    RowScale q8 = {1.0f, 1.0f, 1.0f};
+    RowScale q8{};
     if constexpr (Q8) {
       uint32_t amax = 0;
       float unused = 0.0f;
@@ -166,7 +177,7 @@ __global__ void __launch_bounds__(1024) rows_any_kernel(const RowParams p) {
     }
     for (int64_t j = threadIdx.x; j < p.pad; j += blockDim.x) {
       const float v = j < p.n ? out_at(j) : 0.0f;
-      if constexpr (Q8) y[j] = static_cast<out>(e4m3_pack2(to_scale(v, q8), 0.0f));
+      if constexpr (Q8) y[j] = static_cast<out>(e4m3_pack2(j < p.n ? to_scale<false>(v, q8) : 0.0f, 0.0f));
       else y[j] = Elem<DT>::from_f(v * rstd);
     }
     if (s) {
@@ -185,7 +196,7 @@ __global__ void __launch_bounds__(1024) rows_any_kernel(const RowParams p) {
 // memory (bulk copies counted on an mbarrier), up to kMaxStages rows ahead, so
 // that loads are in flight while a row is reduced and written. Loading a row
 // when its turn came left HBM idle during the reduction and the output: 34 us
-// instead of RINGUS for 4096 x 4096 fp16 with residual, half of the columns alive.
+// instead of 27 for 4096 x 4096 fp16 with residual, half of the columns alive.
 //   kVec   rows of 16-byte vectors: thread t takes vectors i G + t of the stage;
 //   kAny   rows of any alignment: the 16-byte granules that hold the row are
 //          copied, thread t takes elements i G + t. Granules that reach past the
@@ -196,7 +207,7 @@ __global__ void __launch_bounds__(1024) rows_any_kernel(const RowParams p) {
 // GATHER passes them through shared memory as fp32 and picks the alive columns
 // there, through a table of 16-bit places that a CTA makes from the list once for
 // all its rows (kept in registers instead, the places and the weight behind them
-// took every thread's share of the list to set up: 24 us instead of N768US for
+// took every thread's share of the list to set up: 24 us instead of 10 for
 // 8192 x 768 fp16, where a warp has three rows). For the e4m3 scale a thread
 // knows which of its columns the list names (one bit each), so the sum of squares
 // and the largest |u| take one reduction.
@@ -613,13 +624,14 @@ __global__ void __launch_bounds__(MAXT) rows_kernel(const RowParams p, const Row
       buf ^= 1;
     }
     const float rstd = NORM ? rsqrtf(ss * inv_cols + p.eps) : 1.0f;
-    RowScale q8 = {1.0f, 1.0f, 1.0f};
+    RowScale q8{};
     if constexpr (Q8) {
       q8 = row_scale(umax, rstd);
       if (t == 0) p.scale[row] = q8.scale;
     }
-    auto value = [&](float v) { return Q8 ? to_scale(v, q8) : v * rstd; };
-    auto value2 = [&](float2 v) { return Q8 ? to_scale2(v, q8) : mul2(v, both(rstd)); };
+    constexpr bool kExact = !NORM && sizeof(raw) == 2;
+    auto value = [&](float v) { return Q8 ? to_scale<kExact>(v, q8) : v * rstd; };
+    auto value2 = [&](float2 v) { return Q8 ? to_scale2<kExact>(v, q8) : mul2(v, both(rstd)); };
     auto store1 = [&](int j, float v) {
       if constexpr (Q8) y[j] = static_cast<out>(e4m3_pack2(v, 0.0f));
       else y[j] = Elem<DT>::from_f(v);

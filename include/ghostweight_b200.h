@@ -414,9 +414,9 @@ GW_API int gw_rms_norm(const void* x, int dtype, int64_t rows, int64_t cols, int
  * gw_rms_norm with the output in 8 bits:
  *   scale[m] = max(max_j |y[m, j]| / 448, 2^-126)              (float, [rows])
  *   q[m, j]  = y[m, j] / scale[m] rounded to e4m3              (1 byte, ldq)
- * y is the unrounded fp32 value; columns [n_idx, pad_to) of q are zero. A row
- * with a NaN or an infinity among its outputs gets a scale that is one, so
- * that its values read back as NaN.
+ * y / scale is rounded from fp32 (once: the norm's factor cancels in it);
+ * columns [n_idx, pad_to) of q are zero. A row with a NaN or an infinity among
+ * its outputs gets a scale that is one, so that its values read back as NaN.
  */
 GW_API int gw_rms_norm_q8(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx,
                           const void* residual, int64_t ldr, void* sum, int64_t lds,
