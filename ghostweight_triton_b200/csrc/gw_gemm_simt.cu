@@ -16,6 +16,8 @@
 // and eight neighbouring rows cover all 32 banks.
 // Tiles of 64 x 64 outputs where they make four CTAs per SM, 32 x 64 below (their
 // finer grain evens out the SMs' shares), 16 x 32 for at most 16 rows.
+#include <algorithm>
+
 #include "gw_common.cuh"
 #include "gw_internal.h"
 
@@ -57,6 +59,8 @@ struct SimtParams {
   int w_vec;                 // W' rows may be read as 16-byte vectors
 };
 
+constexpr int64_t kGridRows = 32768;               // row tiles in grid.y
+
 template <int BM, int BN, int BK, int TM, int TN, int S>
 struct SimtCfg {
   static constexpr int kThreads = (BM / TM) * (BN / TN);
@@ -79,8 +83,11 @@ gemm_f32_kernel(const SimtParams p) {
   int64_t n_alive = p.n_alive;
   if (p.n_dev) n_alive = min(n_alive, static_cast<int64_t>(max(*p.n_dev, 0)));
   const int tid = threadIdx.x;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * BM;
+  // Row tiles in two grid dimensions: one ends at 65535. (All tiles in grid.x costs
+  // a division per CTA: 28.3 us instead of 25.9 for 1024 x 768 x 384.)
+  const int64_t m0 = (static_cast<int64_t>(blockIdx.z) * kGridRows + blockIdx.y) * BM;
   const int64_t n0 = static_cast<int64_t>(blockIdx.x) * BN;
+  if (m0 >= p.M) return;                           // the last of grid.z, a whole CTA
   // A warp is 4 x 8 threads, eight neighbouring lanes 2 x 4 of them: a vector load
   // takes four rows of W' (two of x) for each eight lanes. 3 to 5% faster than
   // eight lanes along a row.
@@ -245,11 +252,14 @@ cudaError_t launch_simt(const SimtParams& p, cudaStream_t stream) {
   using C = SimtCfg<BM, BN, BK, TM, TN, S>;
   const int64_t gx = (p.N + BN - 1) / BN;
   const int64_t gy = (p.M + BM - 1) / BM;
-  if (gx > 0x7FFFFFFFll || gy > 65535) return cudaErrorInvalidValue;
+  const int64_t gz = (gy + kGridRows - 1) / kGridRows;
+  if (gx > 0x7FFFFFFFll || gz > 65535) return cudaErrorInvalidValue;
+  const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(std::min(gy, kGridRows)),
+                  static_cast<unsigned>(gz));
   auto kern = gemm_f32_kernel<BM, BN, BK, TM, TN, S>;
   cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kern), C::kSmemBytes);
   if (e != cudaSuccess) return e;
-  kern<<<dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy)), C::kThreads, C::kSmemBytes, stream>>>(p);
+  kern<<<grid, C::kThreads, C::kSmemBytes, stream>>>(p);
   return cudaGetLastError();
 }
 

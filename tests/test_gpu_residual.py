@@ -293,3 +293,15 @@ def test_refusals():
     with torch.no_grad():
         ghost_linear(x, wp, idx, residual=r.clone().requires_grad_())
     assert ghost_linear(x, wp, idx, residual=r[:1].expand(8, 48)).shape == (8, 48)
+
+
+def test_fp32_more_row_tiles_than_a_grid_dimension():
+    """65536 tiles of 64 rows and a part of one: past the second grid dimension's limit."""
+    M, K = 65536 * 64 + 5, 4
+    g = gen(3)
+    x, r = randn(g, M, K, dtype=torch.float32), randn(g, M, 1, dtype=torch.float32)
+    w = randn(g, 1, K, dtype=torch.float32)
+    idx = torch.tensor([0, 2, 3], device="cuda")
+    packed = pack_weight(w, idx)
+    y = ghost_linear(x, packed, idx, residual=r)
+    check(y, x[:, idx], w[:, idx], None, None, r)
