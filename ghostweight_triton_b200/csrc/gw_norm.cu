@@ -26,7 +26,7 @@
 // bandwidth (6453 GB/s) over the bytes of one read and one write: 4096 x 4096
 // fp16 with residual, half alive, 19.6 us, 93%; all columns 20.2 us, 103%; 8192 x
 // 8192 bf16 with residual to e4m3, 30% alive, 73.8 us, 89%; 1537 x 11008 bf16
-// rounded 11.1 us, 71% (three rows per CTA: the first load's latency shows).
+// rounded 11.1 us, 71%.
 // Rows of odd length run at a third of it (4096 x 4097 bf16: 52 us): their 2-byte
 // accesses make instructions the limit.
 #include <algorithm>
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(1024) rows_any_kernel(const RowParams p) {
 // GATHER passes them through shared memory as fp32 and picks the alive columns
 // there, through a table of 16-bit places that a CTA makes from the list once for
 // all its rows (kept in registers instead, the places and the weight behind them
-// took every thread's share of the list to set up: 24 us instead of 10 for
+// took every thread's share of the list to set up: 24 us instead of 11 for
 // 8192 x 768 fp16, where a warp has three rows). For the e4m3 scale a thread
 // knows which of its columns the list names (one bit each), so the sum of squares
 // and the largest |u| take one reduction.
