@@ -174,3 +174,23 @@ def test_refusals():
     good.fc.unfreeze_mask()
     with torch.no_grad(), pytest.raises(RuntimeError, match="frozen"):
         good(x)
+
+
+@pytest.mark.parametrize("precision", ["input", "e4m3"])
+def test_two_streams_at_once(precision):
+    """Blocks of one module running on two streams together give what each gives alone."""
+    m = block(512, 1024, torch.bfloat16, 31, precision=precision)
+    for M in (1, 40, 700):
+        data = [inputs(M, 512, torch.bfloat16, seed) for seed in (1, 2)]
+        with torch.no_grad():
+            want = [m(x, r) for x, r in data]
+            torch.cuda.synchronize()
+            streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+            got = [[], []]
+            for _ in range(20):
+                for i, stream in enumerate(streams):
+                    with torch.cuda.stream(stream):
+                        got[i].append(m(*data[i]))
+            torch.cuda.synchronize()
+        for i in range(2):
+            assert all(torch.equal(y, want[i]) for y in got[i])

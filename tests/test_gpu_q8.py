@@ -231,3 +231,18 @@ def test_refusals():
     assert call(lda=72) == _native.GW_ERR_ALIGN and call(ldw=72) == _native.GW_ERR_ALIGN
     assert call(a=a.data_ptr() + 4) == _native.GW_ERR_ALIGN and call(a=None) == _native.GW_ERR_NULL
     assert call(K=-1) == _native.GW_ERR_SHAPE
+
+
+@pytest.mark.parametrize("N", [32768, 32771])
+def test_outputs_past_32_bits(N):
+    """More than 2^31 outputs, and a residual of as many (N odd: rows of 2-byte alignment)."""
+    M, K = 65600, 64
+    g = gen(N)
+    (a, sa), (w, sw) = operand(g, M, K), operand(g, N, K)
+    sa, sw = sa / sa.mean(), sw / sw.mean() / (60 * 60 * math.sqrt(K) * 8)
+    acc = torch.randn(M, N, generator=g, device="cuda", dtype=torch.bfloat16)
+    rows = torch.tensor([0, 1, 40000, M - 200, M - 2, M - 1], device="cuda")
+    r = acc[rows]
+    packed_linear_q8(a, sa, w, sw, residual=acc, out=acc)
+    check(acc[rows], a[rows], sa[rows], w, sw, None, None, r)
+    assert _native.device_error() == 0
