@@ -37,6 +37,7 @@
 // (gw_common.cuh). No TMA multicast.
 #include <cstdlib>
 #include <mutex>
+#include <type_traits>
 
 #include <cuda.h>
 
@@ -83,10 +84,6 @@ struct DcParams {
   uint16_t* y;
   int64_t ldy;
   int y_vec_ok;              // 8-byte stores of four outputs allowed
-  const uint16_t* res;       // residual (or null), leading dimension ldr
-  int64_t ldr;
-  const float* a_scale;      // Q8: scales of a's rows and of W's rows
-  const float* w_scale;
   int num_kb;
   int split;                 // cluster size S
   int x_tx_bytes;            // bytes of one box of a (its rows: M rounded up to 8)
@@ -101,6 +98,17 @@ struct DcParams {
   const int64_t* gidx;
   int64_t n_alive;
 };
+
+// What the kernels with a residual or with e4m3 operands take besides: 32 bytes
+// of parameters (in the plain kernel too they cost 0.08 us of 4.2, 1 x 768 x 384, and
+// twice that in front of the fields that the start of the kernel reads).
+struct DcParamsExt : DcParams {
+  const uint16_t* res;       // residual (or null), leading dimension ldr
+  int64_t ldr;
+  const float* a_scale;      // Q8: scales of a's rows and of W's rows
+  const float* w_scale;
+};
+template <bool Q8, bool RES> using DcArgs = std::conditional_t<Q8 || RES, DcParamsExt, DcParams>;
 
 // Gather mode: one warp fills the a tile (MP rows x 64 columns, 128-byte
 // swizzled rows) of k-block kb. Lane l takes the alive columns 64 kb + 2 l and
@@ -150,8 +158,8 @@ __device__ __forceinline__ void dc_gather_tile(const DcParams& p, uint32_t xs, i
 // Once every slot of its receive buffer has landed it sums the S slots in rank
 // order and writes the slice out. One task = one row m x four features; rows
 // vary fastest across threads (conflict-free reads of the receive rows).
-template <int MP, int DT, bool Q8>
-__device__ __forceinline__ void dc_finish(const DcParams& p, const float* recv, int rank,
+template <int MP, int DT, bool Q8, bool RES>
+__device__ __forceinline__ void dc_finish(const DcArgs<Q8, RES>& p, const float* recv, int rank,
                                           int n_blk, int rows) {
   constexpr int kStride = DcCfg<MP>::kRecvStride;
   const int S = p.split;
@@ -183,8 +191,9 @@ __device__ __forceinline__ void dc_finish(const DcParams& p, const float* recv, 
 #pragma unroll
       for (int j = 0; j < 4; ++j) f[j] = apply_epilogue16(f[j], p.epi);
     }
-    if (p.res)
-      add_residual4<DT>(f, load_residual4(p.res + static_cast<int64_t>(m) * p.ldr, n0, p.N));
+    if constexpr (RES) {
+      if (p.res) add_residual4<DT>(f, load_residual4(p.res + static_cast<int64_t>(m) * p.ldr, n0, p.N));
+    }
     uint16_t* yp = p.y + static_cast<int64_t>(m) * p.ldy + n0;
     if (p.y_vec_ok && n0 + 4 <= p.N) {
       *reinterpret_cast<uint2*>(yp) = make_uint2(Elem<DT>::pack2(f[0], f[1]), Elem<DT>::pack2(f[2], f[3]));
@@ -227,10 +236,11 @@ __device__ __forceinline__ void dc_issue(const DcParams& p, uint32_t sbase, uint
 }
 
 // Q8: a and W' in e4m3 with scales (never gathered here), else 16-bit of type DT.
-template <int MP, int DT, bool Q8>
+// RES: a residual may be given.
+template <int MP, int DT, bool Q8, bool RES>
 __global__ void __launch_bounds__(kDcThreads, 2)
 gemm_decode_kernel(const __grid_constant__ CUtensorMap tmap_w,
-                   const __grid_constant__ CUtensorMap tmap_a, const DcParams p) {
+                   const __grid_constant__ CUtensorMap tmap_a, const DcArgs<Q8, RES> p) {
   using C = DcCfg<MP>;
   constexpr int kCols = atom_cols<Q8>();              // columns of one k-block
   extern __shared__ uint8_t smem_raw[];
@@ -430,20 +440,20 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap tmap_w,
   }
 
   // The residual and the scales of a may come from the previous kernel of the stream.
-  if (Q8 || p.res) asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (Q8 || RES) asm volatile("griddepcontrol.wait;" ::: "memory");
   // Every slot of this CTA's slice has landed: its own and the S - 1 peers'.
   const bool got = mbar_wait_cluster(recv_bar, 0u, nullptr, p.err);
   // Tell every sender that its copy into this CTA has landed.
   if (threadIdx.x < S) mbar_arrive_cluster(mapa_shared(sent_bar, threadIdx.x));
-  if (got) dc_finish<MP, DT, Q8>(p, recv, rank, n_blk, rows);
+  if (got) dc_finish<MP, DT, Q8, RES>(p, recv, rank, n_blk, rows);
   // This CTA's ring is the source of its copies: it stays valid, and the CTA
   // alive, until every owner has received its slice.
   mbar_wait_cluster(sent_bar, 0u, nullptr, p.err);
 }
 
-template <int MP, int DT, bool Q8>
+template <int MP, int DT, bool Q8, bool RES>
 cudaError_t set_decode_attrs() {
-  auto kern = gemm_decode_kernel<MP, DT, Q8>;
+  auto kern = gemm_decode_kernel<MP, DT, Q8, RES>;
   cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kern), DcCfg<MP>::kSmemBytes);
   if (e != cudaSuccess) return e;
   // Clusters of 16 CTAs are a non-portable size; the occupancy query in
@@ -460,11 +470,11 @@ cudaError_t set_decode_attrs() {
   return cudaSuccess;
 }
 
-template <int MP, int DT, bool Q8>
-cudaError_t launch_dc(const CUtensorMap& tw, const CUtensorMap& ta, const DcParams& p,
+template <int MP, int DT, bool Q8, bool RES>
+cudaError_t launch_dc(const CUtensorMap& tw, const CUtensorMap& ta, const DcParamsExt& p,
                       int64_t blocks, cudaStream_t stream) {
-  auto kern = gemm_decode_kernel<MP, DT, Q8>;
-  cudaError_t e = set_decode_attrs<MP, DT, Q8>();
+  auto kern = gemm_decode_kernel<MP, DT, Q8, RES>;
+  cudaError_t e = set_decode_attrs<MP, DT, Q8, RES>();
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(p.split), static_cast<unsigned>(blocks));
@@ -480,7 +490,7 @@ cudaError_t launch_dc(const CUtensorMap& tw, const CUtensorMap& ta, const DcPara
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, kern, tw, ta, p);
+  return cudaLaunchKernelEx(&cfg, kern, tw, ta, static_cast<const DcArgs<Q8, RES>&>(p));
 }
 
 // Clusters of S CTAs of the MP-wide kernel that fit on the device at once, for
@@ -491,8 +501,8 @@ struct DecodeTable {
 
 template <int MP>
 int query_decode_clusters(int s) {
-  auto kern = gemm_decode_kernel<MP, GW_DTYPE_F16, false>;
-  if (set_decode_attrs<MP, GW_DTYPE_F16, false>() != cudaSuccess) {
+  auto kern = gemm_decode_kernel<MP, GW_DTYPE_F16, false, false>;
+  if (set_decode_attrs<MP, GW_DTYPE_F16, false, false>() != cudaSuccess) {
     (void)cudaGetLastError();
     return 0;
   }
@@ -576,7 +586,7 @@ DecodePlan plan_decode(int64_t M, int64_t N, int64_t K, int sm_count) {
 }
 
 namespace {
-cudaError_t launch_decode_params(const DecodePlan& plan, DcParams& p, int dtype, const void* a,
+cudaError_t launch_decode_params(const DecodePlan& plan, DcParamsExt& p, int dtype, const void* a,
                                  int64_t lda, const void* w, int64_t ldw, int64_t K,
                                  cudaStream_t stream) {
   // The box of a covers only the rows that exist (rounded up to 8); the MMA
@@ -595,21 +605,23 @@ cudaError_t launch_decode_params(const DecodePlan& plan, DcParams& p, int dtype,
     return cudaErrorInvalidValue;
   }
   const bool bf = dtype == GW_DTYPE_BF16;
-#define GW_DC(MPV, Q)                                                              \
-  (bf ? launch_dc<MPV, GW_DTYPE_BF16, Q>(tw, ta, p, plan.blocks, stream)            \
-      : launch_dc<MPV, GW_DTYPE_F16, Q>(tw, ta, p, plan.blocks, stream))
+#define GW_DC1(MPV, Q, R)                                                           \
+  (bf ? launch_dc<MPV, GW_DTYPE_BF16, Q, R>(tw, ta, p, plan.blocks, stream)          \
+      : launch_dc<MPV, GW_DTYPE_F16, Q, R>(tw, ta, p, plan.blocks, stream))
+#define GW_DC(MPV) (q8 ? GW_DC1(MPV, true, true) : p.res ? GW_DC1(MPV, false, true) : GW_DC1(MPV, false, false))
   switch (plan.mp) {
-    case 16: return q8 ? GW_DC(16, true) : GW_DC(16, false);
-    case 32: return q8 ? GW_DC(32, true) : GW_DC(32, false);
+    case 16: return GW_DC(16);
+    case 32: return GW_DC(32);
     default: return cudaErrorInvalidValue;
   }
 #undef GW_DC
+#undef GW_DC1
 }
 
-DcParams decode_params(const DecodePlan& plan, int64_t M, int64_t K, int64_t N, const void* bias,
+DcParamsExt decode_params(const DecodePlan& plan, int64_t M, int64_t K, int64_t N, const void* bias,
                        int epilogue, void* y, int64_t ldy, unsigned int* err,
                        const QScale& qs = {}) {
-  DcParams p{};
+  DcParamsExt p{};
   p.M = M;
   p.N = N;
   p.bias = static_cast<const uint16_t*>(bias);
@@ -635,7 +647,7 @@ cudaError_t launch_gemm_decode_gather(const DecodePlan& plan, const void* x, int
   if (plan.split < 2 || plan.split > 16 || plan.blocks <= 0 || plan.blocks > 65535 ||
       M <= 0 || M > plan.mp || n_alive <= 0)
     return cudaErrorInvalidValue;
-  DcParams p = decode_params(plan, M, n_alive, N, bias, epilogue, y, ldy, err);
+  DcParamsExt p = decode_params(plan, M, n_alive, N, bias, epilogue, y, ldy, err);
   if (p.num_kb < plan.split) return cudaErrorInvalidValue;
   p.gx = static_cast<const uint16_t*>(x);
   p.ldx = ldx;
@@ -656,7 +668,7 @@ cudaError_t launch_gemm_decode(const DecodePlan& plan, const void* a, int dtype,
       M <= 0 || M > plan.mp)
     return cudaErrorInvalidValue;
   if (qs.a && (!qs.w || a_cols)) return cudaErrorInvalidValue;
-  DcParams p = decode_params(plan, M, K, N, bias, epilogue, y, ldy, err, qs);
+  DcParamsExt p = decode_params(plan, M, K, N, bias, epilogue, y, ldy, err, qs);
   if (p.num_kb < plan.split) return cudaErrorInvalidValue;
   if (a_cols && (K % kDcK) != 0) return cudaErrorInvalidValue;
   p.a_cols = a_cols;

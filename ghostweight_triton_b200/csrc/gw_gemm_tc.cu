@@ -61,7 +61,7 @@ constexpr int kASmemGather = 1; // producer warps gather into shared memory
 
 constexpr int pow2_at_least(int v) { int p = 32; while (p < v) p <<= 1; return p; }
 
-template <int BN>
+template <int BN, bool STAGED>
 struct TcCfg {
   static constexpr int kABytes = kBM * kBK * 2;
   static constexpr int kBBytes = BN * kBK * 2;
@@ -71,7 +71,7 @@ struct TcCfg {
   static constexpr int kStages = kStagesFit > kMaxStages ? kMaxStages : kStagesFit;
   static constexpr int kTmemCols = pow2_at_least(2 * BN);   // two accumulator buffers
   static constexpr int kBarBytes = 256;
-  static constexpr int kEpiBytes = 8 * WarpTile<32>::kBytes;     // an epilogue tile per warp
+  static constexpr int kEpiBytes = STAGED ? 8 * WarpTile<32>::kBytes : 0;     // an epilogue tile per warp
   static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kEpiBytes + kBarBytes;
   static_assert(kSmemBytes <= 232448, "shared memory budget per CTA");
 };
@@ -105,13 +105,14 @@ struct TcParams {
 
 // Q8: A and W in e4m3 with scales (kATma only), else 16-bit of type DT. STAGED:
 // with a residual or with rows of y that are not 16-byte aligned, which pass
-// through a tile in shared memory (an instantiation of its own: 1024 x 4096 x
-// 1024 without either takes 9.0 us, 10.5 with the tile's code beside it).
+// through a tile in shared memory (an instantiation of its own, and only that one
+// reserves the tile: 1024 x 4096 x 1024 without either takes 9.0 us, 10.5 with the
+// tile's code beside it; 2048 x 768 x 384 8.7 us, 9.05 with its 16 KB reserved).
 template <int BN, int DT, int AMODE, int EPI, bool Q8, bool STAGED>
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_tc_kernel(const __grid_constant__ CUtensorMap tmap_b,
                const __grid_constant__ CUtensorMap tmap_a, const TcParams p) {
-  using C = TcCfg<BN>;
+  using C = TcCfg<BN, STAGED>;
   constexpr int kCols = atom_cols<Q8>();              // columns of one k-block
   static_assert(!Q8 || AMODE == kATma, "e4m3 operands arrive by TMA");
   extern __shared__ uint8_t smem_raw[];
@@ -407,7 +408,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmap_b,
 template <int BN, int DT, int AMODE, bool Q8, bool STAGED>
 cudaError_t launch_tc(const CUtensorMap& tb, const CUtensorMap& ta, const TcParams& p,
                       int sm_count, cudaStream_t stream) {
-  using C = TcCfg<BN>;
+  using C = TcCfg<BN, STAGED>;
   auto kern = p.epi == GW_EPI_GELU_ERF    ? gemm_tc_kernel<BN, DT, AMODE, GW_EPI_GELU_ERF, Q8, STAGED>
               : p.epi == GW_EPI_GELU_TANH ? gemm_tc_kernel<BN, DT, AMODE, GW_EPI_GELU_TANH, Q8, STAGED>
                                           : gemm_tc_kernel<BN, DT, AMODE, GW_EPI_NONE, Q8, STAGED>;
