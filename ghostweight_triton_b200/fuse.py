@@ -160,9 +160,10 @@ class GhostPreNormMLP(GhostMLPChain):
         super().refresh_packed()
         self._plan_q8 = None
 
-    def _eps(self, dtype: torch.dtype) -> float:
+    def _eps(self) -> float:
         eps = getattr(self.norm, "eps", getattr(self.norm, "variance_epsilon", None))
-        return torch.finfo(dtype).eps if eps is None else float(eps)       # None: torch.nn.RMSNorm's default
+        # None: torch.nn.RMSNorm's default, the epsilon of the type it norms 16-bit rows in.
+        return torch.finfo(torch.float32).eps if eps is None else float(eps)
 
     def _operands_q8(self, dtype: torch.dtype):
         w_fc, b_fc, w_proj = self._operands(dtype)
@@ -179,7 +180,7 @@ class GhostPreNormMLP(GhostMLPChain):
         features = self.fc.in_features
         x2 = x.reshape(-1, features)
         r2 = None if residual is None else residual.reshape(-1, features)
-        norm = dict(weight=getattr(self.norm, "weight", None), eps=self._eps(x.dtype), residual=r2,
+        norm = dict(weight=getattr(self.norm, "weight", None), eps=self._eps(), residual=r2,
                     alive_indices=self.fc._frozen_indices)
         bias = self.proj.bias
         if bias is not None and bias.dtype != x.dtype:
