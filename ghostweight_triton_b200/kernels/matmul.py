@@ -244,16 +244,21 @@ def ghost_linear(
 
 
 def _product_out(out, residual, M, N, like):
-    """(output [M, N], residual as a row-major matrix or None) of a product. The output is
+    """(output [M, N], residual as a row-major matrix or None) of a product of `like`'s type
+    and device. A given output has that shape, in row-major rows of their own. The output is
     computed through the residual's rows, so it is these rows or lies apart from them."""
+    given = residual
     if residual is not None:
-        given = residual
         residual = residual_matrix(residual, (M, N), like)
-        if out is not None:
-            in_place_or_apart("out", out, residual)
-            assert residual is given or out is not given, "a residual updated in place must have rows of adjacent elements"
     if out is None:
-        out = torch.empty((M, N), dtype=like.dtype, device=like.device)
+        return torch.empty((M, N), dtype=like.dtype, device=like.device), residual
+    assert out.shape == (M, N) and out.dtype is like.dtype and out.device == like.device, (
+        f"out must be {like.dtype} of shape {(M, N)} on {like.device}, got {out.dtype} {tuple(out.shape)} on {out.device}")
+    assert (out.stride(1) == 1 or N <= 1) and (out.stride(0) >= N or M <= 1), (
+        f"out must be a row-major matrix, got strides {out.stride()}")
+    if residual is not None:
+        in_place_or_apart("out", out, residual)
+        assert residual is given or out is not given, "a residual updated in place must have rows of adjacent elements"
     return out, residual
 
 
@@ -369,9 +374,7 @@ def packed_linear_q8(
         if residual is not None:
             residual = residual_matrix(residual, (M, N), y)
     else:
-        assert out.shape == (M, N) and out.dtype is dtype and out.is_cuda and out.get_device() == dev, (
-            f"out must be {dtype} of shape {(M, N)} on a's device")
-        assert (out.stride(1) == 1 or N <= 1) and (out.stride(0) >= N or M <= 1), "out must be a row-major matrix"
+        assert out.dtype is dtype and out.is_cuda and out.get_device() == dev, f"out must be {dtype} on a's device"
         y, residual = _product_out(out, residual, M, N, out)
         ldy = max(y.stride(0), N)
     if M and N:
@@ -434,6 +437,7 @@ def ghost_linear_pipelined(calls) -> list:
         bias = c[4] if len(c) > 4 else None
         act = c[5] if len(c) > 5 else None
         assert x.ndim == 2 and x.is_cuda and out is not None
+        _product_out(out, None, x.shape[0], wp.shape[0], x)
         norm.append((x, wp, idx, out, bias, act))
     st.gemm.wait_stream(cur)
     st.gather.wait_stream(cur)

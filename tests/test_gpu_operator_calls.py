@@ -8,6 +8,10 @@ import pytest
 import torch
 import torch.nn as nn
 
+from ghostweight_triton_b200.kernels.gather import pack_weight
+from ghostweight_triton_b200.kernels.matmul import (ghost_linear, ghost_linear_dev, ghost_linear_pipelined, packed_linear,
+                                                    packed_linear_q8)
+from ghostweight_triton_b200.kernels.norm import quantize_rows
 from tests.test_gpu_prenorm import block, exact, inputs
 
 pytestmark = pytest.mark.gpu
@@ -35,3 +39,32 @@ def test_block_with_the_norms_default_eps(dtype):
     d = x.double()
     want = d / torch.sqrt((d * d).mean(-1, keepdim=True) + 2.0 ** -23) * m.norm.weight.double()
     assert bool(((n - want).abs() <= 3 * torch.finfo(dtype).eps / 2 * want.abs() + 1e-6).all())
+
+
+def operands(M, N, K, dtype=torch.float16):
+    g = torch.Generator(device="cuda").manual_seed(M + N + K)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda").to(dtype)
+    idx = torch.arange(K, device="cuda")
+    return rnd(M, K), pack_weight(rnd(N, K), idx), idx
+
+
+def test_outputs_refused():
+    """Every product's `out`, with and without a residual, before anything is launched."""
+    M, N, K = 8, 48, 64
+    x, w, idx = operands(M, N, K)
+    count = torch.tensor([K], dtype=torch.int32, device="cuda")
+    qa, sa = quantize_rows(x)
+    qw, sw = quantize_rows(w)
+    res = torch.zeros(M, N, dtype=x.dtype, device="cuda")
+    calls = [lambda out, r: ghost_linear(x, w, idx, out=out, residual=r),
+             lambda out, r: ghost_linear_dev(x, w, idx, count, out=out, residual=r),
+             lambda out, r: packed_linear(x, w, out=out, residual=r),
+             lambda out, r: packed_linear_q8(qa, sa, qw, sw, dtype=x.dtype, out=out, residual=r),
+             lambda out, r: ghost_linear_pipelined([(x, w, idx, out)])]
+    for out in (torch.empty(M - 1, N, dtype=x.dtype, device="cuda"), torch.empty(M, N - 1, dtype=x.dtype, device="cuda"),
+                torch.empty(M, N, dtype=torch.uint8, device="cuda"), torch.empty(M, N, dtype=x.dtype),
+                torch.empty(N, M, dtype=x.dtype, device="cuda").t()):
+        for call in calls:
+            for r in (None, res):
+                with pytest.raises(AssertionError, match="out must be"):
+                    call(out, r)
