@@ -31,17 +31,32 @@ def _span(m: torch.Tensor) -> tuple[int, int]:
     return m.data_ptr(), m.data_ptr() + ((m.shape[0] - 1) * m.stride(0) + m.shape[1]) * m.element_size()
 
 
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two row-major matrices share memory. Columns side by side in one buffer do
+    not; matrices whose rows interleave at different strides are taken to."""
+    if not a.numel() or not b.numel():
+        return False
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    if a1 <= b0 or b1 <= a0:
+        return False
+    # At one stride, the rows of a take the bytes [0, wa) of every period and those of b
+    # [d, d + wb): apart if that ends behind the first and before the next period's.
+    pitches = {t.stride(0) * t.element_size() for t in (a, b) if t.shape[0] > 1}
+    if len(pitches) != 1:
+        return True
+    pitch = pitches.pop()
+    d = (b0 - a0) % pitch
+    return d < a.shape[1] * a.element_size() or d + b.shape[1] * b.element_size() > pitch
+
+
 def in_place_or_apart(what: str, out: torch.Tensor, *inputs: torch.Tensor | None) -> None:
     """Assert that the matrix `out` takes the very place of an input matrix or none of its
     memory (each element is read before it is written only if both have the same rows)."""
     for t in inputs:
-        if t is None or not t.numel() or not out.numel():
+        if t is None or (t.data_ptr() == out.data_ptr() and t.shape == out.shape
+                         and (t.shape[0] <= 1 or t.stride(0) == out.stride(0))):
             continue
-        if (t.data_ptr() == out.data_ptr() and t.shape == out.shape
-                and (t.shape[0] <= 1 or t.stride(0) == out.stride(0))):
-            continue
-        (a0, a1), (b0, b1) = _span(t), _span(out)
-        assert a1 <= b0 or b1 <= a0, f"{what} overlaps an input without being the same rows"
+        assert not overlap(out, t), f"{what} overlaps an input without being the same rows"
 
 
 def out_matrix(what: str, out: torch.Tensor, like: torch.Tensor, *inputs: torch.Tensor | None) -> torch.Tensor:

@@ -11,7 +11,7 @@ import torch.nn as nn
 from ghostweight_triton_b200.kernels.gather import pack_weight
 from ghostweight_triton_b200.kernels.matmul import (ghost_linear, ghost_linear_dev, ghost_linear_pipelined, packed_linear,
                                                     packed_linear_q8)
-from ghostweight_triton_b200.kernels.norm import quantize_rows
+from ghostweight_triton_b200.kernels.norm import quantize_rows, rms_norm
 from tests.test_gpu_prenorm import block, exact, inputs
 
 pytestmark = pytest.mark.gpu
@@ -68,3 +68,24 @@ def test_outputs_refused():
             for r in (None, res):
                 with pytest.raises(AssertionError, match="out must be"):
                     call(out, r)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 96, 64), (5, 200, 128), (300, 768, 512), (2100, 1000, 256)])
+def test_output_beside_the_residual(M, N, K):
+    """Output and residual in two column ranges of one buffer; the row operators likewise."""
+    for dtype in (torch.float16, torch.float32):
+        x, w, idx = operands(M, N, K, dtype)
+        buf = torch.randn(M, 2 * N + 3, device="cuda").to(dtype)
+        keep = buf.clone()
+        y = ghost_linear(x, w, idx, residual=buf[:, :N], out=buf[:, N + 2: 2 * N + 2])
+        assert torch.equal(y, ghost_linear(x, w, idx, residual=keep[:, :N].contiguous()))
+        keep[:, N + 2: 2 * N + 2] = y
+        assert torch.equal(buf, keep)
+        n, s = rms_norm(buf[:, :N], residual=keep[:, :N], residual_out=buf[:, N + 1: 2 * N + 1])
+        assert torch.equal(s, keep[:, :N] + keep[:, :N]) and torch.equal(buf[:, :N], keep[:, :N])
+        # Rounded once; the fp32 sum of N squares is off by at most N 2^-24 of itself (half of that in
+        # its root's inverse), the root and the two products by a few 2^-24.
+        want = 2 * keep[:, :N].double()
+        want /= torch.sqrt((want * want).mean(1, keepdim=True) + 1e-6)
+        assert bool(((n.double() - want).abs() <= (torch.finfo(dtype).eps / 2 + (N / 2 + 16) * 2.0 ** -24)
+                     * want.abs() + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2).all())

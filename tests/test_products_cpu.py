@@ -2,9 +2,12 @@
 
 from __future__ import annotations
 
+import random
+
 import pytest
 import torch
 
+from ghostweight_triton_b200.kernels import _args
 from ghostweight_triton_b200.kernels.matmul import _product_out
 
 F16 = torch.float16
@@ -39,3 +42,43 @@ def test_outputs_taken():
     assert new.shape == (4, 48) and new.dtype is F16
     column = torch.empty(4, 3, dtype=F16)[:, 1:2]
     assert _product_out(column, None, 4, 1, x)[0] is column
+
+
+def test_columns_side_by_side():
+    """Output and residual in the halves of one buffer share no element."""
+    x = torch.empty(6, 32, dtype=F16)
+    buf = torch.empty(6, 100, dtype=F16)
+    for out, residual in ((buf[:, 48:96], buf[:, :48]), (buf[:, :48], buf[:, 52:]), (buf[:, 10:58], buf[:, 58:]),
+                          (buf[:1, 48:96], buf[:1, :48])):
+        n = min(out.shape[1], residual.shape[1])
+        out, residual = out[:, :n], residual[:, :n]
+        y, r = _product_out(out, residual, len(out), n, x)
+        assert y is out and r is residual
+    for out, residual in ((buf[:, 47:95], buf[:, :48]), (buf[1:, :48], buf[:5, 2:50]), (buf[:5, 60:], buf[1:, 50:90])):
+        with pytest.raises(AssertionError, match="overlaps"):
+            _product_out(out, residual, len(out), out.shape[1], x)
+
+
+def test_overlap_against_the_elements():
+    """Random windows of one buffer: never called apart when an element is in both, and
+    called overlapping exactly then where their rows have one stride."""
+    rng = random.Random(1)
+    buf = torch.empty(400, dtype=F16)
+
+    def window():
+        rows, ld = rng.randint(1, 5), rng.randint(1, 12)
+        return buf.as_strided((rows, rng.randint(1, ld)), (ld, 1), rng.randint(0, 60))
+
+    def elements(m):
+        return {m.storage_offset() + r * m.stride(0) + c for r in range(m.shape[0]) for c in range(m.shape[1])}
+
+    one_stride = 0
+    for _ in range(20000):
+        a, b = window(), window()
+        shared = bool(elements(a) & elements(b))
+        got = _args.overlap(a, b)
+        assert got == _args.overlap(b, a) and (got or not shared)
+        if a.shape[0] > 1 and b.shape[0] > 1 and a.stride(0) == b.stride(0):
+            one_stride += 1
+            assert got == shared
+    assert one_stride > 500
