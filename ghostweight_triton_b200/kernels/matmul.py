@@ -21,7 +21,7 @@ from __future__ import annotations
 import torch
 
 from ghostweight_triton_b200 import _native
-from ghostweight_triton_b200.kernels._args import in_place_or_apart, residual_matrix
+from ghostweight_triton_b200.kernels._args import in_place_or_apart, overlap, residual_matrix
 from ghostweight_triton_b200.kernels.gather import pack_weight
 
 
@@ -225,7 +225,9 @@ def ghost_linear(
     """y = act(x[:, alive] @ w_packed^T + bias) + residual for x [M, K], w_packed [N, K_alive].
 
     residual [M, N] (x's dtype, rows may be strided) is added in the epilogue,
-    in fp32, before the one rounding; ``out`` may be the residual itself.
+    in fp32, before the one rounding; ``out`` may be the residual itself. An
+    ``out`` that shares memory with x is allowed: x is copied first, since
+    tiles of y are written while others still read x.
     """
     assert x.ndim == 2 and x.is_cuda
     if not x.is_contiguous():
@@ -238,6 +240,7 @@ def ghost_linear(
             residual = residual_matrix(residual, (M, N), x)
     else:
         y, residual = _product_out(out, residual, M, N, x)
+        x = _apart_from(y, x, w_packed)
     if M and N:
         _gemm(x, w_packed, alive_indices, y, bias, activation, strategy, residual)
     return y
@@ -262,6 +265,17 @@ def _product_out(out, residual, M, N, like):
     return out, residual
 
 
+def _apart_from(out: torch.Tensor, x: torch.Tensor, w_packed: torch.Tensor) -> torch.Tensor:
+    """x, or a copy of it (at its strides) if the output takes any of its memory: a product
+    reads its operands again for every tile, and writes tiles before it has read them all."""
+    assert not overlap(out, w_packed), "out shares memory with w_packed"
+    if not overlap(out, x):
+        return x
+    copy = x.new_empty(x.shape[0] * x.stride(0) if x.shape[0] > 1 else max(x.stride(0), x.shape[1]))
+    copy = copy.as_strided(x.shape, x.stride())
+    return copy.copy_(x)
+
+
 def ghost_linear_dev(
     x: torch.Tensor,
     w_packed: torch.Tensor,
@@ -282,6 +296,8 @@ def ghost_linear_dev(
     M = x.shape[0]
     N = w_packed.shape[0]
     y, residual = _product_out(out, residual, M, N, x)
+    if out is not None:
+        x = _apart_from(y, x, w_packed)
     if M and N:
         _native.gather_gemm_dev(x, w_packed, alive_buffer, alive_count, y, bias=bias,
                                 activation=activation, residual=residual)
@@ -307,6 +323,8 @@ def packed_linear(
                                   or a.data_ptr() % 16):
         a = a.contiguous()
     y, residual = _product_out(out, residual, a.shape[0], w_packed.shape[0], a)
+    if out is not None:
+        a = _apart_from(y, a, w_packed)
     if y.numel():
         _native.packed_gemm(a, w_packed, y, bias=bias, activation=activation, residual=residual)
     return y
@@ -376,6 +394,7 @@ def packed_linear_q8(
     else:
         assert out.dtype is dtype and out.is_cuda and out.get_device() == dev, f"out must be {dtype} on a's device"
         y, residual = _product_out(out, residual, M, N, out)
+        a = _apart_from(y, a, w_packed)
         ldy = max(y.stride(0), N)
     if M and N:
         _native.packed_gemm_q8(a, a_scale, M, K, lda, w_packed, w_scale, N, ldw, y, ldy, bias, activation, residual)

@@ -89,3 +89,39 @@ def test_output_beside_the_residual(M, N, K):
         want /= torch.sqrt((want * want).mean(1, keepdim=True) + 1e-6)
         assert bool(((n.double() - want).abs() <= (torch.finfo(dtype).eps / 2 + (N / 2 + 16) * 2.0 ** -24)
                      * want.abs() + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("M", [1, 7, 130, 700, 3000])
+def test_output_in_the_operands_place(M, dtype):
+    """x + x W'^T written over x (N = K), and over columns of it, equal the same call with an
+    output of its own: no tile of x is read after it was overwritten."""
+    K = 768
+    x, _, _ = operands(M, K, K, dtype)
+    w = (torch.randn(K, K, device="cuda") / 28).to(dtype)
+    idx = torch.randperm(K, device="cuda")[: K // 2].sort().values
+    wp = pack_weight(w, idx)
+    count = torch.tensor([idx.numel()], dtype=torch.int32, device="cuda")
+    calls = [lambda x, r, out, s=s: ghost_linear(x, wp, idx, residual=r, out=out, strategy=s)
+             for s in (("auto",) if dtype is torch.float32 else ("auto", "fused", "overlap"))]
+    calls += [lambda x, r, out: ghost_linear_dev(x, wp, idx, count, residual=r, out=out)]
+    if dtype is not torch.float32:
+        full = pack_weight(w, torch.arange(K, device="cuda"))
+        calls += [lambda x, r, out: packed_linear(x, full, residual=r, out=out),
+                  lambda x, r, out: ghost_linear(x, full, torch.arange(K, device="cuda"), residual=r, out=out, strategy="runs")]
+    for call in calls:
+        want = call(x, x, None)
+        for _ in range(5):
+            y = x.clone()
+            assert call(y, y, y) is y and torch.equal(y, want)
+            y = x.clone()
+            assert torch.equal(call(y, None, y), call(x, None, None))
+    if dtype is not torch.float32:
+        half = pack_weight(w[:, : K // 2], torch.arange(K // 2, device="cuda"))[: 3 * K // 4]
+        for _ in range(3):
+            y = x.clone()                            # both operands strided, the output across them
+            got = packed_linear(y[:, : K // 2], half, out=y[:, K // 4:])
+            assert torch.equal(got, packed_linear(x[:, : K // 2], half))
+            assert torch.equal(y[:, : K // 4], x[:, : K // 4])
+    with pytest.raises(AssertionError, match="w_packed"):
+        ghost_linear(x[:5], wp, idx, out=wp.as_strided((min(M, 5), K), (wp.stride(0) * 2, 1)))

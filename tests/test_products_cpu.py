@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from ghostweight_triton_b200.kernels import _args
-from ghostweight_triton_b200.kernels.matmul import _product_out
+from ghostweight_triton_b200.kernels.matmul import _apart_from, _product_out
 
 F16 = torch.float16
 
@@ -82,3 +82,17 @@ def test_overlap_against_the_elements():
             one_stride += 1
             assert got == shared
     assert one_stride > 500
+
+
+def test_operands_leave_the_output():
+    """An operand that shares memory with the output is copied at its strides, a weight refused."""
+    buf = torch.arange(8 * 40, dtype=F16).view(8, 40)
+    w = torch.zeros(16, 24, dtype=F16)
+    for x, out in ((buf[:, :24], buf[:, :16]), (buf[:, :24], buf[:, 20:36]), (buf[1:2, :24], buf[:, :16]), (buf[1:2], buf[:, 3:19])):
+        copy = _apart_from(out, x, w)
+        assert copy.data_ptr() != x.data_ptr() and torch.equal(copy, x) and not _args.overlap(copy, out)
+        assert copy.shape == x.shape and copy.stride() == x.stride()
+    for x, out in ((buf[:, :24], buf[:, 24:]), (buf[:4, :24], buf[4:, :16]), (buf[:0], buf), (torch.zeros(8, 24), buf)):
+        assert _apart_from(out, x, w) is x
+    with pytest.raises(AssertionError, match="w_packed"):
+        _apart_from(w[:8, :16], buf[:, :24], w)
