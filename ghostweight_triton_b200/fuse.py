@@ -50,6 +50,17 @@ def _epilogue_of(act: nn.Module) -> str | None:
     return _ACT_BY_CLASS.get(type(act).__name__)
 
 
+def _plan_key(dtype: torch.dtype, *tensors: torch.Tensor | None) -> tuple:
+    """What packed operands are made from: the tensors themselves (held, so that none of
+    them can be freed and another take its address), their versions and storage."""
+    return (dtype, *((t, t._version, t.data_ptr()) for t in tensors if t is not None))
+
+
+def _same_key(a: tuple, b: tuple) -> bool:
+    return (len(a) == len(b) and a[0] is b[0]
+            and all(u[0] is v[0] and u[1:] == v[1:] for u, v in zip(a[1:], b[1:])))
+
+
 class GhostMLPChain(nn.Module):
     """fc -> activation -> proj (-> dropout) with proj's dead inputs never computed.
 
@@ -78,10 +89,8 @@ class GhostMLPChain(nn.Module):
     def _operands(self, dtype: torch.dtype):
         fc, proj = self.fc, self.proj
         a_fc, a_proj = fc._frozen_indices, proj._frozen_indices
-        key = (dtype, fc.weight.data_ptr(), fc.weight._version, proj.weight.data_ptr(),
-               proj.weight._version, a_fc.data_ptr(), a_fc._version, a_proj.data_ptr(),
-               a_proj._version, None if fc.bias is None else (fc.bias.data_ptr(), fc.bias._version))
-        if self._plan is not None and self._plan[0] == key:
+        key = _plan_key(dtype, fc.weight, proj.weight, a_fc, a_proj, fc.bias)
+        if self._plan is not None and _same_key(self._plan[0], key):
             return self._plan[1:]
         with torch.no_grad():
             # proj's weight packed over its alive inputs, whole buffer: the fused

@@ -8,6 +8,7 @@ import pytest
 import torch
 import torch.nn as nn
 
+from ghostweight_triton_b200.fuse import GhostMLPChain
 from ghostweight_triton_b200.kernels.gather import pack_weight
 from ghostweight_triton_b200.kernels.matmul import (ghost_linear, ghost_linear_dev, ghost_linear_pipelined, packed_linear,
                                                     packed_linear_q8)
@@ -125,3 +126,52 @@ def test_output_in_the_operands_place(M, dtype):
             assert torch.equal(y[:, : K // 4], x[:, : K // 4])
     with pytest.raises(AssertionError, match="w_packed"):
         ghost_linear(x[:5], wp, idx, out=wp.as_strided((min(M, 5), K), (wp.stride(0) * 2, 1)))
+
+
+def at_address(ptr, make):
+    """A tensor that make() returns at the given address (the allocator hands freed blocks out again)."""
+    others = []
+    for _ in range(50):
+        t = make()
+        if t.data_ptr() == ptr:
+            return t
+        others.append(t)
+    return None
+
+
+@pytest.mark.parametrize("precision", ["input", "e4m3", "chain"])
+@pytest.mark.parametrize("what", ["mask", "weight", "proj mask", "bias"])
+def test_replaced_tensors_at_the_old_address(what, precision):
+    """A mask, weight or bias that replaces another one at its address and version is seen."""
+    D, F = 256, 512
+    g = torch.Generator(device="cuda").manual_seed(3)
+    m = block(D, F, torch.float16, 3, precision="input" if precision == "chain" else precision)
+    if precision == "chain":
+        m = GhostMLPChain(m.fc, m.proj, "gelu")
+    x, _ = inputs(20, D, torch.float16, 3)
+    layer = m.proj if what == "proj mask" else m.fc
+    other = {"weight": torch.randn(F, D, generator=g, device="cuda").half() / 16,
+             "bias": torch.randn(F, generator=g, device="cuda").half(),
+             }.get(what, torch.randperm(layer.in_features, generator=g, device="cuda")[: layer.in_features // 2].sort().values)
+    with torch.no_grad():
+        if what in ("weight", "bias"):
+            setattr(m.fc, what, nn.Parameter(torch.randn_like(other), requires_grad=False))
+        else:
+            layer._set_frozen(other.flip(0).clone())
+        m(x)
+        torch.cuda.synchronize()
+        old = m.fc.weight if what == "weight" else m.fc.bias if what == "bias" else layer._frozen_indices
+        ptr, version = old.data_ptr(), old._version
+        del old
+        if what in ("weight", "bias"):
+            setattr(m.fc, what, None)
+            new = at_address(ptr, other.clone)
+            setattr(m.fc, what, nn.Parameter(other.clone() if new is None else new, requires_grad=False))
+            assert new is None or getattr(m.fc, what)._version == version
+        else:
+            layer.unfreeze_mask()
+            new = at_address(ptr, other.clone)
+            layer._set_frozen(other.clone() if new is None else new)
+        y = m(x)
+        m.refresh_packed()
+        assert torch.equal(y, m(x))
