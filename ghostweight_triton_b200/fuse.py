@@ -110,7 +110,9 @@ class GhostMLPChain(nn.Module):
                 b_fc = fc.bias.detach().index_select(0, a_proj).to(dtype)
                 if pad:
                     b_fc = torch.cat([b_fc, b_fc.new_zeros(pad)])
-        self._plan = (key, w_fc, b_fc, w_proj)
+        # Under graph capture the packing is only recorded, into the graph's own memory: not kept.
+        if not torch.cuda.is_current_stream_capturing():
+            self._plan = (key, w_fc, b_fc, w_proj)
         return w_fc, b_fc, w_proj
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
@@ -176,9 +178,12 @@ class GhostPreNormMLP(GhostMLPChain):
 
     def _operands_q8(self, dtype: torch.dtype):
         w_fc, b_fc, w_proj = self._operands(dtype)
-        if self._plan_q8 is None or self._plan_q8[0] is not w_fc:
-            self._plan_q8 = (w_fc, quantize_rows(w_fc), quantize_rows(w_proj))
-        return self._plan_q8[1], b_fc, self._plan_q8[2]
+        plan = self._plan_q8
+        if plan is None or plan[0] is not w_fc:
+            plan = (w_fc, quantize_rows(w_fc), quantize_rows(w_proj))
+            if not torch.cuda.is_current_stream_capturing():
+                self._plan_q8 = plan
+        return plan[1], b_fc, plan[2]
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
         """x [..., features], and optionally a residual of its shape added in front of the norm."""

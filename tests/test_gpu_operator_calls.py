@@ -175,3 +175,39 @@ def test_replaced_tensors_at_the_old_address(what, precision):
         y = m(x)
         m.refresh_packed()
         assert torch.equal(y, m(x))
+
+
+@pytest.mark.parametrize("updated", [False, True])
+@pytest.mark.parametrize("kind", ["input", "e4m3", "chain"])
+def test_captured_first(kind, updated):
+    """A capture that has to pack the weights (the first call, or the first one after an update)
+    leaves nothing behind that an eager call before the first replay would take as packed."""
+    D, F = 512, 1024
+    m = block(D, F, torch.float16, 11, precision="e4m3" if kind == "e4m3" else "input")
+    if kind == "chain":
+        m = GhostMLPChain(m.fc, m.proj, "gelu")
+    elif kind == "layer":
+        m = m.fc
+    fresh = block(D, F, torch.float16, 11, precision="e4m3" if kind == "e4m3" else "input")
+    if kind in ("chain", "layer"):
+        fresh = GhostMLPChain(fresh.fc, fresh.proj, "gelu") if kind == "chain" else fresh.fc
+    x, _ = inputs(40, D, torch.float16, 11)
+    weight = m.weight if kind == "layer" else m.proj.weight
+    with torch.no_grad():
+        if updated:
+            m(x)
+            for mod in (weight, fresh.weight if kind == "layer" else fresh.proj.weight):
+                mod.mul_(-0.5)
+        want = fresh(x)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = m(x)
+        assert torch.equal(m(x), want)               # before any replay
+        graph.replay()
+        assert torch.equal(y, want) and torch.equal(m(x), want)
+        x2, _ = inputs(40, D, torch.float16, 12)
+        x.copy_(x2)
+        graph.replay()
+        assert torch.equal(y, fresh(x2))
+        del graph
+        assert torch.equal(m(x), fresh(x2))
