@@ -228,7 +228,9 @@ class GhostLinear(nn.Module):
                     and k[4] == alive._version and k[5] is dtype):
                 return c[1]
         packed = pack_weight(w.detach(), alive, dtype=dtype)
-        self._packed = ((w, w._version, w.data_ptr(), alive, alive._version, dtype), packed)
+        # Under graph capture the packing is only recorded, into the graph's own memory: not kept.
+        if not torch.cuda.is_current_stream_capturing():
+            self._packed = ((w, w._version, w.data_ptr(), alive, alive._version, dtype), packed)
         return packed
 
     def _alive_runs(self, alive: torch.Tensor) -> bool:

@@ -178,7 +178,7 @@ def test_replaced_tensors_at_the_old_address(what, precision):
 
 
 @pytest.mark.parametrize("updated", [False, True])
-@pytest.mark.parametrize("kind", ["input", "e4m3", "chain"])
+@pytest.mark.parametrize("kind", ["input", "e4m3", "chain", "layer"])
 def test_captured_first(kind, updated):
     """A capture that has to pack the weights (the first call, or the first one after an update)
     leaves nothing behind that an eager call before the first replay would take as packed."""
