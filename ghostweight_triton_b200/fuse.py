@@ -30,6 +30,7 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
+from ghostweight_triton_b200 import _native
 from ghostweight_triton_b200.kernels.gather import pack_weight
 from ghostweight_triton_b200.kernels._args import refuse_grad
 from ghostweight_triton_b200.kernels.matmul import ghost_linear, packed_linear, packed_linear_q8
@@ -61,13 +62,39 @@ def _same_key(a: tuple, b: tuple) -> bool:
             and all(u[0] is v[0] and u[1:] == v[1:] for u, v in zip(a[1:], b[1:])))
 
 
+class _Plan:
+    """Packed operands kept between calls, with the tensors they were made from (the key).
+
+    Built on one stream and used on any: another stream waits for the build, and the
+    allocator for that stream's work before it hands the memory out again. A capture
+    takes them as they are (it starts when the device is idle).
+    """
+
+    def __init__(self, key: tuple, operands: tuple):
+        self.key = key
+        self.operands = operands
+        self.tensors = [t for o in operands for t in (o if isinstance(o, tuple) else (o,)) if t is not None]
+        self.device = self.tensors[0].device
+        self.stream = _native._stream(self.device)
+        self.built = torch.cuda.current_stream(self.device).record_event()
+
+    def take(self) -> tuple:
+        if _native._stream(self.device) != self.stream and not _native._capturing():
+            stream = torch.cuda.current_stream(self.device)
+            stream.wait_event(self.built)
+            for t in self.tensors:
+                t.record_stream(stream)
+        return self.operands
+
+
 class GhostMLPChain(nn.Module):
     """fc -> activation -> proj (-> dropout) with proj's dead inputs never computed.
 
     ``fc`` and ``proj`` are GhostLinears with frozen masks (``proj.in_features ==
     fc.out_features``); they stay registered as submodules, so parameters and
     state-dict keys are unchanged. The packed operands are built on first use and
-    rebuilt when a weight or a mask changes.
+    rebuilt when a weight or a mask changes. A captured graph reads the operands of
+    the call that it captured: capture again after a change.
     """
 
     def __init__(self, fc: GhostLinear, proj: GhostLinear, activation: str,
@@ -78,7 +105,10 @@ class GhostMLPChain(nn.Module):
         self.proj = proj
         self.activation = activation
         self.dropout = dropout
-        self._plan: tuple | None = None
+        self._plan: _Plan | None = None
+
+    def __getstate__(self):
+        return {k: None if isinstance(v, _Plan) else v for k, v in self.__dict__.items()}    # copies pack anew
 
     def refresh_packed(self) -> None:
         """Rebuild the fused operands at the next forward: needed after in-place
@@ -90,8 +120,8 @@ class GhostMLPChain(nn.Module):
         fc, proj = self.fc, self.proj
         a_fc, a_proj = fc._frozen_indices, proj._frozen_indices
         key = _plan_key(dtype, fc.weight, proj.weight, a_fc, a_proj, fc.bias)
-        if self._plan is not None and _same_key(self._plan[0], key):
-            return self._plan[1:]
+        if self._plan is not None and _same_key(self._plan.key, key):
+            return self._plan.take()
         with torch.no_grad():
             # proj's weight packed over its alive inputs, whole buffer: the fused
             # features padded with zero columns to a multiple of 64 (TMA rows).
@@ -112,7 +142,7 @@ class GhostMLPChain(nn.Module):
                     b_fc = torch.cat([b_fc, b_fc.new_zeros(pad)])
         # Under graph capture the packing is only recorded, into the graph's own memory: not kept.
         if not torch.cuda.is_current_stream_capturing():
-            self._plan = (key, w_fc, b_fc, w_proj)
+            self._plan = _Plan(key, (w_fc, b_fc, w_proj))
         return w_fc, b_fc, w_proj
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
@@ -165,7 +195,7 @@ class GhostPreNormMLP(GhostMLPChain):
             f"norm must be over fc's {fc.in_features} input features")
         self.norm = norm
         self.precision = precision
-        self._plan_q8: tuple | None = None
+        self._plan_q8: _Plan | None = None
 
     def refresh_packed(self) -> None:
         super().refresh_packed()
@@ -178,12 +208,13 @@ class GhostPreNormMLP(GhostMLPChain):
 
     def _operands_q8(self, dtype: torch.dtype):
         w_fc, b_fc, w_proj = self._operands(dtype)
-        plan = self._plan_q8
-        if plan is None or plan[0] is not w_fc:
-            plan = (w_fc, quantize_rows(w_fc), quantize_rows(w_proj))
+        if self._plan_q8 is not None and self._plan_q8.key[0] is w_fc:
+            q_fc, q_proj = self._plan_q8.take()
+        else:
+            q_fc, q_proj = quantize_rows(w_fc), quantize_rows(w_proj)
             if not torch.cuda.is_current_stream_capturing():
-                self._plan_q8 = plan
-        return plan[1], b_fc, plan[2]
+                self._plan_q8 = _Plan((w_fc,), (q_fc, q_proj))
+        return q_fc, b_fc, q_proj
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
         """x [..., features], and optionally a residual of its shape added in front of the norm."""

@@ -4,6 +4,9 @@ those files')."""
 
 from __future__ import annotations
 
+import copy
+import io
+
 import pytest
 import torch
 import torch.nn as nn
@@ -211,3 +214,66 @@ def test_captured_first(kind, updated):
         assert torch.equal(y, fresh(x2))
         del graph
         assert torch.equal(m(x), fresh(x2))
+
+
+def chain_or_block(kind, D, F, seed):
+    m = block(D, F, torch.float16, seed, precision="e4m3" if kind == "e4m3" else "input")
+    return GhostMLPChain(m.fc, m.proj, "gelu") if kind == "chain" else m
+
+
+@pytest.mark.parametrize("kind", ["input", "e4m3", "chain"])
+def test_first_use_on_two_streams(kind):
+    """The operands are packed on one stream, behind other work, and used at once on a second one."""
+    D, F = 512, 1024
+    want = chain_or_block(kind, D, F, 21)
+    x, _ = inputs(40, D, torch.float16, 21)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.no_grad():
+        want = want(x)
+        for _ in range(3):
+            m = chain_or_block(kind, D, F, 21)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(a):
+                torch.cuda._sleep(100_000_000)       # some 50 ms
+                first = m(x)
+            with torch.cuda.stream(b):
+                second = m(x)
+            torch.cuda.synchronize()
+            assert torch.equal(first, want) and torch.equal(second, want)
+
+
+@pytest.mark.parametrize("kind", ["input", "e4m3", "chain"])
+def test_replaced_while_another_stream_uses_them(kind):
+    """Operands replaced (and their memory handed out again) on the stream that packed them,
+    while a call on another stream still has to read them."""
+    D, F = 512, 1024
+    m = chain_or_block(kind, D, F, 22)
+    x, _ = inputs(40, D, torch.float16, 22)
+    b = torch.cuda.Stream()
+    with torch.no_grad():
+        want = m(x)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(b):
+            torch.cuda._sleep(100_000_000)
+            y = m(x)
+        m.refresh_packed()
+        rubbish = [torch.full((n,), 77, dtype=torch.uint8, device="cuda") for n in range(256 * 512, 2 << 20, 64 << 10)]
+        m(x)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and len(rubbish)
+
+
+@pytest.mark.parametrize("kind", ["input", "e4m3", "chain"])
+def test_copies_pack_their_own_operands(kind):
+    m = chain_or_block(kind, 256, 512, 23)
+    x, _ = inputs(5, 256, torch.float16, 23)
+    with torch.no_grad():
+        want = m(x)
+        twin = copy.deepcopy(m)
+        buf = io.BytesIO()
+        torch.save(m, buf)
+        buf.seek(0)
+        loaded = torch.load(buf, weights_only=False)
+        m.proj.weight.zero_()
+        for other in (twin, loaded):
+            assert torch.equal(other(x), want)
