@@ -34,7 +34,7 @@ from ghostweight_triton_b200 import _native
 from ghostweight_triton_b200.kernels.gather import pack_weight
 from ghostweight_triton_b200.kernels._args import refuse_grad
 from ghostweight_triton_b200.kernels.matmul import ghost_linear, packed_linear, packed_linear_q8
-from ghostweight_triton_b200.kernels.norm import quantize_rows, rms_norm, rms_norm_q8
+from ghostweight_triton_b200.kernels.norm import pack_weight_q8, quantize_rows, rms_norm, rms_norm_q8
 from ghostweight_triton_b200.module import GhostLinear
 
 # Activation modules (by class name) that the GEMM epilogue reproduces.
@@ -116,34 +116,42 @@ class GhostMLPChain(nn.Module):
         version counters the plan is keyed on."""
         self._plan = None
 
-    def _operands(self, dtype: torch.dtype):
+    def _operands(self, dtype: torch.dtype) -> tuple:
+        """(w_fc, b_fc, w_proj) as the products take them, for activations of `dtype`."""
         fc, proj = self.fc, self.proj
-        a_fc, a_proj = fc._frozen_indices, proj._frozen_indices
-        key = _plan_key(dtype, fc.weight, proj.weight, a_fc, a_proj, fc.bias)
+        key = _plan_key(dtype, fc.weight, proj.weight, fc._frozen_indices, proj._frozen_indices, fc.bias)
         if self._plan is not None and _same_key(self._plan.key, key):
             return self._plan.take()
         with torch.no_grad():
-            # proj's weight packed over its alive inputs, whole buffer: the fused
-            # features padded with zero columns to a multiple of 64 (TMA rows).
-            wp = pack_weight(proj.weight.detach(), a_proj, dtype=dtype)
-            n_pad = wp.stride(0)
-            w_proj = wp.as_strided((wp.shape[0], n_pad), (n_pad, 1))
-            # Rows of fc's weight for the features proj reads (zero rows for the
-            # padding: their outputs are act(0) = 0), over fc's alive inputs.
-            rows = fc.weight.detach().index_select(0, a_proj)
-            pad = n_pad - rows.shape[0]
-            if pad:
-                rows = torch.cat([rows, rows.new_zeros(pad, rows.shape[1])])
-            w_fc = pack_weight(rows, a_fc, dtype=dtype)
-            b_fc = None
-            if fc.bias is not None:
-                b_fc = fc.bias.detach().index_select(0, a_proj).to(dtype)
-                if pad:
-                    b_fc = torch.cat([b_fc, b_fc.new_zeros(pad)])
+            operands = self._pack(dtype)
         # Under graph capture the packing is only recorded, into the graph's own memory: not kept.
         if not torch.cuda.is_current_stream_capturing():
-            self._plan = _Plan(key, (w_fc, b_fc, w_proj))
-        return w_fc, b_fc, w_proj
+            self._plan = _Plan(key, operands)
+        return operands
+
+    def _pack(self, dtype: torch.dtype) -> tuple:
+        # proj's weight packed over its alive inputs, whole buffer: the fused
+        # features padded with zero columns to a multiple of 64 (TMA rows).
+        wp = pack_weight(self.proj.weight.detach(), self.proj._frozen_indices, dtype=dtype)
+        n_pad = wp.stride(0)
+        w_proj = wp.as_strided((wp.shape[0], n_pad), (n_pad, 1))
+        rows, b_fc = self._features(n_pad, dtype)
+        return pack_weight(rows, self.fc._frozen_indices, dtype=dtype), b_fc, w_proj
+
+    def _features(self, n_pad: int, dtype: torch.dtype) -> tuple:
+        """Rows of fc's weight (in its own type) and its bias for the features proj reads, and
+        zeros up to n_pad of them: their outputs are act(0) = 0."""
+        fc, a_proj = self.fc, self.proj._frozen_indices
+        rows = fc.weight.detach().index_select(0, a_proj)
+        pad = n_pad - rows.shape[0]
+        if pad:
+            rows = torch.cat([rows, rows.new_zeros(pad, rows.shape[1])])
+        b_fc = None
+        if fc.bias is not None:
+            b_fc = fc.bias.detach().index_select(0, a_proj).to(dtype)
+            if pad:
+                b_fc = torch.cat([b_fc, b_fc.new_zeros(pad)])
+        return rows, b_fc
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
         """The chain over x [..., in_features]; residual (the output's shape) is added in
@@ -195,26 +203,24 @@ class GhostPreNormMLP(GhostMLPChain):
             f"norm must be over fc's {fc.in_features} input features")
         self.norm = norm
         self.precision = precision
-        self._plan_q8: _Plan | None = None
-
-    def refresh_packed(self) -> None:
-        super().refresh_packed()
-        self._plan_q8 = None
 
     def _eps(self) -> float:
         eps = getattr(self.norm, "eps", getattr(self.norm, "variance_epsilon", None))
         # None: torch.nn.RMSNorm's default, the epsilon of the type it norms 16-bit rows in.
         return torch.finfo(torch.float32).eps if eps is None else float(eps)
 
-    def _operands_q8(self, dtype: torch.dtype):
-        w_fc, b_fc, w_proj = self._operands(dtype)
-        if self._plan_q8 is not None and self._plan_q8.key[0] is w_fc:
-            q_fc, q_proj = self._plan_q8.take()
-        else:
-            q_fc, q_proj = quantize_rows(w_fc), quantize_rows(w_proj)
-            if not torch.cuda.is_current_stream_capturing():
-                self._plan_q8 = _Plan((w_fc,), (q_fc, q_proj))
-        return q_fc, b_fc, q_proj
+    def _pack(self, dtype: torch.dtype) -> tuple:
+        if self.precision != "e4m3":
+            return super()._pack(dtype)
+        # From the parameters' own type, so that they are rounded once. The fused
+        # features are padded to a multiple of 64 as in 16 bits; proj's rows, padded
+        # with zeros to one of 128, hold as many columns.
+        own = lambda w: w if w.dtype in _native.DTYPE_CODES else w.float()
+        q, s_proj = pack_weight_q8(own(self.proj.weight), self.proj._frozen_indices)
+        n_pad = (q.shape[1] + 63) // 64 * 64
+        rows, b_fc = self._features(n_pad, dtype)
+        q_proj = q.as_strided((q.shape[0], n_pad), q.stride())
+        return pack_weight_q8(own(rows), self.fc._frozen_indices), b_fc, (q_proj, s_proj)
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
         """x [..., features], and optionally a residual of its shape added in front of the norm."""
@@ -232,7 +238,7 @@ class GhostPreNormMLP(GhostMLPChain):
             bias = bias.to(x.dtype)
         identity = self.dropout is None or (isinstance(self.dropout, nn.Dropout) and not self.dropout.training)
         if self.precision == "e4m3":
-            (w_fc, s_fc), b_fc, (w_proj, s_proj) = self._operands_q8(x.dtype)
+            (w_fc, s_fc), b_fc, (w_proj, s_proj) = self._operands(x.dtype)
             q, scale, *rest = rms_norm_q8(x2, **norm)
             s = rest[0] if rest else x2
             h = packed_linear_q8(q, scale, w_fc, s_fc, bias=b_fc, activation=self.activation, dtype=x.dtype)

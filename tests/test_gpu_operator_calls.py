@@ -15,7 +15,7 @@ from ghostweight_triton_b200.fuse import GhostMLPChain
 from ghostweight_triton_b200.kernels.gather import pack_weight
 from ghostweight_triton_b200.kernels.matmul import (ghost_linear, ghost_linear_dev, ghost_linear_pipelined, packed_linear,
                                                     packed_linear_q8)
-from ghostweight_triton_b200.kernels.norm import quantize_rows, rms_norm
+from ghostweight_triton_b200.kernels.norm import pack_weight_q8, quantize_rows, rms_norm, rms_norm_q8
 from tests.test_gpu_prenorm import block, exact, inputs
 
 pytestmark = pytest.mark.gpu
@@ -277,3 +277,47 @@ def test_copies_pack_their_own_operands(kind):
         m.proj.weight.zero_()
         for other in (twin, loaded):
             assert torch.equal(other(x), want)
+
+
+@pytest.mark.parametrize("parameters", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("M", [1, 40, 700])
+def test_e4m3_weights_are_rounded_once(M, parameters):
+    """The block's e4m3 weights are the parameters' own, not those of their copy in the input's type."""
+    D, F, dtype = 256, 600, torch.bfloat16
+    m = block(D, F, parameters, 25, precision="e4m3")
+    x, r = inputs(M, D, dtype, 25)
+    a1, a2 = m.fc._frozen_indices, m.proj._frozen_indices
+    with torch.no_grad():
+        q, sc, s = rms_norm_q8(x, m.norm.weight, 1e-5, residual=r, alive_indices=a1)
+        h = packed_linear_q8(q, sc, *pack_weight_q8(m.fc.weight[a2], a1), bias=m.fc.bias[a2], activation="gelu_tanh", dtype=dtype)
+        h = torch.cat([h, h.new_zeros(M, -a2.numel() % 64)], 1)      # as the block pads them
+        hq, hs = quantize_rows(h)
+        want = packed_linear_q8(hq[:, : a2.numel()], hs, *pack_weight_q8(m.proj.weight, a2), bias=m.proj.bias, residual=s)
+        assert torch.equal(m(x, residual=r), want)
+    # Nothing but e4m3 weights, scales and the bias is kept: a byte a weight, rows padded to 128.
+    padded = lambda n, to: (n + to - 1) // to * to
+    weights = padded(a2.numel(), 64) * padded(a1.numel(), 128) + D * padded(a2.numel(), 128)
+    assert sum(t.untyped_storage().nbytes() for t in m._plan.tensors) <= weights + 4 * (D + F) + 2 * F
+
+
+@pytest.mark.parametrize("precision", ["input", "e4m3"])
+@pytest.mark.parametrize("empty", ["fc", "proj", "both"])
+def test_masks_that_leave_nothing(empty, precision):
+    """fc without a live column gives act(b1) for every row, proj without one leaves s + b2."""
+    D, F, dtype = 128, 256, torch.float16
+    m = block(D, F, dtype, 26, precision=precision)
+    with torch.no_grad():
+        for layer, name in ((m.fc, "fc"), (m.proj, "proj")):
+            if empty in (name, "both"):
+                layer.weight.zero_()
+                layer.freeze_weight_mask()
+                assert layer._frozen_indices.numel() == 0
+        for M in (1, 50, 400):
+            x, r = inputs(M, D, dtype, M)
+            y = m(x, residual=r)
+            if empty == "fc" and precision == "e4m3":
+                s, want, *_ = exact(m, x, r, 1e-5)
+                branch = want - s                    # two roundings to e4m3: see test_gpu_prenorm
+                assert ((y.double() - want).norm() / branch.norm()).item() < 2 / 16
+            else:
+                check_block(y, m, x, r, 1e-5)
