@@ -176,34 +176,53 @@ def clear_packed_cache() -> None:
     _packed_cache.clear()
 
 
-def _gemm(x, w_packed, idx, y, bias, activation, strategy, residual=None):
-    """gw_gather_gemm_residual for a contiguous x; w_packed and y are row-major."""
+def _gemm(x, w_packed, idx, y, bias, activation, strategy, residual=None, shapes=None):
+    """gw_gather_gemm_residual for a contiguous x; y is row-major. shapes: x's and w_packed's."""
     if strategy == "runs" and (x.data_ptr() % 16 or x.stride(0) % 8):
         strategy = "auto"          # direct TMA of x needs 16-byte aligned rows
     dtype = x.dtype
-    M, K = x.shape
-    N, wk = w_packed.shape
+    (M, K), (N, wk) = shapes or (x.shape, w_packed.shape)
     ldw, uw = w_packed.stride()
     ldy, uy = y.stride()
-    assert idx.dtype is torch.int64 and idx.is_contiguous()
-    if (uw != 1 and wk > 1) or (uy != 1 and N > 1) or dtype not in _native.DTYPE_CODES:
-        _native.dtype_code(dtype)                # raises
-        _native._rowmajor(w_packed, y)
     n = idx.numel()
+    assert idx.dtype is torch.int64 and idx.is_contiguous() and idx.is_cuda, "alive_indices must be contiguous int64 on x's device"
+    # _operands_ok for what is usually given; this function is most of a small call's time.
+    if not (w_packed.dtype is dtype and w_packed.is_cuda and wk >= n and uw == 1 and ldw >= wk
+            and (bias is None or (bias.dtype is dtype and bias.numel() == N and bias.is_cuda and bias.is_contiguous()))):
+        ldw = _operands_ok(w_packed, n, bias, dtype, x.get_device())
+    if (uy != 1 and N > 1) or dtype not in _native.DTYPE_CODES:
+        _native.dtype_code(dtype)                # raises
+        _native._rowmajor(y)
     ws_ptr, ws_bytes = None, 0
     if strategy != "fused" and strategy != "runs" and dtype is not torch.float32:
         nbytes = _native.gather_gemm_workspace_bytes(M, n, dtype)
         if nbytes:
             ws = _native.gemm_workspace(x.device, nbytes)
             ws_ptr, ws_bytes = ws.data_ptr(), ws.numel()
-    r_ptr, ldr = (None, 0) if residual is None else (residual.data_ptr(), max(residual.stride(0), N))
+    r_ptr, ldr = (None, 0) if residual is None else (residual.data_ptr(), residual.stride()[0])
     st = _native._call((_native._api or _native.api()).gw_gather_gemm_residual,
                        (x.data_ptr(), _native.DTYPE_CODES[dtype], M, K, K, w_packed.data_ptr(), N, ldw if ldw > n else n,
                         idx.data_ptr(), n, None if bias is None else bias.data_ptr(), _native.epilogue_code(activation),
-                        r_ptr, ldr, y.data_ptr(), ldy if ldy > N else N, _native.GEMM_STRATEGIES[strategy], ws_ptr,
-                        ws_bytes), x.get_device())
+                        r_ptr, ldr if ldr > N else N, y.data_ptr(), ldy if ldy > N else N, _native.GEMM_STRATEGIES[strategy],
+                        ws_ptr, ws_bytes), x.get_device())
     if st:
         _native._check(st, "gw_gather_gemm")
+
+
+def _operands_ok(w_packed, n, bias, dtype, dev) -> int:
+    """The leading dimension of a packed weight [N, n or more] of this type on CUDA device
+    `dev`, in row-major rows of their own; asserts this, and that a bias holds N values."""
+    N, cols = w_packed.shape
+    ld, unit = w_packed.stride()
+    assert (w_packed.dtype is dtype and w_packed.get_device() == dev and cols >= n
+            and (unit == 1 or cols <= 1) and (ld >= cols or N <= 1)), (
+        f"w_packed must be a row-major {dtype} matrix with {n} columns on the activations' device, got "
+        f"{w_packed.dtype} {tuple(w_packed.shape)} with strides {w_packed.stride()} on {w_packed.device}")
+    if bias is not None:
+        assert bias.dtype is dtype and bias.numel() == N and bias.is_contiguous() and bias.get_device() == dev, (
+            f"bias must hold {N} contiguous values of {dtype} on the activations' device, got {bias.dtype} "
+            f"{tuple(bias.shape)} on {bias.device}")
+    return ld if ld > n else n
 
 
 def index_runs(alive_indices: torch.Tensor, K: int) -> int:
@@ -232,8 +251,8 @@ def ghost_linear(
     assert x.ndim == 2 and x.is_cuda
     if not x.is_contiguous():
         x = x.contiguous()
-    M = x.shape[0]
-    N = w_packed.shape[0]
+    shapes = x.shape, w_packed.shape
+    M, N = shapes[0][0], shapes[1][0]
     if out is None:
         y = x.new_empty((M, N))
         if residual is not None:
@@ -242,7 +261,7 @@ def ghost_linear(
         y, residual = _product_out(out, residual, M, N, x)
         x = _apart_from(y, x, w_packed)
     if M and N:
-        _gemm(x, w_packed, alive_indices, y, bias, activation, strategy, residual)
+        _gemm(x, w_packed, alive_indices, y, bias, activation, strategy, residual, shapes)
     return y
 
 
@@ -298,6 +317,7 @@ def ghost_linear_dev(
     y, residual = _product_out(out, residual, M, N, x)
     if out is not None:
         x = _apart_from(y, x, w_packed)
+    _operands_ok(w_packed, alive_buffer.numel(), bias, x.dtype, x.get_device())
     if M and N:
         _native.gather_gemm_dev(x, w_packed, alive_buffer, alive_count, y, bias=bias,
                                 activation=activation, residual=residual)
@@ -316,7 +336,8 @@ def packed_linear(
 
     Both operands arrive by TMA: a's rows may be strided (as ``rms_norm``
     returns them) if they stay 16-byte aligned, else they are copied. residual
-    [M, N] and ``out`` as for :func:`ghost_linear`.
+    [M, N] and ``out`` as for :func:`ghost_linear`. Columns of w_packed from
+    K_alive on are not looked at.
     """
     assert a.ndim == 2 and a.is_cuda
     if not a.is_contiguous() and (a.stride(1) != 1 or a.stride(0) % 8 or a.stride(0) < a.shape[1]
@@ -325,6 +346,7 @@ def packed_linear(
     y, residual = _product_out(out, residual, a.shape[0], w_packed.shape[0], a)
     if out is not None:
         a = _apart_from(y, a, w_packed)
+    _operands_ok(w_packed, a.shape[1], bias, a.dtype, a.get_device())
     if y.numel():
         _native.packed_gemm(a, w_packed, y, bias=bias, activation=activation, residual=residual)
     return y
@@ -457,6 +479,7 @@ def ghost_linear_pipelined(calls) -> list:
         act = c[5] if len(c) > 5 else None
         assert x.ndim == 2 and x.is_cuda and out is not None
         _product_out(out, None, x.shape[0], wp.shape[0], x)
+        _operands_ok(wp, idx.numel(), bias, x.dtype, x.get_device())
         norm.append((x, wp, idx, out, bias, act))
     st.gemm.wait_stream(cur)
     st.gather.wait_stream(cur)

@@ -17,6 +17,7 @@ from ghostweight_triton_b200.kernels.matmul import (ghost_linear, ghost_linear_d
                                                     packed_linear_q8)
 from ghostweight_triton_b200.kernels.norm import pack_weight_q8, quantize_rows, rms_norm, rms_norm_q8
 from tests.test_gpu_prenorm import block, exact, inputs
+from tests.test_products_cpu import weights_and_biases_refused
 
 pytestmark = pytest.mark.gpu
 
@@ -321,3 +322,28 @@ def test_masks_that_leave_nothing(empty, precision):
                 assert ((y.double() - want).norm() / branch.norm()).item() < 2 / 16
             else:
                 check_block(y, m, x, r, 1e-5)
+
+
+def test_operands_refused():
+    """Weights narrower than the product, of another type or device or in overlapping rows, and
+    biases that do not hold N values: refused by every 16-bit product before a launch."""
+    M, N, K = 8, 48, 64
+    x, w, idx = operands(M, N, K)
+    count = torch.tensor([K], dtype=torch.int32, device="cuda")
+    out = torch.empty(M, N, dtype=x.dtype, device="cuda")
+    calls = [lambda w, b: ghost_linear(x, w, idx, bias=b), lambda w, b: ghost_linear_dev(x, w, idx, count, bias=b),
+             lambda w, b: packed_linear(x, w, bias=b), lambda w, b: ghost_linear_pipelined([(x, w, idx, out, b)])]
+    for bad, b in weights_and_biases_refused(N, K, x.dtype):
+        bad = bad.cuda() if bad.stride(0) >= bad.shape[1] and bad.stride(1) == 1 else torch.zeros_like(w).set_(
+            torch.zeros(N * K, dtype=bad.dtype, device="cuda").untyped_storage(), 0, bad.shape, bad.stride())
+        b = None if b is None else b.cuda() if b.is_contiguous() else torch.zeros(2 * N, dtype=b.dtype, device="cuda")[::2]
+        for i, call in enumerate(calls):
+            if bad.shape[0] == N or i < 3:
+                with pytest.raises(AssertionError, match="must"):
+                    call(bad, b)
+    for call in calls:
+        for bad, b in ((w.cpu(), None), (w, torch.zeros(N, dtype=x.dtype))):
+            with pytest.raises(AssertionError, match="must"):
+                call(bad, b)
+    with pytest.raises(AssertionError, match="alive_indices"):
+        ghost_linear(x, w, idx.cpu())

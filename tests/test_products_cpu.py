@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from ghostweight_triton_b200.kernels import _args
-from ghostweight_triton_b200.kernels.matmul import _apart_from, _product_out
+from ghostweight_triton_b200.kernels.matmul import _apart_from, _operands_ok, _product_out
 
 F16 = torch.float16
 
@@ -96,3 +96,25 @@ def test_operands_leave_the_output():
         assert _apart_from(out, x, w) is x
     with pytest.raises(AssertionError, match="w_packed"):
         _apart_from(w[:8, :16], buf[:, :24], w)
+
+
+def weights_and_biases_refused(N, K, dtype):
+    """(weight, bias) pairs that a product of K columns and N features must not read."""
+    w = torch.zeros(N, K, dtype=dtype)
+    b = torch.zeros(N, dtype=dtype)
+    return [(w[:, : K - 1], b), (w[:, : K // 2], None), (w.float() if dtype is not torch.float32 else w.half(), b),
+            (torch.zeros(K, N, dtype=dtype).t(), b), (w[:1].expand(N, K), b), (w.view(-1).as_strided((N // 2, K), (K // 2, 1)), None),
+            (w, b[: N - 1]), (w, torch.zeros(2 * N, dtype=dtype)[::2]), (w, b.double()), (w, b[:1].expand(N))]
+
+
+def test_operands_that_end_too_early():
+    for w, b in weights_and_biases_refused(16, 24, F16):
+        with pytest.raises(AssertionError, match="must"):
+            _operands_ok(w, 24, b, F16, -1)
+    w, b = torch.zeros(16, 24, dtype=F16), torch.zeros(16, dtype=F16)
+    assert _operands_ok(w, 24, b, F16, -1) == 24
+    assert _operands_ok(w[:, :20], 20, None, F16, -1) == 24           # rows with a gap
+    assert _operands_ok(w, 20, b, F16, -1) == 24                     # wider: the first columns
+    assert _operands_ok(torch.zeros(1, 24, dtype=F16).t().contiguous().t(), 24, None, F16, -1) == 24
+    assert _operands_ok(torch.zeros(16, 64, dtype=F16)[:, :0], 0, b, F16, -1) == 64
+    assert _operands_ok(torch.zeros(0, 24, dtype=F16), 24, None, F16, -1) == 24
