@@ -335,20 +335,34 @@ def packed_linear(
     """y = act(a @ w_packed^T + bias) + residual for an already compacted a [M, K_alive].
 
     Both operands arrive by TMA: a's rows may be strided (as ``rms_norm``
-    returns them) if they stay 16-byte aligned, else they are copied. residual
-    [M, N] and ``out`` as for :func:`ghost_linear`. Columns of w_packed from
-    K_alive on are not looked at.
+    returns them) if they start at multiples of 16 bytes, else they are copied
+    into such rows. residual [M, N] and ``out`` as for :func:`ghost_linear`.
+    Columns of w_packed from K_alive on are not looked at.
     """
     assert a.ndim == 2 and a.is_cuda
-    if not a.is_contiguous() and (a.stride(1) != 1 or a.stride(0) % 8 or a.stride(0) < a.shape[1]
-                                  or a.data_ptr() % 16):
-        a = a.contiguous()
-    y, residual = _product_out(out, residual, a.shape[0], w_packed.shape[0], a)
+    M, K = a.shape
+    N = w_packed.shape[0]
+    lda, unit = a.stride()
+    if a.data_ptr() % 16 or (unit != 1 and K > 1) or (M > 1 and (lda % 8 or lda < K)):
+        lda = (K + 7) // 8 * 8
+        buf = a.new_empty((M, lda))              # columns from K on are not looked at
+        buf[:, :K] = a
+        a = buf[:, :K]
+    elif M <= 1:
+        lda = (K + 7) // 8 * 8                   # a row's stride may be anything
+    dev = a.get_device()
+    ldw = _operands_ok(w_packed, K, bias, a.dtype, dev)
+    y, residual = _product_out(out, residual, M, N, a)
     if out is not None:
         a = _apart_from(y, a, w_packed)
-    _operands_ok(w_packed, a.shape[1], bias, a.dtype, a.get_device())
-    if y.numel():
-        _native.packed_gemm(a, w_packed, y, bias=bias, activation=activation, residual=residual)
+    if M and N:
+        r_ptr, ldr = _native._residual(residual)
+        st = _native._call((_native._api or _native.api()).gw_packed_gemm_residual,
+                           (a.data_ptr(), _native.dtype_code(a.dtype), M, K, lda, w_packed.data_ptr(), N, ldw,
+                            None if bias is None else bias.data_ptr(), _native.epilogue_code(activation), r_ptr, ldr,
+                            y.data_ptr(), max(y.stride(0), N)), dev)
+        if st:
+            _native._check(st, "gw_packed_gemm")
     return y
 
 

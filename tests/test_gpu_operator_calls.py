@@ -17,6 +17,7 @@ from ghostweight_triton_b200.kernels.matmul import (ghost_linear, ghost_linear_d
                                                     packed_linear_q8)
 from ghostweight_triton_b200.kernels.norm import pack_weight_q8, quantize_rows, rms_norm, rms_norm_q8
 from tests.test_gpu_prenorm import block, exact, inputs
+from tests.test_gpu_residual import check
 from tests.test_products_cpu import weights_and_biases_refused
 
 pytestmark = pytest.mark.gpu
@@ -347,3 +348,26 @@ def test_operands_refused():
                 call(bad, b)
     with pytest.raises(AssertionError, match="alive_indices"):
         ghost_linear(x, w, idx.cpu())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("M", [1, 3, 17, 300, 2100])
+def test_packed_linear_takes_any_rows(M, dtype):
+    """Rows that TMA cannot load (odd widths, odd offsets, columns of adjacent elements) are copied."""
+    for K in (1, 7, 333, 512):
+        g = torch.Generator(device="cuda").manual_seed(M + K)
+        rnd = lambda *s: torch.randn(*s, generator=g, device="cuda").to(dtype)
+        N, big = 300, rnd(M + 2, K + 13)
+        w, b, r = rnd(N, K) / max(K, 1) ** 0.5, rnd(N), rnd(M, N)
+        wp = pack_weight(w, torch.arange(K, device="cuda"))
+        flat = rnd(M * K + 1)
+        for a in (rnd(M, K), flat[1:].view(M, K), big[1: M + 1, 3: K + 3], big[:M, 8: K + 8], rnd(K, M).t(),
+                  rnd(1, K).expand(M, K), rnd(M, 2 * K)[:, ::2], rnd(2 * M, K)[::2]):
+            keep = a.clone()
+            check(packed_linear(a, wp, bias=b, activation="gelu", residual=r), a, w, b, "gelu", r)
+            assert torch.equal(a, keep)
+    # What rms_norm writes without a list: rows of the width itself.
+    x, weight = rnd(M, 333), rnd(333)
+    w = rnd(64, 333) / 18
+    n = rms_norm(x, weight)
+    check(packed_linear(n, pack_weight(w, torch.arange(333, device="cuda"))), n, w, None, None, None)
