@@ -178,10 +178,13 @@ def clear_packed_cache() -> None:
 
 def _gemm(x, w_packed, idx, y, bias, activation, strategy, residual=None, shapes=None):
     """gw_gather_gemm_residual for a contiguous x; y is row-major. shapes: x's and w_packed's."""
-    if strategy == "runs" and (x.data_ptr() % 16 or x.stride(0) % 8):
-        strategy = "auto"          # direct TMA of x needs 16-byte aligned rows
     dtype = x.dtype
     (M, K), (N, wk) = shapes or (x.shape, w_packed.shape)
+    ldx = K
+    if strategy == "runs":
+        ldx = max(x.stride(0), K)  # a contiguous x of one row may have any stride
+        if x.data_ptr() % 16 or ldx % 8:
+            strategy = "auto"      # direct TMA of x needs 16-byte aligned rows
     ldw, uw = w_packed.stride()
     ldy, uy = y.stride()
     n = idx.numel()
@@ -201,7 +204,7 @@ def _gemm(x, w_packed, idx, y, bias, activation, strategy, residual=None, shapes
             ws_ptr, ws_bytes = ws.data_ptr(), ws.numel()
     r_ptr, ldr = (None, 0) if residual is None else (residual.data_ptr(), residual.stride()[0])
     st = _native._call((_native._api or _native.api()).gw_gather_gemm_residual,
-                       (x.data_ptr(), _native.DTYPE_CODES[dtype], M, K, K, w_packed.data_ptr(), N, ldw if ldw > n else n,
+                       (x.data_ptr(), _native.DTYPE_CODES[dtype], M, K, ldx, w_packed.data_ptr(), N, ldw if ldw > n else n,
                         idx.data_ptr(), n, None if bias is None else bias.data_ptr(), _native.epilogue_code(activation),
                         r_ptr, ldr if ldr > N else N, y.data_ptr(), ldy if ldy > N else N, _native.GEMM_STRATEGIES[strategy],
                         ws_ptr, ws_bytes), x.get_device())

@@ -11,6 +11,7 @@ import pytest
 import torch
 import torch.nn as nn
 
+from ghostweight_triton_b200 import GhostLinear
 from ghostweight_triton_b200.fuse import GhostMLPChain
 from ghostweight_triton_b200.kernels.gather import pack_weight
 from ghostweight_triton_b200.kernels.matmul import (ghost_linear, ghost_linear_dev, ghost_linear_pipelined, packed_linear,
@@ -371,3 +372,27 @@ def test_packed_linear_takes_any_rows(M, dtype):
     w = rnd(64, 333) / 18
     n = rms_norm(x, weight)
     check(packed_linear(n, pack_weight(w, torch.arange(333, device="cuda"))), n, w, None, None, None)
+
+
+@pytest.mark.parametrize("K", [4096, 4100, 4104])
+def test_one_row_of_a_padded_buffer(K):
+    """A row that torch calls contiguous at whatever stride, over 64-column runs; the layer likewise."""
+    g = torch.Generator(device="cuda").manual_seed(K)
+    N, dt = 256, torch.bfloat16
+    runs = torch.randperm(64, generator=g, device="cuda")[:32].sort().values
+    idx = (runs[:, None] * 64 + torch.arange(64, device="cuda")).reshape(-1)
+    w = (torch.randn(N, K, generator=g, device="cuda") / 64).to(dt)
+    wp = pack_weight(w, idx)
+    layer = GhostLinear(K, N, bias=False, device="cuda", dtype=dt)
+    with torch.no_grad():
+        layer.weight.copy_(w)
+        layer._set_frozen(idx)
+    for ld in (K, 4104, 4106, 4160):
+        big = torch.randn(2, ld, generator=g, device="cuda").to(dt)
+        r = torch.randn(1, N, generator=g, device="cuda").to(dt)
+        for x in (big[0:1, :K], big.view(-1)[:K].as_strided((1, K), (1, 1))):
+            assert x.is_contiguous()
+            check(ghost_linear(x, wp, idx, strategy="runs", residual=r), x[:, idx], w[:, idx], None, None, r)
+            with torch.no_grad():
+                for _ in range(2):
+                    check(layer(x, residual=r), x[:, idx], w[:, idx], None, None, r)
