@@ -27,6 +27,9 @@ an extension: the reference replaces the two projections independently
 
 from __future__ import annotations
 
+import copy
+import math
+
 import torch
 import torch.nn as nn
 
@@ -181,8 +184,9 @@ class GhostPreNormMLP(GhostMLPChain):
     """s = x + residual;  y = s + proj(activation(fc(rms_norm(s)))).
 
     ``norm`` is a root-mean-square norm over fc's input features (torch.nn.RMSNorm,
-    or a module with ``weight`` and ``eps`` or ``variance_epsilon``), ``fc`` and
-    ``proj`` are GhostLinears with frozen masks, joined by the GELU ``activation``
+    or a module with ``weight`` and ``eps`` or ``variance_epsilon`` that computes
+    x * rsqrt(mean(x^2) + eps) * weight: two rows are tried when the block is built,
+    at its first forward if the norm is on the meta device then), ``fc`` and ``proj`` are GhostLinears with frozen masks, joined by the GELU ``activation``
     ("gelu" or "gelu_tanh"); all stay registered, so parameters and state-dict
     keys are theirs. fp16 and bf16 inputs. ``precision="e4m3"`` runs both
     products on e4m3 operands (weights rounded once with a scale per feature,
@@ -203,11 +207,36 @@ class GhostPreNormMLP(GhostMLPChain):
             f"norm must be over fc's {fc.in_features} input features")
         self.norm = norm
         self.precision = precision
+        self._norm_known = False
+        if weight is None or not weight.is_meta:
+            self._try_norm()
 
     def _eps(self) -> float:
         eps = getattr(self.norm, "eps", getattr(self.norm, "variance_epsilon", None))
         # None: torch.nn.RMSNorm's default, the epsilon of the type it norms 16-bit rows in.
         return torch.finfo(torch.float32).eps if eps is None else float(eps)
+
+    def _try_norm(self) -> None:
+        """Assert that a copy of the norm in fp32, with a gain of its own, computes what rms_norm does,
+        of a row of ordinary values whose mean is not zero and of one so small that eps counts."""
+        weight = getattr(self.norm, "weight", None)
+        device = torch.device("cpu") if weight is None else weight.device
+        eps = self._eps()
+        row = 1.0 + torch.sin(torch.arange(self.fc.in_features, device=device, dtype=torch.float32))
+        x = torch.stack([row, row * math.sqrt(max(eps, 1e-12))])
+        want = x.double() * torch.rsqrt(x.double().square().mean(-1, keepdim=True) + eps)
+        try:
+            with torch.no_grad():
+                twin = copy.deepcopy(self.norm).float()
+                if weight is not None:
+                    twin.weight.copy_(row - 0.7)
+                    want = want * (row - 0.7).double()
+                got = twin(x).double()
+            same = got.shape == want.shape and bool(((got - want).norm(dim=1) <= 1e-3 * want.norm(dim=1)).all())
+        except Exception as e:
+            raise AssertionError("norm must take rows of fc's input features") from e
+        assert same, "norm must compute x * rsqrt(mean(x^2) + eps) * weight"
+        self._norm_known = True
 
     def _pack(self, dtype: torch.dtype) -> tuple:
         if self.precision != "e4m3":
@@ -228,6 +257,8 @@ class GhostPreNormMLP(GhostMLPChain):
         if not (_frozen(self.fc) and _frozen(self.proj)):
             raise RuntimeError("GhostPreNormMLP needs frozen masks on fc and proj (freeze_mask or freeze_weight_mask)")
         refuse_grad(x=x, residual=residual)
+        if not self._norm_known:
+            self._try_norm()
         features = self.fc.in_features
         x2 = x.reshape(-1, features)
         r2 = None if residual is None else residual.reshape(-1, features)

@@ -12,13 +12,14 @@ import torch
 import torch.nn as nn
 
 from ghostweight_triton_b200 import GhostLinear
-from ghostweight_triton_b200.fuse import GhostMLPChain
+from ghostweight_triton_b200.fuse import GhostMLPChain, GhostPreNormMLP
 from ghostweight_triton_b200.kernels.gather import pack_weight
 from ghostweight_triton_b200.kernels.matmul import (ghost_linear, ghost_linear_dev, ghost_linear_pipelined, packed_linear,
                                                     packed_linear_q8)
 from ghostweight_triton_b200.kernels.norm import pack_weight_q8, quantize_rows, rms_norm, rms_norm_q8
 from tests.test_gpu_prenorm import block, exact, inputs
 from tests.test_gpu_residual import check
+from tests.test_prenorm_cpu import OnePlusWeight
 from tests.test_products_cpu import weights_and_biases_refused
 
 pytestmark = pytest.mark.gpu
@@ -396,3 +397,21 @@ def test_one_row_of_a_padded_buffer(K):
             with torch.no_grad():
                 for _ in range(2):
                     check(layer(x, residual=r), x[:, idx], w[:, idx], None, None, r)
+
+
+def test_norms_told_by_what_they_compute():
+    """A norm that multiplies by 1 + weight is refused; one built on the meta device is tried in the first forward."""
+    m = block(128, 256, torch.float16, 30)
+    with pytest.raises(AssertionError, match="norm must"):
+        GhostPreNormMLP(OnePlusWeight(128).cuda(), m.fc, m.proj, "gelu")
+    x, r = inputs(4, 128, torch.float16, 30)
+    with torch.no_grad():
+        for norm, good in ((nn.RMSNorm(128, eps=1e-5, device="meta"), True), (OnePlusWeight(128).to("meta"), False)):
+            late = GhostPreNormMLP(norm, m.fc, m.proj, m.activation)
+            late.norm.to_empty(device="cuda")
+            late.norm.weight.copy_(m.norm.weight)
+            if good:
+                assert torch.equal(late(x, residual=r), m(x, residual=r))
+            else:
+                with pytest.raises(AssertionError, match="norm must"):
+                    late(x, residual=r)
