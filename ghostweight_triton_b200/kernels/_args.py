@@ -14,6 +14,18 @@ def refuse_grad(**tensors: torch.Tensor | None) -> None:
                                    "call it under torch.no_grad() or on detached tensors")
 
 
+def refuse_grad_out(what: str, out: torch.Tensor) -> None:
+    """Raise if results written into `out` would be lost to its gradient."""
+    if out.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{what} requires a gradient, and this operator has no backward pass: "
+                           "call it under torch.no_grad() or on detached tensors")
+
+
+# Called for every given tensor that a kernel has written: the autograd engine and the
+# caches of packed weights see the write by the tensor's version.
+written = torch.autograd.graph.increment_version
+
+
 def rows(t: torch.Tensor, cols: int) -> torch.Tensor:
     """t as a row-major [rows, cols] matrix (copied only when its strides are not such)."""
     t = t.reshape(-1, cols)

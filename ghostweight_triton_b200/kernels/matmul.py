@@ -21,7 +21,7 @@ from __future__ import annotations
 import torch
 
 from ghostweight_triton_b200 import _native
-from ghostweight_triton_b200.kernels._args import in_place_or_apart, overlap, residual_matrix
+from ghostweight_triton_b200.kernels._args import in_place_or_apart, overlap, refuse_grad_out, residual_matrix, written
 from ghostweight_triton_b200.kernels.gather import pack_weight
 
 
@@ -265,6 +265,8 @@ def ghost_linear(
         x = _apart_from(y, x, w_packed)
     if M and N:
         _gemm(x, w_packed, alive_indices, y, bias, activation, strategy, residual, shapes)
+        if out is not None:
+            written(out)
     return y
 
 
@@ -281,6 +283,7 @@ def _product_out(out, residual, M, N, like):
         f"out must be {like.dtype} of shape {(M, N)} on {like.device}, got {out.dtype} {tuple(out.shape)} on {out.device}")
     assert (out.stride(1) == 1 or N <= 1) and (out.stride(0) >= N or M <= 1), (
         f"out must be a row-major matrix, got strides {out.stride()}")
+    refuse_grad_out("out", out)
     if residual is not None:
         in_place_or_apart("out", out, residual)
         assert residual is given or out is not given, "a residual updated in place must have rows of adjacent elements"
@@ -324,6 +327,8 @@ def ghost_linear_dev(
     if M and N:
         _native.gather_gemm_dev(x, w_packed, alive_buffer, alive_count, y, bias=bias,
                                 activation=activation, residual=residual)
+        if out is not None:
+            written(out)
     return y
 
 
@@ -366,6 +371,8 @@ def packed_linear(
                             y.data_ptr(), max(y.stride(0), N)), dev)
         if st:
             _native._check(st, "gw_packed_gemm")
+        if out is not None:
+            written(out)
     return y
 
 
@@ -437,6 +444,8 @@ def packed_linear_q8(
         ldy = max(y.stride(0), N)
     if M and N:
         _native.packed_gemm_q8(a, a_scale, M, K, lda, w_packed, w_scale, N, ldw, y, ldy, bias, activation, residual)
+        if out is not None:
+            written(out)
     return y
 
 
@@ -536,6 +545,7 @@ def ghost_linear_pipelined(calls) -> list:
                 st.gemm.wait_event(st.ready[b])
                 if out.numel():
                     _native.packed_gemm(xgs.pop(i), wp, out, bias=bias, activation=act)
+                    written(out)
                 st.free[b].record(st.gemm)
             else:
                 ghost_linear(x, wp, idx, bias=bias, activation=act, out=out)

@@ -21,7 +21,7 @@ import math
 import torch
 
 from ghostweight_triton_b200 import _native
-from ghostweight_triton_b200.kernels._args import leading, out_matrix, refuse_grad, rows
+from ghostweight_triton_b200.kernels._args import leading, out_matrix, refuse_grad, refuse_grad_out, rows, written
 from ghostweight_triton_b200.kernels.gather import PACK_ALIGN, _round_up
 
 # e4m3 rows keep a stride of a multiple of 128 bytes: one k-block of the
@@ -70,6 +70,7 @@ def _norm(x, weight, eps, residual, alive_indices, residual_out, q8):
             weight = weight.contiguous()
     total = r_2d = None
     ldr = lds = 0
+    given = residual_out
     if residual is not None:
         assert (residual.shape == shape and residual.dtype is dtype and residual.is_cuda
                 and residual.get_device() == dev), "residual must have x's shape, dtype and device"
@@ -82,6 +83,7 @@ def _norm(x, weight, eps, residual, alive_indices, residual_out, q8):
             total = residual_out = x.new_empty(shape)
             lds = cols
         else:
+            refuse_grad_out("residual_out", residual_out)
             total = out_matrix("residual_out", residual_out, x, x_2d, r_2d)
             lds = leading(total)
     else:
@@ -100,6 +102,8 @@ def _norm(x, weight, eps, residual, alive_indices, residual_out, q8):
         buf = x.new_empty((M, ld))
     if M:
         _native.rms_norm(x_2d, M, cols, ldx, r_2d, ldr, total, lds, weight, eps, idx, n, buf, ld, scale)
+        if given is not None:
+            written(given)
     y = buf if ld == n else buf.narrow(1, 0, n)
     if not flat:
         y = y.view(*shape[:-1], n)

@@ -14,8 +14,8 @@ import torch.nn as nn
 from ghostweight_triton_b200 import GhostLinear
 from ghostweight_triton_b200.fuse import GhostMLPChain, GhostPreNormMLP
 from ghostweight_triton_b200.kernels.gather import pack_weight
-from ghostweight_triton_b200.kernels.matmul import (ghost_linear, ghost_linear_dev, ghost_linear_pipelined, packed_linear,
-                                                    packed_linear_q8)
+from ghostweight_triton_b200.kernels.matmul import (ghost_linear, ghost_linear_dev, ghost_linear_pipelined,
+                                                    ghostweight_matmul, packed_linear, packed_linear_q8)
 from ghostweight_triton_b200.kernels.norm import pack_weight_q8, quantize_rows, rms_norm, rms_norm_q8
 from tests.test_gpu_prenorm import block, exact, inputs
 from tests.test_gpu_residual import check
@@ -415,3 +415,51 @@ def test_norms_told_by_what_they_compute():
             else:
                 with pytest.raises(AssertionError, match="norm must"):
                     late(x, residual=r)
+
+
+def writers(M, N, K, g):
+    """name -> call that writes an [M, N] fp16 tensor that it is given."""
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda").half()
+    x, w, idx = rnd(M, K), rnd(N, K) / 16, torch.arange(K, device="cuda")
+    wp = pack_weight(w, idx)
+    count = torch.tensor([K], dtype=torch.int32, device="cuda")
+    qa, qw, s = quantize_rows(x), quantize_rows(w), rnd(M, N)
+    return {"ghost_linear": lambda out: ghost_linear(x, wp, idx, out=out),
+            "ghost_linear_dev": lambda out: ghost_linear_dev(x, wp, idx, count, out=out),
+            "packed_linear": lambda out: packed_linear(x, wp, residual=s, out=out),
+            "packed_linear_q8": lambda out: packed_linear_q8(*qa, *qw, out=out),
+            "pipelined": lambda out: ghost_linear_pipelined([(x, wp, idx, out)]),
+            "rms_norm": lambda out: rms_norm(s, residual=s, residual_out=out),
+            "rms_norm_q8": lambda out: rms_norm_q8(s, residual=s, residual_out=out)}
+
+
+@pytest.mark.parametrize("name", ["ghost_linear", "ghost_linear_dev", "packed_linear", "packed_linear_q8", "pipelined",
+                                  "rms_norm", "rms_norm_q8"])
+def test_writes_into_given_tensors_are_seen(name):
+    """By the caches of packed weights, by autograd, and under inference mode, where nothing is counted."""
+    g = torch.Generator(device="cuda").manual_seed(40)
+    M, N, K = 64, 256, 128
+    write = writers(M, N, K, g)[name]
+    buf = torch.randn(M, N, generator=g, device="cuda").half()
+    act = torch.randn(9, M, generator=g, device="cuda").half()
+    alive = torch.arange(M, device="cuda")
+    with torch.no_grad():
+        ghostweight_matmul(act, buf, alive)          # buf as a weight: its packed form is kept
+        write(buf)
+        assert torch.equal(ghostweight_matmul(act, buf, alive), ghostweight_matmul(act, buf.clone(), alive))
+    p = torch.randn(M, N, generator=g, device="cuda").half().requires_grad_()
+    z = (buf * p).sum()                              # keeps buf for the gradient of p
+    write(buf)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+    leaf = buf.clone().requires_grad_()
+    before = leaf.detach().clone()
+    with pytest.raises(RuntimeError, match="no backward"):
+        write(leaf)
+    assert torch.equal(leaf, before)
+    with torch.no_grad():
+        write(leaf)
+    with torch.inference_mode():
+        inner = torch.empty(M, N, dtype=torch.float16, device="cuda")
+        write(inner)
+        assert torch.equal(inner, leaf)
