@@ -351,7 +351,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmap_b,
           scale32(f, row_scale, p.w_scale, n_base, p.N);
           bias_activate32<DT, EPI>(f, p.bias, n_base, p.N);
         } else {
-          if (p.bias) add_bias32<DT>(f, p.bias, n_base, p.N);
+          if (p.bias) add_bias32<DT, STAGED>(f, p.bias, n_base, p.N);
           activate32<EPI>(f);
         }
         if (STAGED && p.res) {

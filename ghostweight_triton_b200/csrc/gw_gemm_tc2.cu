@@ -363,16 +363,26 @@ __device__ __forceinline__ void gather_units(const Tc2Params& p, int e, int lane
   if (__any_sync(0xFFFFFFFFu, bad) && lane == 0) raise_error(p.err, GW_DERR_BAD_INDEX);
 }
 
-// Q8: A and W' in e4m3 with scales, else 16-bit of type DT. RES: with a residual
-// (an instantiation of its own: its loads cost the plain epilogue 10% where the
-// epilogue bounds the kernel).
-template <int BN, int DT, int EPI, bool GATHER, bool Q8, bool RES>
+// What the epilogue has to do, each an instantiation of its own. A residual's loads
+// cost the plain epilogue 10% where the epilogue bounds the kernel. The stores of
+// rows that are not 16-byte aligned, unrolled inside its loop though not taken, cost
+// it 0.2 to 0.4 us behind a gather (8192 x 1536 x 384 fp16 with GELU, gather included:
+// 33.3 us, 32.9 with that loop rolled up).
+enum Tc2Out {
+  kOutTma = 0,               // aligned rows of y, by TMA
+  kOutRows = 1,              // rows of any alignment
+  kOutResidual = 2,          // with a residual, rows of any alignment
+};
+
+// Q8: A and W' in e4m3 with scales, else 16-bit of type DT.
+template <int BN, int DT, int EPI, bool GATHER, bool Q8, int OUT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads2, 1)
 gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
                 const __grid_constant__ CUtensorMap tmap_bh,
                 const __grid_constant__ CUtensorMap tmap_a,
                 const __grid_constant__ CUtensorMap tmap_y, const Tc2Params p) {
   using C = Tc2Cfg<BN>;
+  constexpr bool RES = OUT == kOutResidual;
   constexpr int kHalfN = C::kHalfN;
   constexpr int kCols = atom_cols<Q8>();              // columns of one k atom
   static_assert(!(Q8 && GATHER), "the in-kernel gather moves 16-bit elements");
@@ -638,7 +648,7 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
         const int64_t n_base = n_chunk + h * 32;
         if (h == 0) {
           // The staging tile's previous TMA store must have read it.
-          if (p.y_tma && lane == 0) bulk_wait_group_read<0>();
+          if ((OUT == kOutTma || p.y_tma) && lane == 0) bulk_wait_group_read<0>();
           __syncwarp();
           if constexpr (RES) {
             tile.put(rt, p.res_align);
@@ -650,7 +660,7 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
           scale32(f, row_scale, p.w_scale, n_base, p.N);
           bias_activate32<DT, EPI>(f, p.bias, n_base, p.N);
         } else {
-          if (p.bias) add_bias32<DT>(f, p.bias, n_base, p.N);
+          if (p.bias) add_bias32<DT, RES>(f, p.bias, n_base, p.N);
           activate32<EPI>(f);
         }
         if constexpr (RES) {
@@ -662,7 +672,7 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
 #pragma unroll
         for (int j = 0; j < 16; ++j) packed[j] = Elem<DT>::pack2(f[2 * j], f[2 * j + 1]);
         tile.set_own_row(packed, h);      // the 128-byte swizzle that the TMA store reads
-        if (p.y_tma) {
+        if (OUT == kOutTma || p.y_tma) {
           if (h == 1) {
             fence_proxy_async_smem();    // staging writes -> visible to the TMA unit
             __syncwarp();
@@ -855,20 +865,20 @@ cudaError_t launch_tc2_bn(int dtype, Tc2Params& p, const void* a, int64_t M, int
   }
 
   const bool bf = dtype == GW_DTYPE_BF16;
-#define GW_TC2_KERN(G, Q, R)                                                    \
+#define GW_TC2_KERN(G, Q, O)                                                    \
   (p.epi == GW_EPI_GELU_ERF                                                     \
-       ? (bf ? gemm_tc2_kernel<BN, GW_DTYPE_BF16, GW_EPI_GELU_ERF, G, Q, R>     \
-             : gemm_tc2_kernel<BN, GW_DTYPE_F16, GW_EPI_GELU_ERF, G, Q, R>)     \
+       ? (bf ? gemm_tc2_kernel<BN, GW_DTYPE_BF16, GW_EPI_GELU_ERF, G, Q, O>     \
+             : gemm_tc2_kernel<BN, GW_DTYPE_F16, GW_EPI_GELU_ERF, G, Q, O>)     \
    : p.epi == GW_EPI_GELU_TANH                                                  \
-       ? (bf ? gemm_tc2_kernel<BN, GW_DTYPE_BF16, GW_EPI_GELU_TANH, G, Q, R>    \
-             : gemm_tc2_kernel<BN, GW_DTYPE_F16, GW_EPI_GELU_TANH, G, Q, R>)    \
-       : (bf ? gemm_tc2_kernel<BN, GW_DTYPE_BF16, GW_EPI_NONE, G, Q, R>         \
-             : gemm_tc2_kernel<BN, GW_DTYPE_F16, GW_EPI_NONE, G, Q, R>))
-  const bool gather = p.ghdr != nullptr;
-  auto kern = p.res ? (q8 ? GW_TC2_KERN(false, true, true)
-                       : gather ? GW_TC2_KERN(true, false, true) : GW_TC2_KERN(false, false, true))
-                    : (q8 ? GW_TC2_KERN(false, true, false)
-                       : gather ? GW_TC2_KERN(true, false, false) : GW_TC2_KERN(false, false, false));
+       ? (bf ? gemm_tc2_kernel<BN, GW_DTYPE_BF16, GW_EPI_GELU_TANH, G, Q, O>    \
+             : gemm_tc2_kernel<BN, GW_DTYPE_F16, GW_EPI_GELU_TANH, G, Q, O>)    \
+       : (bf ? gemm_tc2_kernel<BN, GW_DTYPE_BF16, GW_EPI_NONE, G, Q, O>         \
+             : gemm_tc2_kernel<BN, GW_DTYPE_F16, GW_EPI_NONE, G, Q, O>))
+#define GW_TC2_OUT(O)                                                           \
+  (q8 ? GW_TC2_KERN(false, true, O)                                             \
+      : p.ghdr ? GW_TC2_KERN(true, false, O) : GW_TC2_KERN(false, false, O))
+  auto kern = p.res ? GW_TC2_OUT(kOutResidual) : p.y_tma ? GW_TC2_OUT(kOutTma) : GW_TC2_OUT(kOutRows);
+#undef GW_TC2_OUT
 #undef GW_TC2_KERN
   cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kern), C::kSmemBytes);
   if (e != cudaSuccess) return e;
