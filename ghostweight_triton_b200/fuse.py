@@ -54,14 +54,14 @@ def _epilogue_of(act: nn.Module) -> str | None:
     return _ACT_BY_CLASS.get(type(act).__name__)
 
 
-def _plan_key(dtype: torch.dtype, *tensors: torch.Tensor | None) -> tuple:
-    """What packed operands are made from: the tensors themselves (held, so that none of
-    them can be freed and another take its address), their versions and storage."""
-    return (dtype, *((t, t._version, t.data_ptr()) for t in tensors if t is not None))
+def _plan_key(form: tuple, *tensors: torch.Tensor | None) -> tuple:
+    """What packed operands are made for and from: the tensors themselves (held, so that none
+    of them can be freed and another take its address), their versions and storage."""
+    return (form, *((t, t._version, t.data_ptr()) for t in tensors if t is not None))
 
 
 def _same_key(a: tuple, b: tuple) -> bool:
-    return (len(a) == len(b) and a[0] is b[0]
+    return (len(a) == len(b) and a[0] == b[0]
             and all(u[0] is v[0] and u[1:] == v[1:] for u, v in zip(a[1:], b[1:])))
 
 
@@ -78,15 +78,17 @@ class _Plan:
         self.operands = operands
         self.tensors = [t for o in operands for t in (o if isinstance(o, tuple) else (o,)) if t is not None]
         self.device = self.tensors[0].device
-        self.stream = _native._stream(self.device)
+        self.streams = {_native._stream(self.device)}      # that the operands are ordered on
         self.built = torch.cuda.current_stream(self.device).record_event()
 
     def take(self) -> tuple:
-        if _native._stream(self.device) != self.stream and not _native._capturing():
+        raw = _native._stream(self.device)
+        if raw not in self.streams and not _native._capturing():
             stream = torch.cuda.current_stream(self.device)
             stream.wait_event(self.built)
             for t in self.tensors:
                 t.record_stream(stream)
+            self.streams.add(raw)
         return self.operands
 
 
@@ -99,6 +101,8 @@ class GhostMLPChain(nn.Module):
     rebuilt when a weight or a mask changes. A captured graph reads the operands of
     the call that it captured: capture again after a change.
     """
+
+    precision = "input"                              # of the operands; GhostPreNormMLP has a choice
 
     def __init__(self, fc: GhostLinear, proj: GhostLinear, activation: str,
                  dropout: nn.Module | None = None):
@@ -122,7 +126,7 @@ class GhostMLPChain(nn.Module):
     def _operands(self, dtype: torch.dtype) -> tuple:
         """(w_fc, b_fc, w_proj) as the products take them, for activations of `dtype`."""
         fc, proj = self.fc, self.proj
-        key = _plan_key(dtype, fc.weight, proj.weight, fc._frozen_indices, proj._frozen_indices, fc.bias)
+        key = _plan_key((dtype, self.precision), fc.weight, proj.weight, fc._frozen_indices, proj._frozen_indices, fc.bias)
         if self._plan is not None and _same_key(self._plan.key, key):
             return self._plan.take()
         with torch.no_grad():
@@ -194,6 +198,8 @@ class GhostPreNormMLP(GhostMLPChain):
     the input's type.
     """
 
+    _norm_known = False                              # tried by _try_norm
+
     def __init__(self, norm: nn.Module, fc: GhostLinear, proj: GhostLinear, activation: str,
                  dropout: nn.Module | None = None, precision: str = "input"):
         super().__init__(fc, proj, activation, dropout)
@@ -207,7 +213,6 @@ class GhostPreNormMLP(GhostMLPChain):
             f"norm must be over fc's {fc.in_features} input features")
         self.norm = norm
         self.precision = precision
-        self._norm_known = False
         if weight is None or not weight.is_meta:
             self._try_norm()
 

@@ -463,3 +463,18 @@ def test_writes_into_given_tensors_are_seen(name):
         inner = torch.empty(M, N, dtype=torch.float16, device="cuda")
         write(inner)
         assert torch.equal(inner, leaf)
+
+
+def test_precision_and_type_change_between_calls():
+    """A block whose precision or input type changes packs what that form needs."""
+    m = block(128, 256, torch.float16, 41)
+    forms = [("input", torch.float16), ("e4m3", torch.float16), ("e4m3", torch.bfloat16), ("input", torch.bfloat16)]
+    want = {}
+    with torch.no_grad():
+        for precision, dtype in forms:
+            twin = copy.deepcopy(m)
+            twin.precision = precision
+            want[precision, dtype] = twin(*inputs(9, 128, dtype, 41))
+        for precision, dtype in forms + forms[::-1] + forms[::2]:
+            m.precision = precision
+            assert torch.equal(m(*inputs(9, 128, dtype, 41)), want[precision, dtype])
