@@ -385,20 +385,24 @@ cudaError_t launch_dense_gemm(const void* a, int dtype, int64_t M, int64_t K, in
                               const gw::Residual& res = {}, const gw::QScale& qs = {}) {
   // The plans count 128-byte k-blocks: two e4m3 columns stand for one of 16 bits.
   const GemmChoice c = choose_gemm(M, N, qs.a ? (K + 1) / 2 : K, d);
-  if (c.kernel == GW_KERNEL_PAIR)
-    return gw::launch_gemm_tc2(a, dtype, M, K, lda, w, N, ldw, bias, epilogue, y, ldy,
-                               d->err_word, d->sm_count, s, peers, n_peers, a_cols, a_width, nullptr,
-                               nullptr, res, qs);
   cudaError_t e;
-  if (c.kernel == GW_KERNEL_DECODE)
+  if (c.kernel == GW_KERNEL_PAIR) {
+    // Its peer stores ride on the TMA stores of y, which rows of 16-byte units need.
+    const int fused = N % 8 == 0 ? n_peers : 0;
+    e = gw::launch_gemm_tc2(a, dtype, M, K, lda, w, N, ldw, bias, epilogue, y, ldy,
+                            d->err_word, d->sm_count, s, fused ? peers : nullptr, fused, a_cols, a_width,
+                            nullptr, nullptr, res, qs);
+    if (fused) return e;
+  } else if (c.kernel == GW_KERNEL_DECODE) {
     e = gw::launch_gemm_decode(c.dp, a, dtype, M, K, lda, w, N, ldw, bias, epilogue, y, ldy,
                                d->err_word, s, a_cols, a_width, res, qs);
-  else if (c.kernel == GW_KERNEL_SPLITK)
+  } else if (c.kernel == GW_KERNEL_SPLITK) {
     e = gw::launch_gemm_splitk(c.sk, a, dtype, M, K, lda, w, N, ldw, bias, epilogue, y, ldy,
                                d->err_word, s, a_cols, a_width, res, qs);
-  else
+  } else {
     e = gw::launch_gemm_tc(0, a, dtype, M, a_cols ? a_width : K, lda, w, N, ldw, nullptr, K, bias,
                            epilogue, y, ldy, d->err_word, d->sm_count, s, a_cols, nullptr, res, qs);
+  }
   if (e != cudaSuccess || n_peers == 0) return e;
   return gw::launch_copy_to_peers(y, M, N, ldy, peers, n_peers, d->sm_count, s);
 }

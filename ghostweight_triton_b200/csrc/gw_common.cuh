@@ -159,8 +159,9 @@ __device__ __forceinline__ void fence_proxy_async_smem() {
 
 // 2-D tile store shared -> global through the TMA unit, tracked by the
 // thread's bulk async-group. x * sizeof(elem) must be a multiple of 16 bytes
-// and x, y non-negative; elements outside the tensor map's extent are not
-// written.
+// and x, y non-negative; rows outside the tensor map's extent and columns from
+// the next 16-byte boundary behind it on are not written. The columns up to that
+// boundary are: an inner extent that is no multiple of 16 bytes acts as the next one.
 __device__ __forceinline__ void tma_store_2d(const void* tmap, uint32_t src, int32_t x, int32_t y) {
   asm volatile(
       "cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"

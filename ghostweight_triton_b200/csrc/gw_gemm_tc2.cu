@@ -13,7 +13,7 @@
 //     to free their stages and publish finished accumulators;
 //   * each CTA's four epilogue warps drain its own TMEM (bias, GELU, one
 //     rounding) into swizzled staging tiles that the TMA unit stores to y (the
-//     warps themselves where y's rows are not 16-byte aligned),
+//     warps themselves where y's rows are not whole 16-byte units),
 //     and arrive on the leader's accumulator-empty barrier (remote arrive for
 //     the second CTA) as soon as their TMEM reads are done;
 //   * launch_dependents right after the prologue lets the next kernel of the
@@ -98,7 +98,7 @@ struct Tc2Params {
   const uint16_t* bias;
   int epi;
   int y_vec_ok;
-  int y_tma;                 // y stored through tmap_y (16-byte aligned rows)
+  int y_tma;                 // y stored through tmap_y (rows of whole 16-byte units)
   uint16_t* y;
   int64_t ldy;
   const uint16_t* res;      // residual (or null), leading dimension ldr
@@ -369,7 +369,7 @@ __device__ __forceinline__ void gather_units(const Tc2Params& p, int e, int lane
 // it 0.2 to 0.4 us behind a gather (8192 x 1536 x 384 fp16 with GELU, gather included:
 // 33.3 us, 32.9 with that loop rolled up).
 enum Tc2Out {
-  kOutTma = 0,               // aligned rows of y, by TMA
+  kOutTma = 0,               // rows of whole 16-byte units, by TMA
   kOutRows = 1,              // rows of any alignment
   kOutResidual = 2,          // with a residual, rows of any alignment
 };
@@ -835,8 +835,10 @@ cudaError_t launch_tc2_bn(int dtype, Tc2Params& p, const void* a, int64_t M, int
     return cudaErrorInvalidValue;
   if (!make_tmap_kmajor(&tb, w, N, K, ldw, kb_cols, C::kHalfN, eb)) return cudaErrorInvalidValue;
   tbh = tb;                  // read only by half jobs (set below)
-  // TMA-store epilogue when y's rows are 16-byte aligned (else direct stores).
-  p.y_tma = p.y_vec_ok && make_tmap_kmajor(&ty, y, M, N, ldy, kEpiCols, 32) ? 1 : 0;
+  // TMA-store epilogue when y's rows are 16-byte aligned and end on such a boundary
+  // (a TMA store writes whole 16-byte units, also over what stands behind a row of N
+  // columns), else the warps' own stores.
+  p.y_tma = p.y_vec_ok && N % 8 == 0 && make_tmap_kmajor(&ty, y, M, N, ldy, kEpiCols, 32) ? 1 : 0;
   if (!p.y_tma) ty = ta;     // not read by the kernel
   p.res_align = row_alignment(p.res, p.ldr);
   if (p.n_peers > 0 && !p.y_tma) return cudaErrorInvalidValue;   // peer stores ride the TMA path

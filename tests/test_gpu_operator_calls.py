@@ -478,3 +478,33 @@ def test_precision_and_type_change_between_calls():
         for precision, dtype in forms + forms[::-1] + forms[::2]:
             m.precision = precision
             assert torch.equal(m(*inputs(9, 128, dtype, 41)), want[precision, dtype])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,N", [(1, 1214), (20, 1526), (300, 1001), (1600, 2878), (2056, 1214), (2100, 4093), (4097, 767)])
+def test_nothing_is_written_beside_the_output(M, N, dtype):
+    """Outputs in aligned rows with a gap behind them: the gap keeps its values, where a row ends
+    inside a 16-byte unit too."""
+    K = 130
+    x, w, idx = operands(M, N, K, dtype)
+    res = torch.randn(M, N, device="cuda").to(dtype)
+    qa, qw = quantize_rows(x), quantize_rows(w)
+    calls = [lambda r, out: ghost_linear(x, w, idx, residual=r, out=out),
+             lambda r, out: ghost_linear_dev(x, pack_weight(w, idx).as_strided((N, 192), (192, 1)), idx,
+                                             torch.tensor([K], dtype=torch.int32, device="cuda"), residual=r, out=out)]
+    if dtype is not torch.float32:
+        calls += [lambda r, out, s=s: ghost_linear(x, w, idx, residual=r, out=out, strategy=s) for s in ("fused", "overlap")]
+        calls += [lambda r, out: packed_linear(x, w, residual=r, out=out),
+                  lambda r, out: packed_linear_q8(*qa, *qw, residual=r, dtype=dtype, out=out)]
+    ld = (N + 7) // 8 * 8
+    for call in calls:
+        for pad in (0, 8) if ld > N else (8,):
+            for r in (None, res, "in place"):
+                buf = torch.full((M + 1, ld + pad), 5.0, dtype=dtype, device="cuda")
+                out = buf[:M, :N]
+                if r == "in place":
+                    out.copy_(res)
+                want = call(res if r == "in place" else r, None)
+                call(out if r == "in place" else r, out)
+                assert torch.equal(out, want)
+                assert bool((buf[:, N:] == 5).all()) and bool((buf[M] == 5).all())
