@@ -11,7 +11,7 @@ import pytest
 import torch
 import torch.nn as nn
 
-from ghostweight_triton_b200 import GhostLinear
+from ghostweight_triton_b200 import GhostLinear, _native
 from ghostweight_triton_b200.fuse import GhostMLPChain, GhostPreNormMLP
 from ghostweight_triton_b200.kernels.gather import pack_weight
 from ghostweight_triton_b200.kernels.matmul import (ghost_linear, ghost_linear_dev, ghost_linear_pipelined,
@@ -508,3 +508,23 @@ def test_nothing_is_written_beside_the_output(M, N, dtype):
                 call(out if r == "in place" else r, out)
                 assert torch.equal(out, want)
                 assert bool((buf[:, N:] == 5).all()) and bool((buf[M] == 5).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("M,N", [(1, 300), (20, 1526), (300, 1001), (700, 4096), (1600, 2880), (2056, 1214)])
+def test_nothing_behind_the_operands_columns_counts(M, N, dtype):
+    """NaN behind the last column of both operands, inside the same 16-byte unit and behind it, and in
+    the workspace that the gathered columns of x pass through."""
+    for K in (1, 63, 130, 333):
+        ld = (K + 7) // 8 * 8 + 8
+        a = torch.full((M, ld), float("nan"), dtype=dtype, device="cuda")[:, :K]
+        w = torch.full((N, ld), float("nan"), dtype=dtype, device="cuda")[:, :K]
+        a.copy_(torch.randn(M, K, device="cuda"))
+        w.copy_(torch.randn(N, K, device="cuda") / K ** 0.5)
+        check(packed_linear(a, w), a, w, None, None, None)
+        idx = torch.arange(K, device="cuda")
+        for strategy in ("pregather", "overlap", "fused", "auto"):
+            for ws in _native._gemm_ws.values():
+                ws[4096:].fill_(0xFF)                # behind the header: NaN in both types
+            x = a.contiguous()
+            check(ghost_linear(x, w, idx, strategy=strategy), a, w, None, None, None)
