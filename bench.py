@@ -183,6 +183,16 @@ class NearGpu:
         return f"{len(self.cpus)} CPUs NVML reports nearest the GPU (of {len(self.prev or self.cpus)} allowed)"
 
 
+def emit(line: dict, extra: dict) -> None:
+    """One JSON line on stdout. The sweep's points (17 KB of 24) go to stderr, as a JSON line of
+    their own: where only the end of a log is kept, they pushed the start of the line out of it."""
+    extra = dict(extra)
+    points = extra.pop("sweep", None)
+    if points is not None:
+        print(json.dumps({"sweep": points}), file=sys.stderr, flush=True)
+    print(json.dumps({**line, **extra}), flush=True)
+
+
 def dist_setup(args):
     world = int(os.environ.get("WORLD_SIZE", "1"))
     rank = int(os.environ.get("RANK", "0"))
@@ -974,8 +984,7 @@ def run_ours(args, world, rank, local):
                          "overlap": "overlap (one launch: the pair GEMM's epilogue warps gather x' while "
                                     "its MMAs run)"}[args.strategy],
         }
-        line.update(extra)
-        print(json.dumps(line), flush=True)
+        emit(line, extra)
 
 
 # ---------------------------------------------------------------------------- ours: sharded MLP

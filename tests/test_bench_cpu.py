@@ -55,3 +55,14 @@ def test_reference_arm_line():
     assert line["impl"] == "reference" and line["steps"] == 2 and line["warmup"] == 3
     assert line["e2e"]["h2d_bytes_per_step"] == 0 and line["e2e"]["value"] == line["value"]
     assert line["cpu_baseline"]["kind"] == "port" and line["value"] > 0
+
+
+def test_sweep_points_leave_the_line(capsys):
+    """stdout holds one JSON line without the sweep's points, which stand on stderr."""
+    points = [{"M": m, "us": 1.0} for m in range(500)]
+    _bench().emit({"metric": "m", "value": 1.0}, {"sweep": points, "kernels": {"k": 2}})
+    out, err = capsys.readouterr()
+    assert json.loads(out) == {"metric": "m", "value": 1.0, "kernels": {"k": 2}} and out.count("\n") == 1
+    assert json.loads(err) == {"sweep": points}
+    _bench().emit({"metric": "m"}, {})
+    assert json.loads(capsys.readouterr().out) == {"metric": "m"}
