@@ -27,8 +27,15 @@
 // fp16 with residual, half alive, 19.6 us, 93%; all columns 20.2 us, 103%; 8192 x
 // 8192 bf16 with residual to e4m3, 30% alive, 73.8 us, 89%; 1537 x 11008 bf16
 // rounded 11.1 us, 71%.
-// Rows of odd length run at a third of it (4096 x 4097 bf16: 52 us): their 2-byte
-// accesses make instructions the limit.
+// Rows of odd length run at a third to a half of it (4096 x 4097 bf16 with residual:
+// 52 us half alive, 41 us full): their 2-byte accesses make instructions the limit.
+// What rows_any_kernel takes (of these, the ones of more than 16384 columns) is read
+// again for each pass, at a quarter: 1024 x 20001 bf16 with residual 96 us half
+// alive, 108 us full, 120 us half alive to e4m3.
+//
+// No kernel here lets the next one of the stream start before it has finished
+// (griddepcontrol.launch_dependents): the products request W' before they wait for
+// the previous kernel, and W' may be what gw_quantize_rows has just written.
 #include <algorithm>
 #include <type_traits>
 

@@ -15,8 +15,10 @@ columns of the second weight are zero. The fused chain therefore
 
 ``GhostPreNormMLP`` puts the residual stream and the root-mean-square norm in
 front of the same chain, so that a whole pre-norm MLP block is three launches
-(five in e4m3): the residual's addition, the norm and the first layer's gather
-are one kernel, and the second addition is the last GEMM's epilogue.
+(four in e4m3, where the hidden rows are rounded by one of their own): the
+residual's addition, the norm and the first layer's gather are one kernel, and
+the second addition is the last GEMM's epilogue. Parameters of another type than
+the input's add a cast of the norm's weight and one of proj's bias to each call.
 
 One gather launch and the dead part of the first GEMM disappear; the result
 equals the unfused chain's (the skipped terms are products with zero weights),

@@ -428,7 +428,8 @@ GW_API int gw_rms_norm_q8(const void* x, int dtype, int64_t rows, int64_t cols, 
  * y[m, j] = x[m, idx[j]] (idx NULL: all columns). With x = nn.Linear.weight
  * [N, K] it packs W[:, alive] for gw_packed_gemm_q8, with x an activation it
  * makes that product's other operand. Entries of x outside the list are not
- * looked at.
+ * looked at. As after the 16-bit weight packs, a product with the packed weight
+ * may follow as the next call on the stream.
  */
 GW_API int gw_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx,
                             const int64_t* idx, int64_t n_idx, void* q, int64_t ldq,
