@@ -192,15 +192,13 @@ class GhostPreNormMLP(GhostMLPChain):
     ``norm`` is a root-mean-square norm over fc's input features (torch.nn.RMSNorm,
     or a module with ``weight`` and ``eps`` or ``variance_epsilon`` that computes
     x * rsqrt(mean(x^2) + eps) * weight: two rows are tried when the block is built,
-    at its first forward if the norm is on the meta device then), ``fc`` and ``proj`` are GhostLinears with frozen masks, joined by the GELU ``activation``
+    or in its next forward if the norm is on the meta device then or replaced later), ``fc`` and ``proj`` are GhostLinears with frozen masks, joined by the GELU ``activation``
     ("gelu" or "gelu_tanh"); all stay registered, so parameters and state-dict
     keys are theirs. fp16 and bf16 inputs. ``precision="e4m3"`` runs both
     products on e4m3 operands (weights rounded once with a scale per feature,
     activations with one per token), with fp32 sums and the residual stream in
     the input's type.
     """
-
-    _norm_known = False                              # tried by _try_norm
 
     def __init__(self, norm: nn.Module, fc: GhostLinear, proj: GhostLinear, activation: str,
                  dropout: nn.Module | None = None, precision: str = "input"):
@@ -223,6 +221,11 @@ class GhostPreNormMLP(GhostMLPChain):
         # None: torch.nn.RMSNorm's default, the epsilon of the type it norms 16-bit rows in.
         return torch.finfo(torch.float32).eps if eps is None else float(eps)
 
+    @property
+    def _norm_known(self) -> bool:
+        """Whether the present norm has been tried."""
+        return self.__dict__.get("_tried") is self.norm
+
     def _try_norm(self) -> None:
         """Assert that a copy of the norm in fp32, with a gain of its own, computes what rms_norm does,
         of a row of ordinary values whose mean is not zero and of one so small that eps counts."""
@@ -243,7 +246,7 @@ class GhostPreNormMLP(GhostMLPChain):
         except Exception as e:
             raise AssertionError("norm must take rows of fc's input features") from e
         assert same, "norm must compute x * rsqrt(mean(x^2) + eps) * weight"
-        self._norm_known = True
+        self.__dict__["_tried"] = self.norm          # not a second submodule
 
     def _pack(self, dtype: torch.dtype) -> tuple:
         if self.precision != "e4m3":

@@ -528,3 +528,21 @@ def test_nothing_behind_the_operands_columns_counts(M, N, dtype):
                 ws[4096:].fill_(0xFF)                # behind the header: NaN in both types
             x = a.contiguous()
             check(ghost_linear(x, w, idx, strategy=strategy), a, w, None, None, None)
+
+
+def test_a_replaced_norm_is_tried():
+    m = block(128, 256, torch.float16, 31)
+    keys = set(m.state_dict())
+    x, r = inputs(4, 128, torch.float16, 31)
+    with torch.no_grad():
+        m(x, residual=r)
+        norm = m.norm
+        m.norm = OnePlusWeight(128).cuda()
+        with pytest.raises(AssertionError, match="norm must"):
+            m(x, residual=r)
+        m.norm = nn.RMSNorm(128, eps=1e-3, device="cuda", dtype=torch.float16)
+        check_block(m(x, residual=r), m, x, r, 1e-3)
+        m.norm = norm
+        for other in (m, copy.deepcopy(m)):
+            check_block(other(x, residual=r), m, x, r, 1e-5)
+            assert set(other.state_dict()) == keys
