@@ -546,3 +546,17 @@ def test_a_replaced_norm_is_tried():
         for other in (m, copy.deepcopy(m)):
             check_block(other(x, residual=r), m, x, r, 1e-5)
             assert set(other.state_dict()) == keys
+
+
+@pytest.mark.parametrize("M,N", [(300, 1214), (2056, 1214), (2056, 1216), (2100, 4093)])
+def test_peer_copies_end_with_the_row(M, N):
+    """The output and its copies in other buffers (here on the same GPU), rows that end inside a
+    16-byte unit included: nothing behind them is written in any."""
+    K = 130
+    x, w, idx = operands(M, N, K)
+    ld = (N + 7) // 8 * 8 + 8
+    bufs = [torch.full((M, ld), 5.0, dtype=x.dtype, device="cuda") for _ in range(3)]
+    want = ghost_linear(x, w, idx)
+    _native.gather_gemm_peers(x, w, idx, bufs[0][:, :N], [b.data_ptr() for b in bufs[1:]], strategy="pregather")
+    for b in bufs:
+        assert torch.equal(b[:, :N], want) and bool((b[:, N:] == 5).all())
