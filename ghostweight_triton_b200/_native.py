@@ -210,6 +210,10 @@ except AttributeError:  # pragma: no cover - older torch
     _raw_stream = None
 
 
+# The raw cudaStream_t of torch's current stream of a device index.
+current_raw_stream = _raw_stream or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
 try:  # torch.cuda.is_current_stream_capturing without its wrapper
     _capturing = torch._C._cuda_isCurrentStreamCapturing
 except AttributeError:  # pragma: no cover - older torch

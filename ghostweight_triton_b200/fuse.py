@@ -37,7 +37,7 @@ import torch.nn as nn
 
 from ghostweight_triton_b200 import _native
 from ghostweight_triton_b200.kernels.gather import pack_weight
-from ghostweight_triton_b200.kernels._args import refuse_grad
+from ghostweight_triton_b200.kernels._args import Kept, refuse_grad
 from ghostweight_triton_b200.kernels.matmul import ghost_linear, packed_linear, packed_linear_q8
 from ghostweight_triton_b200.kernels.norm import pack_weight_q8, quantize_rows, rms_norm, rms_norm_q8
 from ghostweight_triton_b200.module import GhostLinear
@@ -67,30 +67,16 @@ def _same_key(a: tuple, b: tuple) -> bool:
             and all(u[0] is v[0] and u[1:] == v[1:] for u, v in zip(a[1:], b[1:])))
 
 
-class _Plan:
-    """Packed operands kept between calls, with the tensors they were made from (the key).
-
-    Built on one stream and used on any: another stream waits for the build, and the
-    allocator for that stream's work before it hands the memory out again. A capture
-    takes them as they are (it starts when the device is idle).
-    """
+class _Plan(Kept):
+    """Packed operands kept between calls, with the tensors they were made from (the key)."""
 
     def __init__(self, key: tuple, operands: tuple):
+        super().__init__(t for o in operands for t in (o if isinstance(o, tuple) else (o,)) if t is not None)
         self.key = key
         self.operands = operands
-        self.tensors = [t for o in operands for t in (o if isinstance(o, tuple) else (o,)) if t is not None]
-        self.device = self.tensors[0].device
-        self.streams = {_native._stream(self.device)}      # that the operands are ordered on
-        self.built = torch.cuda.current_stream(self.device).record_event()
 
     def take(self) -> tuple:
-        raw = _native._stream(self.device)
-        if raw not in self.streams and not _native._capturing():
-            stream = torch.cuda.current_stream(self.device)
-            stream.wait_event(self.built)
-            for t in self.tensors:
-                t.record_stream(stream)
-            self.streams.add(raw)
+        self.on_this_stream()
         return self.operands
 
 
@@ -192,9 +178,10 @@ class GhostPreNormMLP(GhostMLPChain):
     ``norm`` is a root-mean-square norm over fc's input features (torch.nn.RMSNorm,
     or a module with ``weight`` and ``eps`` or ``variance_epsilon`` that computes
     x * rsqrt(mean(x^2) + eps) * weight: two rows are tried when the block is built,
-    or in its next forward if the norm is on the meta device then or replaced later), ``fc`` and ``proj`` are GhostLinears with frozen masks, joined by the GELU ``activation``
-    ("gelu" or "gelu_tanh"); all stay registered, so parameters and state-dict
-    keys are theirs. fp16 and bf16 inputs. ``precision="e4m3"`` runs both
+    or in its next forward if the norm is on the meta device then or replaced later),
+    ``fc`` and ``proj`` are GhostLinears with frozen masks, joined by the GELU
+    ``activation`` ("gelu" or "gelu_tanh"); all stay registered, so parameters and
+    state-dict keys are theirs. fp16 and bf16 inputs. ``precision="e4m3"`` runs both
     products on e4m3 operands (weights rounded once with a scale per feature,
     activations with one per token), with fp32 sums and the residual stream in
     the input's type.

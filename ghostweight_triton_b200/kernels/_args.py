@@ -4,6 +4,8 @@ from __future__ import annotations
 
 import torch
 
+from ghostweight_triton_b200 import _native
+
 
 def refuse_grad(**tensors: torch.Tensor | None) -> None:
     """Raise if a tensor would need a gradient that the operator cannot give."""
@@ -24,6 +26,29 @@ def refuse_grad_out(what: str, out: torch.Tensor) -> None:
 # Called for every given tensor that a kernel has written: the autograd engine and the
 # caches of packed weights see the write by the tensor's version.
 written = torch.autograd.graph.increment_version
+
+
+class Kept:
+    """Tensors that one call makes and later calls use again, on any stream: another stream
+    than theirs waits until they are made, and the allocator for that stream's work before it
+    hands their memory out again. A capture takes them as they are (it starts when the device
+    is idle).
+    """
+
+    def __init__(self, tensors):
+        self.tensors = list(tensors)
+        self.device = self.tensors[0].device
+        self.streams = {_native._stream(self.device)}      # that the tensors are ordered on
+        self.made = torch.cuda.current_stream(self.device).record_event()
+
+    def on_this_stream(self) -> None:
+        raw = _native._stream(self.device)
+        if raw not in self.streams and not _native._capturing():
+            stream = torch.cuda.current_stream(self.device)
+            stream.wait_event(self.made)
+            for t in self.tensors:
+                t.record_stream(stream)
+            self.streams.add(raw)
 
 
 def rows(t: torch.Tensor, cols: int) -> torch.Tensor:

@@ -36,7 +36,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from ghostweight_triton_b200 import _native
-from ghostweight_triton_b200.kernels._args import residual_matrix
+from ghostweight_triton_b200.kernels._args import Kept, residual_matrix
 from ghostweight_triton_b200.kernels.gather import pack_weight, pack_weight_dev
 from ghostweight_triton_b200.kernels.mask import dead_neuron_mask_compact, alive_indices as _alive
 from ghostweight_triton_b200.kernels.matmul import ghost_linear, ghost_linear_dev, index_runs
@@ -154,9 +154,9 @@ class GhostLinear(nn.Module):
         self.register_buffer("_frozen_indices", None)
         self._mask_frozen: bool = False
         self._last_sparsity: float = 0.0
-        # (key, packed weight) for the frozen index list; rebuilt when the
-        # weight, its dtype/device or the index list changes.
-        self._packed: tuple[tuple, torch.Tensor] | None = None
+        # (key, packed weight, its streams) for the frozen index list; rebuilt when
+        # the weight, its dtype/device or the index list changes.
+        self._packed: tuple[tuple, torch.Tensor, Kept] | None = None
         # (key, whether the frozen list is made of 64-column runs), same key rule.
         self._runs: tuple | None = None
         # Dynamic mode without host synchronisation (see the module docstring).
@@ -215,6 +215,10 @@ class GhostLinear(nn.Module):
             ghost.bias = conv.bias
         return ghost
 
+    def __getstate__(self):
+        # Copies pack their own operands (what is kept holds addresses and events).
+        return {k: None if k in ("_packed", "_fast") else v for k, v in self.__dict__.items()}
+
     # ------------------------------------------------------------------ forward
     def _weight_packed(self, alive: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
         """W' for the frozen list, rebuilt when the weight (object, storage or an
@@ -226,11 +230,12 @@ class GhostLinear(nn.Module):
             k = c[0]
             if (k[0] is w and k[1] == w._version and k[2] == w.data_ptr() and k[3] is alive
                     and k[4] == alive._version and k[5] is dtype):
+                c[2].on_this_stream()
                 return c[1]
         packed = pack_weight(w.detach(), alive, dtype=dtype)
         # Under graph capture the packing is only recorded, into the graph's own memory: not kept.
         if not torch.cuda.is_current_stream_capturing():
-            self._packed = ((w, w._version, w.data_ptr(), alive, alive._version, dtype), packed)
+            self._packed = ((w, w._version, w.data_ptr(), alive, alive._version, dtype), packed, Kept([packed]))
         return packed
 
     def _alive_runs(self, alive: torch.Tensor) -> bool:
@@ -261,14 +266,16 @@ class GhostLinear(nn.Module):
         fast = d.get("_fast")
         if fast is not None:
             (dtype, w, wv, wp, b, bv, bp, alive, av, act, min_sp, in_f, out_f,
-             w_packed, bias_c, prep, sparsity) = fast
+             w_packed, bias_c, prep, sparsity, kept) = fast
             params = d["_parameters"]
             if (x.dtype is dtype and d["_mask_frozen"] and d["_buffers"]["_frozen_indices"] is alive
                     and alive._version == av and params["weight"] is w and w._version == wv
                     and w.data_ptr() == wp and params.get("bias") is b
                     and (b is None or (b._version == bv and b.data_ptr() == bp))
                     and d.get("activation") == act and d["min_sparsity_to_activate"] == min_sp
-                    and x.is_cuda and x.get_device() == torch.cuda.current_device()):
+                    and x.is_cuda and x.get_device() == _native._current_device()):
+                if _native.current_raw_stream(x.get_device()) not in kept.streams:
+                    kept.on_this_stream()
                 shape = x.shape
                 x_2d = x.reshape(-1, in_f)
                 if not x_2d.is_contiguous():
@@ -329,7 +336,7 @@ class GhostLinear(nn.Module):
                     alive, alive._version, self.activation, self.min_sparsity_to_activate,
                     self.in_features, self.out_features, w_packed, bias,
                     _native.prepare_gather_gemm(w_packed, alive, bias, self.activation, strategy, x_2d.dtype),
-                    float(sparsity))
+                    float(sparsity), Kept([w_packed] if bias is None else [w_packed, bias]))
         return out.reshape(*orig_shape[:-1], self.out_features)
 
     def _residual_2d(self, residual: torch.Tensor, x: torch.Tensor, x_2d: torch.Tensor) -> torch.Tensor:

@@ -560,3 +560,50 @@ def test_peer_copies_end_with_the_row(M, N):
     _native.gather_gemm_peers(x, w, idx, bufs[0][:, :N], [b.data_ptr() for b in bufs[1:]], strategy="pregather")
     for b in bufs:
         assert torch.equal(b[:, :N], want) and bool((b[:, N:] == 5).all())
+
+
+@pytest.mark.parametrize("bias_type", [torch.float16, torch.float32])
+@pytest.mark.parametrize("M", [2, 40, 600])
+def test_layer_used_at_once_on_two_streams(M, bias_type):
+    """A frozen layer's packed weight (and its bias in x's type), made on one stream behind other work
+    and used at once on a second one; the next calls alternate."""
+    K, N, dt = 512, 768, torch.float16
+    g = torch.Generator(device="cuda").manual_seed(M)
+    x, r = torch.randn(M, K, generator=g, device="cuda").to(dt), torch.randn(M, N, generator=g, device="cuda").to(dt)
+    w = torch.randn(N, K, generator=g, device="cuda") / 16
+    w[:, torch.randperm(K, generator=g, device="cuda")[: K // 2]] = 0
+    b = torch.randn(N, generator=g, device="cuda")
+
+    def layer():
+        m = GhostLinear(K, N, threshold=0.0, device="cuda", dtype=bias_type)
+        m.weight.copy_(w)
+        m.bias.copy_(b)
+        m.freeze_weight_mask()
+        return m
+
+    a, c = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.no_grad():
+        want = layer()(x, residual=r)
+        for _ in range(3):
+            m = layer()
+            torch.cuda.synchronize()
+            got = []
+            with torch.cuda.stream(a):
+                torch.cuda._sleep(100_000_000)       # some 50 ms
+                got.append(m(x, residual=r))
+            with torch.cuda.stream(c):
+                got.append(m(x, residual=r))
+            for s in (a, c, a, c):
+                with torch.cuda.stream(s):
+                    got.append(m(x, residual=r))
+            torch.cuda.synchronize()
+            assert all(torch.equal(y, want) for y in got)
+        # Copies pack anew, and a captured call uses what is kept.
+        twin = copy.deepcopy(m)
+        m.weight.zero_()
+        assert torch.equal(twin(x, residual=r), want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = twin(x, residual=r)
+        graph.replay()
+        assert torch.equal(y, want)
