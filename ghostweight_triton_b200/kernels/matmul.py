@@ -21,7 +21,7 @@ from __future__ import annotations
 import torch
 
 from ghostweight_triton_b200 import _native
-from ghostweight_triton_b200.kernels._args import in_place_or_apart, overlap, refuse_grad_out, residual_matrix, written
+from ghostweight_triton_b200.kernels._args import Kept, in_place_or_apart, overlap, refuse_grad_out, residual_matrix, written
 from ghostweight_triton_b200.kernels.gather import pack_weight
 
 
@@ -124,10 +124,12 @@ class _PackedCache:
         key = (id(weights), id(idx), dtype)
         e = self._entries.get(key)
         if e is not None:
-            w_ref, i_ref, w_ver, i_ver, packed, prep, ptrs = e
+            w_ref, i_ref, w_ver, i_ver, packed, prep, ptrs, kept = e
             if (w_ref() is weights and i_ref() is idx and w_ver == weights._version
                     and i_ver == idx._version and ptrs == (weights.data_ptr(), idx.data_ptr())
-                    and not torch.cuda.is_current_stream_capturing()):
+                    and not _native._capturing()):
+                if _native.current_raw_stream(weights.get_device()) not in kept.streams:
+                    kept.on_this_stream()
                 self._entries.move_to_end(key)
                 if prep is None and prepare:
                     prep = e[5] = _native.prepare_gather_gemm(packed, idx, None, None, "auto", dtype)
@@ -143,7 +145,7 @@ class _PackedCache:
         prep = _native.prepare_gather_gemm(packed, idx, None, None, "auto", dtype) if prepare else None
         self._entries[key] = [self._weakref.ref(weights, cb), self._weakref.ref(idx, cb),
                               weights._version, idx._version, packed, prep,
-                              (weights.data_ptr(), idx.data_ptr())]
+                              (weights.data_ptr(), idx.data_ptr()), Kept([packed])]
         self.bytes += nbytes
         while len(self._entries) > self.max_entries or self.bytes > self.max_bytes:
             self._drop(next(iter(self._entries)))

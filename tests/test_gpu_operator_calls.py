@@ -607,3 +607,27 @@ def test_layer_used_at_once_on_two_streams(M, bias_type):
             y = twin(x, residual=r)
         graph.replay()
         assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("M", [2, 40, 600])
+def test_cached_weight_used_at_once_on_two_streams(M):
+    """ghostweight_matmul's packed weight, made on one stream behind other work and used at once on a second."""
+    K, N, dt = 512, 768, torch.float16
+    g = torch.Generator(device="cuda").manual_seed(M)
+    x, w = torch.randn(M, K, generator=g, device="cuda").to(dt), torch.randn(K, N, generator=g, device="cuda").to(dt)
+    idx = torch.arange(0, K, 2, device="cuda")
+    a, c = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.no_grad():
+        want = ghostweight_matmul(x, w.clone(), idx)
+        for _ in range(3):
+            fresh = w.clone()
+            torch.cuda.synchronize()
+            got = []
+            with torch.cuda.stream(a):
+                torch.cuda._sleep(100_000_000)       # some 50 ms
+                got.append(ghostweight_matmul(x, fresh, idx))
+            for s in (c, a, c):
+                with torch.cuda.stream(s):
+                    got.append(ghostweight_matmul(x, fresh, idx))
+            torch.cuda.synchronize()
+            assert all(torch.equal(y, want) for y in got)
