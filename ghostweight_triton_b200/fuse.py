@@ -210,8 +210,8 @@ class GhostPreNormMLP(GhostMLPChain):
 
     @property
     def _norm_known(self) -> bool:
-        """Whether the present norm has been tried."""
-        return self.__dict__.get("_tried") is self.norm
+        """Whether the present norm has been tried (a DataParallel replica's is its module's)."""
+        return self.__dict__.get("_tried") is self.norm or getattr(self, "_is_replica", False)
 
     def _try_norm(self) -> None:
         """Assert that a copy of the norm in fp32, with a gain of its own, computes what rms_norm does,

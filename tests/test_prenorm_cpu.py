@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import copy
+
 import pytest
 import torch
 import torch.nn as nn
@@ -110,3 +112,12 @@ def test_the_gain_does_not_hide_the_form(gain):
         else:
             with pytest.raises(AssertionError, match="norm must"):
                 block(norm)
+
+
+def test_replicas_and_copies_are_known():
+    m = block(nn.RMSNorm(16))
+    replica = m._replicate_for_data_parallel()       # what nn.DataParallel makes, with norms of its own
+    replica._modules["norm"] = nn.RMSNorm(16)
+    assert replica._norm_known and copy.deepcopy(m)._norm_known
+    m.norm = nn.RMSNorm(16)
+    assert not m._norm_known
