@@ -205,22 +205,52 @@ __device__ __forceinline__ void dc_finish(const DcArgs<Q8, RES>& p, const float*
   }
 }
 
+// Bounded wait until the k-block `used` or a later one was seen to have landed in a stage.
+__device__ __forceinline__ bool dc_wait_seen(const volatile int* seen, int used, volatile int* abort_flag,
+                                             unsigned int* err) {
+  if (*seen >= used) return true;
+  const unsigned long long t0 = global_timer_ns();
+  for (uint32_t i = 1;; ++i) {
+    if (*seen >= used) return true;
+    if ((i & 255u) == 0u) {
+      if (*abort_flag) return false;
+      if (global_timer_ns() - t0 > GW_WAIT_LIMIT_NS) {
+        *abort_flag = 1;
+        raise_error(err, GW_DERR_WAIT_TIMEOUT);
+        return false;
+      }
+    }
+  }
+}
+
 // Issues the MMAs of k-blocks first, first + step, ... of this CTA's range
 // (local indices; `used` counts ring slots in order) into accumulator d, with
 // one commit per k-block to its stage's empty barrier, then one to tfull (or
 // raises the abort flag) and one to drain_bar.
+//
+// In a ring of an odd number of stages two issuers (step 2) hand each stage to one
+// another. A wait by parity tells a barrier's phase from the one before it only: while
+// the stage's previous use had not landed (loads land in any order), a wait for the
+// present one passed at once, on a stage still being written. So an issuer writes down
+// in `seen` what it found landed, and waits for the other's note before its own wait.
 template <int MP, int DT, bool Q8, typename FullF, typename EmptyF>
 __device__ __forceinline__ void dc_issue(const DcParams& p, uint32_t sbase, uint32_t d, int nk,
                                          int first, int step, FullF full, EmptyF empty,
                                          uint32_t tfull, uint32_t drain_bar,
-                                         volatile int* abort_flag) {
+                                         volatile int* abort_flag, volatile int* seen) {
   using C = DcCfg<MP>;
   constexpr uint32_t idesc = idesc_for<Q8, DT>(kDcN, MP);
+  const bool handed = (C::kStages & 1) != 0 && step == 2;
   bool ok = true;
   for (int used = first; used < nk; used += step) {
     const int s = used % C::kStages;
     const uint32_t ph = (used / C::kStages) & 1u;
+    if (handed && used >= C::kStages && !dc_wait_seen(seen + s, used - C::kStages, abort_flag, p.err)) {
+      ok = false;
+      break;
+    }
     if (!mbar_wait(full(s), ph, abort_flag, p.err)) { ok = false; break; }
+    if (handed) seen[s] = used;
     tc_fence_after();
     const uint32_t w_s = sbase + s * C::kStageBytes;
     const uint64_t w_desc = smem_desc_kmajor_sw128(w_s);
@@ -260,6 +290,8 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap tmap_w,
   static_assert(8 * (2 * C::kStages + 4) <= 192, "barrier region overflows into the TMEM slot");
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_region + 192);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bar_region + 196);
+  volatile int* seen = abort_flag + 1;     // per stage: the last k-block that an issuer saw landed
+  static_assert(200 + 4 * C::kStages <= 256, "barrier region");
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -280,6 +312,7 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap tmap_w,
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
+      seen[s] = -1;
       mbar_init(full(s), p.gx ? 2 : 1);    // gather mode: the producer's and the gathering warp's arrivals
       mbar_init(empty(s), 1);
     }
@@ -357,7 +390,7 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap tmap_w,
     // ------------------------------------------------------------ MMA issuer (even k-blocks)
     if (lane == 0) {
       dc_issue<MP, DT, Q8>(p, sbase, tmem_base, kb1 - kb0, 0, dual ? 2 : 1, full, empty, tfull,
-                       drain_bar, abort_flag);
+                       drain_bar, abort_flag, seen);
       // Every MMA (of both issuers) has finished writing TMEM before TMEM is freed.
       mbar_wait(drain_bar, 0u, nullptr, p.err, 100000000ull);
     }
@@ -367,7 +400,7 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap tmap_w,
       // ---------------------------------------------------------- MMA issuer (odd k-blocks)
       if (lane == 0)
         dc_issue<MP, DT, Q8>(p, sbase, tmem_base + MP, kb1 - kb0, 1, 2, full, empty, tfull, drain_bar,
-                         abort_flag);
+                         abort_flag, seen);
       __syncwarp();
     }
     if (p.gx) {

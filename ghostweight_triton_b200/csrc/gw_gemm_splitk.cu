@@ -66,6 +66,9 @@ struct SkCfg {
   static constexpr int kAccCols = kDual ? 2 * BN : BN;
   static constexpr int kTmemCols = kAccCols < 32 ? 32 : kAccCols;  // power of two >= 32
   static constexpr int kSmemBytes = 1024 + kRingBytes + 256;
+  // Each issuer takes every use of its stages: it waits for a phase by its parity, which
+  // tells it from the one before only (see dc_issue in gw_gemm_decode.cu).
+  static_assert(!kDual || kStages % 2 == 0, "an odd ring hands stages from issuer to issuer");
   static_assert(kSmemBytes <= 232448, "shared memory budget per CTA");
 };
 
