@@ -631,3 +631,25 @@ def test_cached_weight_used_at_once_on_two_streams(M):
                     got.append(ghostweight_matmul(x, fresh, idx))
             torch.cuda.synchronize()
             assert all(torch.equal(y, want) for y in got)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("M", [1, 16])
+def test_decode_products_over_cold_weights(M, q8):
+    """Up to 16 rows with more k-blocks per CTA than the ring has stages, back to back over weights that
+    lie in HBM (their loads land in any order): the same bits in every round, and the formula's values."""
+    N, K, dt = 4096, 4096, torch.bfloat16
+    g = torch.Generator(device="cuda").manual_seed(M)
+    x, r = torch.randn(M, K, generator=g, device="cuda").to(dt), torch.randn(M, N, generator=g, device="cuda").to(dt)
+    ws = [(torch.randn(N, K, generator=g, device="cuda") / 64).to(dt) for _ in range(12)]      # 400 MB
+    if q8:
+        a, packed = quantize_rows(x), [quantize_rows(w) for w in ws]
+        call = lambda i: packed_linear_q8(*a, *packed[i], residual=r)
+    else:
+        call = lambda i: packed_linear(x, ws[i], residual=r)
+    first = [call(i) for i in range(len(ws))]
+    rounds = [[call(i) for i in range(len(ws))] for _ in range(20)]
+    for i, y in enumerate(first):
+        assert all(torch.equal(y, later[i]) for later in rounds)
+        if not q8:
+            check(y, x, ws[i], None, None, r)
