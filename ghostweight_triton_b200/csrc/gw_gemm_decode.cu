@@ -214,7 +214,7 @@ __device__ __forceinline__ bool dc_wait_seen(const volatile int* seen, int used,
     if (*seen >= used) return true;
     if ((i & 255u) == 0u) {
       if (*abort_flag) return false;
-      if (global_timer_ns() - t0 > GW_WAIT_LIMIT_NS) {
+      if (past_limit(t0, GW_WAIT_LIMIT_NS)) {
         *abort_flag = 1;
         raise_error(err, GW_DERR_WAIT_TIMEOUT);
         return false;
@@ -260,8 +260,12 @@ __device__ __forceinline__ void dc_issue(const DcParams& p, uint32_t sbase, uint
       tc_mma<Q8>(d, w_desc + 2u * k, a_desc + 2u * k, idesc, (used > first || k > 0) ? 1u : 0u);
     tc_commit(empty(s));
   }
-  if (ok) tc_commit(tfull);
-  else *abort_flag = 1;            // the drain warps stop waiting for tfull
+  if (ok) {
+    tc_commit(tfull);
+  } else {
+    *abort_flag = 1;               // the drain warps stop waiting for tfull
+    drain_full(full(0), C::kStages, p.err);
+  }
   tc_commit(drain_bar);
 }
 
@@ -378,12 +382,10 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap tmap_w,
           tma_load_2d(w_s + kDcWBytes, &tmap_a, ax, 0, full(s));
         }
       }
-      if (!ok) {
-        // Loads still in flight complete before the CTA exits.
-        const int first = issued > C::kStages ? issued - C::kStages : 0;
-        for (int i = first; i < issued; ++i)
-          mbar_wait(full(i % C::kStages), (i / C::kStages) & 1u, nullptr, p.err, 100000000ull);
-      }
+      // Loads in flight land before the CTA exits. An issuer that gave up
+      // raises the flag before it waits for the loads of that time: a producer that
+      // does not see the flag here had issued all of its own by then.
+      if (!ok || *abort_flag) drain_full(full(0), C::kStages, p.err);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -474,14 +476,17 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap tmap_w,
 
   // The residual and the scales of a may come from the previous kernel of the stream.
   if (Q8 || RES) asm volatile("griddepcontrol.wait;" ::: "memory");
-  // Every slot of this CTA's slice has landed: its own and the S - 1 peers'.
-  const bool got = mbar_wait_cluster(recv_bar, 0u, nullptr, p.err);
+  // Every slot of this CTA's slice has landed: its own and the S - 1 peers'. A peer
+  // whose own waits run out sends zeros, after at most two of them and its drain: this
+  // CTA, into which it sends, stays for longer than that.
+  constexpr unsigned long long kPeerLimit = 4 * GW_WAIT_LIMIT_NS;
+  const bool got = mbar_wait_cluster(recv_bar, 0u, nullptr, p.err, kPeerLimit);
   // Tell every sender that its copy into this CTA has landed.
   if (threadIdx.x < S) mbar_arrive_cluster(mapa_shared(sent_bar, threadIdx.x));
   if (got) dc_finish<MP, DT, Q8, RES>(p, recv, rank, n_blk, rows);
   // This CTA's ring is the source of its copies: it stays valid, and the CTA
   // alive, until every owner has received its slice.
-  mbar_wait_cluster(sent_bar, 0u, nullptr, p.err);
+  mbar_wait_cluster(sent_bar, 0u, nullptr, p.err, kPeerLimit);
 }
 
 template <int MP, int DT, bool Q8, bool RES>

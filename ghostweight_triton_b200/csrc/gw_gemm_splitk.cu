@@ -234,8 +234,12 @@ __device__ __forceinline__ void sk_issue(const SkParams& p, uint32_t sbase, uint
       tc_mma<Q8>(d, a_desc + 2u * k, b_desc + 2u * k, idesc, (used > first || k > 0) ? 1u : 0u);
     tc_commit(empty(s));
   }
-  if (ok) tc_commit(tfull);
-  else *abort_flag = 1;            // the drain warps stop waiting for tfull
+  if (ok) {
+    tc_commit(tfull);
+  } else {
+    *abort_flag = 1;               // the drain warps stop waiting for tfull
+    drain_full(full(0), C::kStages, p.err);
+  }
   tc_commit(drain_bar);
 }
 
@@ -318,12 +322,10 @@ gemm_splitk_kernel(const __grid_constant__ CUtensorMap tmap_b,
         const int ax = p.a_cols ? run_start_check(cur, p.a_width, p.err) : kb * kCols;
         tma_load_2d(a_s, &tmap_a, ax, m_blk * kSkBM, full(s));
       }
-      if (!ok) {
-        // Loads still in flight complete before the ring is reused or the CTA exits.
-        const int first = issued > C::kStages ? issued - C::kStages : 0;
-        for (int i = first; i < issued; ++i)
-          mbar_wait(full(i % C::kStages), (i / C::kStages) & 1u, nullptr, p.err, 100000000ull);
-      }
+      // Loads in flight land before the ring is reused or the CTA exits. An issuer that gave up
+      // raises the flag before it waits for the loads of that time: a producer that
+      // does not see the flag here had issued all of its own by then.
+      if (!ok || *abort_flag) drain_full(full(0), C::kStages, p.err);
     }
     __syncwarp();
   } else if (warp == 1) {

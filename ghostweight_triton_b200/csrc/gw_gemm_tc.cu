@@ -199,12 +199,9 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmap_b,
           }
         }
       }
-      if (!ok) {
-        // Drain loads still in flight before the CTA exits (bounded, 100 ms).
-        const uint32_t first = it > static_cast<uint32_t>(C::kStages) ? it - C::kStages : 0u;
-        for (uint32_t i = first; i < it; ++i)
-          mbar_wait(full_b(i % C::kStages), (i / C::kStages) & 1u, nullptr, p.err, 100000000ull);
-      }
+      // Loads in flight land before the CTA exits: those issued since an issuer gave up
+      // here, those before it by itself (it raises the flag first).
+      if (!ok || *abort_flag) drain_full(full_b(0), C::kStages, p.err);
     }
   } else if (warp == kWarpMma) {
     // ------------------------------------------------------------ MMA issuer
@@ -242,6 +239,10 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmap_b,
         }
         if (!ok) break;
         tc_commit(tfull(b));
+      }
+      if (!ok) {
+        *abort_flag = 1;
+        drain_full(full_b(0), C::kStages, p.err);
       }
       // All MMAs of this thread complete before TMEM can be released.
       tc_commit(drain_bar);

@@ -240,7 +240,7 @@ __device__ __forceinline__ bool wait_flag_eq(const unsigned long long* flag, uin
     if (ld_acquire_gpu_u64(flag) == value) return true;
     if ((i & 63u) == 0u) {
       if (abort_flag && *abort_flag) return false;
-      if (global_timer_ns() - t0 > GW_WAIT_LIMIT_NS) {
+      if (past_limit(t0, GW_WAIT_LIMIT_NS)) {
         if (abort_flag) *abort_flag = 1;
         raise_error(err, GW_DERR_WAIT_TIMEOUT);
         return false;
@@ -526,11 +526,10 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
           }
         }
       }
-      if (!ok && rank == 0) {
-        const uint32_t first = it > static_cast<uint32_t>(kStages2) ? it - kStages2 : 0u;
-        for (uint32_t i = first; i < it; ++i)
-          mbar_wait_cluster(full(i % kStages2), (i / kStages2) & 1u, nullptr, p.err, 100000000ull);
-      }
+      // Both CTAs' loads are counted on the leader's barriers. They land before the pair
+      // exits: those issued since the issuer gave up are waited for here, those before it
+      // by the issuer (it raises the flag first).
+      if (rank == 0 && (!ok || *abort_flag)) drain_full(full(0), kStages2, p.err);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (leader only)
@@ -579,6 +578,10 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_b,
         }
         if (!ok) break;
         tc_commit_pair_mc(tfull(b), 0x3);
+      }
+      if (!ok) {
+        *abort_flag = 1;
+        drain_full(full(0), kStages2, p.err);
       }
       tc_commit_pair_mc(drain_bar, 0x1);
       mbar_wait(drain_bar, 0u, nullptr, p.err, 100000000ull);
